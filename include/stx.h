@@ -748,6 +748,121 @@ STX_API stx_status stx_separate_audio(const stx_audio_view* input, int model_cha
                                       size_t workspace_bytes, stx_stream stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Transformer-layer operators over fp32, fp16 and bf16 tensors, with their gradients: what the
+ * models' layers need in half precision, on longer clips than they were trained on, and to be
+ * fine-tuned. They have no counterpart of their own in the reference, which runs these layers
+ * forward, in fp32, at the trained length; the neighbours they extend are named at each.
+ * All data tensors of a call have one element type (nb[0] is its size); parameters and
+ * statistics have the types given below whatever the data's. Sums and statistics are kept in
+ * 32 bits or more and results rounded once. Results are deterministic. Nothing is allocated, and
+ * every call may be captured into a graph. Tensors, workspace and stream belong to the current
+ * device. Inputs of no elements are valid: outputs that are sums over them are zeros.
+ * ---------------------------------------------------------------------------------------- */
+typedef int32_t stx_type;          /* ggml's numbers of these types */
+enum {
+    STX_TYPE_F32  = 0,
+    STX_TYPE_F16  = 1,
+    STX_TYPE_BF16 = 30
+};
+
+typedef int32_t stx_act;           /* act(z) */
+enum {
+    STX_ACT_NONE    = 0,           /* z */
+    STX_ACT_GELU    = 1,           /* z/2 * (1 + erf(z / sqrt2)), stx_gelu_erf's */
+    STX_ACT_SILU    = 2,           /* z / (1 + exp(-z)) */
+    STX_ACT_SIGMOID = 3            /* 1 / (1 + exp(-z)), the gate of stx_glu */
+};
+
+/* The rotation of stx_rope_scaled. For pair i of n_dims/2 and position p:
+ *   far   = p * freq_base^(-2i/n_dims) / freq_factors[i]      (factors of 1 where NULL)
+ *   theta = freq_scale * far                                  when ext_factor == 0
+ *         = freq_scale * far * (1 - mix_i) + far * mix_i      otherwise, where
+ *   mix_i = ext_factor * (1 - clamp((i - lo) / max(0.001, hi - lo), 0, 1)),
+ *   lo    = max(0, floor(d(beta_fast))), hi = min(n_dims - 1, ceil(d(beta_slow))),
+ *   d(r)  = n_dims * ln(n_ctx_orig / (2 pi r)) / (2 ln freq_base)
+ * (linear interpolation; the by-parts interpolation of Peng et al., "YaRN", 2023, section 3.2),
+ * and the rotated pair is scaled by attn_factor, times 1 + 0.1 ln(1 / freq_scale) when
+ * ext_factor != 0. Mode 0 rotates adjacent pairs (2i, 2i+1), mode 2 the pairs
+ * (i, i + n_dims/2); elements from n_dims on are copied. Size tagged: set size to the struct's. */
+typedef struct {
+    uint32_t size;
+    int32_t  n_dims;               /* even, 2 .. min(ne0, 8192) */
+    int32_t  mode;                 /* 0 or 2 */
+    int32_t  n_ctx_orig;           /* trained length; used when ext_factor != 0 */
+    float    freq_base;            /* > 0, and != 1 when ext_factor != 0 */
+    float    freq_scale;           /* > 0 */
+    float    ext_factor;
+    float    attn_factor;
+    float    beta_fast;            /* > 0 when ext_factor != 0 */
+    float    beta_slow;
+    const float* freq_factors;     /* device [n_dims/2], or NULL */
+} stx_rope_params;
+
+/* stx_rope_ext (above) over typed tensors, with scaled positions, for the queries q
+ * [dim, heads, N, batch] and, where k is not NULL, the keys k [dim, kv heads, N, batch] of one
+ * attention in one launch. pos is device int32: token i2 of batch i3 is at
+ * pos[i3 * pos_stride + i2] (pos_stride 0: every sequence has the same positions). Angles are
+ * formed in double, the rotation in float. Rows are contiguous; any other strides, so q and k may be
+ * slices of a projection's output. q_dst may be q and k_dst may be k; outputs overlap nothing
+ * else. At most 2^31 - 1 tokens (N * batch) and 2^24 - 1 rows a token. */
+STX_API stx_status stx_rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
+                                   int64_t pos_stride, const stx_rope_params* params, const stx_tensor* q_dst,
+                                   const stx_tensor* k_dst, stx_stream stream);
+/* Its gradient: q and k are the gradients of the rotated tensors, q_dst and k_dst those of the
+ * tensors before (the rotation is linear: the same scaling, by -theta). */
+STX_API stx_status stx_rope_scaled_back(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
+                                        int64_t pos_stride, const stx_rope_params* params, const stx_tensor* q_dst,
+                                        const stx_tensor* k_dst, stx_stream stream);
+
+/* GroupNorm over channels-last tensors: a is [C, T1, T2, B], contiguous. stx_group_norm has
+ * the channels in ne2; the norm over tokens [D, N] at the end of HTDemucs' transformer
+ * (src/htdemucs.cpp:223-227) is this one with one group. The channels are split into n_groups
+ * groups of ceil(C / n_groups), the last of what is left (every group has a channel); each is
+ * normalised per ne3 slice over T1 x T2 x its channels with the biased variance:
+ *   y = act((a - mean) / sqrt(var + eps) * weight[c] + bias[c]).
+ * weight and bias: device float[C], either may be NULL (1 and 0). stats: device double
+ * [B][n_groups][2], receives mean and 1 / sqrt(var + eps) for stx_group_norm_cl_back (NULL: not
+ * kept); without elements (T1 or T2 0) they are 0 and 1 / sqrt(eps). dst may be a. workspace:
+ * device, 256-byte aligned, no initialisation; calls that share one must not overlap. */
+STX_API size_t     stx_group_norm_cl_workspace_size(const stx_tensor* a, stx_type type, int n_groups);
+STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_groups, double eps, const float* weight,
+                                     const float* bias, stx_act act, const stx_tensor* dst, double* stats,
+                                     void* workspace, size_t workspace_bytes, stx_stream stream);
+/* Its gradients, from dy (of y), a and stats as the forward call left them: dx (of a; may be dy),
+ * dweight and dbias (device float[C], summed over T1, T2 and B). Any of the three may be NULL.
+ * The same workspace size. */
+STX_API stx_status stx_group_norm_cl_back(const stx_tensor* dy, const stx_tensor* a, stx_type type, const double* stats,
+                                          int n_groups, const float* weight, const float* bias, stx_act act,
+                                          const stx_tensor* dx, float* dweight, float* dbias, void* workspace,
+                                          size_t workspace_bytes, stx_stream stream);
+
+/* The gated feed-forward block, both projections and the gate in one kernel:
+ *   dst[n, m] = act(sum_k x[k, m] w_gate[k, n] + b_gate[n]) * (sum_k x[k, m] w_value[k, n] + b_value[n]).
+ * With STX_ACT_SIGMOID it is stx_glu of a linear layer (the mask heads, src/roformer.cpp:193-204).
+ * x [K, tokens...] (up to three token dimensions, evenly spaced rows), w_gate and w_value [K, N]
+ * (ggml's weight layout), dst [N, tokens...] (the same token dimensions, evenly spaced rows);
+ * rows are contiguous, row strides any. b_gate, b_value: device float[N], either may be NULL.
+ * Products are accumulated in fp32 (matrix instructions of the data's type). dst overlaps no
+ * input. At most 2^30 tokens, K and N at most 2^20. */
+STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, const stx_tensor* w_value, stx_type type,
+                                const float* b_gate, const float* b_value, stx_act act, const stx_tensor* dst,
+                                stx_stream stream);
+/* Its gradients, from dh (of dst) and the forward call's inputs; the two products are formed
+ * again, so the forward call keeps nothing. dx (of x), dw_gate and dw_value (of the weights),
+ * db_gate and db_value (device float[N]); any may be NULL, and the work for it is left out (both
+ * weights' gradients or neither). For fp16 and bf16 the gradients of the two products are rounded
+ * to the data's type before the matrix products that use them; db_gate and db_value are summed from
+ * the unrounded ones. Outputs overlap no input. workspace: device, 256-byte aligned, no
+ * initialisation; calls that share one must not overlap. The size is for n_tokens tokens, K =
+ * n_in, N = n_hidden (0 for sizes that stx_gated_ff_back rejects). */
+STX_API size_t     stx_gated_ff_back_workspace_size(int64_t n_tokens, int64_t n_in, int64_t n_hidden, stx_type type);
+STX_API stx_status stx_gated_ff_back(const stx_tensor* dh, const stx_tensor* x, const stx_tensor* w_gate,
+                                     const stx_tensor* w_value, stx_type type, const float* b_gate, const float* b_value,
+                                     stx_act act, const stx_tensor* dx, const stx_tensor* dw_gate,
+                                     const stx_tensor* dw_value, float* db_gate, float* db_value, void* workspace,
+                                     size_t workspace_bytes, stx_stream stream);
+
+/* ------------------------------------------------------------------------------------------
  * Versioned function table (after libstems V1, src/libstems_v1.h:146-189). Every entry point
  * above, in header order; a later revision of V1 may append entries (never reorder them), so
  * a consumer checks `size` against the prefix it needs.
@@ -937,6 +1052,35 @@ typedef struct stx_api_v1 {
                                  void* separate_user, const stx_separate_options* options,
                                  float* out, void* workspace, size_t workspace_bytes,
                                  stx_stream stream);
+    /* Appended: the transformer-layer operators over typed tensors. */
+    stx_status (*rope_scaled)(const stx_tensor* q, const stx_tensor* k, stx_type type,
+                              const int32_t* pos, int64_t pos_stride, const stx_rope_params* params,
+                              const stx_tensor* q_dst, const stx_tensor* k_dst, stx_stream stream);
+    stx_status (*rope_scaled_back)(const stx_tensor* q, const stx_tensor* k, stx_type type,
+                                   const int32_t* pos, int64_t pos_stride,
+                                   const stx_rope_params* params, const stx_tensor* q_dst,
+                                   const stx_tensor* k_dst, stx_stream stream);
+    size_t (*group_norm_cl_workspace_size)(const stx_tensor* a, stx_type type, int n_groups);
+    stx_status (*group_norm_cl)(const stx_tensor* a, stx_type type, int n_groups, double eps,
+                                const float* weight, const float* bias, stx_act act,
+                                const stx_tensor* dst, double* stats, void* workspace,
+                                size_t workspace_bytes, stx_stream stream);
+    stx_status (*group_norm_cl_back)(const stx_tensor* dy, const stx_tensor* a, stx_type type,
+                                     const double* stats, int n_groups, const float* weight,
+                                     const float* bias, stx_act act, const stx_tensor* dx,
+                                     float* dweight, float* dbias, void* workspace,
+                                     size_t workspace_bytes, stx_stream stream);
+    stx_status (*gated_ff)(const stx_tensor* x, const stx_tensor* w_gate, const stx_tensor* w_value,
+                           stx_type type, const float* b_gate, const float* b_value, stx_act act,
+                           const stx_tensor* dst, stx_stream stream);
+    size_t (*gated_ff_back_workspace_size)(int64_t n_tokens, int64_t n_in, int64_t n_hidden,
+                                           stx_type type);
+    stx_status (*gated_ff_back)(const stx_tensor* dh, const stx_tensor* x, const stx_tensor* w_gate,
+                                const stx_tensor* w_value, stx_type type, const float* b_gate,
+                                const float* b_value, stx_act act, const stx_tensor* dx,
+                                const stx_tensor* dw_gate, const stx_tensor* dw_value,
+                                float* db_gate, float* db_value, void* workspace,
+                                size_t workspace_bytes, stx_stream stream);
     void (*reserved[16])(void);
 } stx_api_v1;
 

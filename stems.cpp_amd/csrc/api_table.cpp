@@ -95,6 +95,14 @@ const stx_api_v1 kApiV1 = {
     &stx_concat,
     &stx_separate_audio_workspace_size,
     &stx_separate_audio,
+    &stx_rope_scaled,
+    &stx_rope_scaled_back,
+    &stx_group_norm_cl_workspace_size,
+    &stx_group_norm_cl,
+    &stx_group_norm_cl_back,
+    &stx_gated_ff,
+    &stx_gated_ff_back_workspace_size,
+    &stx_gated_ff_back,
     {},
 };
 }  // namespace

@@ -1,0 +1,173 @@
+// typed.hpp — element types of the transformer-layer operators (fp32, fp16, bf16): checks of
+// typed tensors on the host, conversions, vector access and activations on the device.
+#pragma once
+
+#include <type_traits>
+
+#include "tensor.hpp"
+
+namespace stx {
+
+using f16 = _Float16;
+using bf16 = __bf16;
+
+inline int type_size(stx_type t) {
+    switch (t) {
+    case STX_TYPE_F32: return 4;
+    case STX_TYPE_F16:
+    case STX_TYPE_BF16: return 2;
+    default: fail(STX_STATUS_INVALID_ARGUMENT, "unknown element type %d", (int)t);
+    }
+}
+
+// Calls f(T{}) with the device type of t.
+template <class F>
+void with_type(stx_type t, F&& f) {
+    switch (t) {
+    case STX_TYPE_F32: return f(float{});
+    case STX_TYPE_F16: return f(f16{});
+    case STX_TYPE_BF16: return f(bf16{});
+    default: fail(STX_STATUS_INVALID_ARGUMENT, "unknown element type %d", (int)t);
+    }
+}
+
+inline void check_act(stx_act act) {
+    STX_REQUIRE(act >= STX_ACT_NONE && act <= STX_ACT_SIGMOID, "unknown activation %d", (int)act);
+}
+
+// check_tensor (tensor.hpp) for elements of `size` bytes; the data is aligned to its elements.
+inline void check_typed(const stx_tensor* t, int size, const char* what) {
+    STX_REQUIRE(t != nullptr, "%s is NULL", what);
+    bool none = false;
+    for (int i = 0; i < 4; i++) {
+        STX_REQUIRE(t->ne[i] >= 0, "%s: negative ne[%d]", what, i);
+        none = none || t->ne[i] == 0;
+    }
+    long long n = none ? 0 : 1;
+    for (int i = 0; i < 4 && !none; i++) {
+        STX_REQUIRE(t->ne[i] < (1LL << 40) / n, "%s too large", what);
+        n *= t->ne[i];
+    }
+    STX_REQUIRE(t->nb[0] == size, "%s: rows must be contiguous (nb[0] == %d, the element size)", what, size);
+    for (int i = 1; i < 4; i++) STX_REQUIRE(t->nb[i] >= 0 && t->nb[i] % size == 0, "%s: bad stride nb[%d]", what, i);
+    STX_REQUIRE(n == 0 || t->data != nullptr, "%s has no data", what);
+    STX_REQUIRE(reinterpret_cast<uintptr_t>(t->data) % size == 0, "%s: data is not aligned to its elements", what);
+}
+
+inline bool contiguous_typed(const stx_tensor* t, int size) {
+    long long expect = size;
+    bool dense = true;
+    for (int i = 0; i < 4; i++) {
+        if (t->ne[i] == 0) return true;
+        dense = dense && (t->ne[i] == 1 || t->nb[i] == expect);
+        expect *= t->ne[i];
+    }
+    return dense;
+}
+
+// First and last byte past the end that a tensor's elements span; {0, 0} without elements.
+struct Span {
+    uintptr_t lo, hi;
+};
+inline Span span_of(const stx_tensor* t, int size) {
+    uintptr_t lo = reinterpret_cast<uintptr_t>(t->data), hi = lo + size;
+    for (int i = 0; i < 4; i++) {
+        if (t->ne[i] == 0) return {0, 0};
+        hi += (uintptr_t)((t->ne[i] - 1) * t->nb[i]);
+    }
+    return {lo, hi};
+}
+inline Span span_of(const void* p, size_t bytes) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return p && bytes ? Span{lo, lo + bytes} : Span{0, 0};
+}
+inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+inline void check_workspace(const void* ws, size_t have, size_t need, const char* what) {
+    if (need == 0) return;
+    STX_REQUIRE(ws != nullptr && have >= need, "%s: workspace of %zu bytes needed, %zu given", what, need, ws ? have : (size_t)0);
+    STX_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, "%s: the workspace must be 256-byte aligned", what);
+}
+
+// ------------------------------------------------------------------------------- device
+// N elements moved as one access of N * sizeof(T) bytes.
+template <class T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(f16 x) { return (float)x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return (float)x; }
+// Rounded to nearest even. The float is made opaque before fp16's rounding: the compiler otherwise
+// takes v_fma_mixlo_f16 for some fused results and not for others, and that one rounds the
+// exact sum to fp16 where the rest round the float, so vector and scalar paths would differ by a bit.
+template <class T>
+__device__ __forceinline__ T from_f32(float x) {
+    if constexpr (std::is_same_v<T, f16>) asm("" : "+v"(x));
+    return (T)x;
+}
+
+// 1 / (1 + exp(-z)) with the hardware reciprocal (1 ulp).
+__device__ __forceinline__ float sigmoid_f32(float z) { return __builtin_amdgcn_rcpf(1.f + expf(-z)); }
+
+// Phi(z), the normal distribution, and phi = exp(-z^2/2): Phi(-|z|) = phi t P(t) / 2 with
+// t = 1 / (1 + |z| / (2 sqrt2)), P the polynomial of stx_gelu_erf (gelu_phi_neg in ops.hip).
+__device__ __forceinline__ float normal_cdf(float z, float& phi) {
+    phi = expf(-0.5f * z * z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35355339059327376220f, fabsf(z), 1.f));
+    float p = -1.5161373655e-02f;
+    p = fmaf(p, t, 9.183117002e-02f);
+    p = fmaf(p, t, -2.2204872965e-01f);
+    p = fmaf(p, t, 2.545801103e-01f);
+    p = fmaf(p, t, -1.139718890e-01f);
+    p = fmaf(p, t, 4.3268962765e-03f);
+    p = fmaf(p, t, -3.3629499375e-02f);
+    p = fmaf(p, t, -1.2177567695e-03f);
+    p = fmaf(p, t, 4.1566714645e-02f);
+    p = fmaf(p, t, 8.82191360e-02f);
+    p = fmaf(p, t, 1.234102100e-01f);
+    p = fmaf(p, t, 1.4104762675e-01f);
+    p = fmaf(p, t, 1.410473883e-01f);
+    const float q = phi * (t * p);
+    return z < 0.f ? q : 1.f - q;
+}
+
+// act(z), and its derivative d.
+template <int ACT>
+__device__ __forceinline__ float act_f32(float z) {
+    float phi;
+    if constexpr (ACT == STX_ACT_GELU) return z * normal_cdf(z, phi);
+    if constexpr (ACT == STX_ACT_SILU) return z * sigmoid_f32(z);
+    if constexpr (ACT == STX_ACT_SIGMOID) return sigmoid_f32(z);
+    return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_f32(float z, float& d) {
+    if constexpr (ACT == STX_ACT_GELU) {
+        float phi;
+        const float c = normal_cdf(z, phi);
+        d = fmaf(z * phi, 0.39894228040143267794f, c);               // Phi + z phi / sqrt(2 pi)
+        return z * c;
+    } else if constexpr (ACT == STX_ACT_SILU || ACT == STX_ACT_SIGMOID) {
+        const float s = sigmoid_f32(z);
+        d = ACT == STX_ACT_SILU ? s * fmaf(z, 1.f - s, 1.f) : s * (1.f - s);
+        return ACT == STX_ACT_SILU ? z * s : s;
+    } else {
+        d = 1.f;
+        return z;
+    }
+}
+
+// Calls f(std::integral_constant<int, act>{}), on the host or (act uniform over the launch) in a kernel.
+template <class F>
+__host__ __device__ __forceinline__ void with_act(int act, F&& f) {
+    switch (act) {
+    case STX_ACT_GELU: return f(std::integral_constant<int, STX_ACT_GELU>{});
+    case STX_ACT_SILU: return f(std::integral_constant<int, STX_ACT_SILU>{});
+    case STX_ACT_SIGMOID: return f(std::integral_constant<int, STX_ACT_SIGMOID>{});
+    default: return f(std::integral_constant<int, STX_ACT_NONE>{});
+    }
+}
+
+}  // namespace stx

@@ -121,6 +121,15 @@ _SIGNATURES = {
     "stx_concat": (_i, [_vp, _i, _i, _vp, _vp]),
     "stx_separate_audio_workspace_size": (ctypes.c_size_t, [_vp, _i, _i, _i]),
     "stx_separate_audio": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "stx_rope_scaled": (_i, [_vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp]),
+    "stx_rope_scaled_back": (_i, [_vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp]),
+    "stx_group_norm_cl_workspace_size": (ctypes.c_size_t, [_vp, _i, _i]),
+    "stx_group_norm_cl": (_i, [_vp, _i, _i, ctypes.c_double, _vp, _vp, _i, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "stx_group_norm_cl_back": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "stx_gated_ff": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp]),
+    "stx_gated_ff_back_workspace_size": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _i]),
+    "stx_gated_ff_back": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                               _vp]),
 }
 
 
@@ -1093,3 +1102,228 @@ def concat(tensors, dim, out=None, stream=None):
     arr = (ctypes.c_void_p * len(descs))(*[ctypes.addressof(d) for d in descs])
     check(lib().stx_concat(arr, len(descs), int(dim), _t(out), _stream(stream)))
     return out
+
+
+# ----------------------------------------- transformer-layer operators (fp32, fp16, bf16)
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 30
+
+ACT_NONE = 0
+ACT_GELU = 1
+ACT_SILU = 2
+ACT_SIGMOID = 3
+
+
+class RopeParams(ctypes.Structure):
+    """stx_rope_params; rope_params() fills it and keeps the frequency factors' tensor alive."""
+    _fields_ = [("size", ctypes.c_uint32), ("n_dims", ctypes.c_int32), ("mode", ctypes.c_int32),
+                ("n_ctx_orig", ctypes.c_int32), ("freq_base", ctypes.c_float), ("freq_scale", ctypes.c_float),
+                ("ext_factor", ctypes.c_float), ("attn_factor", ctypes.c_float), ("beta_fast", ctypes.c_float),
+                ("beta_slow", ctypes.c_float), ("freq_factors", ctypes.c_void_p)]
+
+
+def rope_params(n_dims, mode=0, freq_factors=None, freq_base=10000.0, freq_scale=1.0, n_ctx_orig=0, ext_factor=0.0,
+                attn_factor=1.0, beta_fast=32.0, beta_slow=1.0):
+    """The rotation of rope_scaled; freq_factors is a float32 device tensor of n_dims / 2 values, or None."""
+    if freq_factors is not None:
+        import torch
+        _require(freq_factors, torch.float32, "freq_factors")
+        if freq_factors.numel() != n_dims // 2:
+            raise ValueError("freq_factors must have n_dims / 2 values")
+    p = RopeParams(ctypes.sizeof(RopeParams), int(n_dims), int(mode), int(n_ctx_orig), float(freq_base), float(freq_scale),
+                   float(ext_factor), float(attn_factor), float(beta_fast), float(beta_slow),
+                   None if freq_factors is None else freq_factors.data_ptr())
+    p.factors = freq_factors
+    return p
+
+
+def _type(t):
+    import torch
+    try:
+        return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}[t.dtype]
+    except KeyError:
+        raise TypeError(f"operands must be float32, float16 or bfloat16, got {t.dtype}") from None
+
+
+def _typed(t, like, what):
+    """stx_tensor of a tensor of up to 4 dims with the element type and device of `like`."""
+    if t.dtype != like.dtype:
+        raise TypeError(f"{what} must be {like.dtype}, got {t.dtype}")
+    if t.device != like.device or not t.is_cuda:
+        raise ValueError(f"{what} must be a CUDA (HIP) tensor on {like.device}")
+    size, n = t.element_size(), t.dim()
+    if n > 4:
+        raise ValueError(f"{what} has more than 4 dimensions")
+    shape, strides = t.shape, t.stride()
+    d = Tensor()
+    d.data = t.data_ptr()
+    at = size
+    for i in range(4):
+        e = shape[n - 1 - i] if i < n else 1
+        d.ne[i] = e
+        d.nb[i] = at if e == 1 else size * strides[n - 1 - i]
+        at = d.nb[i] * e
+    return d
+
+
+def _floats(t, like, count, what, dtype=None):
+    """Pointer of a contiguous float32 (or dtype) vector of `count` values on like's device, or None."""
+    if t is None:
+        return None
+    import torch
+    _require(t, dtype or torch.float32, what)
+    if t.device != like.device:
+        raise ValueError(f"{what} must be on {like.device}")
+    if t.numel() != count:
+        raise ValueError(f"{what} must have {count} values, has {t.numel()}")
+    return t.data_ptr()
+
+
+def _launch(fn, like, stream, *args):
+    """fn(*args, stream) with like's device current, on `stream` (default: that device's current stream)."""
+    import torch
+    if like.device.index == torch.cuda.current_device():
+        s = stream if stream is not None else torch.cuda.current_stream()
+        check(fn(*args, s.cuda_stream))
+        return
+    with torch.cuda.device(like.device):
+        s = stream if stream is not None else torch.cuda.current_stream()
+        check(fn(*args, s.cuda_stream))
+
+
+def _scratch(need, workspace, like, stream):
+    """(pointer, bytes) of the caller's workspace, or of a new one that belongs to `stream` (so that memory freed on
+    return is not handed to another stream while the call still uses it); and the tensor that owns it."""
+    if workspace is None:
+        import torch
+        with torch.cuda.stream(stream):              # None: the current stream
+            workspace = torch.empty(max(256, need), dtype=torch.uint8, device=like.device)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def _rope_scaled(fn, q, pos, params, k, out, k_out, stream):
+    import torch
+    if pos.dtype != torch.int32 or pos.device != q.device or (pos.dim() > 0 and pos.numel() > 1 and pos.stride(-1) != 1):
+        raise TypeError("pos must be an int32 tensor on the queries' device with contiguous rows")
+    if q.dim() > 4 or q.dim() < 3:
+        raise ValueError("q must be (batch, tokens, heads, head size) or (tokens, heads, head size)")
+    batch, n = (q.shape[0] if q.dim() == 4 else 1), q.shape[-3]
+    if tuple(pos.shape) not in ((n,), (batch, n)):
+        raise ValueError(f"pos must be ({n},) or ({batch}, {n}), is {tuple(pos.shape)}")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    dq, do = _typed(q, q, "q"), _typed(out, q, "out")
+    dk = dko = None
+    if k is not None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        dk, dko = _typed(k, q, "k"), _typed(k_out, q, "k_out")
+    ref = lambda d: None if d is None else ctypes.byref(d)  # noqa: E731
+    _launch(fn, q, stream, ref(dq), ref(dk), _type(q), pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0,
+            ctypes.byref(params), ref(do), ref(dko))
+    return out if k is None else (out, k_out)
+
+
+def rope_scaled(q, pos, params, k=None, out=None, k_out=None, stream=None):
+    """Rotary positions of q (batch, tokens, heads, head size) and, in the same launch, of k (batch, tokens, kv heads,
+    head size): out, or (out, k_out). pos: int32 device (tokens,) or (batch, tokens); params: rope_params(). Rows are
+    contiguous, other strides any (slices of a projection); out may be q and k_out may be k."""
+    return _rope_scaled(lib().stx_rope_scaled, q, pos, params, k, out, k_out, stream)
+
+
+def rope_scaled_back(q, pos, params, k=None, out=None, k_out=None, stream=None):
+    """The gradient of rope_scaled: q and k are the gradients of its outputs."""
+    return _rope_scaled(lib().stx_rope_scaled_back, q, pos, params, k, out, k_out, stream)
+
+
+def _slices(t, like, what):
+    """stx_tensor [C, T1, T2, B] of a (B, T1, T2, C), (B, T, C) or (T, C) tensor."""
+    d = _typed(t, like, what)
+    if t.dim() == 3:                                # ggml order [C, T, B]: B moves to ne3
+        d.ne[2], d.ne[3], d.nb[3], d.nb[2] = 1, d.ne[2], d.nb[2], d.nb[1] * d.ne[1]
+    return d
+
+
+def group_norm_cl_workspace_size(x, n_groups):
+    return lib().stx_group_norm_cl_workspace_size(ctypes.byref(_slices(x, x, "x")), _type(x), int(n_groups))
+
+
+def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, out=None, stats=None, workspace=None,
+                  stream=None):
+    """act(GroupNorm(x) * weight + bias) with the channels last: x (B, T1, T2, C), (B, T, C) or (T, C), contiguous;
+    weight and bias: float32 device (C,) or None. Returns (out, stats): stats is float64 (B, n_groups, 2), mean and
+    1 / sqrt(var + eps), for group_norm_cl_back. out may be x."""
+    import torch
+    out = _out(out, x)
+    dx, do = _slices(x, x, "x"), _slices(out, x, "out")
+    C, B = dx.ne[0], dx.ne[3]
+    if stats is None:
+        stats = torch.empty((B, n_groups, 2), dtype=torch.float64, device=x.device)
+    w, b = _floats(weight, x, C, "weight"), _floats(bias, x, C, "bias")
+    s = _floats(stats, x, B * n_groups * 2, "stats", torch.float64)
+    L, t = lib(), _type(x)
+    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(ctypes.byref(dx), t, int(n_groups)), workspace, x, stream)
+    _launch(L.stx_group_norm_cl, x, stream, ctypes.byref(dx), t, int(n_groups), float(eps), w, b, int(act),
+            ctypes.byref(do), s, ws, nbytes)
+    return out, stats
+
+
+def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_NONE, dx=None, dweight=None, dbias=None,
+                       workspace=None, stream=None):
+    """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy."""
+    import torch
+    dx = _out(dx, x)
+    da, dd, do = _slices(x, x, "x"), _slices(dy, x, "dy"), _slices(dx, x, "dx")
+    C, B = da.ne[0], da.ne[3]
+    dweight = torch.empty(C, dtype=torch.float32, device=x.device) if dweight is None else dweight
+    dbias = torch.empty(C, dtype=torch.float32, device=x.device) if dbias is None else dbias
+    L, t = lib(), _type(x)
+    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(ctypes.byref(da), t, int(n_groups)), workspace, x, stream)
+    _launch(L.stx_group_norm_cl_back, x, stream, ctypes.byref(dd), ctypes.byref(da), t,
+            _floats(stats, x, B * n_groups * 2, "stats", torch.float64), int(n_groups), _floats(weight, x, C, "weight"),
+            _floats(bias, x, C, "bias"), int(act), ctypes.byref(do), _floats(dweight, x, C, "dweight"),
+            _floats(dbias, x, C, "dbias"), ws, nbytes)
+    return dx, dweight, dbias
+
+
+def gated_ff(x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=None, out=None, stream=None):
+    """act(x @ w_gate.T + b_gate) * (x @ w_value.T + b_value): x (..., K) of up to 4 dims, weights (N, K), biases
+    float32 (N,) or None; out (..., N)."""
+    import torch
+    N = w_gate.shape[0]
+    if out is None:
+        out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    dx, dg, dv, do = (_typed(t, x, n) for t, n in ((x, "x"), (w_gate, "w_gate"), (w_value, "w_value"), (out, "out")))
+    _launch(lib().stx_gated_ff, x, stream, ctypes.byref(dx), ctypes.byref(dg), ctypes.byref(dv), _type(x),
+            _floats(b_gate, x, N, "b_gate"), _floats(b_value, x, N, "b_value"), int(act), ctypes.byref(do))
+    return out
+
+
+def gated_ff_back_workspace_size(n_tokens, n_in, n_hidden, dtype):
+    import torch
+    t = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}[dtype]
+    return lib().stx_gated_ff_back_workspace_size(int(n_tokens), int(n_in), int(n_hidden), t)
+
+
+def gated_ff_back(dh, x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=None, dx=None, dw_gate=None,
+                  dw_value=None, db_gate=None, db_value=None, workspace=None, stream=None):
+    """Gradients (dx, dw_gate, dw_value, db_gate, db_value) of gated_ff; the last two are float32, and None where
+    there is no such bias."""
+    import torch
+    N, K = w_gate.shape
+    dev = x.device
+    dx = _out(dx, x)
+    dw_gate, dw_value = _out(dw_gate, w_gate), _out(dw_value, w_value)
+    if db_gate is None and b_gate is not None:
+        db_gate = torch.empty(N, dtype=torch.float32, device=dev)
+    if db_value is None and b_value is not None:
+        db_value = torch.empty(N, dtype=torch.float32, device=dev)
+    d = [_typed(t, x, n) for t, n in ((dh, "dh"), (x, "x"), (w_gate, "w_gate"), (w_value, "w_value"), (dx, "dx"),
+                                      (dw_gate, "dw_gate"), (dw_value, "dw_value"))]
+    r = [ctypes.byref(t) for t in d]
+    L, t = lib(), _type(x)
+    tokens = x.numel() // max(1, K)
+    ws, nbytes, keep = _scratch(L.stx_gated_ff_back_workspace_size(tokens, K, N, t), workspace, x, stream)
+    _launch(L.stx_gated_ff_back, x, stream, r[0], r[1], r[2], r[3], t, _floats(b_gate, x, N, "b_gate"),
+            _floats(b_value, x, N, "b_value"), int(act), r[4], r[5], r[6], _floats(db_gate, x, N, "db_gate"),
+            _floats(db_value, x, N, "db_value"), ws, nbytes)
+    return dx, dw_gate, dw_value, db_gate, db_value
