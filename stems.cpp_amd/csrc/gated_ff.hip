@@ -29,31 +29,44 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 acc, bf16) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
 
-// The products of the block, all of the form out[m][j] = sum_r P[j][r] Q[m][r] with r contiguous:
+// The products of the block, all of the form out[m][j] = sum_r P(j, r) Q(m, r):
 //   FORWARD  P = rows of Wg and Wv, 16 by 16 in turn (a lane then holds gate and value of the same
 //            outputs), Q = x; the epilogue forms act(g) v.
 //   GRAD     the same products again; the epilogue takes dh and writes dg = dh v act'(g) and
 //            dv = dh act(g), and per wave the sums of its columns for the biases' gradients.
-//   DX       P = the transposed weights, Q = dg, then dv: both reductions into one accumulator.
-//   DW       P = x^T, Q = dg^T or dv^T (grid z), a part of the tokens (split), fp32 partial sums.
+//   DX       P = the weights, Q = dg, then dv: both reductions (over the N outputs) into one
+//            accumulator.
+//   DW       P = x, Q = dg or dv, reduced over the tokens.
+// In FORWARD and GRAD r is the fastest dimension of both operands, in DX of Q only and in DW of
+// neither; an operand whose r is not its fastest dimension is "strided" below.
 enum Mode { FORWARD, GRAD, DX, DW };
+
+// Tiles of TJ x TM outputs, WJ x WM waves, SLOTS blocks a CU.
+template <int TJ_, int TM_, int WJ_, int WM_, int SLOTS_>
+struct Tile {
+    static constexpr int TJ = TJ_, TM = TM_, WJ = WJ_, WM = WM_, SLOTS = SLOTS_, NT = 64 * WJ * WM;
+};
+using Large = Tile<256, 256, 2, 4, 1>;
+using Medium = Tile<128, 128, 2, 2, 2>;
+using Small = Tile<128, 64, 2, 2, 3>;
 
 struct FfArgs {
     const char* p[2];
     const char* q[2];
     long long ps[2], qs[2];              // row strides in bytes
-    int J, M;                            // rows of one P, rows of Q
-    long long R;                         // reduction length
-    long long split;                     // DW: reduction length of a part
-    int jtiles, mtiles;
+    int J, M;                            // extents of P's and Q's other dimension
+    long long RP, RQ;                    // reduction lengths: past RP (of a strided P or Q past its own) zeros are taken
+    int steps, chunk;                    // steps of one reduction; steps of a part of it (DX, DW: split)
+    int jtiles, tiles, items;            // column tiles, output tiles, tiles x parts (x 2 in DW)
     const float* b[2];
     int act;
     const char* dh;
     long long dhs;
     char* out[2];
-    long long os;                        // output row stride in bytes
-    int jpad;                            // GRAD: columns written, zeros from J on
-    float* db;                           // GRAD: [wave rows][2][J]
+    long long os[2];                     // output row strides in bytes
+    int jpad;                            // columns written: J, in GRAD padded with zeros
+    int qpad;                            // DW: columns that a row of Q has
+    float* part;                         // GRAD: column sums [wave rows][2][J]; DX, DW: [parts][M][J] or NULL
 };
 
 __device__ const u32x4 zero_chunk = {0, 0, 0, 0};
@@ -73,7 +86,6 @@ __device__ __forceinline__ u32x4 load_chunk(const char* p, long long left) {
     }
     return v;
 }
-
 __device__ __forceinline__ void load_to_lds(const void* src, void* lds) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                      (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
@@ -114,175 +126,369 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// Tiles of TJ x TM outputs, WAVES_J x WAVES_M waves. A stage of LDS holds 128 bytes of every row
-// (8 chunks); chunk c of row r lies at position c ^ (r % 8), so the 16 rows that a fragment reads
-// spread over all banks. Two stages: the next is filled (ALIGNED: straight from memory to LDS;
-// otherwise through registers, any alignment and length) while the waves multiply the other.
-template <class T, int MODE, int TJ, int TM, int WAVES_J, int WAVES_M, bool ALIGNED>
-__global__ __launch_bounds__(64 * WAVES_J* WAVES_M) void ff_kernel(FfArgs a) {
-    constexpr int NT = 64 * WAVES_J * WAVES_M, E = 16 / sizeof(T);
-    constexpr int NJ = TJ / WAVES_J / 16, NM = TM / WAVES_M / 16;   // 16 x 16 tiles of a wave
-    constexpr int PL = TJ * 8 / NT, QL = TM * 8 / NT;                // chunks a thread fetches for a stage
-    constexpr bool GATED = MODE == FORWARD || MODE == GRAD;
-    __shared__ __align__(128) char lds[2][(TJ + TM) * 128];
+constexpr int CH = 8;                    // 16-byte chunks of the reduction in a step: 128 bytes, 64 or 32 elements
 
-    // Tiles in groups of 8 along m, m fastest: the tiles that an XCD works on share rows of both.
-    int id = xcd_block();
-    if (id >= a.jtiles * a.mtiles) return;
-    const int per = 8 * a.jtiles, group = id / per, in = id - group * per;
-    const int gm = min(8, a.mtiles - group * 8);
-    const int m0 = (group * 8 + in % gm) * TM, jt = in / gm;
-    const int j0 = GATED ? jt * (TJ / 2) : jt * TJ;
+// An operand's tile of X rows (or columns) in a stage of LDS. Plain: [X][CH] chunks, chunk c of row x
+// at c ^ (x % 8), so that the 16 rows a fragment reads spread over all banks. Strided: rows of
+// the reduction, [CH E][X / E] chunks, chunk c of row r at c ^ turn(r), so that the rows which
+// one read takes (4 rows of 32 bytes for the transposing 16-bit read, 4 of 64 bytes in
+// fp32) do.
+template <class T, int X>
+__device__ __forceinline__ int turn(int r) {
+    constexpr int E = 16 / sizeof(T), CHUNKS = X / E;
+    return (sizeof(T) == 2 ? 2 * (r % 4 + r / 8 % 2 * 4) : 4 * (r / 4 % 4)) % CHUNKS;
+}
 
-    long long r0 = 0, r1 = a.R;
-    int which = 0;
-    if constexpr (MODE == DW) {
-        which = blockIdx.y;
-        r0 = blockIdx.z * a.split;
-        r1 = min(r0 + a.split, a.R);
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Fragments of N 16-row tiles from `first` on, for lane l: the chunk of row l % 16 at position l / 16
+// of group kk (see mma).
+template <class T, int X, int N, bool STRIDED>
+struct Fragments {
+    int at[STRIDED ? N : 1];
+    __device__ __forceinline__ Fragments(int lane, int first) {
+        constexpr int E = 16 / sizeof(T);
+        const int s = lane % 16, q = lane / 16;
+        if constexpr (!STRIDED) {
+            at[0] = (first * 16 + s) * CH * 16 + (q ^ (s % 8)) * 16;
+        } else if constexpr (sizeof(T) == 2) {                       // lane s reads row s / 4, columns 4 (s % 4) .. + 3
+            const int row = q * 8 + s / 4;
+#pragma unroll
+            for (int i = 0; i < N; i++) at[i] = row * X * 2 + (((first + i) * 2 + s % 4 / 2) ^ turn<T, X>(row)) * 16 + s % 2 * 8;
+        } else {
+            const int row = q * 4;
+#pragma unroll
+            for (int i = 0; i < N; i++) at[i] = row * X * 4 + (((first + i) * 4 + s / 4) ^ turn<T, X>(row)) * 16 + s % 4 * 4;
+        }
+        (void)E;
     }
-    constexpr int SEGMENTS = MODE == DX ? 2 : 1;
+    __device__ __forceinline__ void read(const char* lds, int kk, u32x4 (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if constexpr (!STRIDED) {
+                f[i] = *reinterpret_cast<const u32x4*>(lds + i * 256 * CH + (at[0] ^ (kk * 64)));
+            } else if constexpr (sizeof(T) == 2) {
+                s16x4 h[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at[i] + (kk * 32 + e * 4) * X * 2));
+                __builtin_memcpy(&f[i], h, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[i][e] = *reinterpret_cast<const unsigned*>(lds + at[i] + (kk * 16 + e) * X * 4);
+            }
+        }
+    }
+};
+
+// The chunks of an operand's tile that a thread fetches in a step.
+template <class T, int X, int NT, bool STRIDED>
+struct Source {
+    static constexpr int E = 16 / sizeof(T), N = X * CH / NT, PER = STRIDED ? X / E : CH;   // chunks a thread; chunks a row
+    static __device__ __forceinline__ int row(int i) { return (i * NT + (int)threadIdx.x) / PER; }
+    static __device__ __forceinline__ int chunk(int i) {
+        return (i * NT + (int)threadIdx.x) % PER ^ (STRIDED ? turn<T, X>(row(i)) : row(i) % 8);
+    }
+};
+
+// Persistent blocks: each takes tiles of its XCD's share in turn, and the steps of all its tiles
+// form one stream. Two stages of LDS: while the waves multiply one, the other is filled with
+// the next step, the next tile's first included (ALIGNED: straight from memory to LDS; otherwise
+// through registers, for any alignment and length).
+template <class T, int MODE, class C, bool ALIGNED>
+__global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
+    constexpr int NT = C::NT, E = 16 / sizeof(T), TJ = C::TJ, TM = C::TM;
+    constexpr int NJ = TJ / C::WJ / 16, NM = TM / C::WM / 16;       // 16 x 16 tiles of a wave
+    constexpr bool GATED = MODE == FORWARD || MODE == GRAD, PS = !GATED, QS = MODE == DW;
+    constexpr int WIDTH = GATED ? TJ / 2 : TJ;                       // output columns of a tile
+    constexpr int STAGE = (TJ + TM) * CH * 16;
+    using PSource = Source<T, TJ, NT, PS>;
+    using QSource = Source<T, TM, NT, QS>;
+    __shared__ __align__(128) char lds[2][STAGE];
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    const int wj = wave / WAVES_M, wm = wave % WAVES_M;
-    const char *pp[PL], *qq[QL];
-    const int chunk = (tid % 8) ^ (tid / 8 % 8);                     // rows of a thread differ by multiples of NT / 8
-    auto aim = [&](int seg) {
+    const int wj = wave / C::WM, wm = wave % C::WM;
+
+    // Item `id`: part z of a tile. Tiles in groups of 8 along m, m fastest: the tiles that an XCD
+    // works on at a time share rows of both operands.
+    struct Item {
+        int m0, j0, z, begin, end;       // end: steps [begin, end) of the reduction (DX: of both)
+    };
+    const int mtiles = a.tiles / a.jtiles;
+    auto item_of = [&](int id) {
+        Item t;
+        t.z = id / a.tiles;
+        id -= t.z * a.tiles;
+        const int per = 8 * a.jtiles, group = id / per, in = id - group * per, gm = min(8, mtiles - group * 8);
+        t.m0 = (group * 8 + in % gm) * TM;
+        t.j0 = in / gm * WIDTH;
+        t.begin = 0;
+        t.end = a.steps;
+        if constexpr (!GATED) {
+            t.begin = (MODE == DW ? t.z / 2 : t.z) * a.chunk;
+            t.end = min(t.begin + a.chunk, MODE == DX ? 2 * a.steps : a.steps);
+        }
+        return t;
+    };
+    const int per = (a.items + kXcds - 1) / kXcds, last = min(((int)blockIdx.x % kXcds + 1) * per, a.items);
+    int id = (int)blockIdx.x % kXcds * per + (int)blockIdx.x / kXcds;
+    const int stride = (int)gridDim.x / kXcds;
+    if (id >= last) return;
+
+    // A step's chunks lie at a base (of the tile and step, in scalar registers) plus a lane's own
+    // offset of less than 2^31 (ALIGNED: row strides below 2^23), which changes with the tile only
+    // where rows are clamped. With unaligned operands the offset is 64-bit.
+    using Off = std::conditional_t<ALIGNED, unsigned, long long>;
+    Off poff[PSource::N], qoff[QSource::N];
+    const int pside = GATED ? __builtin_amdgcn_readfirstlane(tid / CH / 16 % 2) : 0;   // a wave's rows are of one matrix
+    auto aim = [&](const Item& t, int seg, int qs) {
 #pragma unroll
-        for (int i = 0; i < PL; i++) {
-            const int row = (i * NT + tid) / 8;
-            const int s = GATED ? row / 16 % 2 : seg;
-            const int j = min(GATED ? j0 + row / 32 * 16 + row % 16 : j0 + row, a.J - 1);
-            pp[i] = a.p[s] + j * a.ps[s] + (r0 + chunk * E) * (long long)sizeof(T);
+        for (int i = 0; i < PSource::N; i++) {
+            const int row = PSource::row(i), at = PSource::chunk(i) * E;
+            if constexpr (PS) poff[i] = (Off)(row * a.ps[seg] + (ALIGNED ? min(at, a.J - E - t.j0) : at) * (long long)sizeof(T));
+            else poff[i] = (Off)(min(row / 32 * 16 + row % 16, a.J - 1 - t.j0) * a.ps[pside] + at * (long long)sizeof(T));
         }
 #pragma unroll
-        for (int i = 0; i < QL; i++) {
-            const int s = MODE == DW ? which : seg;
-            qq[i] = a.q[s] + min(m0 + (i * NT + tid) / 8, a.M - 1) * a.qs[s] + (r0 + chunk * E) * (long long)sizeof(T);
+        for (int i = 0; i < QSource::N; i++) {
+            const int row = QSource::row(i), at = QSource::chunk(i) * E;
+            if constexpr (QS) qoff[i] = (Off)(row * a.qs[qs] + min(at, a.qpad - E - t.m0) * (long long)sizeof(T));
+            else qoff[i] = (Off)(min(row, a.M - 1 - t.m0) * a.qs[qs] + at * (long long)sizeof(T));
         }
     };
-    const int steps = (int)((r1 - r0 + 8 * E - 1) / (8 * E));
-    u32x4 hold[ALIGNED ? 1 : PL + QL];
-    auto fetch = [&](int step, int stage) {
-        const long long at = (long long)step * 128, left = r1 - r0 - (long long)step * 8 * E - chunk * E;
+    u32x4 hold[ALIGNED ? 1 : PSource::N + QSource::N];
+    auto fetch = [&](const Item& t, int step, int stage) {
+        const int seg = MODE == DX && step >= a.steps ? 1 : 0, qs = MODE == DW ? t.z % 2 : seg;
+        if (step == t.begin || (MODE == DX && step == a.steps)) aim(t, seg, qs);
+        const long long r = (long long)(step - seg * a.steps) * CH * E;
+        const char* pb = PS ? a.p[seg] + r * a.ps[seg] + t.j0 * (long long)sizeof(T) : a.p[pside] + t.j0 * a.ps[pside] + r * (long long)sizeof(T);
+        const char* qb = QS ? a.q[qs] + r * a.qs[qs] + t.m0 * (long long)sizeof(T) : a.q[qs] + t.m0 * a.qs[qs] + r * (long long)sizeof(T);
+        char* pl = lds[stage] + wave * 1024;
+        char* ql = lds[stage] + TJ * CH * 16 + wave * 1024;
+        if constexpr (ALIGNED) {
+            if (r + CH * E <= a.RP && r + CH * E <= a.RQ) {
 #pragma unroll
-        for (int i = 0; i < PL + QL; i++) {
-            const char* src = (i < PL ? pp[i < PL ? i : 0] : qq[i < PL ? 0 : i - PL]) + at;
-            if constexpr (ALIGNED) load_to_lds(left > 0 ? (const void*)src : (const void*)&zero_chunk, &lds[stage][(i * NT + wave * 64) * 16]);
-            else hold[i] = load_chunk<T>(src, left);
+                for (int i = 0; i < PSource::N; i++) load_to_lds(pb + poff[i], pl + i * NT * 16);
+#pragma unroll
+                for (int i = 0; i < QSource::N; i++) load_to_lds(qb + qoff[i], ql + i * NT * 16);
+            } else {                                     // the reduction's end: zeros for what is past it
+#pragma unroll
+                for (int i = 0; i < PSource::N; i++)
+                    load_to_lds(r + (PS ? PSource::row(i) : PSource::chunk(i) * E) < a.RP ? (const void*)(pb + poff[i]) : (const void*)&zero_chunk, pl + i * NT * 16);
+#pragma unroll
+                for (int i = 0; i < QSource::N; i++)
+                    load_to_lds(r + (QS ? QSource::row(i) : QSource::chunk(i) * E) < a.RQ ? (const void*)(qb + qoff[i]) : (const void*)&zero_chunk, ql + i * NT * 16);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PSource::N; i++)
+                hold[i] = load_chunk<T>(pb + poff[i], !PS ? a.RP - r - PSource::chunk(i) * E : r + PSource::row(i) < a.RP ? a.J - t.j0 - PSource::chunk(i) * E : 0);
+#pragma unroll
+            for (int i = 0; i < QSource::N; i++)
+                hold[PSource::N + i] = load_chunk<T>(qb + qoff[i], !QS ? a.RQ - r - QSource::chunk(i) * E : r + QSource::row(i) < a.RQ ? E : 0);
         }
     };
     auto settle = [&](int stage) {
-        if constexpr (!ALIGNED) {
-#pragma unroll
-            for (int i = 0; i < PL + QL; i++) *reinterpret_cast<u32x4*>(&lds[stage][(i * NT + tid) * 16]) = hold[i];
-        } else {
+        if constexpr (ALIGNED) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < PSource::N + QSource::N; i++)
+                *reinterpret_cast<u32x4*>(&lds[stage][(i < PSource::N ? i * NT : TJ * CH + (i - PSource::N) * NT) * 16 + tid * 16]) = hold[i];
         }
         __syncthreads();
     };
 
+    const Fragments<T, TJ, NJ, PS> pf(lane, wj * NJ);
+    const Fragments<T, TM, NM, QS> qf(lane, wm * NM);
     f32x4 acc[NJ][NM];
-#pragma unroll
-    for (int j = 0; j < NJ; j++)
-#pragma unroll
-        for (int m = 0; m < NM; m++) acc[j][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    const int frag = (lane % 16) * 128 + ((lane / 16) ^ (lane % 8)) * 16;
-    const int pbase = wj * NJ * 16 * 128, qbase = (TJ + wm * NM * 16) * 128;
-#pragma unroll 1
-    for (int seg = 0; seg < SEGMENTS; seg++) {
-        aim(seg);
-        fetch(0, 0);
-        settle(0);
-#pragma unroll 1
-        for (int s = 0; s < steps; s++) {
-            const int stage = s & 1;
-            if (s + 1 < steps) fetch(s + 1, stage ^ 1);
+    // A wave's outputs leave 16 rows at a time. 16-bit results go through the wave's share of the
+    // stage that was multiplied last, as 16-byte pieces of rows of COLS columns: stored from the
+    // accumulators' own layout they would be runs of 32 bytes (the forward product of 48,060 tokens,
+    // K 384, N 1536 then spends 41 us of 167 on its stores).
+    constexpr int COLS = GATED ? NJ * 8 : NJ * 16, CR = COLS / 8, AREA = 16 * COLS * 2, SHARE = STAGE / (NT / 64), PIECES = 16 * CR / 64;
+    static_assert(AREA * (MODE == GRAD ? 4 : 2) <= SHARE && PIECES >= 1, "staging");
+    auto spot = [&](int row, int col) { return row * COLS * 2 + (col / 8 ^ row % (CR < 8 ? CR : 8)) * 16 + col % 8 * 2; };
+    auto pack = [&](char* p, const float (&f)[4]) {
+        T v[4];
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
+        for (int i = 0; i < 4; i++) v[i] = from_f32<T>(f[i]);
+        __builtin_memcpy(__builtin_assume_aligned(p, 8), v, sizeof v);
+    };
+    auto flush = [&](const char* area, char* out, long long os, int row0, int col0) {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const int row = (i * 64 + lane) / CR, c = (i * 64 + lane) % CR * 8, left = a.jpad - col0 - c;
+            const char* from = area + spot(row, c);
+            char* to = out + (row0 + row) * os + (col0 + c) * (long long)sizeof(T);
+            if (row0 + row >= a.M) continue;
+            if (left >= 8) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(from);
+                __builtin_memcpy(to, &v, 16);
+            } else {
+#pragma unroll 1
+                for (int e = 0; e < left; e++) reinterpret_cast<T*>(to)[e] = reinterpret_cast<const T*>(from)[e];
+            }
+        }
+    };
+    constexpr bool WIDE = sizeof(T) == 2, TAKES = MODE == GRAD && WIDE;
+    u32x4 dhv[TAKES ? PIECES : 1];                       // dh of the next 16 rows
+    auto take = [&](const Item& t, int m) {
+        if constexpr (TAKES) {
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const int row = t.m0 + (wm * NM + m) * 16 + (i * 64 + lane) / CR, col = t.j0 + wj * NJ * 8 + (i * 64 + lane) % CR * 8;
+                dhv[i] = load_chunk<T>(a.dh + row * a.dhs + col * (long long)sizeof(T), row < a.M ? a.J - col : 0);
+            }
+        }
+    };
+
+    auto gated = [&](const Item& t, char* share, auto act) {
+        const int nw = t.j0 + wj * NJ * 8;               // the wave's first column
+        float sg[MODE == GRAD ? NJ / 2 : 1][4] = {}, sv[MODE == GRAD ? NJ / 2 : 1][4] = {};
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + lane % 16;
+            char* area = share + (MODE == GRAD ? m % 2 * 2 : m % 2) * AREA;
+            if constexpr (TAKES) {
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) *reinterpret_cast<u32x4*>(area + spot((i * 64 + lane) / CR, (i * 64 + lane) % CR * 8)) = dhv[i];
+                if (m + 1 < NM) take(t, m + 1);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2) {
+                const int col = j * 8 + lane / 16 * 4, n = nw + col;
+                char* here = area + spot(lane % 16, col);
+                if constexpr (MODE == FORWARD) {
+                    float h[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) h[r] = act_f32<act()>(acc[j][m][r]) * acc[j + 1][m][r];
+                    if constexpr (WIDE) pack(here, h);
+                    else if (row < a.M) store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.J - n, h);
+                } else {
+                    float dh[4], dg[4], dv[4];
+                    if constexpr (WIDE) load4<T>(static_cast<const char*>(__builtin_assume_aligned(here, 8)), 4, dh);
+                    else load4<T>(a.dh + row * a.dhs + n * (long long)sizeof(T), row < a.M ? a.J - n : 0, dh);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float d;
+                        const float g = act_f32<act()>(acc[j][m][r], d);
+                        const bool in = row < a.M && n + r < a.J;    // what lies past the edges may be anything, NaN too
+                        dg[r] = in ? dh[r] * acc[j + 1][m][r] * d : 0.f;
+                        dv[r] = in ? dh[r] * g : 0.f;
+                        sg[j / 2][r] += dg[r];
+                        sv[j / 2][r] += dv[r];
+                    }
+                    if constexpr (WIDE) {
+                        pack(here, dg);
+                        pack(here + AREA, dv);
+                    } else if (row < a.M && a.out[0]) {
+                        store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.jpad - n, dg);
+                        store4<T>(a.out[1] + row * a.os[1] + n * (long long)sizeof(T), a.jpad - n, dv);
+                    }
+                }
+            }
+            if constexpr (WIDE) {
+                if (MODE == FORWARD || a.out[0]) {
+                    flush(area, a.out[0], a.os[0], row0, nw);
+                    if constexpr (MODE == GRAD) flush(area + AREA, a.out[1], a.os[1], row0, nw);
+                }
+            }
+        }
+        if constexpr (MODE == GRAD) {
+            if (!a.part) return;
+            float* part = a.part + ((long long)(t.m0 / TM) * C::WM + wm) * 2 * a.J;
+#pragma unroll
+            for (int j = 0; j < NJ / 2; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int n = nw + j * 16 + lane / 16 * 4 + r;
+                    const float g = row_sum(sg[j][r]), v = row_sum(sv[j][r]);
+                    if (lane % 16 == 0 && n < a.J) {
+                        part[n] = g;
+                        part[a.J + n] = v;
+                    }
+                }
+        }
+    };
+    auto plain = [&](const Item& t, char* share) {
+        const int jw = t.j0 + wj * NJ * 16, which = MODE == DW ? t.z % 2 : 0;
+        float* part = a.part ? a.part + (long long)t.z * a.M * a.J : nullptr;
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + lane % 16;
+            char* area = share + m % 2 * AREA;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const float f[4] = {acc[j][m][0], acc[j][m][1], acc[j][m][2], acc[j][m][3]};
+                const int c = j * 16 + lane / 16 * 4, col = jw + c;
+                if (part) {
+                    if (row < a.M) store4<float>(reinterpret_cast<char*>(part + (long long)row * a.J + col), a.J - col, f);
+                } else if constexpr (WIDE) {
+                    pack(area + spot(lane % 16, c), f);
+                } else if (row < a.M) {
+                    store4<T>(a.out[which] + row * a.os[which] + col * (long long)sizeof(T), a.J - col, f);
+                }
+            }
+            if constexpr (WIDE)
+                if (!part) flush(area, a.out[which], a.os[which], row0, jw);
+        }
+    };
+    // A tile starts from its biases, or from zeros.
+    auto start = [&](const Item& t) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            float b[4] = {};
+            if constexpr (GATED) {
+                const int n = t.j0 + (wj * NJ + j) / 2 * 16 + lane / 16 * 4;
+                if (a.b[j % 2]) load4<float>(reinterpret_cast<const char*>(a.b[j % 2] + n), a.J - n, b);
+            }
+#pragma unroll
+            for (int m = 0; m < NM; m++) acc[j][m] = f32x4{b[0], b[1], b[2], b[3]};
+        }
+    };
+
+    Item t = item_of(id);
+    fetch(t, t.begin, 0);
+    settle(0);
+    int stage = 0;
+    while (true) {
+        start(t);
+        const int next = id + stride;
+        Item n = t;
+#pragma unroll 1
+        for (int s = t.begin; s < t.end; s++) {
+            if (s + 1 < t.end) {
+                fetch(t, s + 1, stage ^ 1);
+            } else if (next < last) {
+                n = item_of(next);
+                fetch(n, n.begin, stage ^ 1);
+            }
+#pragma unroll
+            for (int kk = 0; kk < CH / 4; kk++) {
                 u32x4 fp[NJ], fq[NM];
-#pragma unroll
-                for (int j = 0; j < NJ; j++) fp[j] = *reinterpret_cast<const u32x4*>(&lds[stage][pbase + j * 2048 + (frag ^ (kk * 64))]);
-#pragma unroll
-                for (int m = 0; m < NM; m++) fq[m] = *reinterpret_cast<const u32x4*>(&lds[stage][qbase + m * 2048 + (frag ^ (kk * 64))]);
+                pf.read(lds[stage], kk, fp);
+                qf.read(lds[stage] + TJ * CH * 16, kk, fq);
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
 #pragma unroll
                     for (int m = 0; m < NM; m++) acc[j][m] = mma(fp[j], fq[m], acc[j][m], T{});
             }
-            if (s + 1 < steps) settle(stage ^ 1);
-        }
-        if (seg + 1 < SEGMENTS) __syncthreads();
-    }
-
-    const int mrow = m0 + wm * NM * 16 + lane % 16;
-    if constexpr (GATED) with_act(a.act, [&](auto act) {
-#pragma unroll
-        for (int j = 0; j < NJ; j += 2) {
-            const int n = j0 + (wj * NJ + j) * 8 + lane / 16 * 4, left = a.J - n;
-            float bg[4], bv[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                bg[r] = a.b[0] && r < left ? a.b[0][n + r] : 0.f;
-                bv[r] = a.b[1] && r < left ? a.b[1][n + r] : 0.f;
-            }
-            float sg[4] = {}, sv[4] = {};
-#pragma unroll
-            for (int m = 0; m < NM; m++) {
-                const int row = mrow + m * 16;
-                if constexpr (MODE == FORWARD) {
-                    float h[4];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) h[r] = act_f32<act()>(acc[j][m][r] + bg[r]) * (acc[j + 1][m][r] + bv[r]);
-                    if (row < a.M) store4<T>(a.out[0] + row * a.os + n * (long long)sizeof(T), left, h);
-                } else {
-                    float dh[4], dg[4], dv[4];
-                    load4<T>(a.dh + row * a.dhs + n * (long long)sizeof(T), row < a.M ? left : 0, dh);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        float d;
-                        const float g = act_f32<act()>(acc[j][m][r] + bg[r], d), v = acc[j + 1][m][r] + bv[r];
-                        const bool in = row < a.M && r < left;
-                        dg[r] = in ? dh[r] * v * d : 0.f;
-                        dv[r] = in ? dh[r] * g : 0.f;
-                        sg[r] += dg[r];
-                        sv[r] += dv[r];
-                    }
-                    if (row < a.M && a.out[0]) {
-                        store4<T>(a.out[0] + row * a.os + n * (long long)sizeof(T), a.jpad - n, dg);
-                        store4<T>(a.out[1] + row * a.os + n * (long long)sizeof(T), a.jpad - n, dv);
-                    }
-                }
-            }
-            if constexpr (MODE == GRAD) {
-                if (a.db) {
-                    float* part = a.db + ((long long)(m0 / TM) * WAVES_M + wm) * 2 * a.J;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float g = row_sum(sg[r]), v = row_sum(sv[r]);
-                        if (lane % 16 == 0 && r < left) {
-                            part[n + r] = g;
-                            part[a.J + n + r] = v;
-                        }
-                    }
-                }
+            if (s + 1 < t.end) {
+                settle(stage ^ 1);
+                stage ^= 1;
             }
         }
-    });
-    else {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            const int c = j0 + (wj * NJ + j) * 16 + lane / 16 * 4;
-#pragma unroll
-            for (int m = 0; m < NM; m++) {
-                const int row = mrow + m * 16;
-                const float f[4] = {acc[j][m][0], acc[j][m][1], acc[j][m][2], acc[j][m][3]};
-                if (row >= a.M) continue;
-                if constexpr (MODE == DX) store4<T>(a.out[0] + row * a.os + c * (long long)sizeof(T), a.J - c, f);
-                else store4<float>(a.out[0] + (((long long)blockIdx.z * 2 + which) * a.M + row) * a.os + c * 4LL, a.J - c, f);
-            }
-        }
+        take(t, 0);
+        __syncthreads();                                 // the last stage is read; its shares are free
+        char* share = lds[stage] + wave * SHARE;
+        if constexpr (GATED) with_act(a.act, [&](auto act) { gated(t, share, act); });
+        else plain(t, share);
+        if (next >= last) return;
+        settle(stage ^ 1);
+        stage ^= 1;
+        id = next;
+        t = n;
     }
 }
 
@@ -300,9 +506,9 @@ __global__ __launch_bounds__(512) void ff_few_kernel(FfArgs a) {
 #pragma unroll
     for (int m = 0; m < NM; m++) q[m] = a.q[0] + min(m * 16 + lane % 16, a.M - 1) * a.qs[0];
     f32x4 acc[2][NM] = {};
-    const int steps = (int)((a.R + 4 * E - 1) / (4 * E));
+    const int steps = (int)((a.RP + 4 * E - 1) / (4 * E));
     auto take = [&](int s, auto whole) {
-        const long long r = (long long)s * 4 * E + lane / 16 * E, at = r * (long long)sizeof(T), left = whole() ? E : a.R - r;
+        const long long r = (long long)s * 4 * E + lane / 16 * E, at = r * (long long)sizeof(T), left = whole() ? E : a.RP - r;
         const u32x4 g = load_chunk<T>(p[0] + at, left), v = load_chunk<T>(p[1] + at, left);
 #pragma unroll
         for (int m = 0; m < NM; m++) {
@@ -311,7 +517,7 @@ __global__ __launch_bounds__(512) void ff_few_kernel(FfArgs a) {
             acc[1][m] = mma(v, x, acc[1][m], T{});
         }
     };
-    const int full = (int)(a.R / (4 * E));
+    const int full = (int)(a.RP / (4 * E));
     int s = wave;
     for (; s + 3 * WAVES < full; s += 4 * WAVES) {
 #pragma unroll
@@ -340,43 +546,42 @@ __global__ __launch_bounds__(512) void ff_few_kernel(FfArgs a) {
         h[r] = act_f32<act()>(g[r] + (a.b[0] && in ? a.b[0][n + r] : 0.f)) * (v[r] + (a.b[1] && in ? a.b[1][n + r] : 0.f));
     }
     });
-    store4<T>(a.out[0] + row * a.os + n * (long long)sizeof(T), a.J - n, h);
+    store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.J - n, h);
 }
 
-// src [rows][cols] -> dst [cols][ld], zeros from `rows` to the next multiple of 64.
-template <class T>
-__global__ __launch_bounds__(256) void ff_transpose_kernel(const char* src, long long ss, int rows, int cols, T* dst, long long ld) {
-    __shared__ T tile[64][66];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, x = threadIdx.x % 64, y = threadIdx.x / 64;
-    for (int i = y; i < 64; i += 4)
-        tile[i][x] = r0 + i < rows && c0 + x < cols ? reinterpret_cast<const T*>(src + (r0 + i) * ss)[c0 + x] : T(0.f);
-    __syncthreads();
-    for (int i = y; i < 64; i += 4)
-        if (c0 + i < cols) dst[(long long)(c0 + i) * ld + r0 + x] = tile[x][i];
+// Sums of the parts of a split reduction, in order: part [splits][W][rows][cols] to out[w][rows][cols].
+template <class T, int V>
+__global__ __launch_bounds__(256) void ff_fold_kernel(const float* part, int splits, long long rows, int cols, int w, char* o0, char* o1, long long s0, long long s1) {
+    const long long n = rows * cols, i = (blockIdx.x * 256LL + threadIdx.x) * V;
+    if (i >= w * n) return;
+    float s[V] = {};
+#pragma unroll 4
+    for (int k = 0; k < splits; k++) {
+        float f[V];
+        __builtin_memcpy(f, part + k * w * n + i, sizeof f);
+#pragma unroll
+        for (int e = 0; e < V; e++) s[e] += f[e];
+    }
+    const long long e = i < n ? i : i - n, row = e / cols, col = e - row * cols;
+    T v[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) v[k] = from_f32<T>(s[k]);
+    __builtin_memcpy((i < n ? o0 + row * s0 : o1 + row * s1) + col * (long long)sizeof(T), v, sizeof v);
 }
 
-// Weight gradients: the parts of the tokens added in order.
-template <class T>
-__global__ __launch_bounds__(256) void ff_dw_fold_kernel(const float* part, int splits, int N, int K, char* dg, char* dv, long long sg, long long sv) {
-    const long long i = blockIdx.x * 256LL + threadIdx.x, n = (long long)N * K;
-    if (i >= 2 * n) return;
-    float s = 0.f;
-    for (int k = 0; k < splits; k++) s += part[k * 2 * n + i];
-    const long long e = i < n ? i : i - n, row = e / K, col = e - row * K;
-    reinterpret_cast<T*>(i < n ? dg + row * sg : dv + row * sv)[col] = from_f32<T>(s);
-}
-
-// Bias gradients: the waves' column sums, 32 columns x 8 lanes a block.
-__global__ __launch_bounds__(256) void ff_db_fold_kernel(const float* part, long long rows, int N, float* dg, float* dv) {
-    __shared__ double red[8][33];
+// Bias gradients: the waves' column sums, 32 columns x 32 lanes a block.
+__global__ __launch_bounds__(1024) void ff_db_fold_kernel(const float* part, long long rows, int N, float* dg, float* dv) {
+    __shared__ double red[32][33];
     const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
     double s = 0.0;
-    if (c < 2 * N)
-        for (long long r = lane; r < rows; r += 8) s += (double)part[r * 2 * N + c];
+    if (c < 2 * N) {
+#pragma unroll 8
+        for (long long r = lane; r < rows; r += 32) s += (double)part[r * 2 * N + c];
+    }
     red[lane][threadIdx.x % 32] = s;
     __syncthreads();
     if (lane || c >= 2 * N) return;
-    for (int i = 1; i < 8; i++) s += red[i][threadIdx.x];
+    for (int i = 1; i < 32; i++) s += red[i][threadIdx.x];
     float* d = c < N ? dg : dv;
     if (d) d[c < N ? c : c - N] = (float)s;
 }
@@ -406,27 +611,66 @@ Rows rows_of(const stx_tensor* t, int size, const char* what) {
     return r;
 }
 
-bool aligned_rows(const void* p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0; }
+bool aligned_rows(const void* p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride < (1 << 23); }
 
-template <class T, int MODE, int TJ, int TM, int WJ, int WM, bool AL>
-void launch_tiles(FfArgs a, dim3 yz, hipStream_t stream) {
-    const int width = MODE == FORWARD || MODE == GRAD ? TJ / 2 : TJ;
+constexpr int kFew = 64;
+constexpr long long kMaxWidth = 1 << 20, kMaxTokens = 1 << 30;   // of K and N; of the tokens (row indexes of tiles fit 32 bits)
+constexpr int kCus = 256;                                         // of an MI355X: plans are made without a device at hand
+
+// How a product is run: its tile and the number of parts of its reduction, by the least estimated time.
+// A step of a tile takes cycles in proportion to its area, the larger tiles' by a better rate (the
+// measured ones of a long reduction); a part ends in an epilogue and a fold.
+struct Plan {
+    int tile, splits, steps;             // 0 Large, 1 Medium, 2 Small; steps of a part
+};
+Plan plan_of(long long J, long long M, long long steps, int width_of_two, int w, int size, bool split) {
+    struct Kind {
+        int tj, tm, slots;
+        double rate[2];                  // relative, 16-bit and fp32
+    };
+    static constexpr Kind kinds[] = {{256, 256, 1, {1.0, 1.0}}, {128, 128, 2, {0.86, 0.96}}, {128, 64, 3, {0.62, 0.85}}};
+    Plan best{};
+    double least = 0;
+    steps = std::max(1LL, steps);                                 // no tokens: nothing is launched
+    for (int k = 0; k < 3; k++) {
+        const long long jt = (J * width_of_two + kinds[k].tj - 1) / kinds[k].tj, tiles = jt * ((M + kinds[k].tm - 1) / kinds[k].tm) * w;
+        const double step = kinds[k].tj * (double)kinds[k].tm / 65536 / kinds[k].rate[size == 4] * (size == 4 ? 7.1 : 0.95);   // us on a whole CU
+        for (int s = 1; s <= (split ? 32 : 1) && (s == 1 || steps / s >= 4); s++) {
+            const long long part = (steps + s - 1) / s, slots = (long long)kCus * kinds[k].slots, items = tiles * ((steps + part - 1) / part);
+            // Full rounds share a CU; in the last, fewer blocks a CU run faster, but not as fast as their number.
+            const long long rounds = items / slots, rest = items - rounds * slots;
+            const double busy = rounds * kinds[k].slots + (rest ? (double)((rest + kCus - 1) / kCus) : 0.0);
+            double us = busy * (part * step + 4.0 * kinds[k].tj * kinds[k].tm / 65536) + 2.0;
+            if (s > 1) us += 4.0 + 8.0 * s * J * M * w / 4e6;
+            if (least == 0 || us < least) {
+                least = us;
+                best = {k, (int)((steps + part - 1) / part), (int)part};
+            }
+        }
+    }
+    return best;
+}
+
+template <class T, int MODE, class C, bool AL>
+void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
+    const int width = MODE == FORWARD || MODE == GRAD ? C::TJ / 2 : C::TJ;
     a.jtiles = (a.J + width - 1) / width;
-    a.mtiles = (int)(((long long)a.M + TM - 1) / TM);
-    const long long tiles = (long long)a.jtiles * a.mtiles;
-    if (tiles >= (1LL << 30)) fail(STX_STATUS_UNSUPPORTED, "gated_ff: too many tiles");
-    hipLaunchKernelGGL((ff_kernel<T, MODE, TJ, TM, WJ, WM, AL>), dim3(xcd_grid(tiles), yz.y, yz.z), dim3(64 * WJ * WM), 0, stream, a);
+    const long long tiles = (long long)a.jtiles * (((long long)a.M + C::TM - 1) / C::TM);
+    if (tiles * parts >= (1LL << 30)) fail(STX_STATUS_UNSUPPORTED, "gated_ff: too many tiles");
+    a.tiles = (int)tiles;
+    a.items = (int)(tiles * parts);
+    const long long blocks = std::min<long long>(a.items, (long long)device_cus() * C::SLOTS);
+    hipLaunchKernelGGL((ff_kernel<T, MODE, C, AL>), dim3(xcd_grid(blocks)), dim3(C::NT), 0, stream, a);
     launch_check("ff_kernel");
 }
 
-constexpr int kSmall = 128;              // tile edge; its waves' rows of bias sums are 64 tokens
-constexpr int kFew = 64;
-constexpr long long kMaxWidth = 1 << 20, kMaxTokens = 1 << 30;   // of K and N; of the tokens (row indexes of tiles fit 32 bits)
-
+// Unaligned operands go through registers, which the large tile has none to spare of.
 template <class T, int MODE>
-void launch_ff(const FfArgs& a, bool aligned, dim3 yz, hipStream_t stream) {
-    if (aligned) launch_tiles<T, MODE, kSmall, kSmall, 2, 2, true>(a, yz, stream);
-    else launch_tiles<T, MODE, kSmall, kSmall, 2, 2, false>(a, yz, stream);
+void launch_ff(const FfArgs& a, bool aligned, int tile, int parts, hipStream_t stream) {
+    if (!aligned) tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
+    else if (tile == 0) launch_tiles<T, MODE, Large, true>(a, parts, stream);
+    else if (tile == 1) launch_tiles<T, MODE, Medium, true>(a, parts, stream);
+    else launch_tiles<T, MODE, Small, true>(a, parts, stream);
 }
 
 struct Block {
@@ -459,7 +703,9 @@ void check_output(const stx_tensor* t, const Rows& r, int size, const char* what
     STX_REQUIRE(r.n <= 1 || r.stride >= t->ne[0] * size, "gated_ff: rows of %s overlap", what);
 }
 
-FfArgs products(const Block& b, const float* bg, const float* bv, stx_act act) {
+int steps_of(long long r, int size) { return (int)((r * size + CH * 16 - 1) / (CH * 16)); }
+
+FfArgs products(const Block& b, const float* bg, const float* bv, stx_act act, int size) {
     FfArgs k{};
     k.p[0] = b.wg.data;
     k.p[1] = b.wv.data;
@@ -469,7 +715,9 @@ FfArgs products(const Block& b, const float* bg, const float* bv, stx_act act) {
     k.qs[0] = b.x.stride;
     k.J = b.N;
     k.M = (int)b.M;
-    k.R = b.K;
+    k.RP = k.RQ = b.K;
+    k.steps = steps_of(b.K, size);
+    k.jpad = b.N;
     k.b[0] = bg;
     k.b[1] = bv;
     k.act = act;
@@ -479,23 +727,20 @@ bool products_aligned(const Block& b, int size) {
     return b.K % (16 / size) == 0 && aligned_rows(b.x.data, b.x.stride) && aligned_rows(b.wg.data, b.wg.stride) && aligned_rows(b.wv.data, b.wv.stride);
 }
 
-// Workspace of the backward pass. The split of the token reduction of the weights' gradients is
-// chosen so that its tiles come to about two a CU of the MI355X's 256.
+// Workspace of the backward pass: dg and dv with rows of a multiple of 64 elements, the parts of
+// split reductions, the biases' column sums (for the smallest tile's waves).
 struct BackPlan {
-    long long Mp, Np;
-    int splits;
-    long long split, db_rows;
-    size_t dg, dgt, xt, wt, dw, db, total;
+    long long Np;
+    Plan grad, dx, dw;
+    size_t dg, part, db, total;
 };
+constexpr int kWaveRows[] = {Large::TM / Large::WM, Medium::TM / Medium::WM, Small::TM / Small::WM};
 BackPlan back_plan(long long M, long long K, long long N, int size) {
     BackPlan p{};
-    p.Mp = pad64(M);
     p.Np = pad64(N);
-    const long long tiles = 2 * ((K + kSmall - 1) / kSmall) * ((N + kSmall - 1) / kSmall);
-    const long long most = std::max(1LL, std::min(p.Mp / 512, 512 / tiles));
-    p.split = pad64((p.Mp + most - 1) / most);
-    p.splits = p.split ? (int)std::max(1LL, (p.Mp + p.split - 1) / p.split) : 1;
-    p.db_rows = (M + kSmall - 1) / kSmall * 2;
+    p.grad = plan_of(N, M, steps_of(K, size), 2, 1, size, false);
+    p.dx = plan_of(K, M, 2LL * steps_of(N, size), 1, 1, size, true);
+    p.dw = plan_of(K, N, steps_of(M, size), 1, 2, size, true);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -503,89 +748,98 @@ BackPlan back_plan(long long M, long long K, long long N, int size) {
         return here;
     };
     p.dg = take(2 * (size_t)(M * p.Np) * size);
-    p.dgt = take(2 * (size_t)(N * p.Mp) * size);
-    p.xt = take((size_t)(K * p.Mp) * size);
-    p.wt = take(2 * (size_t)(K * p.Np) * size);
-    p.dw = take((size_t)p.splits * 2 * N * K * sizeof(float));
-    p.db = take((size_t)p.db_rows * 2 * N * sizeof(float));
+    // One after another, in the same place: the products run in one stream.
+    const size_t dx = p.dx.splits > 1 ? (size_t)p.dx.splits * M * K : 0, dw = p.dw.splits > 1 ? (size_t)p.dw.splits * 2 * N * K : 0;
+    p.part = take(std::max(dx, dw) * sizeof(float));
+    p.db = take((size_t)((M + 63) / 64 * 2 + 2) * 2 * N * sizeof(float));   // rows of waves: M / 64 or M / 32, up to a whole tile
     p.total = at;
     return p;
 }
 
 template <class T>
-void transpose(const char* src, long long stride, long long rows, int cols, T* dst, long long ld, hipStream_t stream) {
-    hipLaunchKernelGGL(ff_transpose_kernel<T>, dim3((unsigned)(pad64(rows) / 64), (cols + 63) / 64), dim3(256), 0, stream, src, stride, (int)rows, cols, dst, ld);
-    launch_check("ff_transpose_kernel");
+void fold(const float* part, int splits, long long rows, int cols, int w, char* o0, char* o1, long long s0, long long s1, hipStream_t stream) {
+    const long long n = rows * cols * w;
+    auto launch = [&](auto v) {
+        constexpr int V = v();
+        hipLaunchKernelGGL((ff_fold_kernel<T, V>), dim3((unsigned)((n / V + 255) / 256)), dim3(256), 0, stream, part, splits, rows, cols, w, o0, o1, s0, s1);
+    };
+    STX_REQUIRE(n / 256 < (1LL << 31), "gated_ff_back: gradients too large");
+    if (cols % 4 == 0) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 1>{});
+    launch_check("ff_fold_kernel");
 }
 
 template <class T>
 void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, stx_act act, const Rows* dx, const Rows* dwg, const Rows* dwv,
               float* dbg, float* dbv, char* ws, hipStream_t stream) {
-    const BackPlan p = back_plan(b.M, b.K, b.N, sizeof(T));
-    T* dg = reinterpret_cast<T*>(ws + p.dg);
-    T* dv = dg + b.M * p.Np;
-    T* dgt = reinterpret_cast<T*>(ws + p.dgt);
-    T* dvt = dgt + b.N * p.Mp;
-    T* xt = reinterpret_cast<T*>(ws + p.xt);
-    T* wgt = reinterpret_cast<T*>(ws + p.wt);
-    T* wvt = wgt + b.K * p.Np;
-    float* dw = reinterpret_cast<float*>(ws + p.dw);
+    constexpr int size = sizeof(T);
+    const BackPlan p = back_plan(b.M, b.K, b.N, size);
+    char* dg = ws + p.dg;
+    char* dv = dg + b.M * p.Np * size;
+    float* part = reinterpret_cast<float*>(ws + p.part);
     float* db = reinterpret_cast<float*>(ws + p.db);
+    const bool aligned = products_aligned(b, size);
     if (b.M > 0) {
-        FfArgs k = products(b, bg, bv, act);
+        FfArgs k = products(b, bg, bv, act, size);
         k.dh = dh.data;
         k.dhs = dh.stride;
-        k.out[0] = dx || dwg ? reinterpret_cast<char*>(dg) : nullptr;
-        k.out[1] = reinterpret_cast<char*>(dv);
-        k.os = p.Np * (long long)sizeof(T);
+        k.out[0] = dx || dwg ? dg : nullptr;
+        k.out[1] = dv;
+        k.os[0] = k.os[1] = p.Np * size;
         k.jpad = (int)p.Np;
-        k.db = dbg || dbv ? db : nullptr;
-        launch_ff<T, GRAD>(k, products_aligned(b, sizeof(T)), dim3(1), stream);
+        k.part = dbg || dbv ? db : nullptr;
+        launch_ff<T, GRAD>(k, aligned, p.grad.tile, 1, stream);
     }
     if (dbg || dbv) {
-        hipLaunchKernelGGL(ff_db_fold_kernel, dim3((2 * b.N + 31) / 32), dim3(256), 0, stream, db, b.M > 0 ? p.db_rows : 0, b.N, dbg, dbv);
+        const int tile = aligned || p.grad.tile == 2 ? p.grad.tile : 1;
+        const long long tm = tile == 0 ? Large::TM : tile == 1 ? Medium::TM : Small::TM;
+        const long long rows = (b.M + tm - 1) / tm * (tm / kWaveRows[tile]);
+        hipLaunchKernelGGL(ff_db_fold_kernel, dim3((2 * b.N + 31) / 32), dim3(1024), 0, stream, db, rows, b.N, dbg, dbv);
         launch_check("ff_db_fold_kernel");
     }
     if (dx && b.M > 0) {
-        transpose<T>(b.wg.data, b.wg.stride, b.N, b.K, wgt, p.Np, stream);
-        transpose<T>(b.wv.data, b.wv.stride, b.N, b.K, wvt, p.Np, stream);
         FfArgs k{};
-        k.p[0] = reinterpret_cast<char*>(wgt);
-        k.p[1] = reinterpret_cast<char*>(wvt);
-        k.q[0] = reinterpret_cast<char*>(dg);
-        k.q[1] = reinterpret_cast<char*>(dv);
-        k.ps[0] = k.ps[1] = k.qs[0] = k.qs[1] = p.Np * (long long)sizeof(T);
-        k.J = b.K;
+        k.p[0] = b.wg.data;
+        k.p[1] = b.wv.data;
+        k.ps[0] = b.wg.stride;
+        k.ps[1] = b.wv.stride;
+        k.q[0] = dg;
+        k.q[1] = dv;
+        k.qs[0] = k.qs[1] = p.Np * size;
+        k.J = k.jpad = b.K;
         k.M = (int)b.M;
-        k.R = p.Np;
+        k.RP = b.N;
+        k.RQ = p.Np;
+        k.steps = steps_of(b.N, size);
+        k.chunk = p.dx.steps;
         k.out[0] = dx->data;
-        k.os = dx->stride;
-        launch_ff<T, DX>(k, true, dim3(1), stream);
+        k.os[0] = dx->stride;
+        k.part = p.dx.splits > 1 ? part : nullptr;
+        launch_ff<T, DX>(k, aligned, p.dx.tile, p.dx.splits, stream);
+        if (k.part) fold<T>(part, p.dx.splits, b.M, b.K, 1, dx->data, dx->data, dx->stride, dx->stride, stream);
     }
-    if (dwg) {
-        int splits = 0;
-        if (b.M > 0) {
-            splits = p.splits;
-            transpose<T>(b.x.data, b.x.stride, b.M, b.K, xt, p.Mp, stream);
-            transpose<T>(reinterpret_cast<char*>(dg), p.Np * (long long)sizeof(T), b.M, b.N, dgt, p.Mp, stream);
-            transpose<T>(reinterpret_cast<char*>(dv), p.Np * (long long)sizeof(T), b.M, b.N, dvt, p.Mp, stream);
-            FfArgs k{};
-            k.p[0] = reinterpret_cast<char*>(xt);
-            k.q[0] = reinterpret_cast<char*>(dgt);
-            k.q[1] = reinterpret_cast<char*>(dvt);
-            k.ps[0] = k.qs[0] = k.qs[1] = p.Mp * (long long)sizeof(T);
-            k.J = b.K;
-            k.M = b.N;
-            k.R = p.Mp;
-            k.split = p.split;
-            k.out[0] = reinterpret_cast<char*>(dw);
-            k.os = b.K * 4LL;
-            launch_ff<T, DW>(k, true, dim3(1, 2, splits), stream);
-        }
-        const long long n = 2LL * b.N * b.K;
-        hipLaunchKernelGGL(ff_dw_fold_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, dw, splits, b.N, b.K, dwg->data, dwv->data, dwg->stride, dwv->stride);
-        launch_check("ff_dw_fold_kernel");
+    if (dwg && b.M > 0) {
+        FfArgs k{};
+        k.p[0] = b.x.data;
+        k.ps[0] = b.x.stride;
+        k.q[0] = dg;
+        k.q[1] = dv;
+        k.qs[0] = k.qs[1] = p.Np * size;
+        k.J = k.jpad = b.K;
+        k.M = b.N;
+        k.qpad = (int)p.Np;
+        k.RP = k.RQ = b.M;
+        k.steps = steps_of(b.M, size);
+        k.chunk = p.dw.steps;
+        k.out[0] = dwg->data;
+        k.out[1] = dwv->data;
+        k.os[0] = dwg->stride;
+        k.os[1] = dwv->stride;
+        k.part = p.dw.splits > 1 ? part : nullptr;
+        launch_ff<T, DW>(k, aligned, p.dw.tile, 2 * p.dw.splits, stream);
     }
+    if (dwg && (p.dw.splits > 1 || b.M == 0))                        // without tokens: sums of no parts
+        fold<T>(part, b.M > 0 ? p.dw.splits : 0, b.N, b.K, 2, dwg->data, dwv->data, dwg->stride, dwv->stride, stream);
 }
 
 }  // namespace
@@ -608,12 +862,13 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
         for (const stx_tensor* t : {x, w_gate, w_value})
             STX_REQUIRE(!overlap(span_of(t, size), span_of(dst, size)), "gated_ff: dst overlaps an input");
         if (b.M == 0) return;
-        FfArgs k = products(b, b_gate, b_value, act);
+        FfArgs k = products(b, b_gate, b_value, act, size);
         k.out[0] = d.data;
-        k.os = d.stride;
+        k.os[0] = d.stride;
         with_type(type, [&](auto t) {
             using T = decltype(t);
-            if (b.M > kFew) return launch_ff<T, FORWARD>(k, products_aligned(b, size), dim3(1), as_stream(stream));
+            if (b.M > kFew)
+                return launch_ff<T, FORWARD>(k, products_aligned(b, size), plan_of(b.N, b.M, k.steps, 2, 1, size, false).tile, 1, as_stream(stream));
             const dim3 grid((b.N + 15) / 16), block(512);
             if (b.M <= 16) hipLaunchKernelGGL((ff_few_kernel<T, 1>), grid, block, 0, as_stream(stream), k);
             else if (b.M <= 32) hipLaunchKernelGGL((ff_few_kernel<T, 2>), grid, block, 0, as_stream(stream), k);

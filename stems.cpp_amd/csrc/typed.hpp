@@ -108,13 +108,17 @@ __device__ __forceinline__ T from_f32(float x) {
     return (T)x;
 }
 
-// 1 / (1 + exp(-z)) with the hardware reciprocal (1 ulp).
-__device__ __forceinline__ float sigmoid_f32(float z) { return __builtin_amdgcn_rcpf(1.f + expf(-z)); }
+// 1 / (1 + exp(-z)) on the hardware's 2^y and reciprocal (1 ulp each): the rounding of y = -z log2 e
+// costs |z| ulps of exp(-z), which the result meets only where exp(-z) dominates it, z < 0. Four
+// instructions; with a library exp the epilogue of the gated block took longer than its products.
+__device__ __forceinline__ float sigmoid_f32(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+}
 
 // Phi(z), the normal distribution, and phi = exp(-z^2/2): Phi(-|z|) = phi t P(t) / 2 with
 // t = 1 / (1 + |z| / (2 sqrt2)), P the polynomial of stx_gelu_erf (gelu_phi_neg in ops.hip).
 __device__ __forceinline__ float normal_cdf(float z, float& phi) {
-    phi = expf(-0.5f * z * z);
+    phi = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f);   // z^2 / 2 ulps, in the tails
     const float t = __builtin_amdgcn_rcpf(fmaf(0.35355339059327376220f, fabsf(z), 1.f));
     float p = -1.5161373655e-02f;
     p = fmaf(p, t, 9.183117002e-02f);
