@@ -41,7 +41,10 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 acc, bf16) {
 // neither; an operand whose r is not its fastest dimension is "strided" below.
 enum Mode { FORWARD, GRAD, DX, DW };
 
-// Tiles of TJ x TM outputs, WJ x WM waves, SLOTS blocks a CU.
+// Tiles of TJ x TM outputs, WJ x WM waves, SLOTS blocks a CU. A step of the reduction is 8 chunks of
+// 16 bytes of every row, in two stages of LDS: five stages of 4 chunks, which keep twice as much
+// in flight, took 5 to 10 % longer everywhere (twice the barriers).
+constexpr int CH = 8;
 template <int TJ_, int TM_, int WJ_, int WM_, int SLOTS_>
 struct Tile {
     static constexpr int TJ = TJ_, TM = TM_, WJ = WJ_, WM = WM_, SLOTS = SLOTS_, NT = 64 * WJ * WM;
@@ -56,7 +59,7 @@ struct FfArgs {
     long long ps[2], qs[2];              // row strides in bytes
     int J, M;                            // extents of P's and Q's other dimension
     long long RP, RQ;                    // reduction lengths: past RP (of a strided P or Q past its own) zeros are taken
-    int steps, chunk;                    // steps of one reduction; steps of a part of it (DX, DW: split)
+    int steps, chunk;                    // steps of one reduction; of a part of it (DX, DW)
     int jtiles, tiles, items;            // column tiles, output tiles, tiles x parts (x 2 in DW)
     const float* b[2];
     int act;
@@ -79,16 +82,28 @@ __device__ __forceinline__ u32x4 load_chunk(const char* p, long long left) {
     if (left >= E) {
         __builtin_memcpy(&v, p, 16);
     } else if (left > 0) {
-        T e[E];
+        T e[E];                                          // clamped, not skipped: a load each, no branches
 #pragma unroll
-        for (int i = 0; i < E; i++) e[i] = i < left ? reinterpret_cast<const T*>(p)[i] : T(0.f);
+        for (int i = 0; i < E; i++) {
+            const T x = reinterpret_cast<const T*>(p)[i < left ? i : 0];
+            e[i] = i < left ? x : T(0.f);
+        }
         __builtin_memcpy(&v, e, 16);
     }
     return v;
 }
-__device__ __forceinline__ void load_to_lds(const void* src, void* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// 16 bytes a lane from memory to LDS at lds + lane * 16 (lds uniform over the wave): at base + off,
+// base uniform; or at p. Written out because the compiler takes every such load for one that a
+// transposing LDS read might depend on, and waits for all of them before it; the waits are
+// settle()'s. No register is written.
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)p);
+}
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void load_to_lds(const void* p, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "m0", "memory");
 }
 
 template <class T>
@@ -100,7 +115,11 @@ __device__ __forceinline__ void load4(const char* p, int left, float (&f)[4]) {
         for (int i = 0; i < 4; i++) f[i] = to_f32(v[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = i < left ? to_f32(reinterpret_cast<const T*>(p)[i]) : 0.f;
+        for (int i = 0; i < 4; i++) f[i] = 0.f;
+        if (left > 0) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[i] = to_f32(reinterpret_cast<const T*>(p)[i < left ? i : 0]);
+        }
     }
 }
 template <class T>
@@ -126,10 +145,8 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-constexpr int CH = 8;                    // 16-byte chunks of the reduction in a step: 128 bytes, 64 or 32 elements
-
 // An operand's tile of X rows (or columns) in a stage of LDS. Plain: [X][CH] chunks, chunk c of row x
-// at c ^ (x % 8), so that the 16 rows a fragment reads spread over all banks. Strided: rows of
+// at c ^ (x % 8), so that eight rows which a fragment reads together lie in different banks. Strided: rows of
 // the reduction, [CH E][X / E] chunks, chunk c of row r at c ^ turn(r), so that the rows which
 // one read takes (4 rows of 32 bytes for the transposing 16-bit read, 4 of 64 bytes in
 // fp32) do.
@@ -150,7 +167,7 @@ struct Fragments {
         constexpr int E = 16 / sizeof(T);
         const int s = lane % 16, q = lane / 16;
         if constexpr (!STRIDED) {
-            at[0] = (first * 16 + s) * CH * 16 + (q ^ (s % 8)) * 16;
+            at[0] = (first * 16 + s) * CH * 16 + (q ^ s % 8) * 16;
         } else if constexpr (sizeof(T) == 2) {                       // lane s reads row s / 4, columns 4 (s % 4) .. + 3
             const int row = q * 8 + s / 4;
 #pragma unroll
@@ -192,9 +209,9 @@ struct Source {
 };
 
 // Persistent blocks: each takes tiles of its XCD's share in turn, and the steps of all its tiles
-// form one stream. Two stages of LDS: while the waves multiply one, the other is filled with
-// the next step, the next tile's first included (ALIGNED: straight from memory to LDS; otherwise
-// through registers, for any alignment and length).
+// form one stream: while the waves multiply one stage of LDS, the other is filled with the next
+// step, the next tile's first included (ALIGNED: straight from memory to LDS; otherwise through
+// registers, for any alignment and length).
 template <class T, int MODE, class C, bool ALIGNED>
 __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     constexpr int NT = C::NT, E = 16 / sizeof(T), TJ = C::TJ, TM = C::TM;
@@ -240,7 +257,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     // where rows are clamped. With unaligned operands the offset is 64-bit.
     using Off = std::conditional_t<ALIGNED, unsigned, long long>;
     Off poff[PSource::N], qoff[QSource::N];
-    const int pside = GATED ? __builtin_amdgcn_readfirstlane(tid / CH / 16 % 2) : 0;   // a wave's rows are of one matrix
+    const int pside = GATED ? __builtin_amdgcn_readfirstlane(tid / CH / 16 % 2) : 0;   // the matrix of a wave's rows
     auto aim = [&](const Item& t, int seg, int qs) {
 #pragma unroll
         for (int i = 0; i < PSource::N; i++) {
@@ -262,14 +279,13 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         const long long r = (long long)(step - seg * a.steps) * CH * E;
         const char* pb = PS ? a.p[seg] + r * a.ps[seg] + t.j0 * (long long)sizeof(T) : a.p[pside] + t.j0 * a.ps[pside] + r * (long long)sizeof(T);
         const char* qb = QS ? a.q[qs] + r * a.qs[qs] + t.m0 * (long long)sizeof(T) : a.q[qs] + t.m0 * a.qs[qs] + r * (long long)sizeof(T);
-        char* pl = lds[stage] + wave * 1024;
-        char* ql = lds[stage] + TJ * CH * 16 + wave * 1024;
         if constexpr (ALIGNED) {
+            const unsigned pl = lds_address(lds[stage] + wave * 1024), ql = pl + TJ * CH * 16;
             if (r + CH * E <= a.RP && r + CH * E <= a.RQ) {
 #pragma unroll
-                for (int i = 0; i < PSource::N; i++) load_to_lds(pb + poff[i], pl + i * NT * 16);
+                for (int i = 0; i < PSource::N; i++) load_to_lds(pb, poff[i], pl + i * NT * 16);
 #pragma unroll
-                for (int i = 0; i < QSource::N; i++) load_to_lds(qb + qoff[i], ql + i * NT * 16);
+                for (int i = 0; i < QSource::N; i++) load_to_lds(qb, qoff[i], ql + i * NT * 16);
             } else {                                     // the reduction's end: zeros for what is past it
 #pragma unroll
                 for (int i = 0; i < PSource::N; i++)
@@ -287,6 +303,23 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 hold[PSource::N + i] = load_chunk<T>(qb + qoff[i], !QS ? a.RQ - r - QSource::chunk(i) * E : r + QSource::row(i) < a.RQ ? E : 0);
         }
     };
+    // The stream of fetches, one step ahead of the products.
+    Item ft = item_of(id);
+    int fid = id, fstep = ft.begin, fstage = 0;
+    bool more = true;
+    auto fetch_next = [&] {
+        fetch(ft, fstep, fstage);
+        fstage ^= 1;
+        if (++fstep == ft.end) {
+            fid += stride;
+            more = fid < last;
+            if (more) {
+                ft = item_of(fid);
+                fstep = ft.begin;
+            }
+        }
+    };
+    // Waits for the step in `stage`.
     auto settle = [&](int stage) {
         if constexpr (ALIGNED) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -307,15 +340,23 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     // accumulators' own layout they would be runs of 32 bytes (the forward product of 48,060 tokens,
     // K 384, N 1536 then spends 41 us of 167 on its stores).
     constexpr int COLS = GATED ? NJ * 8 : NJ * 16, CR = COLS / 8, AREA = 16 * COLS * 2, SHARE = STAGE / (NT / 64), PIECES = 16 * CR / 64;
-    static_assert(AREA * (MODE == GRAD ? 4 : 2) <= SHARE && PIECES >= 1, "staging");
-    auto spot = [&](int row, int col) { return row * COLS * 2 + (col / 8 ^ row % (CR < 8 ? CR : 8)) * 16 + col % 8 * 2; };
+    constexpr int AREAS = MODE == GRAD ? 2 : 1, TURNS = AREA * AREAS * 2 <= SHARE ? 2 : 1;   // areas of 16 rows; groups in turn
+    static_assert(AREA * AREAS <= SHARE && PIECES >= 1 && 16 * CR % 64 == 0, "staging");
+    auto spot = [&](int row, int col) { return row * COLS * 2 + (col / 8 + row) % CR * 16 + col % 8 * 2; };
     auto pack = [&](char* p, const float (&f)[4]) {
         T v[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = from_f32<T>(f[i]);
         __builtin_memcpy(__builtin_assume_aligned(p, 8), v, sizeof v);
     };
-    auto flush = [&](const char* area, char* out, long long os, int row0, int col0) {
+    // The lane's number as a new value: addresses formed from it are not kept from one group of rows
+    // for the next, there being no registers for them beside the accumulators.
+    auto fresh = [&] {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
+    auto flush = [&](int lane, const char* area, char* out, long long os, int row0, int col0) {
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
             const int row = (i * 64 + lane) / CR, c = (i * 64 + lane) % CR * 8, left = a.jpad - col0 - c;
@@ -332,13 +373,13 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         }
     };
     constexpr bool WIDE = sizeof(T) == 2, TAKES = MODE == GRAD && WIDE;
-    u32x4 dhv[TAKES ? PIECES : 1];                       // dh of the next 16 rows
-    auto take = [&](const Item& t, int m) {
+    u32x4 dhv[TAKES ? NM : 1][TAKES ? PIECES : 1];       // the wave's part of dh
+    auto take = [&](int lane, const Item& t, int m) {
         if constexpr (TAKES) {
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
                 const int row = t.m0 + (wm * NM + m) * 16 + (i * 64 + lane) / CR, col = t.j0 + wj * NJ * 8 + (i * 64 + lane) % CR * 8;
-                dhv[i] = load_chunk<T>(a.dh + row * a.dhs + col * (long long)sizeof(T), row < a.M ? a.J - col : 0);
+                dhv[m][i] = load_chunk<T>(a.dh + row * a.dhs + col * (long long)sizeof(T), row < a.M ? a.J - col : 0);
             }
         }
     };
@@ -348,12 +389,12 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         float sg[MODE == GRAD ? NJ / 2 : 1][4] = {}, sv[MODE == GRAD ? NJ / 2 : 1][4] = {};
 #pragma unroll
         for (int m = 0; m < NM; m++) {
+            const int lane = fresh();
             const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + lane % 16;
-            char* area = share + (MODE == GRAD ? m % 2 * 2 : m % 2) * AREA;
+            char* area = share + m % TURNS * AREAS * AREA;
             if constexpr (TAKES) {
 #pragma unroll
-                for (int i = 0; i < PIECES; i++) *reinterpret_cast<u32x4*>(area + spot((i * 64 + lane) / CR, (i * 64 + lane) % CR * 8)) = dhv[i];
-                if (m + 1 < NM) take(t, m + 1);
+                for (int i = 0; i < PIECES; i++) *reinterpret_cast<u32x4*>(area + spot((i * 64 + lane) / CR, (i * 64 + lane) % CR * 8)) = dhv[m][i];
             }
 #pragma unroll
             for (int j = 0; j < NJ; j += 2) {
@@ -386,12 +427,13 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                         store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.jpad - n, dg);
                         store4<T>(a.out[1] + row * a.os[1] + n * (long long)sizeof(T), a.jpad - n, dv);
                     }
+                    __builtin_amdgcn_sched_barrier(0);   // one at a time: there are no registers for more
                 }
             }
             if constexpr (WIDE) {
                 if (MODE == FORWARD || a.out[0]) {
-                    flush(area, a.out[0], a.os[0], row0, nw);
-                    if constexpr (MODE == GRAD) flush(area + AREA, a.out[1], a.os[1], row0, nw);
+                    flush(lane, area, a.out[0], a.os[0], row0, nw);
+                    if constexpr (MODE == GRAD) flush(lane, area + AREA, a.out[1], a.os[1], row0, nw);
                 }
             }
         }
@@ -416,8 +458,9 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         float* part = a.part ? a.part + (long long)t.z * a.M * a.J : nullptr;
 #pragma unroll
         for (int m = 0; m < NM; m++) {
+            const int lane = fresh();
             const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + lane % 16;
-            char* area = share + m % 2 * AREA;
+            char* area = share + m % TURNS * AREA;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 const float f[4] = {acc[j][m][0], acc[j][m][1], acc[j][m][2], acc[j][m][3]};
@@ -431,7 +474,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 }
             }
             if constexpr (WIDE)
-                if (!part) flush(area, a.out[which], a.os[which], row0, jw);
+                if (!part) flush(lane, area, a.out[which], a.os[which], row0, jw);
         }
     };
     // A tile starts from its biases, or from zeros.
@@ -441,29 +484,26 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
             float b[4] = {};
             if constexpr (GATED) {
                 const int n = t.j0 + (wj * NJ + j) / 2 * 16 + lane / 16 * 4;
-                if (a.b[j % 2]) load4<float>(reinterpret_cast<const char*>(a.b[j % 2] + n), a.J - n, b);
+                if (a.b[j % 2]) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) b[r] = a.b[j % 2][min(n + r, a.J - 1)];
+                }
             }
 #pragma unroll
             for (int m = 0; m < NM; m++) acc[j][m] = f32x4{b[0], b[1], b[2], b[3]};
         }
     };
 
-    Item t = item_of(id);
-    fetch(t, t.begin, 0);
-    settle(0);
+    fetch_next();
     int stage = 0;
     while (true) {
+        const Item t = item_of(id);
         start(t);
-        const int next = id + stride;
-        Item n = t;
+        char* share = nullptr;
 #pragma unroll 1
         for (int s = t.begin; s < t.end; s++) {
-            if (s + 1 < t.end) {
-                fetch(t, s + 1, stage ^ 1);
-            } else if (next < last) {
-                n = item_of(next);
-                fetch(n, n.begin, stage ^ 1);
-            }
+            settle(stage);                               // every wave is done with the stage before it, too
+            if (more) fetch_next();
 #pragma unroll
             for (int kk = 0; kk < CH / 4; kk++) {
                 u32x4 fp[NJ], fq[NM];
@@ -474,21 +514,19 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
 #pragma unroll
                     for (int m = 0; m < NM; m++) acc[j][m] = mma(fp[j], fq[m], acc[j][m], T{});
             }
-            if (s + 1 < t.end) {
-                settle(stage ^ 1);
-                stage ^= 1;
-            }
+            share = lds[stage];
+            stage ^= 1;
         }
-        take(t, 0);
-        __syncthreads();                                 // the last stage is read; its shares are free
-        char* share = lds[stage] + wave * SHARE;
+        if constexpr (TAKES) {
+#pragma unroll
+            for (int m = 0; m < NM; m++) take(lane, t, m);
+        }
+        __syncthreads();                                 // the last stage is read; its shares are free until the next step settles
+        share += wave * SHARE;
         if constexpr (GATED) with_act(a.act, [&](auto act) { gated(t, share, act); });
         else plain(t, share);
-        if (next >= last) return;
-        settle(stage ^ 1);
-        stage ^= 1;
-        id = next;
-        t = n;
+        id += stride;
+        if (id >= last) return;
     }
 }
 
@@ -618,29 +656,34 @@ constexpr long long kMaxWidth = 1 << 20, kMaxTokens = 1 << 30;   // of K and N; 
 constexpr int kCus = 256;                                         // of an MI355X: plans are made without a device at hand
 
 // How a product is run: its tile and the number of parts of its reduction, by the least estimated time.
-// A step of a tile takes cycles in proportion to its area, the larger tiles' by a better rate (the
-// measured ones of a long reduction); a part ends in an epilogue and a fold.
+// A step (128 bytes of the reduction) of a tile takes time in proportion to its area, the larger
+// tiles' at a better rate (the measured ones of a long reduction); a part ends in an epilogue
+// and a fold.
 struct Plan {
-    int tile, splits, steps;             // 0 Large, 1 Medium, 2 Small; steps of a part
+    int tile, splits, part;              // 0 Large, 1 Medium, 2 Small; parts, steps of a part
 };
-Plan plan_of(long long J, long long M, long long steps, int width_of_two, int w, int size, bool split) {
+long long steps_of(long long r, int size) { return std::max(1LL, (r * size + CH * 16 - 1) / (CH * 16)); }
+Plan plan_of(Mode mode, long long J, long long M, long long steps, int size) {
     struct Kind {
         int tj, tm, slots;
-        double rate[2];                  // relative, 16-bit and fp32
+        double rate[2], alone[3];        // relative rate, 16-bit and fp32; and of 1, 2, 3 blocks on a CU
     };
-    static constexpr Kind kinds[] = {{256, 256, 1, {1.0, 1.0}}, {128, 128, 2, {0.86, 0.96}}, {128, 64, 3, {0.62, 0.85}}};
+    static constexpr Kind kinds[] = {{256, 256, 1, {1.0, 1.0}, {1, 1, 1}},
+                                     {128, 128, 2, {0.86, 0.96}, {0.6, 1, 1}},
+                                     {128, 64, 3, {0.62, 0.85}, {0.4, 0.75, 1}}};
+    const bool gated = mode == FORWARD || mode == GRAD;
+    const int w = mode == DW ? 2 : 1;
     Plan best{};
     double least = 0;
-    steps = std::max(1LL, steps);                                 // no tokens: nothing is launched
-    for (int k = 0; k < 3; k++) {
-        const long long jt = (J * width_of_two + kinds[k].tj - 1) / kinds[k].tj, tiles = jt * ((M + kinds[k].tm - 1) / kinds[k].tm) * w;
-        const double step = kinds[k].tj * (double)kinds[k].tm / 65536 / kinds[k].rate[size == 4] * (size == 4 ? 7.1 : 0.95);   // us on a whole CU
-        for (int s = 1; s <= (split ? 32 : 1) && (s == 1 || steps / s >= 4); s++) {
-            const long long part = (steps + s - 1) / s, slots = (long long)kCus * kinds[k].slots, items = tiles * ((steps + part - 1) / part);
-            // Full rounds share a CU; in the last, fewer blocks a CU run faster, but not as fast as their number.
-            const long long rounds = items / slots, rest = items - rounds * slots;
-            const double busy = rounds * kinds[k].slots + (rest ? (double)((rest + kCus - 1) / kCus) : 0.0);
-            double us = busy * (part * step + 4.0 * kinds[k].tj * kinds[k].tm / 65536) + 2.0;
+    for (int k = mode == GRAD ? 1 : 0; k < 3; k++) {                 // Large has no registers for GRAD's epilogue: 460 us where Medium takes 250
+        const Kind& c = kinds[k];
+        const long long tiles = (J * (gated ? 2 : 1) + c.tj - 1) / c.tj * ((M + c.tm - 1) / c.tm) * w;
+        const double area = c.tj * (double)c.tm / 65536, step = area / c.rate[size == 4] * (size == 4 ? 7.1 : 0.95);   // us on a whole CU
+        for (int s = 1; s <= (gated ? 1 : 32) && (s == 1 || steps / s >= 4); s++) {
+            const long long part = (steps + s - 1) / s, items = tiles * ((steps + part - 1) / part), rest = items % (kCus * c.slots);
+            const long long k_rest = (rest + kCus - 1) / kCus;
+            const double busy = (double)(items / (kCus * c.slots)) * c.slots + (rest ? k_rest / c.alone[k_rest - 1] : 0.0);
+            double us = busy * (part * step + 4.0 * area) + 2.0;
             if (s > 1) us += 4.0 + 8.0 * s * J * M * w / 4e6;
             if (least == 0 || us < least) {
                 least = us;
@@ -668,7 +711,7 @@ void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
 template <class T, int MODE>
 void launch_ff(const FfArgs& a, bool aligned, int tile, int parts, hipStream_t stream) {
     if (!aligned) tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
-    else if (tile == 0) launch_tiles<T, MODE, Large, true>(a, parts, stream);
+    else if (MODE != GRAD && tile == 0) launch_tiles<T, MODE == GRAD ? FORWARD : MODE, Large, true>(a, parts, stream);
     else if (tile == 1) launch_tiles<T, MODE, Medium, true>(a, parts, stream);
     else launch_tiles<T, MODE, Small, true>(a, parts, stream);
 }
@@ -703,8 +746,6 @@ void check_output(const stx_tensor* t, const Rows& r, int size, const char* what
     STX_REQUIRE(r.n <= 1 || r.stride >= t->ne[0] * size, "gated_ff: rows of %s overlap", what);
 }
 
-int steps_of(long long r, int size) { return (int)((r * size + CH * 16 - 1) / (CH * 16)); }
-
 FfArgs products(const Block& b, const float* bg, const float* bv, stx_act act, int size) {
     FfArgs k{};
     k.p[0] = b.wg.data;
@@ -716,7 +757,7 @@ FfArgs products(const Block& b, const float* bg, const float* bv, stx_act act, i
     k.J = b.N;
     k.M = (int)b.M;
     k.RP = k.RQ = b.K;
-    k.steps = steps_of(b.K, size);
+    k.steps = (int)steps_of(b.K, size);
     k.jpad = b.N;
     k.b[0] = bg;
     k.b[1] = bv;
@@ -738,9 +779,9 @@ constexpr int kWaveRows[] = {Large::TM / Large::WM, Medium::TM / Medium::WM, Sma
 BackPlan back_plan(long long M, long long K, long long N, int size) {
     BackPlan p{};
     p.Np = pad64(N);
-    p.grad = plan_of(N, M, steps_of(K, size), 2, 1, size, false);
-    p.dx = plan_of(K, M, 2LL * steps_of(N, size), 1, 1, size, true);
-    p.dw = plan_of(K, N, steps_of(M, size), 1, 2, size, true);
+    p.grad = plan_of(GRAD, N, M, steps_of(K, size), size);
+    p.dx = plan_of(DX, K, M, 2 * steps_of(N, size), size);
+    p.dw = plan_of(DW, K, N, steps_of(M, size), size);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -810,8 +851,8 @@ void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, 
         k.M = (int)b.M;
         k.RP = b.N;
         k.RQ = p.Np;
-        k.steps = steps_of(b.N, size);
-        k.chunk = p.dx.steps;
+        k.steps = (int)steps_of(b.N, size);
+        k.chunk = p.dx.part;
         k.out[0] = dx->data;
         k.os[0] = dx->stride;
         k.part = p.dx.splits > 1 ? part : nullptr;
@@ -829,8 +870,8 @@ void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, 
         k.M = b.N;
         k.qpad = (int)p.Np;
         k.RP = k.RQ = b.M;
-        k.steps = steps_of(b.M, size);
-        k.chunk = p.dw.steps;
+        k.steps = (int)steps_of(b.M, size);
+        k.chunk = p.dw.part;
         k.out[0] = dwg->data;
         k.out[1] = dwv->data;
         k.os[0] = dwg->stride;
@@ -868,7 +909,7 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
         with_type(type, [&](auto t) {
             using T = decltype(t);
             if (b.M > kFew)
-                return launch_ff<T, FORWARD>(k, products_aligned(b, size), plan_of(b.N, b.M, k.steps, 2, 1, size, false).tile, 1, as_stream(stream));
+                return launch_ff<T, FORWARD>(k, products_aligned(b, size), plan_of(FORWARD, b.N, b.M, k.steps, size).tile, 1, as_stream(stream));
             const dim3 grid((b.N + 15) / 16), block(512);
             if (b.M <= 16) hipLaunchKernelGGL((ff_few_kernel<T, 1>), grid, block, 0, as_stream(stream), k);
             else if (b.M <= 32) hipLaunchKernelGGL((ff_few_kernel<T, 2>), grid, block, 0, as_stream(stream), k);

@@ -401,6 +401,25 @@ def test_gated_ff(device, dtype, shape, act):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(5000, 392, 1030), (2600, 1160, 2056), (9001, 128, 96)], ids=str)
+def test_gated_ff_large(device, dtype, shape):
+    """The larger tiles, several of them a block, with edges in every direction and reductions split or not."""
+    M, K, N = shape
+    dt = TYPES[dtype]
+    x, dh = randn(device, (M, K), 37, dtype=dt), randn(device, (M, N), 38, dtype=dt)
+    wg, wv = (randn(device, (N, K), 39 + i, K ** -0.5, dtype=dt) for i in range(2))
+    bg, bv = randn(device, (N,), 34, 0.2), randn(device, (N,), 35, 0.2)
+    ref = ff_ref(x, wg, wv, "sigmoid", bg, bv, dh)
+    h = stx.gated_ff(x, wg, wv, stx.ACT_SIGMOID, bg, bv)
+    close(h, ref["h"], ref["eh"], "h")
+    norm_close(h, ref["h"], 1, "h")
+    for name, got in zip(("dx", "dwg", "dwv", "dbg", "dbv"), stx.gated_ff_back(dh, x, wg, wv, stx.ACT_SIGMOID, bg, bv)):
+        close(got, ref[name], ref["e" + name], name)
+        if not name.startswith("db"):
+            norm_close(got, ref[name], 2, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M", [5, 150])
 def test_gated_ff_strides_and_token_dims(device, dtype, M):
     """Rows of larger buffers (x, weights, dh and every output), at odd offsets; token dimensions; the bytes between
