@@ -13,16 +13,24 @@ namespace {
 // thread meets the same channels in every vector it takes whatever C is, the slice is walked in
 // super-rows of R = V / gcd(C, V) rows, which hold a whole number of vectors: vector j of a
 // super-row covers channels (j V + e) mod C. Accesses may be unaligned (odd C, odd slices); only
-// the slice's last vector can be partial.
+// the slice's last super-row can be partial.
 //
 // A block has a tile of `cols` vector columns x `rws` super-rows at a time, and one chunk of the
-// slice's super-rows. Three steps, forward and backward alike:
-//   sums:  per (slice, chunk, slot = position in the super-row) two sums in double
-//          (x, x^2 or dz, dz xhat); in double because E[x^2] - mean^2 cancels otherwise;
-//   fold:  over chunks and the R slots of a channel, to [slice][C] pairs;
-//   apply: each block adds the channels of the groups it needs from those pairs, then streams its
-//          elements, one fused multiply-add and the activation each.
+// slice's super-rows. Two kernels, forward and backward alike:
+//   sums:  two sums of every slot (position in the super-row) over the chunk: x, x^2 or dz, dz xhat;
+//          added up to groups (backward: times w), one pair a (slice, chunk, tile, group), and in the
+//          backward pass also kept per slot, for dweight and dbias;
+//   apply: each block adds the pairs of its slice's groups, then streams its elements, one fused
+//          multiply-add and the activation each. In the backward pass extra blocks add the
+//          slots' sums to dweight and dbias.
+// (slices with more than kDirect pairs have them added by a small kernel in between). x and x^2 are
+// summed in double, since E[x^2] - mean^2 cancels; the backward sums in float over kHeld rows
+// of a thread (64 terms drift by about 1e-7 of their sum), then in double. Both passes are bound by HBM, the second by what the last-level cache still holds.
 constexpr int kThreads = 256;
+constexpr int kBatch = 4;                // super-rows a thread has in flight
+constexpr int kHeld = 64;                // rows summed in float before they join the sums in double
+constexpr int kDirect = 2048;            // pairs that every apply block adds by itself
+constexpr int kParamChannels = 8;        // of a block that adds dweight and dbias: 32 lanes a channel
 
 struct Geometry {
     long long B, T;
@@ -58,9 +66,10 @@ Geometry geometry(const stx_tensor* a, int size, int n_groups) {
     g.tiles = (g.ncol + g.cols - 1) / g.cols;
     g.rws = kThreads / g.cols;
     g.srows = (g.T + g.R - 1) / g.R;
-    // Chunks: enough blocks for eight a CU, each of at least 16 super-rows and 8 passes of its threads.
-    const long long most = std::max(1LL, std::min(2048 / std::max(1LL, g.B * g.tiles), g.srows / std::max(16, 8 * g.rws)));
-    g.chunk_srows = std::max(1LL, (g.srows + most - 1) / most);
+    // Chunks: enough blocks for four a CU, each of at least one batch of its threads' rows.
+    const long long most = std::max(1LL, std::min(1024 / std::max(1LL, g.B * g.tiles), g.srows / (kBatch * g.rws)));
+    const long long batch = kBatch * g.rws;
+    g.chunk_srows = std::max(1LL, ((g.srows + most - 1) / most + batch - 1) / batch) * batch;
     g.chunks = (int)std::max(1LL, (g.srows + g.chunk_srows - 1) / g.chunk_srows);
     return g;
 }
@@ -74,24 +83,26 @@ struct NormArgs {
     const float *w, *b;
     const double2* stats_in;             // [B][G] mean, 1 / sqrt(var + eps)
     double2* stats_out;
-    double2* part;                       // [B][chunks][slots]
-    double2* chan;                       // [B][C]
+    double2* part;                       // [B][rows][G], rows = chunks x tiles
+    double2* folded;                     // [B][G]
+    double2* slot;                       // backward: [B][chunks][slots]
+    long long rows;                      // of `part`, or 1 where they are folded (0: no elements)
+    unsigned first;                      // backward: apply blocks before this one add dweight and dbias
     float *dw, *db;
     double eps;
     int act;
 };
 
 template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* p, long long left, float (&f)[V]) {
+__device__ __forceinline__ Pack<T, V> load_vec(const T* p, long long left) {
+    Pack<T, V> v;
     if (left >= V) {
-        T v[V];
-        __builtin_memcpy(v, p, sizeof v);
-#pragma unroll
-        for (int e = 0; e < V; e++) f[e] = to_f32(v[e]);
+        __builtin_memcpy(&v, p, sizeof v);
     } else {
 #pragma unroll
-        for (int e = 0; e < V; e++) f[e] = e < left ? to_f32(p[e]) : 0.f;
+        for (int e = 0; e < V; e++) v.v[e] = e < left ? p[e] : T(0.f);
     }
+    return v;
 }
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T* p, long long left, const float (&f)[V]) {
@@ -109,143 +120,181 @@ __device__ __forceinline__ void store_vec(T* p, long long left, const float (&f)
 
 // Where a thread is: its slice, column and super-rows.
 struct Place {
-    long long slice, begin, end, chunk;
-    int col, row;
+    long long slice, begin, end, full, chunk;            // super-rows before `full` are whole
+    int col, row, tile;
     bool on;
 };
-__device__ __forceinline__ Place place(const NormArgs& a) {
+__device__ __forceinline__ Place place(const NormArgs& a, unsigned bid) {
     Place p;
-    const unsigned bid = blockIdx.x;
-    const unsigned bc = a.tiles.div(bid), tile = bid - bc * a.tiles.d;
+    const unsigned bc = a.tiles.div(bid);
+    p.tile = (int)(bid - bc * a.tiles.d);
     const unsigned b = a.chunks.div(bc);
     p.slice = b;
     p.chunk = bc - b * a.chunks.d;
-    const int c = (int)threadIdx.x % a.g.cols;
     p.row = (int)threadIdx.x / a.g.cols;
-    p.col = (int)tile * a.g.cols + c;
+    p.col = p.tile * a.g.cols + (int)threadIdx.x % a.g.cols;
     p.begin = p.chunk * a.g.chunk_srows;
     p.end = min(p.begin + a.g.chunk_srows, a.g.srows);
+    p.full = a.g.T % a.g.R ? a.g.srows - 1 : a.g.srows;
     p.on = p.row < a.g.rws && p.col < a.g.ncol;
     return p;
 }
 
-// Per-channel constants of a normalisation: xhat = (x - mh) r - d, with mean = mh + the rest in d
-// (a float mean alone would cost |mean| 2^-24 / std).
-struct Chan {
-    float mh, r, d, w, b;
-};
-__device__ __forceinline__ Chan chan_of(const NormArgs& a, double mean, double rstd, int c) {
-    Chan k;
-    k.mh = (float)mean;
-    k.r = (float)rstd;
-    k.d = (float)((mean - (double)k.mh) * rstd);
-    k.w = a.w ? a.w[c] : 1.f;
-    k.b = a.b ? a.b[c] : 0.f;
-    return k;
+// f(r, batch) over a thread's super-rows, kBatch of them at a time: their loads are in flight together.
+// whole: every vector of the batch exists in full.
+template <class F>
+__device__ __forceinline__ void for_rows(const Place& p, int rws, F&& f) {
+    long long r = p.begin + p.row;
+    const long long end = min(p.end, p.full);
+    for (; r + (kBatch - 1) * rws < end; r += kBatch * rws) f(r, std::integral_constant<int, kBatch>{}, std::true_type{});
+    for (; r < p.end; r += rws) f(r, std::integral_constant<int, 1>{}, std::false_type{});
 }
+
+// Sum of red[rows][width] over the rows, into red[0][]. All threads; the order depends on the shape alone.
+__device__ __forceinline__ void fold_rows(double2* red, int rows, int width) {
+    while (rows > 1) {
+        const int half = (rows + 1) / 2;
+        __syncthreads();
+        for (int i = (int)threadIdx.x; i < (rows - half) * width; i += kThreads) {
+            const double2 v = red[half * width + i];
+            red[i].x += v.x;
+            red[i].y += v.y;
+        }
+        rows = half;
+    }
+    __syncthreads();
+}
+
+// Per-channel constants, all of the centred t = x - mh, where mean = mh + a rest that joins the
+// additive constants (a float mean alone would cost |mean| 2^-24 / std; a product x r - mean r, which
+// would save the subtraction, costs as much):
+//   xhat = t r - d,  z = xhat w + b = t A + B,  dx = r (w dz - S1/n - xhat S2/n) = t q + (dz A + p).
+struct Chan {
+    float mh, r, d, A, B, p, q;
+    __device__ __forceinline__ void set(const NormArgs& a, double mean, double rstd, int c) {
+        const double w = a.w ? (double)a.w[c] : 1.0, b = a.b ? (double)a.b[c] : 0.0;
+        mh = (float)mean;
+        const double rest = (mean - (double)mh) * rstd;
+        r = (float)rstd;
+        d = (float)rest;
+        A = (float)(rstd * w);
+        B = (float)(b - rest * w);
+    }
+    __device__ __forceinline__ void set_back(double mean, double rstd, double s1, double s2) {   // S1 / n, S2 / n
+        p = (float)(((mean - (double)mh) * rstd * s2 - s1) * rstd);
+        q = (float)(-rstd * rstd * s2);
+    }
+};
 
 template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
     constexpr int V = 16 / sizeof(T);
     __shared__ double2 red[kThreads * V];
-    const Place p = place(a);
-    double s1[V] = {}, s2[V] = {};
+    const Place p = place(a, blockIdx.x);
+    const int width = a.g.cols * V, first = p.tile * width, here = min(width, a.g.slots - first);
+    double2* mine = red + p.row * width + (int)threadIdx.x % a.g.cols * V;
+    if (p.row < a.g.rws) {
+#pragma unroll
+        for (int e = 0; e < V; e++) mine[e] = make_double2(0.0, 0.0);
+    }
     if (p.on) {
         const long long n = a.g.T * a.g.C;
         const T* x = static_cast<const T*>(a.x) + p.slice * n;
         const T* dy = static_cast<const T*>(a.dy) + p.slice * n;
-        Chan k[V];
+        Chan k[BACK ? V : 1];
         if constexpr (BACK) {
 #pragma unroll
             for (int e = 0; e < V; e++) {
                 const int c = (p.col * V + e) % a.g.C;
                 const double2 st = a.stats_in[p.slice * a.g.G + c / a.g.width];
-                k[e] = chan_of(a, st.x, st.y, c);
+                k[e].set(a, st.x, st.y, c);
             }
         }
-        for (long long r = p.begin + p.row; r < p.end; r += a.g.rws) {
-            const long long at = r * a.g.slots + (long long)p.col * V;
-            float f[V];
-            load_vec<T, V>(x + at, n - at, f);
-            if constexpr (BACK) {
-                float g[V];
-                load_vec<T, V>(dy + at, n - at, g);
+        std::conditional_t<BACK, float, double> s1[V] = {}, s2[V] = {};
+        int held = 0;
+        auto flush = [&] {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                mine[e] = make_double2(mine[e].x + (double)s1[e], mine[e].y + (double)s2[e]);
+                s1[e] = s2[e] = 0;
+            }
+            held = 0;
+        };
+        for_rows(p, a.g.rws, [&](long long r, auto batch, auto whole) {
+            constexpr int N = batch();
+            Pack<T, V> f[N], g[BACK ? N : 1];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const long long at = (r + i * a.g.rws) * a.g.slots + (long long)p.col * V, left = whole() ? V : n - at;
+                f[i] = load_vec<T, V>(x + at, left);
+                if constexpr (BACK) g[i] = load_vec<T, V>(dy + at, left);
+            }
+            const long long left = whole() ? V : n - r * a.g.slots - (long long)p.col * V;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
 #pragma unroll
                 for (int e = 0; e < V; e++) {
-                    const float xh = fmaf(f[e] - k[e].mh, k[e].r, -k[e].d);
-                    float d;
-                    (void)act_f32<ACT>(fmaf(xh, k[e].w, k[e].b), d);
-                    const double dz = (double)(g[e] * d);        // past the end g is 0
-                    s1[e] += at + e < n ? dz : 0.0;
-                    s2[e] = at + e < n ? fma(dz, (double)xh, s2[e]) : s2[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const double d = (double)f[e];
-                    s1[e] += d;
-                    s2[e] = fma(d, d, s2[e]);
+                    if (!whole() && e >= left) continue;
+                    const float xe = to_f32(f[i].v[e]);
+                    if constexpr (BACK) {
+                        const float t = xe - k[e].mh;
+                        float d;
+                        (void)act_f32<ACT>(fmaf(t, k[e].A, k[e].B), d);
+                        const float dz = to_f32(g[i].v[e]) * d;
+                        s1[e] += dz;
+                        s2[e] = fmaf(dz, fmaf(t, k[e].r, -k[e].d), s2[e]);
+                    } else {
+                        s1[e] += (double)xe;
+                        s2[e] = fma((double)xe, (double)xe, s2[e]);
+                    }
                 }
             }
-        }
+            if (BACK && (held += N) >= kHeld) flush();
+        });
+        flush();
     }
-    const int width = a.g.cols * V;
-#pragma unroll
-    for (int e = 0; e < V; e++)
-        if (p.row < a.g.rws) red[p.row * width + ((int)threadIdx.x % a.g.cols) * V + e] = make_double2(s1[e], s2[e]);
-    __syncthreads();
-    const int first = (p.col - (int)threadIdx.x % a.g.cols) * V;
-    for (int i = (int)threadIdx.x; i < width && first + i < a.g.slots; i += kThreads) {
-        double2 s = red[i];
-        for (int r = 1; r < a.g.rws; r++) {
-            s.x += red[r * width + i].x;
-            s.y += red[r * width + i].y;
+    fold_rows(red, a.g.rws, width);
+    if constexpr (BACK) {
+        double2* slot = a.slot + (p.slice * a.g.chunks + p.chunk) * a.g.slots + first;
+        for (int i = (int)threadIdx.x; i < here; i += kThreads) slot[i] = red[i];
+    }
+    // A group's slots: one run in each of the super-row's R rows. Wide groups by a wave each, narrow
+    // ones by a thread.
+    double2* part = a.part + ((p.slice * a.g.chunks + p.chunk) * a.g.tiles + p.tile) * a.g.G;
+    const bool wide = a.g.width >= 64;
+    const int lanes = wide ? 64 : 1, lane = wide ? (int)threadIdx.x % 64 : 0;
+    for (int g = (int)threadIdx.x / lanes; g < a.g.G; g += kThreads / lanes) {
+        double2 s = make_double2(0.0, 0.0);
+        for (int r = 0; r < a.g.R; r++) {
+            const int row = r * a.g.C - first, lo = max(0, row + g * a.g.width), hi = min(here, row + min((g + 1) * a.g.width, a.g.C));
+            for (int i = lo + lane; i < hi; i += lanes) {
+                const double w = BACK && a.w ? (double)a.w[i - row] : 1.0;
+                s.x = fma(red[i].x, w, s.x);
+                s.y = fma(red[i].y, w, s.y);
+            }
         }
-        a.part[(p.slice * a.g.chunks + p.chunk) * a.g.slots + first + i] = s;
+        if (wide) {
+            s.x = lane_sum<64>(s.x);
+            s.y = lane_sum<64>(s.y);
+        }
+        if (lane == 0) part[g] = s;
     }
 }
 
-// [B][chunks][R][C] -> [B][C]: 32 channels x 8 parts a block, in a fixed order.
-__global__ __launch_bounds__(256) void gn_cl_fold_kernel(NormArgs a, FastDiv ctiles) {
-    __shared__ double2 red[8][33];
-    const unsigned b = ctiles.div(blockIdx.x);
-    const int c = (int)(blockIdx.x - b * ctiles.d) * 32 + (int)threadIdx.x % 32, lane = (int)threadIdx.x / 32;
+// The pairs of one group of one slice.
+__global__ __launch_bounds__(kThreads) void gn_cl_fold_kernel(NormArgs a, long long rows) {
+    __shared__ double2 red[kThreads];
+    const long long b = blockIdx.x / (unsigned)a.g.G, g = blockIdx.x % (unsigned)a.g.G;
     double2 s = make_double2(0.0, 0.0);
-    if (c < a.g.C) {
-        const double2* p = a.part + (long long)b * a.g.chunks * a.g.slots + c;
-        const int rows = a.g.srows ? a.g.chunks * a.g.R : 0;
-        for (int i = lane; i < rows; i += 8) {
-            const double2 v = p[(long long)i * a.g.C];
-            s.x += v.x;
-            s.y += v.y;
-        }
+#pragma unroll 4
+    for (long long r = threadIdx.x; r < rows; r += kThreads) {
+        const double2 v = a.part[(b * rows + r) * a.g.G + g];
+        s.x += v.x;
+        s.y += v.y;
     }
-    red[lane][threadIdx.x % 32] = s;
-    __syncthreads();
-    if (lane == 0 && c < a.g.C) {
-        for (int i = 1; i < 8; i++) {
-            s.x += red[i][threadIdx.x].x;
-            s.y += red[i][threadIdx.x].y;
-        }
-        a.chan[(long long)b * a.g.C + c] = s;
-    }
-}
-
-// Group values a block's columns need: a wave adds the channels of a group (weighted in the
-// backward pass, where the channel's xhat = dxhat / w).
-template <bool BACK>
-__device__ double2 group_total(const NormArgs& a, long long slice, int group) {
-    const int lo = group * a.g.width, hi = min(lo + a.g.width, a.g.C);
-    double2 s = make_double2(0.0, 0.0);
-    for (int c = lo + (int)threadIdx.x % 64; c < hi; c += 64) {
-        const double2 v = a.chan[slice * a.g.C + c];
-        const double w = BACK && a.w ? (double)a.w[c] : 1.0;
-        s.x = fma(v.x, w, s.x);
-        s.y = fma(v.y, w, s.y);
-    }
-    s.x = lane_sum<64>(s.x);
-    s.y = lane_sum<64>(s.y);
-    return s;
+    red[threadIdx.x] = s;
+    fold_rows(red, kThreads, 1);
+    if (threadIdx.x == 0) a.folded[blockIdx.x] = red[0];
 }
 
 __device__ __forceinline__ double2 moments(const NormArgs& a, double2 s, double n) {
@@ -254,18 +303,54 @@ __device__ __forceinline__ double2 moments(const NormArgs& a, double2 s, double 
     return make_double2(mean, 1.0 / sqrt(fmax(0.0, s.y / n - mean * mean) + a.eps));
 }
 
+// dbias and dweight of kParamChannels channels: the slots' sums over slices, chunks and R.
+__device__ void add_params(const NormArgs& a, double2* red, unsigned block) {
+    const int c = (int)block * kParamChannels + (int)threadIdx.x % kParamChannels, lane = (int)threadIdx.x / kParamChannels;
+    const long long rows = a.g.srows ? a.g.B * a.g.chunks * a.g.R : 0;
+    double2 s = make_double2(0.0, 0.0);
+    if (c < a.g.C) {
+#pragma unroll 8
+        for (long long r = lane; r < rows; r += kThreads / kParamChannels) {
+            const double2 v = a.slot[r * a.g.C + c];
+            s.x += v.x;
+            s.y += v.y;
+        }
+    }
+    red[threadIdx.x] = s;
+    fold_rows(red, kThreads / kParamChannels, kParamChannels);
+    if (lane || c >= a.g.C) return;
+    if (a.db) a.db[c] = (float)red[threadIdx.x].x;
+    if (a.dw) a.dw[c] = (float)red[threadIdx.x].y;
+}
+
 template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
     constexpr int V = 16 / sizeof(T);
-    extern __shared__ double2 groups[];                  // [G]
-    const Place p = place(a);
-    // Every group of the slice (a column tile of odd C meets channels of several places).
-    for (int g = (int)threadIdx.x / 64; g < a.g.G; g += kThreads / 64) {
-        const double n = (double)a.g.T * (min((g + 1) * a.g.width, a.g.C) - g * a.g.width);
-        const double2 s = group_total<BACK>(a, p.slice, g);
-        if (threadIdx.x % 64 == 0) {
+    extern __shared__ double2 groups[];                  // [max(G, kThreads)]
+    if (BACK && blockIdx.x < a.first) return add_params(a, groups, blockIdx.x);
+    const Place p = place(a, blockIdx.x - a.first);
+    {
+        const int G = a.g.G, parts = max(1, kThreads / G);
+        const double2* from = a.part + p.slice * a.rows * G;
+        for (int g0 = 0; g0 < G; g0 += kThreads) {       // one pass unless there are more groups than threads
+            const int g = g0 + (int)threadIdx.x % min(G, kThreads), part = (int)threadIdx.x / min(G, kThreads);
+            double2 s = make_double2(0.0, 0.0);
+            if (g < G && part < parts) {
+#pragma unroll 4
+                for (long long r = part; r < a.rows; r += parts) {
+                    const double2 v = from[r * G + g];
+                    s.x += v.x;
+                    s.y += v.y;
+                }
+                groups[g0 + (int)threadIdx.x] = s;
+            }
+        }
+        fold_rows(groups, parts, G);
+        for (int g = (int)threadIdx.x; g < G; g += kThreads) {
+            const double n = (double)a.g.T * (min((g + 1) * a.g.width, a.g.C) - g * a.g.width);
+            const double2 s = groups[g];
             groups[g] = BACK ? make_double2(s.x / n, s.y / n) : moments(a, s, n);
-            if (!BACK && a.stats_out && p.chunk == 0 && p.col == (int)threadIdx.x % a.g.cols) a.stats_out[p.slice * a.g.G + g] = groups[g];
+            if (!BACK && a.stats_out && p.chunk == 0 && p.tile == 0) a.stats_out[p.slice * G + g] = groups[g];
         }
     }
     __syncthreads();
@@ -275,60 +360,59 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
     const T* dy = static_cast<const T*>(a.dy) + p.slice * n;
     T* out = static_cast<T*>(a.out) + p.slice * n;
     Chan k[V];
-    float k1[V], k2[V];
 #pragma unroll
     for (int e = 0; e < V; e++) {
         const int c = (p.col * V + e) % a.g.C, g = c / a.g.width;
         if constexpr (BACK) {
             const double2 st = a.stats_in[p.slice * a.g.G + g];
-            k[e] = chan_of(a, st.x, st.y, c);
-            k1[e] = (float)(groups[g].x * st.y);
-            k2[e] = (float)(groups[g].y * st.y);
+            k[e].set(a, st.x, st.y, c);
+            k[e].set_back(st.x, st.y, groups[g].x, groups[g].y);
         } else {
-            k[e] = chan_of(a, groups[g].x, groups[g].y, c);
+            k[e].set(a, groups[g].x, groups[g].y, c);
         }
     }
-    for (long long r = p.begin + p.row; r < p.end; r += a.g.rws) {
-        const long long at = r * a.g.slots + (long long)p.col * V;
-        float f[V], y[V];
-        load_vec<T, V>(x + at, n - at, f);
-        if constexpr (BACK) {
-            float g[V];
-            load_vec<T, V>(dy + at, n - at, g);
+    for_rows(p, a.g.rws, [&](long long r, auto batch, auto whole) {
+        constexpr int N = batch();
+        Pack<T, V> f[N], g[BACK ? N : 1];
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float xh = fmaf(f[e] - k[e].mh, k[e].r, -k[e].d);
-                float d;
-                (void)act_f32<ACT>(fmaf(xh, k[e].w, k[e].b), d);
-                y[e] = fmaf(-xh, k2[e], fmaf(g[e] * d, k[e].r * k[e].w, -k1[e]));
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float xh = fmaf(f[e] - k[e].mh, k[e].r, -k[e].d);
-                y[e] = act_f32<ACT>(fmaf(xh, k[e].w, k[e].b));
-            }
+        for (int i = 0; i < N; i++) {
+            const long long at = (r + i * a.g.rws) * a.g.slots + (long long)p.col * V, left = whole() ? V : n - at;
+            f[i] = load_vec<T, V>(x + at, left);
+            if constexpr (BACK) g[i] = load_vec<T, V>(dy + at, left);
         }
-        if (at < n) store_vec<T, V>(out + at, n - at, y);
-    }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const long long at = (r + i * a.g.rws) * a.g.slots + (long long)p.col * V, left = whole() ? V : n - at;
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float t = to_f32(f[i].v[e]) - k[e].mh, z = fmaf(t, k[e].A, k[e].B);
+                if constexpr (BACK) {
+                    float d;
+                    (void)act_f32<ACT>(z, d);
+                    y[e] = fmaf(t, k[e].q, fmaf(to_f32(g[i].v[e]) * d, k[e].A, k[e].p));
+                } else {
+                    y[e] = act_f32<ACT>(z);
+                }
+            }
+            store_vec<T, V>(out + at, left, y);
+        }
+    });
 }
 
-// dbias and dweight: the channels' sums over the slices.
-__global__ __launch_bounds__(256) void gn_cl_params_kernel(NormArgs a) {
-    const int c = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (c >= a.g.C) return;
-    double s1 = 0.0, s2 = 0.0;
-    for (long long b = 0; b < a.g.B; b++) {
-        const double2 v = a.chan[b * a.g.C + c];
-        s1 += v.x;
-        s2 += v.y;
-    }
-    if (a.db) a.db[c] = (float)s1;
-    if (a.dw) a.dw[c] = (float)s2;
+long long pair_rows(const Geometry& g) { return g.srows ? (long long)g.chunks * g.tiles : 0; }
+bool folds(const Geometry& g) { return pair_rows(g) > 1 && (g.G > kThreads || pair_rows(g) * g.G > kDirect); }
+struct Spaces {
+    size_t folded, slot, total;          // `part` is at 0
+};
+Spaces spaces(const Geometry& g) {
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    Spaces s{};
+    s.folded = up((size_t)g.B * pair_rows(g) * g.G * sizeof(double2));
+    s.slot = s.folded + up(folds(g) ? (size_t)g.B * g.G * sizeof(double2) : 0);
+    s.total = s.slot + (size_t)g.B * g.chunks * g.slots * sizeof(double2);
+    return s;
 }
-
-size_t chan_bytes(const Geometry& g) { return ((size_t)g.B * g.C * sizeof(double2) + 255) / 256 * 256; }
-size_t workspace_bytes(const Geometry& g) { return chan_bytes(g) + (size_t)g.B * g.chunks * g.slots * sizeof(double2); }
 
 constexpr int kMaxGroups = 4096;         // of the apply kernel's LDS: 64 KB
 
@@ -343,37 +427,41 @@ Geometry check_norm(const stx_tensor* a, stx_type type, int n_groups) {
                 n_groups);
     if (n_groups > kMaxGroups) fail(STX_STATUS_UNSUPPORTED, "group_norm_cl: more than %d groups", kMaxGroups);
     const Geometry g = geometry(a, size, n_groups);
-    STX_REQUIRE(g.B * g.chunks * g.tiles < (1LL << 31) && g.B * ((C + 31) / 32) < (1LL << 31), "group_norm_cl: too many slices");
+    STX_REQUIRE(g.B < (1LL << 31) && g.B * g.chunks * g.tiles < (1LL << 30) && g.B * g.G < (1LL << 31), "group_norm_cl: too many slices");
     return g;
 }
 
 template <bool BACK>
 void run_norm(NormArgs& a, stx_type type, void* ws, hipStream_t stream) {
     const Geometry& g = a.g;
+    const Spaces at = spaces(g);
     a.chunks = FastDiv((unsigned)g.chunks);
     a.tiles = FastDiv((unsigned)g.tiles);
-    a.chan = static_cast<double2*>(ws);
-    a.part = reinterpret_cast<double2*>(static_cast<char*>(ws) + chan_bytes(g));
-    const dim3 grid((unsigned)(g.B * g.chunks * g.tiles)), block(kThreads);
-    const unsigned ctiles = (unsigned)((g.C + 31) / 32);
+    a.part = static_cast<double2*>(ws);
+    a.folded = reinterpret_cast<double2*>(static_cast<char*>(ws) + at.folded);
+    a.slot = reinterpret_cast<double2*>(static_cast<char*>(ws) + at.slot);
+    a.rows = pair_rows(g);
+    a.first = BACK && (a.dw || a.db) ? (unsigned)((g.C + kParamChannels - 1) / kParamChannels) : 0;
+    const unsigned blocks = (unsigned)(g.B * g.chunks * g.tiles);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (g.B == 0) return;
-        if (g.srows) {
-            if constexpr (BACK) with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_sums_kernel<T, true, act()>), grid, block, 0, stream, a); });
-            else hipLaunchKernelGGL((gn_cl_sums_kernel<T, false, STX_ACT_NONE>), grid, block, 0, stream, a);
+        if (g.srows && g.B) {
+            if constexpr (BACK) with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_sums_kernel<T, true, act()>), dim3(blocks), dim3(kThreads), 0, stream, a); });
+            else hipLaunchKernelGGL((gn_cl_sums_kernel<T, false, STX_ACT_NONE>), dim3(blocks), dim3(kThreads), 0, stream, a);
             launch_check("gn_cl_sums_kernel");
         }
-        hipLaunchKernelGGL(gn_cl_fold_kernel, dim3((unsigned)g.B * ctiles), dim3(256), 0, stream, a, FastDiv(ctiles));
-        launch_check("gn_cl_fold_kernel");
-        if (BACK && !a.out) return;
-        with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_apply_kernel<T, BACK, act()>), grid, block, sizeof(double2) * g.G, stream, a); });
+        const bool apply = !BACK || a.out;
+        if (folds(g) && g.B && apply) {
+            hipLaunchKernelGGL(gn_cl_fold_kernel, dim3((unsigned)(g.B * g.G)), dim3(kThreads), 0, stream, a, a.rows);
+            launch_check("gn_cl_fold_kernel");
+            a.part = a.folded;
+            a.rows = 1;
+        }
+        const unsigned grid = a.first + (apply ? blocks : 0);
+        if (grid == 0) return;
+        with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_apply_kernel<T, BACK, act()>), dim3(grid), dim3(kThreads), sizeof(double2) * std::max(g.G, kThreads), stream, a); });
         launch_check("gn_cl_apply_kernel");
     });
-    if (BACK && (a.dw || a.db)) {
-        hipLaunchKernelGGL(gn_cl_params_kernel, dim3((g.C + 255) / 256), dim3(256), 0, stream, a);
-        launch_check("gn_cl_params_kernel");
-    }
 }
 
 }  // namespace
@@ -389,7 +477,7 @@ STX_API size_t stx_group_norm_cl_workspace_size(const stx_tensor* a, stx_type ty
         STX_REQUIRE(a != nullptr, "group_norm_cl: a is NULL");
         stx_tensor t = *a;
         t.data = reinterpret_cast<void*>((uintptr_t)256);          // a query may have no data yet
-        bytes = workspace_bytes(check_norm(&t, type, n_groups));
+        bytes = spaces(check_norm(&t, type, n_groups)).total;
     });
     return bytes;
 }
@@ -407,7 +495,7 @@ STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_g
         STX_REQUIRE(contiguous_typed(dst, size), "group_norm_cl: dst must be contiguous");
         STX_REQUIRE(dst->data == a->data || !overlap(span_of(a, size), span_of(dst, size)), "group_norm_cl: dst overlaps a in part");
         STX_REQUIRE(eps >= 0.0, "group_norm_cl: negative eps");
-        check_workspace(workspace, workspace_bytes_, workspace_bytes(k.g), "group_norm_cl");
+        check_workspace(workspace, workspace_bytes_, spaces(k.g).total, "group_norm_cl");
         k.x = a->data;
         k.dy = a->data;                  // not read
         k.out = dst->data;
@@ -440,7 +528,7 @@ STX_API stx_status stx_group_norm_cl_back(const stx_tensor* dy, const stx_tensor
             STX_REQUIRE(dx->data == dy->data || !overlap(span_of(dy, size), span_of(dx, size)), "group_norm_cl_back: dx overlaps dy in part");
         }
         STX_REQUIRE(stats != nullptr || k.g.B == 0, "group_norm_cl_back: stats is NULL");
-        check_workspace(workspace, workspace_bytes_, workspace_bytes(k.g), "group_norm_cl_back");
+        check_workspace(workspace, workspace_bytes_, spaces(k.g).total, "group_norm_cl_back");
         if (!dx && !dweight && !dbias) return;
         k.x = a->data;
         k.dy = dy->data;
