@@ -186,6 +186,26 @@ struct Chan {
     }
 };
 
+// f(e, c, g) for the channels c and groups g of a column's elements.
+template <int V, class F>
+__device__ __forceinline__ void for_channels(const Geometry& g, int col, F&& f) {
+    int c = (int)((unsigned)(col * V) % (unsigned)g.C), group = (int)((unsigned)c / (unsigned)g.width), next = (group + 1) * g.width;
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        f(e, c, group);
+        c++;
+        if (c == next) {
+            group++;
+            next += g.width;
+        }
+        if (c == g.C) {
+            c = 0;
+            group = 0;
+            next = g.width;
+        }
+    }
+}
+
 template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
     constexpr int V = 16 / sizeof(T);
@@ -203,12 +223,10 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
         const T* dy = static_cast<const T*>(a.dy) + p.slice * n;
         Chan k[BACK ? V : 1];
         if constexpr (BACK) {
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                const int c = (p.col * V + e) % a.g.C;
-                const double2 st = a.stats_in[p.slice * a.g.G + c / a.g.width];
+            for_channels<V>(a.g, p.col, [&](int e, int c, int g) {
+                const double2 st = a.stats_in[p.slice * a.g.G + g];
                 k[e].set(a, st.x, st.y, c);
-            }
+            });
         }
         std::conditional_t<BACK, float, double> s1[V] = {}, s2[V] = {};
         int held = 0;
@@ -256,7 +274,13 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
     fold_rows(red, a.g.rws, width);
     if constexpr (BACK) {
         double2* slot = a.slot + (p.slice * a.g.chunks + p.chunk) * a.g.slots + first;
-        for (int i = (int)threadIdx.x; i < here; i += kThreads) slot[i] = red[i];
+        for (int i = (int)threadIdx.x; i < here; i += kThreads) {
+            const double2 v = red[i];
+            slot[i] = v;
+            const double w = a.w ? (double)a.w[(unsigned)(first + i) % (unsigned)a.g.C] : 1.0;
+            red[i] = make_double2(v.x * w, v.y * w);
+        }
+        __syncthreads();
     }
     // A group's slots: one run in each of the super-row's R rows. Wide groups by a wave each, narrow
     // ones by a thread.
@@ -268,9 +292,8 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
         for (int r = 0; r < a.g.R; r++) {
             const int row = r * a.g.C - first, lo = max(0, row + g * a.g.width), hi = min(here, row + min((g + 1) * a.g.width, a.g.C));
             for (int i = lo + lane; i < hi; i += lanes) {
-                const double w = BACK && a.w ? (double)a.w[i - row] : 1.0;
-                s.x = fma(red[i].x, w, s.x);
-                s.y = fma(red[i].y, w, s.y);
+                s.x += red[i].x;
+                s.y += red[i].y;
             }
         }
         if (wide) {
@@ -360,9 +383,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
     const T* dy = static_cast<const T*>(a.dy) + p.slice * n;
     T* out = static_cast<T*>(a.out) + p.slice * n;
     Chan k[V];
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-        const int c = (p.col * V + e) % a.g.C, g = c / a.g.width;
+    for_channels<V>(a.g, p.col, [&](int e, int c, int g) {
         if constexpr (BACK) {
             const double2 st = a.stats_in[p.slice * a.g.G + g];
             k[e].set(a, st.x, st.y, c);
@@ -370,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
         } else {
             k[e].set(a, groups[g].x, groups[g].y, c);
         }
-    }
+    });
     for_rows(p, a.g.rws, [&](long long r, auto batch, auto whole) {
         constexpr int N = batch();
         Pack<T, V> f[N], g[BACK ? N : 1];

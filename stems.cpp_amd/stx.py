@@ -7,6 +7,7 @@ loading it raises.
 """
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libstx.so")
@@ -1138,58 +1139,62 @@ def rope_params(n_dims, mode=0, freq_factors=None, freq_base=10000.0, freq_scale
     return p
 
 
+_TENSOR = struct.Struct("P8q")                       # stx_tensor: data, ne[4], nb[4]
+_types = {}                                         # torch dtype -> (stx_type, bytes)
+
+
 def _type(t):
-    import torch
+    if not _types:
+        import torch
+        _types.update({torch.float32: (TYPE_F32, 4), torch.float16: (TYPE_F16, 2), torch.bfloat16: (TYPE_BF16, 2)})
     try:
-        return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}[t.dtype]
+        return _types[t.dtype][0]
     except KeyError:
         raise TypeError(f"operands must be float32, float16 or bfloat16, got {t.dtype}") from None
 
 
 def _typed(t, like, what):
-    """stx_tensor of a tensor of up to 4 dims with the element type and device of `like`."""
-    if t.dtype != like.dtype:
+    """stx_tensor (packed) of a tensor of up to 4 dims with the element type and device of `like`."""
+    if t.dtype is not like.dtype:
         raise TypeError(f"{what} must be {like.dtype}, got {t.dtype}")
-    if t.device != like.device or not t.is_cuda:
+    if not t.is_cuda or t.device != like.device:
         raise ValueError(f"{what} must be a CUDA (HIP) tensor on {like.device}")
-    size, n = t.element_size(), t.dim()
+    shape, stride, size = t.shape, t.stride(), t.element_size()
+    n = len(shape)
     if n > 4:
         raise ValueError(f"{what} has more than 4 dimensions")
-    shape, strides = t.shape, t.stride()
-    d = Tensor()
-    d.data = t.data_ptr()
-    at = size
-    for i in range(4):
-        e = shape[n - 1 - i] if i < n else 1
-        d.ne[i] = e
-        d.nb[i] = at if e == 1 else size * strides[n - 1 - i]
-        at = d.nb[i] * e
-    return d
+    if n < 4:
+        shape = (1,) * (4 - n) + tuple(shape)
+        stride = (shape[4 - n] * stride[0] if n else 1,) * (4 - n) + stride
+    d, c, b, a = shape
+    w, z, y, x = stride
+    return _TENSOR.pack(t.data_ptr(), a, b, c, d, size if a == 1 else size * x, size * y, size * z, size * w)
 
 
 def _floats(t, like, count, what, dtype=None):
     """Pointer of a contiguous float32 (or dtype) vector of `count` values on like's device, or None."""
     if t is None:
         return None
-    import torch
-    _require(t, dtype or torch.float32, what)
-    if t.device != like.device:
-        raise ValueError(f"{what} must be on {like.device}")
-    if t.numel() != count:
-        raise ValueError(f"{what} must have {count} values, has {t.numel()}")
+    if dtype is None:
+        import torch
+        dtype = torch.float32
+    if t.dtype is not dtype or t.device != like.device or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{what} must be {count} contiguous {dtype} values on {like.device}, is {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
 def _launch(fn, like, stream, *args):
     """fn(*args, stream) with like's device current, on `stream` (default: that device's current stream)."""
     import torch
-    if like.device.index == torch.cuda.current_device():
-        s = stream if stream is not None else torch.cuda.current_stream()
-        check(fn(*args, s.cuda_stream))
-        return
-    with torch.cuda.device(like.device):
-        s = stream if stream is not None else torch.cuda.current_stream()
-        check(fn(*args, s.cuda_stream))
+    index = like.device.index
+    s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, s)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, s)
+    if status:
+        check(status)
 
 
 def _scratch(need, workspace, like, stream):
@@ -1197,29 +1202,29 @@ def _scratch(need, workspace, like, stream):
     return is not handed to another stream while the call still uses it); and the tensor that owns it."""
     if workspace is None:
         import torch
-        with torch.cuda.stream(stream):              # None: the current stream
+        if stream is None:
             workspace = torch.empty(max(256, need), dtype=torch.uint8, device=like.device)
+        else:
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(max(256, need), dtype=torch.uint8, device=like.device)
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 def _rope_scaled(fn, q, pos, params, k, out, k_out, stream):
     import torch
-    if pos.dtype != torch.int32 or pos.device != q.device or (pos.dim() > 0 and pos.numel() > 1 and pos.stride(-1) != 1):
-        raise TypeError("pos must be an int32 tensor on the queries' device with contiguous rows")
-    if q.dim() > 4 or q.dim() < 3:
+    shape = q.shape
+    if len(shape) not in (3, 4):
         raise ValueError("q must be (batch, tokens, heads, head size) or (tokens, heads, head size)")
-    batch, n = (q.shape[0] if q.dim() == 4 else 1), q.shape[-3]
-    if tuple(pos.shape) not in ((n,), (batch, n)):
-        raise ValueError(f"pos must be ({n},) or ({batch}, {n}), is {tuple(pos.shape)}")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    dq, do = _typed(q, q, "q"), _typed(out, q, "out")
+    batch, n = (shape[0] if len(shape) == 4 else 1), shape[-3]
+    if pos.dtype is not torch.int32 or pos.device != q.device or tuple(pos.shape) not in ((n,), (batch, n)) or (n > 1 and pos.stride(-1) != 1):
+        raise ValueError(f"pos must be ({n},) or ({batch}, {n}) int32 with contiguous rows on {q.device}, is {tuple(pos.shape)} {pos.dtype}")
+    out = q.new_empty(q.shape) if out is None else out
     dk = dko = None
     if k is not None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        k_out = k.new_empty(k.shape) if k_out is None else k_out
         dk, dko = _typed(k, q, "k"), _typed(k_out, q, "k_out")
-    ref = lambda d: None if d is None else ctypes.byref(d)  # noqa: E731
-    _launch(fn, q, stream, ref(dq), ref(dk), _type(q), pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0,
-            ctypes.byref(params), ref(do), ref(dko))
+    _launch(fn, q, stream, _typed(q, q, "q"), dk, _type(q), pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0,
+            ctypes.byref(params), _typed(out, q, "out"), dko)
     return out if k is None else (out, k_out)
 
 
@@ -1235,16 +1240,13 @@ def rope_scaled_back(q, pos, params, k=None, out=None, k_out=None, stream=None):
     return _rope_scaled(lib().stx_rope_scaled_back, q, pos, params, k, out, k_out, stream)
 
 
-def _slices(t, like, what):
-    """stx_tensor [C, T1, T2, B] of a (B, T1, T2, C), (B, T, C) or (T, C) tensor."""
-    d = _typed(t, like, what)
-    if t.dim() == 3:                                # ggml order [C, T, B]: B moves to ne3
-        d.ne[2], d.ne[3], d.nb[3], d.nb[2] = 1, d.ne[2], d.nb[2], d.nb[1] * d.ne[1]
-    return d
+def _slices(t):
+    """(B, T1, T2, C) view of a (B, T1, T2, C), (B, T, C) or (T, C) tensor."""
+    return t.unsqueeze(1) if t.dim() == 3 else t
 
 
 def group_norm_cl_workspace_size(x, n_groups):
-    return lib().stx_group_norm_cl_workspace_size(ctypes.byref(_slices(x, x, "x")), _type(x), int(n_groups))
+    return lib().stx_group_norm_cl_workspace_size(_typed(_slices(x), x, "x"), _type(x), int(n_groups))
 
 
 def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, out=None, stats=None, workspace=None,
@@ -1253,17 +1255,16 @@ def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, o
     weight and bias: float32 device (C,) or None. Returns (out, stats): stats is float64 (B, n_groups, 2), mean and
     1 / sqrt(var + eps), for group_norm_cl_back. out may be x."""
     import torch
-    out = _out(out, x)
-    dx, do = _slices(x, x, "x"), _slices(out, x, "out")
-    C, B = dx.ne[0], dx.ne[3]
+    out = x.new_empty(x.shape) if out is None else out
+    v = _slices(x)
+    dx, t, L = _typed(v, x, "x"), _type(x), lib()
+    C, B = v.shape[-1], v.shape[0] if v.dim() == 4 else 1
     if stats is None:
         stats = torch.empty((B, n_groups, 2), dtype=torch.float64, device=x.device)
-    w, b = _floats(weight, x, C, "weight"), _floats(bias, x, C, "bias")
-    s = _floats(stats, x, B * n_groups * 2, "stats", torch.float64)
-    L, t = lib(), _type(x)
-    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(ctypes.byref(dx), t, int(n_groups)), workspace, x, stream)
-    _launch(L.stx_group_norm_cl, x, stream, ctypes.byref(dx), t, int(n_groups), float(eps), w, b, int(act),
-            ctypes.byref(do), s, ws, nbytes)
+    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(dx, t, int(n_groups)), workspace, x, stream)
+    _launch(L.stx_group_norm_cl, x, stream, dx, t, int(n_groups), float(eps), _floats(weight, x, C, "weight"),
+            _floats(bias, x, C, "bias"), int(act), _typed(_slices(out), x, "out"),
+            _floats(stats, x, B * n_groups * 2, "stats", torch.float64), ws, nbytes)
     return out, stats
 
 
@@ -1271,16 +1272,16 @@ def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_N
                        workspace=None, stream=None):
     """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy."""
     import torch
-    dx = _out(dx, x)
-    da, dd, do = _slices(x, x, "x"), _slices(dy, x, "dy"), _slices(dx, x, "dx")
-    C, B = da.ne[0], da.ne[3]
+    dx = x.new_empty(x.shape) if dx is None else dx
+    v = _slices(x)
+    da, t, L = _typed(v, x, "x"), _type(x), lib()
+    C, B = v.shape[-1], v.shape[0] if v.dim() == 4 else 1
     dweight = torch.empty(C, dtype=torch.float32, device=x.device) if dweight is None else dweight
     dbias = torch.empty(C, dtype=torch.float32, device=x.device) if dbias is None else dbias
-    L, t = lib(), _type(x)
-    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(ctypes.byref(da), t, int(n_groups)), workspace, x, stream)
-    _launch(L.stx_group_norm_cl_back, x, stream, ctypes.byref(dd), ctypes.byref(da), t,
+    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(da, t, int(n_groups)), workspace, x, stream)
+    _launch(L.stx_group_norm_cl_back, x, stream, _typed(_slices(dy), x, "dy"), da, t,
             _floats(stats, x, B * n_groups * 2, "stats", torch.float64), int(n_groups), _floats(weight, x, C, "weight"),
-            _floats(bias, x, C, "bias"), int(act), ctypes.byref(do), _floats(dweight, x, C, "dweight"),
+            _floats(bias, x, C, "bias"), int(act), _typed(_slices(dx), x, "dx"), _floats(dweight, x, C, "dweight"),
             _floats(dbias, x, C, "dbias"), ws, nbytes)
     return dx, dweight, dbias
 
@@ -1288,13 +1289,11 @@ def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_N
 def gated_ff(x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=None, out=None, stream=None):
     """act(x @ w_gate.T + b_gate) * (x @ w_value.T + b_value): x (..., K) of up to 4 dims, weights (N, K), biases
     float32 (N,) or None; out (..., N)."""
-    import torch
     N = w_gate.shape[0]
     if out is None:
-        out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-    dx, dg, dv, do = (_typed(t, x, n) for t, n in ((x, "x"), (w_gate, "w_gate"), (w_value, "w_value"), (out, "out")))
-    _launch(lib().stx_gated_ff, x, stream, ctypes.byref(dx), ctypes.byref(dg), ctypes.byref(dv), _type(x),
-            _floats(b_gate, x, N, "b_gate"), _floats(b_value, x, N, "b_value"), int(act), ctypes.byref(do))
+        out = x.new_empty((*x.shape[:-1], N))
+    _launch(lib().stx_gated_ff, x, stream, _typed(x, x, "x"), _typed(w_gate, x, "w_gate"), _typed(w_value, x, "w_value"),
+            _type(x), _floats(b_gate, x, N, "b_gate"), _floats(b_value, x, N, "b_value"), int(act), _typed(out, x, "out"))
     return out
 
 
@@ -1319,11 +1318,10 @@ def gated_ff_back(dh, x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=
         db_value = torch.empty(N, dtype=torch.float32, device=dev)
     d = [_typed(t, x, n) for t, n in ((dh, "dh"), (x, "x"), (w_gate, "w_gate"), (w_value, "w_value"), (dx, "dx"),
                                       (dw_gate, "dw_gate"), (dw_value, "dw_value"))]
-    r = [ctypes.byref(t) for t in d]
     L, t = lib(), _type(x)
     tokens = x.numel() // max(1, K)
     ws, nbytes, keep = _scratch(L.stx_gated_ff_back_workspace_size(tokens, K, N, t), workspace, x, stream)
-    _launch(L.stx_gated_ff_back, x, stream, r[0], r[1], r[2], r[3], t, _floats(b_gate, x, N, "b_gate"),
-            _floats(b_value, x, N, "b_value"), int(act), r[4], r[5], r[6], _floats(db_gate, x, N, "db_gate"),
+    _launch(L.stx_gated_ff_back, x, stream, d[0], d[1], d[2], d[3], t, _floats(b_gate, x, N, "b_gate"),
+            _floats(b_value, x, N, "b_value"), int(act), d[4], d[5], d[6], _floats(db_gate, x, N, "db_gate"),
             _floats(db_value, x, N, "db_value"), ws, nbytes)
     return dx, dw_gate, dw_value, db_gate, db_value

@@ -482,7 +482,6 @@ def test_gated_ff_nonfinite_rows_stay_rows(device):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_gated_ff_partial_gradients(device, dtype):
     """Only some of the outputs through the C ABI: the same bits as with all of them."""
-    import ctypes
     M, K, N, dt = 150, 48, 40, TYPES[dtype]
     x, dh = randn(device, (M, K), 61, dtype=dt), randn(device, (M, N), 62, dtype=dt)
     wg, wv = (randn(device, (N, K), 63 + i, 0.2, dtype=dt) for i in range(2))
@@ -493,9 +492,9 @@ def test_gated_ff_partial_gradients(device, dtype):
         out = [torch.empty_like(t) for t in full]
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         d = [stx._typed(t, x, "t") for t in (dh, x, wg, wv)]
-        o = [ctypes.byref(stx._typed(out[i], x, "o")) if i in pick else None for i in range(3)]
+        o = [stx._typed(out[i], x, "o") if i in pick else None for i in range(3)]
         f = [out[i].data_ptr() if i in pick else None for i in (3, 4)]
-        stx.check(stx.lib().stx_gated_ff_back(*map(ctypes.byref, d), stx._type(x), bg.data_ptr(), bv.data_ptr(), stx.ACT_GELU, *o, *f,
+        stx.check(stx.lib().stx_gated_ff_back(*d, stx._type(x), bg.data_ptr(), bv.data_ptr(), stx.ACT_GELU, *o, *f,
                                               ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
         for i in pick:
             assert torch.equal(out[i], full[i]), i
