@@ -9,7 +9,7 @@
 namespace stx {
 namespace {
 
-// One slice (ne3 index) is [T][C], dense. Threads move 16-byte vectors of V elements; so that a
+// One slice (ne3 index) is [T][C], dense. Threads move vectors of V elements; so that a
 // thread meets the same channels in every vector it takes whatever C is, the slice is walked in
 // super-rows of R = V / gcd(C, V) rows, which hold a whole number of vectors: vector j of a
 // super-row covers channels (j V + e) mod C. Accesses may be unaligned (odd C, odd slices); only
@@ -27,7 +27,8 @@ namespace {
 // summed in double, since E[x^2] - mean^2 cancels; the backward sums in float over kHeld rows
 // of a thread (64 terms drift by about 1e-7 of their sum), then in double. Both passes are bound by HBM, the second by what the last-level cache still holds.
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;                // super-rows a thread has in flight
+constexpr int kVec = 4;                  // elements of a vector: with 8 of 16 bits a channel's constants leave four waves a SIMD
+constexpr int kBatch = 2;                // super-rows a thread has in flight
 constexpr int kHeld = 64;                // rows summed in float before they join the sums in double
 constexpr int kDirect = 2048;            // pairs that every apply block adds by itself
 constexpr int kParamChannels = 8;        // of a block that adds dweight and dbias: 32 lanes a channel
@@ -41,14 +42,14 @@ struct Geometry {
     long long srows, chunk_srows;        // super-rows of a slice, of a chunk
 };
 
-Geometry geometry(const stx_tensor* a, int size, int n_groups) {
+Geometry geometry(const stx_tensor* a, int n_groups) {
     Geometry g{};
     g.C = (int)a->ne[0];
     g.T = a->ne[1] * a->ne[2];
     g.B = a->ne[3];
     g.G = n_groups;
     g.width = (g.C + n_groups - 1) / n_groups;
-    g.V = 16 / size;
+    g.V = kVec;
     g.R = g.V / std::gcd(g.C, g.V);
     g.slots = g.C * g.R;
     g.ncol = g.slots / g.V;
@@ -66,10 +67,10 @@ Geometry geometry(const stx_tensor* a, int size, int n_groups) {
     g.tiles = (g.ncol + g.cols - 1) / g.cols;
     g.rws = kThreads / g.cols;
     g.srows = (g.T + g.R - 1) / g.R;
-    // Chunks: enough blocks for four a CU, each of at least one batch of its threads' rows.
-    const long long most = std::max(1LL, std::min(1024 / std::max(1LL, g.B * g.tiles), g.srows / (kBatch * g.rws)));
-    const long long batch = kBatch * g.rws;
-    g.chunk_srows = std::max(1LL, ((g.srows + most - 1) / most + batch - 1) / batch) * batch;
+    // Chunks: four blocks a CU, all resident at once and none more than the others (840 blocks took as
+    // long as 1,020 that do a fifth more between them), each of at least four super-rows a thread.
+    const long long most = std::max(1LL, std::min(1024 / std::max(1LL, g.B * g.tiles), g.srows / (4 * g.rws)));
+    g.chunk_srows = std::max(1LL, (g.srows + most - 1) / most);
     g.chunks = (int)std::max(1LL, (g.srows + g.chunk_srows - 1) / g.chunk_srows);
     return g;
 }
@@ -140,15 +141,33 @@ __device__ __forceinline__ Place place(const NormArgs& a, unsigned bid) {
     return p;
 }
 
-// f(r, batch) over a thread's super-rows, kBatch of them at a time: their loads are in flight together.
-// whole: every vector of the batch exists in full.
-template <class F>
-__device__ __forceinline__ void for_rows(const Place& p, int rws, F&& f) {
+// use(r, whole, load(r, whole)) over a thread's super-rows, kBatch of them at a time, the next batch's
+// loads issued before the last one's are used. whole: every vector exists in full.
+template <class L, class F>
+__device__ __forceinline__ void for_rows(const Place& p, int rws, L&& load, F&& use) {
+    constexpr std::integral_constant<int, kBatch> batch{};
+    constexpr std::integral_constant<int, 1> one{};
     long long r = p.begin + p.row;
-    const long long end = min(p.end, p.full);
-    for (; r + (kBatch - 1) * rws < end; r += kBatch * rws) f(r, std::integral_constant<int, kBatch>{}, std::true_type{});
-    for (; r < p.end; r += rws) f(r, std::integral_constant<int, 1>{}, std::false_type{});
+    const long long end = min(p.end, p.full), ahead = (kBatch - 1) * rws, step = kBatch * rws;
+    if (r + ahead < end) {
+        auto now = load(r, batch, std::true_type{});
+        for (; r + step + ahead < end; r += step) {
+            const auto next = load(r + step, batch, std::true_type{});
+            use(r, batch, std::true_type{}, now);
+            now = next;
+        }
+        use(r, batch, std::true_type{}, now);
+        r += step;
+    }
+    for (; r < end; r += rws) use(r, one, std::true_type{}, load(r, one, std::true_type{}));
+    if (r < p.end) use(r, one, std::false_type{}, load(r, one, std::false_type{}));
 }
+
+// N vectors of x, and of dy in the backward pass.
+template <class T, int V, int N, bool BACK>
+struct Rows {
+    Pack<T, V> x[N], dy[BACK ? N : 1];
+};
 
 // Sum of red[rows][width] over the rows, into red[0][]. All threads; the order depends on the shape alone.
 __device__ __forceinline__ void fold_rows(double2* red, int rows, int width) {
@@ -208,7 +227,7 @@ __device__ __forceinline__ void for_channels(const Geometry& g, int col, F&& f) 
 
 template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = kVec;
     __shared__ double2 red[kThreads * V];
     const Place p = place(a, blockIdx.x);
     const int width = a.g.cols * V, first = p.tile * width, here = min(width, a.g.slots - first);
@@ -233,34 +252,39 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
         auto flush = [&] {
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                mine[e] = make_double2(mine[e].x + (double)s1[e], mine[e].y + (double)s2[e]);
+                double t1 = (double)s1[e], t2 = (double)s2[e];
+                if constexpr (BACK) t2 = fma(t2, (double)k[e].r, -t1 * (double)k[e].d);   // from dz t to dz xhat
+                mine[e] = make_double2(mine[e].x + t1, mine[e].y + t2);
                 s1[e] = s2[e] = 0;
             }
             held = 0;
         };
-        for_rows(p, a.g.rws, [&](long long r, auto batch, auto whole) {
-            constexpr int N = batch();
-            Pack<T, V> f[N], g[BACK ? N : 1];
+        auto load = [&](long long r, auto batch, auto whole) {
+            Rows<T, V, batch(), BACK> f;
 #pragma unroll
-            for (int i = 0; i < N; i++) {
+            for (int i = 0; i < batch(); i++) {
                 const long long at = (r + i * a.g.rws) * a.g.slots + (long long)p.col * V, left = whole() ? V : n - at;
-                f[i] = load_vec<T, V>(x + at, left);
-                if constexpr (BACK) g[i] = load_vec<T, V>(dy + at, left);
+                f.x[i] = load_vec<T, V>(x + at, left);
+                if constexpr (BACK) f.dy[i] = load_vec<T, V>(dy + at, left);
             }
+            return f;
+        };
+        for_rows(p, a.g.rws, load, [&](long long r, auto batch, auto whole, const auto& f) {
+            constexpr int N = batch();
             const long long left = whole() ? V : n - r * a.g.slots - (long long)p.col * V;
 #pragma unroll
             for (int i = 0; i < N; i++) {
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     if (!whole() && e >= left) continue;
-                    const float xe = to_f32(f[i].v[e]);
+                    const float xe = to_f32(f.x[i].v[e]);
                     if constexpr (BACK) {
                         const float t = xe - k[e].mh;
                         float d;
                         (void)act_f32<ACT>(fmaf(t, k[e].A, k[e].B), d);
-                        const float dz = to_f32(g[i].v[e]) * d;
+                        const float dz = to_f32(f.dy[i].v[e]) * d;
                         s1[e] += dz;
-                        s2[e] = fmaf(dz, fmaf(t, k[e].r, -k[e].d), s2[e]);
+                        s2[e] = fmaf(dz, t, s2[e]);
                     } else {
                         s1[e] += (double)xe;
                         s2[e] = fma((double)xe, (double)xe, s2[e]);
@@ -348,7 +372,7 @@ __device__ void add_params(const NormArgs& a, double2* red, unsigned block) {
 
 template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = kVec;
     extern __shared__ double2 groups[];                  // [max(G, kThreads)]
     if (BACK && blockIdx.x < a.first) return add_params(a, groups, blockIdx.x);
     const Place p = place(a, blockIdx.x - a.first);
@@ -392,26 +416,29 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
             k[e].set(a, groups[g].x, groups[g].y, c);
         }
     });
-    for_rows(p, a.g.rws, [&](long long r, auto batch, auto whole) {
-        constexpr int N = batch();
-        Pack<T, V> f[N], g[BACK ? N : 1];
+    auto load = [&](long long r, auto batch, auto whole) {
+        Rows<T, V, batch(), BACK> f;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < batch(); i++) {
             const long long at = (r + i * a.g.rws) * a.g.slots + (long long)p.col * V, left = whole() ? V : n - at;
-            f[i] = load_vec<T, V>(x + at, left);
-            if constexpr (BACK) g[i] = load_vec<T, V>(dy + at, left);
+            f.x[i] = load_vec<T, V>(x + at, left);
+            if constexpr (BACK) f.dy[i] = load_vec<T, V>(dy + at, left);
         }
+        return f;
+    };
+    for_rows(p, a.g.rws, load, [&](long long r, auto batch, auto whole, const auto& f) {
+        constexpr int N = batch();
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const long long at = (r + i * a.g.rws) * a.g.slots + (long long)p.col * V, left = whole() ? V : n - at;
             float y[V];
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                const float t = to_f32(f[i].v[e]) - k[e].mh, z = fmaf(t, k[e].A, k[e].B);
+                const float t = to_f32(f.x[i].v[e]) - k[e].mh, z = fmaf(t, k[e].A, k[e].B);
                 if constexpr (BACK) {
                     float d;
                     (void)act_f32<ACT>(z, d);
-                    y[e] = fmaf(t, k[e].q, fmaf(to_f32(g[i].v[e]) * d, k[e].A, k[e].p));
+                    y[e] = fmaf(t, k[e].q, fmaf(to_f32(f.dy[i].v[e]) * d, k[e].A, k[e].p));
                 } else {
                     y[e] = act_f32<ACT>(z);
                 }
@@ -447,7 +474,7 @@ Geometry check_norm(const stx_tensor* a, stx_type type, int n_groups) {
     STX_REQUIRE((n_groups - 1LL) * ((C + n_groups - 1) / n_groups) < C, "group_norm_cl: %lld channels leave a group of %d empty", C,
                 n_groups);
     if (n_groups > kMaxGroups) fail(STX_STATUS_UNSUPPORTED, "group_norm_cl: more than %d groups", kMaxGroups);
-    const Geometry g = geometry(a, size, n_groups);
+    const Geometry g = geometry(a, n_groups);
     STX_REQUIRE(g.B < (1LL << 31) && g.B * g.chunks * g.tiles < (1LL << 30) && g.B * g.G < (1LL << 31), "group_norm_cl: too many slices");
     return g;
 }
