@@ -33,29 +33,25 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 acc, bf16) {
 // x - h, l the rest, all exact (8 bits each of the 24). A product of two such sums without its
 // three smallest terms, which are below 2^-23 of it together, is six bf16 products: 2.7 times the rate
 // of the fp32 matrix instruction, at its accuracy. An infinity's rest is inf - inf: NaN.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 struct Split {
-    u32x4 h, m, l;                       // 8 values a lane, as bf16
-    __device__ __forceinline__ void set(u32x4 a, u32x4 b) {
+    u32x2 part[3];                       // four values' h, m, l as bf16
+    __device__ __forceinline__ explicit Split(u32x4 x) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const unsigned x0 = i < 2 ? a[2 * i] : b[2 * i - 4], x1 = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
-            const float r0 = rest(x0), r1 = rest(x1);
-            const unsigned y0 = __float_as_uint(r0), y1 = __float_as_uint(r1);
-            h[i] = upper(x0, x1);
-            m[i] = upper(y0, y1);
-            l[i] = upper(__float_as_uint(rest(y0)), __float_as_uint(rest(y1)));
+        for (int k = 0; k < 3; k++) {
+            part[k] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(x[i] & 0xffff0000u));
         }
     }
-    static __device__ __forceinline__ float rest(unsigned x) { return __uint_as_float(x) - __uint_as_float(x & 0xffff0000u); }
-    static __device__ __forceinline__ unsigned upper(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 };
-__device__ __forceinline__ f32x4 mma(const Split& a, const Split& b, f32x4 acc) {
-    acc = mma(a.l, b.h, acc, bf16{});
-    acc = mma(a.h, b.l, acc, bf16{});
-    acc = mma(a.m, b.m, acc, bf16{});
-    acc = mma(a.m, b.h, acc, bf16{});
-    acc = mma(a.h, b.m, acc, bf16{});
-    return mma(a.h, b.h, acc, bf16{});
+__device__ __forceinline__ f32x4 mma(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x4 acc) {   // smallest terms first
+    acc = mma(a[2], b[0], acc, bf16{});
+    acc = mma(a[0], b[2], acc, bf16{});
+    acc = mma(a[1], b[1], acc, bf16{});
+    acc = mma(a[1], b[0], acc, bf16{});
+    acc = mma(a[0], b[1], acc, bf16{});
+    return mma(a[0], b[0], acc, bf16{});
 }
 
 // The products of the block, all of the form out[m][j] = sum_r P(j, r) Q(m, r):
@@ -174,82 +170,90 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// An operand's tile of X rows (or columns) in a stage of LDS. Plain: [X][CH] chunks, chunk c of row x
-// at c ^ (x % 8), so that eight rows which a fragment reads together lie in different banks. Strided: rows of
-// the reduction, [CH E][X / E] chunks, chunk c of row r at c ^ turn(r), so that the rows which
-// one read takes (4 rows of 32 bytes for the transposing 16-bit read, 4 of 64 bytes in
-// fp32) do.
-template <class T, int X>
+// An operand's tile of X rows (or columns) of 16-bit values in a stage of LDS. Plain: [X][PER] chunks
+// of 8 values, chunk c of row x at c ^ bend(x), so that eight rows which a fragment reads together
+// lie in different banks. Strided: rows of the reduction, [8 PER][X / 8] chunks, chunk c of row r at
+// c ^ turn(r), so that the 4 rows of 32 bytes which the transposing read takes do. A 16-bit
+// operand is fetched in this form (PER 8: a step of 64); an fp32 one is split on its way into three
+// planes of it (PER 4: a step of 32).
+template <int PER>
+__device__ __forceinline__ int bend(int x) {
+    return PER == 8 ? x % 8 : x / 2 % 4;
+}
+template <int X>
 __device__ __forceinline__ int turn(int r) {
-    constexpr int E = 16 / sizeof(T), CHUNKS = X / E;
-    return (sizeof(T) == 2 ? 2 * (r % 4 + r / 8 % 2 * 4) : 4 * (r / 4 % 4)) % CHUNKS;
+    return 2 * (r % 4 + r / 8 % 2 * 4) % (X / 8);
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// Fragments of N 16-row tiles from `first` on, for lane l: the chunk of row l % 16 at position l / 16
-// of group kk (see mma).
-template <class T, int X, int N, bool STRIDED>
+// Fragments of 16-row tiles from `first` on, for lane l: the chunk of row l % 16 at position l / 16 of
+// group kk (see mma).
+template <int X, int N, int PER, bool STRIDED>
 struct Fragments {
     int at[STRIDED ? N : 1];
     __device__ __forceinline__ Fragments(int lane, int first) {
-        constexpr int E = 16 / sizeof(T);
         const int s = lane % 16, q = lane / 16;
         if constexpr (!STRIDED) {
-            at[0] = (first * 16 + s) * CH * 16 + (q ^ s % 8) * 16;
-        } else if constexpr (sizeof(T) == 2) {                       // lane s reads row s / 4, columns 4 (s % 4) .. + 3
+            at[0] = (first * 16 + s) * PER * 16 + (q ^ bend<PER>(s)) * 16;
+        } else {                                         // lane s reads row s / 4, columns 4 (s % 4) .. + 3
             const int row = q * 8 + s / 4;
 #pragma unroll
-            for (int i = 0; i < N; i++) at[i] = row * X * 2 + (((first + i) * 2 + s % 4 / 2) ^ turn<T, X>(row)) * 16 + s % 2 * 8;
-        } else {
-            const int row = q * 4;
-#pragma unroll
-            for (int i = 0; i < N; i++) at[i] = row * X * 4 + (((first + i) * 4 + s / 4) ^ turn<T, X>(row)) * 16 + s % 4 * 4;
+            for (int i = 0; i < N; i++) at[i] = row * X * 2 + (((first + i) * 2 + s % 4 / 2) ^ turn<X>(row)) * 16 + s % 2 * 8;
         }
-        (void)E;
     }
     __device__ __forceinline__ u32x4 read(const char* lds, int kk, int i) const {
         u32x4 f;
         if constexpr (!STRIDED) {
-            f = *reinterpret_cast<const u32x4*>(lds + i * 256 * CH + (at[0] ^ (kk * 64)));
-        } else if constexpr (sizeof(T) == 2) {
+            f = *reinterpret_cast<const u32x4*>(lds + i * 256 * PER + (at[0] ^ (kk * 64)));
+        } else {
             s16x4 h[2];
 #pragma unroll
             for (int e = 0; e < 2; e++)
                 h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at[i] + (kk * 32 + e * 4) * X * 2));
             __builtin_memcpy(&f, h, 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) f[e] = *reinterpret_cast<const unsigned*>(lds + at[i] + (kk * 16 + e) * X * 4);
         }
         return f;
     }
 };
 
-// The chunks of an operand's tile that a thread fetches in a step.
+// The 16-byte chunks of an operand's tile that a thread fetches in a step: [X][8], strided [8 E][X / E].
 template <class T, int X, int NT, bool STRIDED>
 struct Source {
     static constexpr int E = 16 / sizeof(T), N = X * CH / NT, PER = STRIDED ? X / E : CH;   // chunks a thread; chunks a row
     static __device__ __forceinline__ int row(int i) { return (i * NT + (int)threadIdx.x) / PER; }
     static __device__ __forceinline__ int chunk(int i) {
-        return (i * NT + (int)threadIdx.x) % PER ^ (STRIDED ? turn<T, X>(row(i)) : row(i) % 8);
+        const int c = (i * NT + (int)threadIdx.x) % PER;
+        if constexpr (sizeof(T) == 4) return c;
+        else return c ^ (STRIDED ? turn<X>(row(i)) : bend<CH>(row(i)));
+    }
+    // fp32: where the four values of chunk i lie in a plane.
+    static __device__ __forceinline__ int spot(int i) {
+        const int r = row(i), c = chunk(i);
+        return (STRIDED ? r * X * 2 + ((c / 2) ^ turn<X>(r)) * 16 : r * 64 + ((c / 2) ^ bend<4>(r)) * 16) + c % 2 * 8;
     }
 };
 
 // Persistent blocks: each takes tiles of its XCD's share in turn, and the steps of all its tiles
 // form one stream: while the waves multiply one stage of LDS, the other is filled with the next
-// step, the next tile's first included (ALIGNED: straight from memory to LDS; otherwise through
-// registers, for any alignment and length).
+// step, the next tile's first included: straight from memory to LDS for aligned 16-bit operands
+// (ALIGNED), otherwise through registers, for any alignment and length. fp32 operands are split
+// between the registers and LDS, once a block (by every wave from its fragments, splitting took
+// longer than the products), and have one stage of three planes: two would leave room for one
+// block a CU.
 template <class T, int MODE, class C, bool ALIGNED>
 __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     constexpr int NT = C::NT, E = 16 / sizeof(T), TJ = C::TJ, TM = C::TM;
     constexpr int NJ = TJ / C::WJ / 16, NM = TM / C::WM / 16;       // 16 x 16 tiles of a wave
     constexpr bool GATED = MODE == FORWARD || MODE == GRAD, PS = !GATED, QS = MODE == DW;
     constexpr int WIDTH = GATED ? TJ / 2 : TJ;                       // output columns of a tile
-    constexpr int STAGE = (TJ + TM) * CH * 16;
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int PER = SPLIT ? 4 : CH, PLANES = SPLIT ? 3 : 1, STAGES = SPLIT ? 1 : 2, QAT = TJ * PER * 16 * PLANES;   // Q's place
+    constexpr int STAGE = (TJ + TM) * PER * 16 * PLANES;
+    static_assert(!(SPLIT && ALIGNED));
     using PSource = Source<T, TJ, NT, PS>;
     using QSource = Source<T, TM, NT, QS>;
-    __shared__ __align__(128) char lds[2][STAGE];
+    __shared__ __align__(128) char lds[STAGES][STAGE];
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int wj = wave / C::WM, wm = wave % C::WM;
@@ -322,6 +326,11 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 for (int i = 0; i < QSource::N; i++)
                     load_to_lds(r + (QS ? QSource::row(i) : QSource::chunk(i) * E) < a.RQ ? (const void*)(qb + qoff[i]) : (const void*)&zero_chunk, ql + i * NT * 16);
             }
+        } else if (r + CH * E <= a.RP && r + CH * E <= a.RQ && (!PS || t.j0 + TJ <= a.J)) {
+#pragma unroll
+            for (int i = 0; i < PSource::N; i++) __builtin_memcpy(&hold[i], pb + poff[i], 16);
+#pragma unroll
+            for (int i = 0; i < QSource::N; i++) __builtin_memcpy(&hold[PSource::N + i], qb + qoff[i], 16);
         } else {
 #pragma unroll
             for (int i = 0; i < PSource::N; i++)
@@ -337,7 +346,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     bool more = true;
     auto fetch_next = [&] {
         fetch(ft, fstep, fstage);
-        fstage ^= 1;
+        if constexpr (STAGES == 2) fstage ^= 1;
         if (++fstep == ft.end) {
             fid += stride;
             more = fid < last;
@@ -351,6 +360,15 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     auto settle = [&](int stage) {
         if constexpr (ALIGNED) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else if constexpr (SPLIT) {
+            __syncthreads();                             // the one stage is read
+#pragma unroll
+            for (int i = 0; i < PSource::N + QSource::N; i++) {
+                const Split v(hold[i]);
+                char* to = lds[0] + (i < PSource::N ? PSource::spot(i) : QAT + QSource::spot(i - PSource::N));
+#pragma unroll
+                for (int k = 0; k < 3; k++) *reinterpret_cast<u32x2*>(to + k * (i < PSource::N ? TJ : TM) * 64) = v.part[k];
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < PSource::N + QSource::N; i++)
@@ -359,8 +377,8 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         __syncthreads();
     };
 
-    const Fragments<T, TJ, NJ, PS> pf(lane, wj * NJ);
-    const Fragments<T, TM, NM, QS> qf(lane, wm * NM);
+    const Fragments<TJ, NJ, PER, PS> pf(lane, wj * NJ);
+    const Fragments<TM, NM, PER, QS> qf(lane, wm * NM);
     f32x4 acc[NJ][NM];
 
     // A wave's outputs leave 16 rows at a time. 16-bit results go through the wave's share of the
@@ -532,17 +550,20 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         for (int s = t.begin; s < t.end; s++) {
             settle(stage);                               // every wave is done with the stage before it, too
             if (more) fetch_next();
-            const char *pl = lds[stage], *ql = pl + TJ * CH * 16;
-            if constexpr (sizeof(T) == 4) {              // the step's two groups of 16 as one of 32
-                Split sq[NM];
+            const char *pl = lds[stage], *ql = pl + QAT;
+            if constexpr (SPLIT) {
+                u32x4 fq[NM][3];
 #pragma unroll
-                for (int m = 0; m < NM; m++) sq[m].set(qf.read(ql, 0, m), qf.read(ql, 1, m));
+                for (int m = 0; m < NM; m++)
+#pragma unroll
+                    for (int k = 0; k < 3; k++) fq[m][k] = qf.read(ql + k * TM * 64, 0, m);
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    Split sp;
-                    sp.set(pf.read(pl, 0, j), pf.read(pl, 1, j));
+                    u32x4 fp[3];
 #pragma unroll
-                    for (int m = 0; m < NM; m++) acc[j][m] = mma(sp, sq[m], acc[j][m]);
+                    for (int k = 0; k < 3; k++) fp[k] = pf.read(pl + k * TJ * 64, 0, j);
+#pragma unroll
+                    for (int m = 0; m < NM; m++) acc[j][m] = mma(fp, fq[m], acc[j][m]);
                 }
             } else {
 #pragma unroll
@@ -559,7 +580,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 }
             }
             share = lds[stage];
-            stage ^= 1;
+            if constexpr (STAGES == 2) stage ^= 1;
         }
         if constexpr (TAKES) {
 #pragma unroll
@@ -719,10 +740,10 @@ Plan plan_of(Mode mode, long long J, long long M, long long steps, int size) {
     const int w = mode == DW ? 2 : 1;
     Plan best{};
     double least = 0;
-    for (int k = mode == GRAD ? 1 : 0; k < 3; k++) {                 // Large has no registers for GRAD's epilogue: 460 us where Medium takes 250
+    for (int k = mode == GRAD || size == 4 ? 1 : 0; k < 3; k++) {    // Large has no registers for GRAD's epilogue: 460 us where Medium takes 250
         const Kind& c = kinds[k];
         const long long tiles = (J * (gated ? 2 : 1) + c.tj - 1) / c.tj * ((M + c.tm - 1) / c.tm) * w;
-        const double area = c.tj * (double)c.tm / 65536, step = area / c.rate[size == 4] * (size == 4 ? 7.1 : 0.95);   // us on a whole CU
+        const double area = c.tj * (double)c.tm / 65536, step = area / c.rate[size == 4] * (size == 4 ? 5.5 : 0.95);   // us on a whole CU
         for (int s = 1; s <= (gated ? 1 : 32) && (s == 1 || steps / s >= 4); s++) {
             const long long part = (steps + s - 1) / s, items = tiles * ((steps + part - 1) / part), rest = items % (kCus * c.slots);
             const long long k_rest = (rest + kCus - 1) / kCus;
@@ -751,10 +772,11 @@ void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
     launch_check("ff_kernel");
 }
 
-// Unaligned operands go through registers, which the large tile has none to spare of.
+// What goes through registers has no Large tile.
 template <class T, int MODE>
 void launch_ff(const FfArgs& a, bool aligned, int tile, int parts, hipStream_t stream) {
-    if (!aligned) tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
+    if constexpr (sizeof(T) == 4) return tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
+    else if (!aligned) tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
     else if (MODE != GRAD && tile == 0) launch_tiles<T, MODE == GRAD ? FORWARD : MODE, Large, true>(a, parts, stream);
     else if (tile == 1) launch_tiles<T, MODE, Medium, true>(a, parts, stream);
     else launch_tiles<T, MODE, Small, true>(a, parts, stream);
