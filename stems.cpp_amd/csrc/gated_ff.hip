@@ -388,7 +388,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     constexpr int COLS = GATED ? NJ * 8 : NJ * 16, CR = COLS / 8, AREA = 16 * COLS * 2, SHARE = STAGE / (NT / 64), PIECES = 16 * CR / 64;
     constexpr int AREAS = MODE == GRAD ? 2 : 1, TURNS = AREA * AREAS * 2 <= SHARE ? 2 : 1;   // areas of 16 rows; groups in turn
     static_assert(AREA * AREAS <= SHARE && PIECES >= 1 && 16 * CR % 64 == 0, "staging");
-    auto spot = [&](int row, int col) { return row * COLS * 2 + (col / 8 + row) % CR * 16 + col % 8 * 2; };
+    auto spot = [&](unsigned row, unsigned col) { return row * COLS * 2 + (col / 8 + row) % CR * 16 + col % 8 * 2; };
     auto pack = [&](char* p, const float (&f)[4]) {
         T v[4];
 #pragma unroll
@@ -398,14 +398,14 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     // The lane's number as a new value: addresses formed from it are not kept from one group of rows
     // for the next, there being no registers for them beside the accumulators.
     auto fresh = [&] {
-        int l = lane;
+        unsigned l = lane;
         asm volatile("" : "+v"(l));
         return l;
     };
-    auto flush = [&](int lane, const char* area, char* out, long long os, int row0, int col0) {
+    auto flush = [&](unsigned lane, const char* area, char* out, long long os, int row0, int col0) {
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            const int row = (i * 64 + lane) / CR, c = (i * 64 + lane) % CR * 8, left = a.jpad - col0 - c;
+            const int row = (int)((i * 64 + lane) / CR), c = (int)((i * 64 + lane) % CR * 8), left = a.jpad - col0 - c;
             const char* from = area + spot(row, c);
             char* to = out + (row0 + row) * os + (col0 + c) * (long long)sizeof(T);
             if (row0 + row >= a.M) continue;
@@ -420,23 +420,23 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     };
     constexpr bool WIDE = sizeof(T) == 2, TAKES = MODE == GRAD && WIDE;
     u32x4 dhv[TAKES ? NM : 1][TAKES ? PIECES : 1];       // the wave's part of dh
-    auto take = [&](int lane, const Item& t, int m) {
+    auto take = [&](unsigned lane, const Item& t, int m) {
         if constexpr (TAKES) {
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
-                const int row = t.m0 + (wm * NM + m) * 16 + (i * 64 + lane) / CR, col = t.j0 + wj * NJ * 8 + (i * 64 + lane) % CR * 8;
+                const int row = t.m0 + (wm * NM + m) * 16 + (int)((i * 64 + lane) / CR), col = t.j0 + wj * NJ * 8 + (int)((i * 64 + lane) % CR * 8);
                 dhv[m][i] = load_chunk<T>(a.dh + row * a.dhs + col * (long long)sizeof(T), row < a.M ? a.J - col : 0);
             }
         }
     };
 
-    auto gated = [&](const Item& t, char* share, auto act) {
+    auto gated = [&](const Item& t, char* share, auto act, auto whole) {
         const int nw = t.j0 + wj * NJ * 8;               // the wave's first column
         float sg[MODE == GRAD ? NJ / 2 : 1][4] = {}, sv[MODE == GRAD ? NJ / 2 : 1][4] = {};
 #pragma unroll
         for (int m = 0; m < NM; m++) {
-            const int lane = fresh();
-            const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + lane % 16;
+            const unsigned lane = fresh();
+            const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + (int)(lane % 16);
             char* area = share + m % TURNS * AREAS * AREA;
             if constexpr (TAKES) {
 #pragma unroll
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
             }
 #pragma unroll
             for (int j = 0; j < NJ; j += 2) {
-                const int col = j * 8 + lane / 16 * 4, n = nw + col;
+                const int col = j * 8 + (int)(lane / 16 * 4), n = nw + col;
                 char* here = area + spot(lane % 16, col);
                 if constexpr (MODE == FORWARD) {
                     float h[4];
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                     for (int r = 0; r < 4; r++) {
                         float d;
                         const float g = act_f32<act()>(acc[j][m][r], d);
-                        const bool in = row < a.M && n + r < a.J;    // what lies past the edges may be anything, NaN too
+                        const bool in = whole() || (row < a.M && n + r < a.J);   // what lies past the edges may be anything, NaN too
                         dg[r] = in ? dh[r] * acc[j + 1][m][r] * d : 0.f;
                         dv[r] = in ? dh[r] * g : 0.f;
                         sg[j / 2][r] += dg[r];
@@ -504,13 +504,13 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         float* part = a.part ? a.part + (long long)t.z * a.M * a.J : nullptr;
 #pragma unroll
         for (int m = 0; m < NM; m++) {
-            const int lane = fresh();
-            const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + lane % 16;
+            const unsigned lane = fresh();
+            const int row0 = t.m0 + (wm * NM + m) * 16, row = row0 + (int)(lane % 16);
             char* area = share + m % TURNS * AREA;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 const float f[4] = {acc[j][m][0], acc[j][m][1], acc[j][m][2], acc[j][m][3]};
-                const int c = j * 16 + lane / 16 * 4, col = jw + c;
+                const int c = j * 16 + (int)(lane / 16 * 4), col = jw + c;
                 if (part) {
                     if (row < a.M) store4<float>(reinterpret_cast<char*>(part + (long long)row * a.J + col), a.J - col, f);
                 } else if constexpr (WIDE) {
@@ -550,6 +550,12 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
         for (int s = t.begin; s < t.end; s++) {
             settle(stage);                               // every wave is done with the stage before it, too
             if (more) fetch_next();
+            if constexpr (TAKES) {
+                if (s + 1 == t.end) {
+#pragma unroll
+                    for (int m = 0; m < NM; m++) take(lane, t, m);
+                }
+            }
             const char *pl = lds[stage], *ql = pl + QAT;
             if constexpr (SPLIT) {
                 u32x4 fq[NM][3];
@@ -582,13 +588,14 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
             share = lds[stage];
             if constexpr (STAGES == 2) stage ^= 1;
         }
-        if constexpr (TAKES) {
-#pragma unroll
-            for (int m = 0; m < NM; m++) take(lane, t, m);
-        }
         __syncthreads();                                 // the last stage is read; its shares are free until the next step settles
         share += wave * SHARE;
-        if constexpr (GATED) with_act(a.act, [&](auto act) { gated(t, share, act); });
+        if constexpr (MODE == FORWARD) {
+            with_act(a.act, [&](auto act) { gated(t, share, act, std::true_type{}); });
+        } else if constexpr (MODE == GRAD) {
+            if (t.m0 + TM <= a.M && t.j0 + WIDTH <= a.J) with_act(a.act, [&](auto act) { gated(t, share, act, std::true_type{}); });
+            else with_act(a.act, [&](auto act) { gated(t, share, act, std::false_type{}); });
+        }
         else plain(t, share);
         id += stride;
         if (id >= last) return;
@@ -841,7 +848,9 @@ struct BackPlan {
     Plan grad, dx, dw;
     size_t dg, part, db, total;
 };
-constexpr int kWaveRows[] = {Large::TM / Large::WM, Medium::TM / Medium::WM, Small::TM / Small::WM};
+// Rows of column sums that GRAD writes with a tile: one a wave along the tokens, of whole tiles.
+template <class C>
+long long sum_rows(long long M) { return (M + C::TM - 1) / C::TM * C::WM; }
 BackPlan back_plan(long long M, long long K, long long N, int size) {
     BackPlan p{};
     p.Np = pad64(N);
@@ -858,7 +867,7 @@ BackPlan back_plan(long long M, long long K, long long N, int size) {
     // One after another, in the same place: the products run in one stream.
     const size_t dx = p.dx.splits > 1 ? (size_t)p.dx.splits * M * K : 0, dw = p.dw.splits > 1 ? (size_t)p.dw.splits * 2 * N * K : 0;
     p.part = take(std::max(dx, dw) * sizeof(float));
-    p.db = take((size_t)((M + 63) / 64 * 2 + 2) * 2 * N * sizeof(float));   // rows of waves: M / 64 or M / 32, up to a whole tile
+    p.db = take((size_t)std::max(sum_rows<Medium>(M), sum_rows<Small>(M)) * 2 * N * sizeof(float));
     p.total = at;
     return p;
 }
@@ -898,9 +907,7 @@ void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, 
         launch_ff<T, GRAD>(k, aligned, p.grad.tile, 1, stream);
     }
     if (dbg || dbv) {
-        const int tile = aligned || p.grad.tile == 2 ? p.grad.tile : 1;
-        const long long tm = tile == 0 ? Large::TM : tile == 1 ? Medium::TM : Small::TM;
-        const long long rows = (b.M + tm - 1) / tm * (tm / kWaveRows[tile]);
+        const long long rows = b.M == 0 ? 0 : p.grad.tile == 2 ? sum_rows<Small>(b.M) : sum_rows<Medium>(b.M);
         hipLaunchKernelGGL(ff_db_fold_kernel, dim3((2 * b.N + 31) / 32), dim3(1024), 0, stream, db, rows, b.N, dbg, dbv);
         launch_check("ff_db_fold_kernel");
     }

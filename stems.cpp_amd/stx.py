@@ -1153,8 +1153,9 @@ def _type(t):
         raise TypeError(f"operands must be float32, float16 or bfloat16, got {t.dtype}") from None
 
 
-def _typed(t, like, what):
-    """stx_tensor (packed) of a tensor of up to 4 dims with the element type and device of `like`."""
+def _typed(t, like, what, slices=False):
+    """stx_tensor (packed) of a tensor of up to 4 dims with the element type and device of `like`; with slices, a
+    (B, T, C) tensor as (B, 1, T, C)."""
     if t.dtype is not like.dtype:
         raise TypeError(f"{what} must be {like.dtype}, got {t.dtype}")
     if not t.is_cuda or t.device != like.device:
@@ -1163,7 +1164,10 @@ def _typed(t, like, what):
     n = len(shape)
     if n > 4:
         raise ValueError(f"{what} has more than 4 dimensions")
-    if n < 4:
+    if slices and n == 3:
+        shape = (shape[0], 1, shape[1], shape[2])
+        stride = (stride[0], shape[2] * stride[1], stride[1], stride[2])
+    elif n < 4:
         shape = (1,) * (4 - n) + tuple(shape)
         stride = (shape[4 - n] * stride[0] if n else 1,) * (4 - n) + stride
     d, c, b, a = shape
@@ -1240,13 +1244,8 @@ def rope_scaled_back(q, pos, params, k=None, out=None, k_out=None, stream=None):
     return _rope_scaled(lib().stx_rope_scaled_back, q, pos, params, k, out, k_out, stream)
 
 
-def _slices(t):
-    """(B, T1, T2, C) view of a (B, T1, T2, C), (B, T, C) or (T, C) tensor."""
-    return t.unsqueeze(1) if t.dim() == 3 else t
-
-
 def group_norm_cl_workspace_size(x, n_groups):
-    return lib().stx_group_norm_cl_workspace_size(_typed(_slices(x), x, "x"), _type(x), int(n_groups))
+    return lib().stx_group_norm_cl_workspace_size(_typed(x, x, "x", True), _type(x), int(n_groups))
 
 
 def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, out=None, stats=None, workspace=None,
@@ -1256,14 +1255,13 @@ def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, o
     1 / sqrt(var + eps), for group_norm_cl_back. out may be x."""
     import torch
     out = x.new_empty(x.shape) if out is None else out
-    v = _slices(x)
-    dx, t, L = _typed(v, x, "x"), _type(x), lib()
-    C, B = v.shape[-1], v.shape[0] if v.dim() == 4 else 1
+    dx, t, L = _typed(x, x, "x", True), _type(x), lib()
+    C, B = x.shape[-1], x.shape[0] if x.dim() > 2 else 1
     if stats is None:
         stats = torch.empty((B, n_groups, 2), dtype=torch.float64, device=x.device)
     ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(dx, t, int(n_groups)), workspace, x, stream)
     _launch(L.stx_group_norm_cl, x, stream, dx, t, int(n_groups), float(eps), _floats(weight, x, C, "weight"),
-            _floats(bias, x, C, "bias"), int(act), _typed(_slices(out), x, "out"),
+            _floats(bias, x, C, "bias"), int(act), _typed(out, x, "out", True),
             _floats(stats, x, B * n_groups * 2, "stats", torch.float64), ws, nbytes)
     return out, stats
 
@@ -1273,15 +1271,14 @@ def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_N
     """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy."""
     import torch
     dx = x.new_empty(x.shape) if dx is None else dx
-    v = _slices(x)
-    da, t, L = _typed(v, x, "x"), _type(x), lib()
-    C, B = v.shape[-1], v.shape[0] if v.dim() == 4 else 1
+    da, t, L = _typed(x, x, "x", True), _type(x), lib()
+    C, B = x.shape[-1], x.shape[0] if x.dim() > 2 else 1
     dweight = torch.empty(C, dtype=torch.float32, device=x.device) if dweight is None else dweight
     dbias = torch.empty(C, dtype=torch.float32, device=x.device) if dbias is None else dbias
     ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(da, t, int(n_groups)), workspace, x, stream)
-    _launch(L.stx_group_norm_cl_back, x, stream, _typed(_slices(dy), x, "dy"), da, t,
+    _launch(L.stx_group_norm_cl_back, x, stream, _typed(dy, x, "dy", True), da, t,
             _floats(stats, x, B * n_groups * 2, "stats", torch.float64), int(n_groups), _floats(weight, x, C, "weight"),
-            _floats(bias, x, C, "bias"), int(act), _typed(_slices(dx), x, "dx"), _floats(dweight, x, C, "dweight"),
+            _floats(bias, x, C, "bias"), int(act), _typed(dx, x, "dx", True), _floats(dweight, x, C, "dweight"),
             _floats(dbias, x, C, "dbias"), ws, nbytes)
     return dx, dweight, dbias
 

@@ -605,3 +605,74 @@ def test_differences(device):
         up[i], down[i] = args[i] + step * d, args[i] - step * d
         slope = (loss(up) - loss(down)) / (2 * step)
         assert abs(slope - float((g.to(F64) * d).sum())) <= 1e-5 * float((g.to(F64) * d).abs().sum()), i
+
+
+# ------------------------------------------------------------------- far offsets, shared devices
+def test_offsets_past_32_bits(device):
+    """Elements and bytes beyond 2^32 in every operator: the last rows against the definition."""
+    dt = torch.bfloat16
+    q = torch.zeros((1, 70000, 512, 64), dtype=dt, device=device)                  # 2.3e9 elements, 4.6 GB
+    q[:, -3:] = randn(device, (1, 3, 512, 64), 401, dtype=dt)
+    pos = torch.arange(70000, device=device, dtype=torch.int32)
+    y = stx.rope_scaled(q, pos, stx.rope_params(64), out=q.clone())
+    want, mag = rope_ref(q[:, -3:], pos[-3:], 64, 0)
+    close(y[:, -3:], want, 4 * U * mag, "rope")
+    del q, y
+    x = torch.zeros((2, 1100000, 1024), dtype=dt, device=device)                   # the second slice starts past 2^31 bytes
+    x[1, ::1000] = randn(device, (1100, 1024), 402, dtype=dt)
+    y, stats = stx.group_norm_cl(x, 4, act=stx.ACT_SILU)
+    assert not bool(y[0].any())
+    part = x[1, ::1000].to(F64).view(1100, 4, 256)
+    n = 1100000 * 256
+    mean = part.sum((0, 2)) / n
+    var = part.square().sum((0, 2)) / n - mean * mean
+    assert torch.allclose(stats[1], torch.stack([mean, (var + 1e-5).rsqrt()], -1), rtol=1e-10, atol=1e-13)
+    z = (part[-3:] - mean[:, None]) * (var + 1e-5).rsqrt()[:, None]
+    close(y[1, ::1000][-3:], (z * torch.sigmoid(z)).view(3, 1024), 64 * U * (1 + z.abs()).view(3, 1024), "norm")
+    dx, dw, db = stx.group_norm_cl_back(x, x, stats, 4, act=stx.ACT_SILU, dx=y)
+    ref = norm_ref(x[1:, ::1000], 4, 1e-5, None, None, "silu", x[1:, ::1000])      # the other rows of dy are 0
+    s = (part - mean[:, None]) * (var + 1e-5).rsqrt()[:, None]
+    sg = torch.sigmoid(s)
+    dz = part * (sg + s * sg * (1 - sg))
+    close(db, dz.sum(0).reshape(1024), (64 * U * (1 + s.abs()) * part.abs()).sum(0).reshape(1024), "db")
+    assert ref["dx"].shape == (1, 1100, 1024) and bool(dx[1].isfinite().all())
+    del x, y, dx
+    M, K, N = 600000, 40, 4096                                                     # out: 2.5e9 elements
+    x = torch.zeros((M, K), dtype=dt, device=device)
+    x[-70:] = randn(device, (70, K), 403, dtype=dt)
+    wg, wv = (randn(device, (N, K), 404 + i, K ** -0.5, dtype=dt) for i in range(2))
+    h = stx.gated_ff(x, wg, wv, stx.ACT_SILU)
+    ref = ff_ref(x[-70:], wg, wv, "silu", None, None, randn(device, (70, N), 406, dtype=dt))
+    close(h[-70:], ref["h"], ref["eh"], "h")
+    assert not bool(h[:1000].any())
+    h.zero_()
+    h[-70:] = randn(device, (70, N), 406, dtype=dt)                               # as dh: the other tokens add nothing
+    dx, dwg, dwv, _, _ = stx.gated_ff_back(h, x, wg, wv, stx.ACT_SILU)
+    close(dx[-70:], ref["dx"], ref["edx"], "dx")
+    assert not bool(dx[:1000].any())
+    close(dwg, ref["dwg"], ref["edwg"], "dwg")
+    close(dwv, ref["dwv"], ref["edwv"], "dwv")
+
+
+def test_two_streams_at_once(device):
+    """Calls of the same operators on two streams, each with its own workspace, many times over: each stream's results."""
+    x = [randn(device, (3, 501, 96), 411 + i, dtype=torch.bfloat16) for i in range(2)]
+    dh = [randn(device, (3, 501, 160), 413 + i, dtype=torch.bfloat16) for i in range(2)]
+    wg, wv = (randn(device, (160, 96), 415 + i, 0.1, dtype=torch.bfloat16) for i in range(2))
+
+    def step(i, s=None):
+        y, stats = stx.group_norm_cl(x[i], 8, act=stx.ACT_GELU, stream=s)
+        return [y, *stx.group_norm_cl_back(x[i], x[i], stats, 8, act=stx.ACT_GELU, stream=s),
+                *stx.gated_ff_back(dh[i], y, wg, wv, stx.ACT_SILU, stream=s)[:3]]
+
+    want = [[t.clone() for t in step(i)] for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i, s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for run in got[i] for a, b in zip(run, want[i]))
