@@ -802,9 +802,10 @@ typedef struct {
  * [dim, heads, N, batch] and, where k is not NULL, the keys k [dim, kv heads, N, batch] of one
  * attention in one launch. pos is device int32: token i2 of batch i3 is at
  * pos[i3 * pos_stride + i2] (pos_stride 0: every sequence has the same positions). Angles are
- * formed in double, the rotation in float. Rows are contiguous; any other strides, so q and k may be
- * slices of a projection's output. q_dst may be q and k_dst may be k; outputs overlap nothing
- * else. At most 2^31 - 1 tokens (N * batch) and 2^24 - 1 rows a token. */
+ * formed in double (up to 2^40 in magnitude), the rotation in float. Rows are contiguous; any
+ * other strides, so q and k may be slices of a projection's output. q_dst may be q and k_dst may
+ * be k; outputs overlap nothing else. At most 2^31 - 1 tokens (N * batch), 2^24 - 1 rows and
+ * fewer than 2^27 elements a token. */
 STX_API stx_status stx_rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
                                    int64_t pos_stride, const stx_rope_params* params, const stx_tensor* q_dst,
                                    const stx_tensor* k_dst, stx_stream stream);
@@ -817,8 +818,9 @@ STX_API stx_status stx_rope_scaled_back(const stx_tensor* q, const stx_tensor* k
 /* GroupNorm over channels-last tensors: a is [C, T1, T2, B], contiguous. stx_group_norm has
  * the channels in ne2; the norm over tokens [D, N] at the end of HTDemucs' transformer
  * (src/htdemucs.cpp:223-227) is this one with one group. The channels are split into n_groups
- * groups of ceil(C / n_groups), the last of what is left (every group has a channel); each is
- * normalised per ne3 slice over T1 x T2 x its channels with the biased variance:
+ * groups (4,096 at most) of ceil(C / n_groups), the last of what is left (every group has a
+ * channel); each is normalised per ne3 slice over T1 x T2 x its channels with the biased
+ * variance:
  *   y = act((a - mean) / sqrt(var + eps) * weight[c] + bias[c]).
  * weight and bias: device float[C], either may be NULL (1 and 0). stats: device double
  * [B][n_groups][2], receives mean and 1 / sqrt(var + eps) for stx_group_norm_cl_back (NULL: not
@@ -842,8 +844,11 @@ STX_API stx_status stx_group_norm_cl_back(const stx_tensor* dy, const stx_tensor
  * x [K, tokens...] (up to three token dimensions, evenly spaced rows), w_gate and w_value [K, N]
  * (ggml's weight layout), dst [N, tokens...] (the same token dimensions, evenly spaced rows);
  * rows are contiguous, row strides any. b_gate, b_value: device float[N], either may be NULL.
- * Products are accumulated in fp32 (matrix instructions of the data's type). dst overlaps no
- * input. At most 2^30 tokens, K and N at most 2^20. */
+ * Products are accumulated in fp32, on the matrix cores: of fp16 and bf16 as they are; of fp32,
+ * above 64 tokens and in the gradients, as the six larger products of three bf16 parts an element,
+ * which hold all of a finite element above 2^-100 (smaller ones lose low bits; an infinity gives
+ * NaN where a sum of products might have been infinite). dst overlaps no input. At most 2^30
+ * tokens, K and N at most 2^20. */
 STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, const stx_tensor* w_value, stx_type type,
                                 const float* b_gate, const float* b_value, stx_act act, const stx_tensor* dst,
                                 stx_stream stream);

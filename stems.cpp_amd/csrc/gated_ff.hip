@@ -120,12 +120,13 @@ __device__ __forceinline__ u32x4 load_chunk(const char* p, long long left) {
 // 16 bytes a lane from memory to LDS at lds + lane * 16 (lds uniform over the wave): at base + off,
 // base uniform; or at p. Written out because the compiler takes every such load for one that a
 // transposing LDS read might depend on, and waits for all of them before it; the waits are
-// settle()'s. No register is written.
+// settle()'s. No register is written. s_nop: a wait state between m0 and its use, five between a
+// vector instruction that may have written the base (a lane read, a reloaded spill) and its use.
 __device__ __forceinline__ unsigned lds_address(const void* p) {
     return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)p);
 }
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void load_to_lds(const void* p, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");

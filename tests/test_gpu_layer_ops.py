@@ -259,6 +259,23 @@ def test_group_norm_cl(device, dtype, shape, act):
     assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 40, 300, 300), (1, 2000, 1024, 512), (1, 20, 4096, 4096), (2, 9, 8000, 4000)], ids=str)
+def test_group_norm_cl_many_groups(device, dtype, shape):
+    """More groups than a block has threads, up to the most."""
+    B, T, C, G = shape
+    x, dy = (randn(device, (B, T, C), 71 + i, 1.3, 0.4 - 0.4 * i, TYPES[dtype]) for i in range(2))
+    w, b = randn(device, (C,), 73, 0.3, 1.0), randn(device, (C,), 74, 0.3)
+    ref = norm_ref(x, G, 1e-5, w, b, "silu", dy)
+    y, stats = stx.group_norm_cl(x, G, 1e-5, w, b, stx.ACT_SILU)
+    close(y, ref["y"], ref["ey"], "y")
+    assert torch.allclose(stats, ref["stats"], rtol=1e-10, atol=1e-13)
+    dx, dw, db = stx.group_norm_cl_back(dy, x, stats, G, w, b, stx.ACT_SILU)
+    close(dx, ref["dx"], ref["edx"], "dx")
+    close(dw, ref["dw"], ref["edw"], "dw")
+    close(db, ref["db"], ref["edb"], "db")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("C,shift", [(48, 0), (48, 1), (37, 1)])
 def test_group_norm_cl_in_place_alignment_and_4d(device, dtype, C, shift):
