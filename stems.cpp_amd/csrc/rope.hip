@@ -12,7 +12,9 @@ namespace {
 // large batch fill tiles too): it forms cos and sin of the tile's angles once, in LDS, and rotates
 // all rows (heads of q, then of k) of those tokens with them. The operator reads and writes every
 // element once and is bound by HBM; the angles cost half / (rows * dim) of a double-precision
-// evaluation an element.
+// evaluation an element. 60 x 801 tokens of 16 rows of 64 fp32 values, slices of a projection (394 MB):
+// 73 us, 5.4 TB/s; the gradient of 2 x 16,384 tokens of 40 rows of 128 bf16 values, 96 of them rotated
+// (671 MB): 132 us, 5.1 TB/s, the rate of a large copy; one token of 16 rows: 2.5 us.
 //
 // Angles are products of a position and a frequency in double (a float angle of 10^5 radians
 // would be off by 2^-8); cos and sin are reduced and evaluated in double and rounded to float
@@ -87,7 +89,9 @@ __device__ __forceinline__ void rope_store(T* p, Pack<T, V> r, int valid) {
 }
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeItems = 4;            // units a thread loads before it stores the first
+// Units a thread of a tile, one after another. The two calls above by it: 1: 81, 134 us; 2: 72, 136; 4: 73, 132;
+// 8: 77, 149. Four loaded before the first is stored: 76, 150 (the waves' registers, hence fewer waves).
+constexpr int kRopeUnits = 4;
 constexpr int kRopeTable = 4096;         // pairs in LDS: 32 KB
 constexpr int kRopeTile = 16;
 
@@ -111,62 +115,44 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(RopeScaledArg
     }
     __syncthreads();
     const unsigned total = nt * a.rows.d * a.units.d;
-    for (unsigned base = threadIdx.x; base < total; base += kRopeThreads * kRopeItems) {
-        Pack<T, V> x[kRopeItems], y[kRopeItems];
-        T* out[kRopeItems];
-        int at[kRopeItems];              // first element within the row
-        const float2* tab[kRopeItems];
+    for (unsigned e = threadIdx.x; e < total; e += kRopeThreads) {
+        const unsigned row = a.units.div(e), u = e - row * a.units.d;
+        const unsigned tk = a.rows.div(row), h = row - tk * a.rows.d;
+        const unsigned t = t0 + tk, i3 = a.n.div(t), i2 = t - i3 * a.n.d;
+        const bool is_k = h >= a.q_rows;
+        const RopeSide& side = is_k ? a.k : a.q;
+        const long long i1 = is_k ? h - a.q_rows : h;
+        const T* src = reinterpret_cast<const T*>(side.src + i1 * side.s1 + i2 * side.s2 + i3 * side.s3);
+        T* out = reinterpret_cast<T*>(side.dst + i1 * side.d1 + i2 * side.d2 + i3 * side.d3);
+        const float2* tab = cs + tk * half;
+        if constexpr (MODE == 0) {
+            const int at = (int)u * V;
+            Pack<T, V> x = rope_load<T, V, VEC>(src + at, a.dim - at);
 #pragma unroll
-        for (int j = 0; j < kRopeItems; j++) {
-            const unsigned e = base + j * kRopeThreads;
-            out[j] = nullptr;
-            if (e >= total) continue;
-            const unsigned row = a.units.div(e), u = e - row * a.units.d;
-            const unsigned tk = a.rows.div(row), h = row - tk * a.rows.d;
-            const unsigned t = t0 + tk, i3 = a.n.div(t), i2 = t - i3 * a.n.d;
-            const bool is_k = h >= a.q_rows;
-            const RopeSide& side = is_k ? a.k : a.q;
-            const long long i1 = is_k ? h - a.q_rows : h;
-            const T* src = reinterpret_cast<const T*>(side.src + i1 * side.s1 + i2 * side.s2 + i3 * side.s3);
-            out[j] = reinterpret_cast<T*>(side.dst + i1 * side.d1 + i2 * side.d2 + i3 * side.d3);
-            tab[j] = cs + tk * half;
-            if constexpr (MODE == 0) {
-                at[j] = (int)u * V;
-                x[j] = rope_load<T, V, VEC>(src + at[j], a.dim - at[j]);
-            } else {
-                const int pairs = half / V;
-                at[j] = (int)u < pairs ? (int)u * V : a.n_dims + ((int)u - pairs) * V;
-                x[j] = rope_load<T, V, VEC>(src + at[j], V);
-                if (at[j] < half) y[j] = rope_load<T, V, VEC>(src + at[j] + half, V);
+            for (int v = 0; v < V; v += 2) {
+                const int pair = (at + v) / 2;
+                if (pair >= half) continue;
+                const float2 r = tab[pair];
+                const float x0 = to_f32(x.v[v]), x1 = to_f32(x.v[v + 1]);
+                x.v[v] = from_f32<T>(fmaf(x0, r.x, -(x1 * r.y)));
+                x.v[v + 1] = from_f32<T>(fmaf(x0, r.y, x1 * r.x));
             }
-        }
+            rope_store<T, V, VEC>(out + at, x, a.dim - at);
+        } else {
+            const int pairs = half / V, at = (int)u < pairs ? (int)u * V : a.n_dims + ((int)u - pairs) * V;
+            Pack<T, V> x = rope_load<T, V, VEC>(src + at, V);
+            if (at < half) {
+                Pack<T, V> y = rope_load<T, V, VEC>(src + at + half, V);
 #pragma unroll
-        for (int j = 0; j < kRopeItems; j++) {
-            if (!out[j]) continue;
-            if constexpr (MODE == 0) {
-#pragma unroll
-                for (int v = 0; v < V; v += 2) {
-                    const int pair = (at[j] + v) / 2;
-                    if (pair >= half) continue;
-                    const float2 r = tab[j][pair];
-                    const float x0 = to_f32(x[j].v[v]), x1 = to_f32(x[j].v[v + 1]);
-                    x[j].v[v] = from_f32<T>(fmaf(x0, r.x, -(x1 * r.y)));
-                    x[j].v[v + 1] = from_f32<T>(fmaf(x0, r.y, x1 * r.x));
+                for (int v = 0; v < V; v++) {
+                    const float2 r = tab[at + v];
+                    const float x0 = to_f32(x.v[v]), x1 = to_f32(y.v[v]);
+                    x.v[v] = from_f32<T>(fmaf(x0, r.x, -(x1 * r.y)));
+                    y.v[v] = from_f32<T>(fmaf(x0, r.y, x1 * r.x));
                 }
-                rope_store<T, V, VEC>(out[j] + at[j], x[j], a.dim - at[j]);
-            } else {
-                if (at[j] < half) {
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        const float2 r = tab[j][at[j] + v];
-                        const float x0 = to_f32(x[j].v[v]), x1 = to_f32(y[j].v[v]);
-                        x[j].v[v] = from_f32<T>(fmaf(x0, r.x, -(x1 * r.y)));
-                        y[j].v[v] = from_f32<T>(fmaf(x0, r.y, x1 * r.x));
-                    }
-                    rope_store<T, V, VEC>(out[j] + at[j] + half, y[j], V);
-                }
-                rope_store<T, V, VEC>(out[j] + at[j], x[j], V);
+                rope_store<T, V, VEC>(out + at + half, y, V);
             }
+            rope_store<T, V, VEC>(out + at, x, V);
         }
     }
 }
@@ -263,9 +249,9 @@ void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const 
     }
     const int w = v ? v : p->mode == 0 ? 2 : 1;
     a.units = FastDiv((unsigned)(p->mode == 0 ? (dim + w - 1) / w : half / w + (dim - a.n_dims + w - 1) / w));
-    // Tokens a block: kRopeItems units a thread, as long as two blocks a CU remain.
+    // Tokens a block: kRopeUnits units a thread, as long as two blocks a CU remain.
     const long long items = (long long)a.rows.d * a.units.d;
-    long long tile = std::max(1LL, std::min<long long>(kRopeTile, kRopeThreads * kRopeItems / items));
+    long long tile = std::max(1LL, std::min<long long>(kRopeTile, kRopeThreads * kRopeUnits / items));
     tile = std::min(tile, std::max(1LL, (long long)a.tokens / 512));
     a.tile = (unsigned)std::min<long long>(tile, kRopeTable / half);
     const size_t lds = sizeof(float2) * a.tile * half;
