@@ -1211,6 +1211,8 @@ def _scratch(need, workspace, like, stream):
         else:
             with torch.cuda.stream(stream):
                 workspace = torch.empty(max(256, need), dtype=torch.uint8, device=like.device)
+    elif not workspace.is_cuda or workspace.device != like.device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous CUDA (HIP) tensor on {like.device}, is on {workspace.device}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
@@ -1222,6 +1224,9 @@ def _rope_scaled(fn, q, pos, params, k, out, k_out, stream):
     batch, n = (shape[0] if len(shape) == 4 else 1), shape[-3]
     if pos.dtype is not torch.int32 or pos.device != q.device or tuple(pos.shape) not in ((n,), (batch, n)) or (n > 1 and pos.stride(-1) != 1):
         raise ValueError(f"pos must be ({n},) or ({batch}, {n}) int32 with contiguous rows on {q.device}, is {tuple(pos.shape)} {pos.dtype}")
+    factors = getattr(params, "factors", None)
+    if factors is not None and factors.device != q.device:
+        raise ValueError(f"freq_factors are on {factors.device}, q is on {q.device}")
     out = q.new_empty(q.shape) if out is None else out
     dk = dko = None
     if k is not None:

@@ -151,3 +151,19 @@ def test_parameter_helpers():
         stx.rope_params(64, freq_factors=[1.0])
     p = stx.rope_params(64, 2, n_ctx_orig=4096, ext_factor=1.0)
     assert p.size == ctypes.sizeof(stx.RopeParams) == 48 and (p.mode, p.n_ctx_orig) == (2, 4096)
+
+
+def test_workspace_of_another_device():
+    """A workspace in host memory never reaches a kernel."""
+    import torch
+    with pytest.raises(ValueError):
+        stx._scratch(256, torch.empty(256, dtype=torch.uint8), torch.empty(1, device="meta"), None)
+
+
+def test_frequency_factors_of_another_device():
+    import torch
+    q, pos = torch.empty(2, 4, 8), torch.zeros(2, dtype=torch.int32)
+    p = stx.rope_params(8)
+    p.factors = torch.ones(4, device="meta")
+    with pytest.raises(ValueError, match="freq_factors"):
+        stx.rope_scaled(q, pos, p)
