@@ -830,7 +830,7 @@ STX_API size_t     stx_group_norm_cl_workspace_size(const stx_tensor* a, stx_typ
 STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_groups, double eps, const float* weight,
                                      const float* bias, stx_act act, const stx_tensor* dst, double* stats,
                                      void* workspace, size_t workspace_bytes, stx_stream stream);
-/* Its gradients, from dy (of y), a and stats as the forward call left them: dx (of a; may be dy),
+/* Its gradients, from dy (of y), a and stats as the forward call left them: dx (of a; may be dy or a),
  * dweight and dbias (device float[C], summed over T1, T2 and B). Any of the three may be NULL.
  * The same workspace size. */
 STX_API stx_status stx_group_norm_cl_back(const stx_tensor* dy, const stx_tensor* a, stx_type type, const double* stats,

@@ -1273,7 +1273,7 @@ def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, o
 
 def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_NONE, dx=None, dweight=None, dbias=None,
                        workspace=None, stream=None):
-    """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy."""
+    """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy or x."""
     import torch
     dx = x.new_empty(x.shape) if dx is None else dx
     da, t, L = _typed(x, x, "x", True), _type(x), lib()

@@ -693,3 +693,29 @@ def test_two_streams_at_once(device):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for run in got[i] for a, b in zip(run, want[i]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_over_the_input(device, dtype):
+    """group_norm_cl_back with dx in x's memory gives the same bits."""
+    x, dy = (randn(device, (3, 211, 40), 81 + i, dtype=TYPES[dtype]) for i in range(2))
+    w = randn(device, (40,), 83, 0.3, 1.0)
+    _, stats = stx.group_norm_cl(x, 5, weight=w, act=stx.ACT_SILU)
+    want = stx.group_norm_cl_back(dy, x, stats, 5, w, act=stx.ACT_SILU)
+    got = stx.group_norm_cl_back(dy, x, stats, 5, w, act=stx.ACT_SILU, dx=x)
+    assert got[0] is x and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [9, 200])
+def test_gated_ff_of_one_row_for_every_token(device, dtype, M):
+    """x and dh broadcast (a row stride of 0): the bits of the same rows written out."""
+    row, dh = (randn(device, (1, n), 84 + n, dtype=TYPES[dtype]) for n in (48, 24))
+    wg, wv = (randn(device, (24, 48), 86 + i, 0.2, dtype=TYPES[dtype]) for i in range(2))
+    x, g = row.expand(M, 48), dh.expand(M, 24)
+    assert x.stride(0) == 0
+    assert torch.equal(stx.gated_ff(x, wg, wv), stx.gated_ff(x.contiguous(), wg, wv))
+    dx = torch.empty(M, 48, device=device, dtype=TYPES[dtype])
+    got = stx.gated_ff_back(g, x, wg, wv, dx=dx)
+    want = stx.gated_ff_back(g.contiguous(), x.contiguous(), wg, wv)
+    assert all(torch.equal(p, q) for p, q in zip(got[:3], want[:3]))
