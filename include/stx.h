@@ -855,9 +855,10 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
 /* Its gradients, from dh (of dst) and the forward call's inputs; the two products are formed
  * again, so the forward call keeps nothing. dx (of x), dw_gate and dw_value (of the weights),
  * db_gate and db_value (device float[N]); any may be NULL, and the work for it is left out (both
- * weights' gradients or neither). For fp16 and bf16 the gradients of the two products are rounded
- * to the data's type before the matrix products that use them; db_gate and db_value are summed from
- * the unrounded ones. Outputs overlap no input. workspace: device, 256-byte aligned, no
+ * weights' gradients or neither). Results are rounded once: the gradients of the two products are
+ * held in fp32, for fp16 and bf16 in two bf16 parts (16 bits at any fp32 exponent), so they may pass
+ * fp16's range where the results do not; an infinite x or weight gives NaN in the gradients it enters.
+ * Outputs overlap no input. workspace: device, 256-byte aligned, no
  * initialisation; calls that share one must not overlap. The size is for n_tokens tokens, K =
  * n_in, N = n_hidden (0 for sizes that stx_gated_ff_back rejects). */
 STX_API size_t     stx_gated_ff_back_workspace_size(int64_t n_tokens, int64_t n_in, int64_t n_hidden, stx_type type);

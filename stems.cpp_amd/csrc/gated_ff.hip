@@ -45,7 +45,22 @@ struct Split {
         }
     }
 };
-__device__ __forceinline__ f32x4 mma(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x4 acc) {   // smallest terms first
+// x as a high and a low bf16 part; an infinity has a low part of 0.
+__device__ __forceinline__ void halves(float x, bf16& hi, bf16& lo) {
+    hi = (bf16)x;
+    const float rest = x - (float)hi;
+    lo = (bf16)(rest == rest ? rest : 0.f);
+}
+__device__ __forceinline__ f32x4 mma(const u32x4 (&a)[1], const u32x4 (&b)[2], f32x4 acc) {   // smallest terms first
+    acc = mma(a[0], b[1], acc, bf16{});
+    return mma(a[0], b[0], acc, bf16{});
+}
+__device__ __forceinline__ f32x4 mma(const u32x4 (&a)[2], const u32x4 (&b)[2], f32x4 acc) {
+    acc = mma(a[1], b[0], acc, bf16{});
+    acc = mma(a[0], b[1], acc, bf16{});
+    return mma(a[0], b[0], acc, bf16{});
+}
+__device__ __forceinline__ f32x4 mma(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x4 acc) {
     acc = mma(a[2], b[0], acc, bf16{});
     acc = mma(a[0], b[2], acc, bf16{});
     acc = mma(a[1], b[1], acc, bf16{});
@@ -62,21 +77,32 @@ __device__ __forceinline__ f32x4 mma(const u32x4 (&a)[3], const u32x4 (&b)[3], f
 //   DX       P = the weights, Q = dg, then dv: both reductions (over the N outputs) into one
 //            accumulator.
 //   DW       P = x, Q = dg or dv, reduced over the tokens.
+// GRAD leaves dg and dv in fp32, of 16-bit data as two bf16 parts, high and low: 16 bits at any
+// exponent. Rounded to the data's type instead they would add an error as large as that of the
+// results' own rounding (bf16, 48,060 tokens, K 384, N 1,536: 2.3e-3 where it is 1.65e-3), and fp16's would end
+// at 65,504 and 2^-24, where a sum that they enter need not. DX and DW multiply both parts, by
+// bf16's P as it is and by fp16's in two bf16 parts (without the product of the two low ones, below
+// 2^-17 of the whole). An infinity in P gives NaN there: infinity times a low part of 0.
 // In FORWARD and GRAD r is the fastest dimension of both operands, in DX of Q only and in DW of
 // neither; an operand whose r is not its fastest dimension is "strided" below.
 enum Mode { FORWARD, GRAD, DX, DW };
 
-// Tiles of TJ x TM outputs, WJ x WM waves, SLOTS blocks a CU. A step of the reduction is 8 chunks of
-// 16 bytes of every row, in two stages of LDS: five stages of 4 chunks, which keep twice as much
-// in flight, took 5 to 10 % longer everywhere (twice the barriers).
-constexpr int CH = 8;
-template <int TJ_, int TM_, int WJ_, int WM_, int SLOTS_>
+// Tiles of TJ x TM outputs, WJ x WM waves. A step of the reduction is 64 values
+// of every row in FORWARD and GRAD of 16-bit data, in two stages of LDS (five stages of 32, which keep
+// twice as much in flight, took 5 to 10 % longer: twice the barriers), and 32 elsewhere, where an
+// operand has two or three parts.
+constexpr int step_of(Mode mode, int size) { return size == 2 && (mode == FORWARD || mode == GRAD) ? 64 : 32; }
+template <int TJ_, int TM_, int WJ_, int WM_>
 struct Tile {
-    static constexpr int TJ = TJ_, TM = TM_, WJ = WJ_, WM = WM_, SLOTS = SLOTS_, NT = 64 * WJ * WM;
+    static constexpr int TJ = TJ_, TM = TM_, WJ = WJ_, WM = WM_, NT = 64 * WJ * WM;
 };
-using Large = Tile<256, 256, 2, 4, 1>;
-using Medium = Tile<128, 128, 2, 2, 2>;
-using Small = Tile<128, 64, 2, 2, 3>;
+using Large = Tile<256, 256, 2, 4>;
+using Medium = Tile<128, 128, 2, 2>;
+using Small = Tile<128, 64, 2, 2>;
+// Blocks of a tile (0 Large, 1 Medium, 2 Small) that a CU holds: what its registers and LDS have room for.
+constexpr int slots_of(int tile, Mode mode, stx_type type) {
+    return tile == 0 ? 1 : tile == 1 && !(type == STX_TYPE_BF16 && (mode == DX || mode == DW)) ? 2 : 3;
+}
 
 struct FfArgs {
     const char* p[2];
@@ -94,6 +120,7 @@ struct FfArgs {
     long long os[2];                     // output row strides in bytes
     int jpad;                            // columns written: J, in GRAD padded with zeros
     int qpad;                            // DW: columns that a row of Q has
+    long long plane;                     // of 16-bit data: bytes from dg's and dv's high parts to their low ones
     float* part;                         // GRAD: column sums [wave rows][2][J]; DX, DW: [parts][M][J] or NULL
 };
 
@@ -175,8 +202,8 @@ __device__ __forceinline__ float row_sum(float v) {
 // of 8 values, chunk c of row x at c ^ bend(x), so that eight rows which a fragment reads together
 // lie in different banks. Strided: rows of the reduction, [8 PER][X / 8] chunks, chunk c of row r at
 // c ^ turn(r), so that the 4 rows of 32 bytes which the transposing read takes do. A 16-bit
-// operand is fetched in this form (PER 8: a step of 64); an fp32 one is split on its way into three
-// planes of it (PER 4: a step of 32).
+// operand is fetched in this form (PER 8: a step of 64; 4: of 32), dg and dv in two planes of it; an
+// fp32 one is split on its way into three planes, fp16's P of DX and DW into two.
 template <int PER>
 __device__ __forceinline__ int bend(int x) {
     return PER == 8 ? x % 8 : x / 2 % 4;
@@ -218,15 +245,17 @@ struct Fragments {
     }
 };
 
-// The 16-byte chunks of an operand's tile that a thread fetches in a step: [X][8], strided [8 E][X / E].
-template <class T, int X, int NT, bool STRIDED>
+// The 16-byte chunks of an operand's tile that a thread fetches in a step of R values: [X][R / E],
+// strided [R][X / E].
+template <class T, int X, int NT, bool STRIDED, int R>
 struct Source {
-    static constexpr int E = 16 / sizeof(T), N = X * CH / NT, PER = STRIDED ? X / E : CH;   // chunks a thread; chunks a row
+    static constexpr int E = 16 / sizeof(T), N = X * R / E / NT, PER = STRIDED ? X / E : R / E;   // chunks a thread; chunks a row
+    static_assert(X * R / E % NT == 0);
     static __device__ __forceinline__ int row(int i) { return (i * NT + (int)threadIdx.x) / PER; }
     static __device__ __forceinline__ int chunk(int i) {
         const int c = (i * NT + (int)threadIdx.x) % PER;
         if constexpr (sizeof(T) == 4) return c;
-        else return c ^ (STRIDED ? turn<X>(row(i)) : bend<CH>(row(i)));
+        else return c ^ (STRIDED ? turn<X>(row(i)) : bend<R / 8>(row(i)));
     }
     // fp32: where the four values of chunk i lie in a plane.
     static __device__ __forceinline__ int spot(int i) {
@@ -241,19 +270,21 @@ struct Source {
 // (ALIGNED), otherwise through registers, for any alignment and length. fp32 operands are split
 // between the registers and LDS, once a block (by every wave from its fragments, splitting took
 // longer than the products), and have one stage of three planes: two would leave room for one
-// block a CU.
+// block a CU. fp16's P of DX and DW is split there too.
 template <class T, int MODE, class C, bool ALIGNED>
 __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     constexpr int NT = C::NT, E = 16 / sizeof(T), TJ = C::TJ, TM = C::TM;
     constexpr int NJ = TJ / C::WJ / 16, NM = TM / C::WM / 16;       // 16 x 16 tiles of a wave
     constexpr bool GATED = MODE == FORWARD || MODE == GRAD, PS = !GATED, QS = MODE == DW;
     constexpr int WIDTH = GATED ? TJ / 2 : TJ;                       // output columns of a tile
-    constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int PER = SPLIT ? 4 : CH, PLANES = SPLIT ? 3 : 1, STAGES = SPLIT ? 1 : 2, QAT = TJ * PER * 16 * PLANES;   // Q's place
-    constexpr int STAGE = (TJ + TM) * PER * 16 * PLANES;
-    static_assert(!(SPLIT && ALIGNED));
-    using PSource = Source<T, TJ, NT, PS>;
-    using QSource = Source<T, TM, NT, QS>;
+    constexpr bool SPLIT = sizeof(T) == 4, HALVE = !GATED && std::is_same_v<T, f16>;
+    constexpr int R = step_of((Mode)MODE, sizeof(T)), PER = R / 8, STAGES = SPLIT ? 1 : 2;
+    constexpr int PP = SPLIT ? 3 : HALVE ? 2 : 1, QP = SPLIT ? 3 : GATED ? 1 : 2;              // planes
+    constexpr int QIN = SPLIT ? 1 : QP;                              // of Q in memory
+    constexpr int PPLANE = TJ * PER * 16, QPLANE = TM * PER * 16, QAT = PPLANE * PP, STAGE = QAT + QPLANE * QP;
+    static_assert(!((SPLIT || HALVE) && ALIGNED));
+    using PSource = Source<T, TJ, NT, PS, R>;
+    using QSource = Source<T, TM, NT, QS, R>;
     __shared__ __align__(128) char lds[STAGES][STAGE];
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
@@ -290,7 +321,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     // where rows are clamped. With unaligned operands the offset is 64-bit.
     using Off = std::conditional_t<ALIGNED, unsigned, long long>;
     Off poff[PSource::N], qoff[QSource::N];
-    const int pside = GATED ? __builtin_amdgcn_readfirstlane(tid / CH / 16 % 2) : 0;   // the matrix of a wave's rows
+    const int pside = GATED ? __builtin_amdgcn_readfirstlane(tid / PSource::PER / 16 % 2) : 0;   // the matrix of a wave's rows
     auto aim = [&](const Item& t, int seg, int qs) {
 #pragma unroll
         for (int i = 0; i < PSource::N; i++) {
@@ -305,40 +336,49 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
             else qoff[i] = (Off)(min(row, a.M - 1 - t.m0) * a.qs[qs] + at * (long long)sizeof(T));
         }
     };
-    u32x4 hold[ALIGNED ? 1 : PSource::N + QSource::N];
+    constexpr int HELD = PSource::N + QSource::N * QIN;
+    u32x4 hold[ALIGNED ? 1 : HELD];
     auto fetch = [&](const Item& t, int step, int stage) {
         const int seg = MODE == DX && step >= a.steps ? 1 : 0, qs = MODE == DW ? t.z % 2 : seg;
         if (step == t.begin || (MODE == DX && step == a.steps)) aim(t, seg, qs);
-        const long long r = (long long)(step - seg * a.steps) * CH * E;
+        const long long r = (long long)(step - seg * a.steps) * R;
         const char* pb = PS ? a.p[seg] + r * a.ps[seg] + t.j0 * (long long)sizeof(T) : a.p[pside] + t.j0 * a.ps[pside] + r * (long long)sizeof(T);
         const char* qb = QS ? a.q[qs] + r * a.qs[qs] + t.m0 * (long long)sizeof(T) : a.q[qs] + t.m0 * a.qs[qs] + r * (long long)sizeof(T);
         if constexpr (ALIGNED) {
-            const unsigned pl = lds_address(lds[stage] + wave * 1024), ql = pl + TJ * CH * 16;
-            if (r + CH * E <= a.RP && r + CH * E <= a.RQ) {
+            const unsigned pl = lds_address(lds[stage] + wave * 1024), ql = pl + QAT;
+            if (r + R <= a.RP && r + R <= a.RQ) {
 #pragma unroll
                 for (int i = 0; i < PSource::N; i++) load_to_lds(pb, poff[i], pl + i * NT * 16);
 #pragma unroll
-                for (int i = 0; i < QSource::N; i++) load_to_lds(qb, qoff[i], ql + i * NT * 16);
+                for (int k = 0; k < QIN; k++)
+#pragma unroll
+                    for (int i = 0; i < QSource::N; i++) load_to_lds(qb + k * a.plane, qoff[i], ql + k * QPLANE + i * NT * 16);
             } else {                                     // the reduction's end: zeros for what is past it
 #pragma unroll
                 for (int i = 0; i < PSource::N; i++)
                     load_to_lds(r + (PS ? PSource::row(i) : PSource::chunk(i) * E) < a.RP ? (const void*)(pb + poff[i]) : (const void*)&zero_chunk, pl + i * NT * 16);
 #pragma unroll
-                for (int i = 0; i < QSource::N; i++)
-                    load_to_lds(r + (QS ? QSource::row(i) : QSource::chunk(i) * E) < a.RQ ? (const void*)(qb + qoff[i]) : (const void*)&zero_chunk, ql + i * NT * 16);
+                for (int k = 0; k < QIN; k++)
+#pragma unroll
+                    for (int i = 0; i < QSource::N; i++)
+                        load_to_lds(r + (QS ? QSource::row(i) : QSource::chunk(i) * E) < a.RQ ? (const void*)(qb + k * a.plane + qoff[i]) : (const void*)&zero_chunk,
+                                    ql + k * QPLANE + i * NT * 16);
             }
-        } else if (r + CH * E <= a.RP && r + CH * E <= a.RQ && (!PS || t.j0 + TJ <= a.J)) {
+        } else if (r + R <= a.RP && r + R <= a.RQ && (!PS || t.j0 + TJ <= a.J)) {
 #pragma unroll
             for (int i = 0; i < PSource::N; i++) __builtin_memcpy(&hold[i], pb + poff[i], 16);
 #pragma unroll
-            for (int i = 0; i < QSource::N; i++) __builtin_memcpy(&hold[PSource::N + i], qb + qoff[i], 16);
+            for (int i = 0; i < QSource::N * QIN; i++) __builtin_memcpy(&hold[PSource::N + i], qb + i / QSource::N * a.plane + qoff[i % QSource::N], 16);
         } else {
 #pragma unroll
             for (int i = 0; i < PSource::N; i++)
                 hold[i] = load_chunk<T>(pb + poff[i], !PS ? a.RP - r - PSource::chunk(i) * E : r + PSource::row(i) < a.RP ? a.J - t.j0 - PSource::chunk(i) * E : 0);
 #pragma unroll
-            for (int i = 0; i < QSource::N; i++)
-                hold[PSource::N + i] = load_chunk<T>(qb + qoff[i], !QS ? a.RQ - r - QSource::chunk(i) * E : r + QSource::row(i) < a.RQ ? E : 0);
+            for (int k = 0; k < QIN; k++)
+#pragma unroll
+                for (int i = 0; i < QSource::N; i++)
+                    hold[PSource::N + k * QSource::N + i] =
+                        load_chunk<T>(qb + k * a.plane + qoff[i], !QS ? a.RQ - r - QSource::chunk(i) * E : r + QSource::row(i) < a.RQ ? E : 0);
         }
     };
     // The stream of fetches, one step ahead of the products.
@@ -368,12 +408,28 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 const Split v(hold[i]);
                 char* to = lds[0] + (i < PSource::N ? PSource::spot(i) : QAT + QSource::spot(i - PSource::N));
 #pragma unroll
-                for (int k = 0; k < 3; k++) *reinterpret_cast<u32x2*>(to + k * (i < PSource::N ? TJ : TM) * 64) = v.part[k];
+                for (int k = 0; k < 3; k++) *reinterpret_cast<u32x2*>(to + k * (i < PSource::N ? PPLANE : QPLANE)) = v.part[k];
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < PSource::N + QSource::N; i++)
-                *reinterpret_cast<u32x4*>(&lds[stage][(i < PSource::N ? i * NT : TJ * CH + (i - PSource::N) * NT) * 16 + tid * 16]) = hold[i];
+            for (int i = 0; i < HELD; i++) {
+                char* to = lds[stage] + (i < PSource::N ? i * NT * 16 : QAT + (i - PSource::N) * NT * 16) + tid * 16;   // planes of Q follow one another
+                if (HALVE && i < PSource::N) {
+                    f16 x[8];
+                    bf16 part[2][8];
+                    __builtin_memcpy(x, &hold[i], 16);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) halves(to_f32(x[e]), part[0][e], part[1][e]);
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        u32x4 v;
+                        __builtin_memcpy(&v, part[k], 16);
+                        *reinterpret_cast<u32x4*>(to + k * PPLANE) = v;
+                    }
+                } else {
+                    *reinterpret_cast<u32x4*>(to) = hold[i];
+                }
+            }
         }
         __syncthreads();
     };
@@ -387,7 +443,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
     // accumulators' own layout they would be runs of 32 bytes (the forward product of 48,060 tokens,
     // K 384, N 1536 then spends 41 us of 167 on its stores).
     constexpr int COLS = GATED ? NJ * 8 : NJ * 16, CR = COLS / 8, AREA = 16 * COLS * 2, SHARE = STAGE / (NT / 64), PIECES = 16 * CR / 64;
-    constexpr int AREAS = MODE == GRAD ? 2 : 1, TURNS = AREA * AREAS * 2 <= SHARE ? 2 : 1;   // areas of 16 rows; groups in turn
+    constexpr int AREAS = MODE == GRAD ? 4 : 1, TURNS = AREA * AREAS * 2 <= SHARE ? 2 : 1;   // areas of 16 rows; groups in turn
     static_assert(AREA * AREAS <= SHARE && PIECES >= 1 && 16 * CR % 64 == 0, "staging");
     auto spot = [&](unsigned row, unsigned col) { return row * COLS * 2 + (col / 8 + row) % CR * 16 + col % 8 * 2; };
     auto pack = [&](char* p, const float (&f)[4]) {
@@ -395,6 +451,13 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = from_f32<T>(f[i]);
         __builtin_memcpy(__builtin_assume_aligned(p, 8), v, sizeof v);
+    };
+    auto pack_halves = [&](char* p, const float (&f)[4]) {
+        bf16 hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) halves(f[i], hi[i], lo[i]);
+        __builtin_memcpy(__builtin_assume_aligned(p, 8), hi, sizeof hi);
+        __builtin_memcpy(__builtin_assume_aligned(p + AREA, 8), lo, sizeof lo);
     };
     // The lane's number as a new value: addresses formed from it are not kept from one group of rows
     // for the next, there being no registers for them beside the accumulators.
@@ -468,8 +531,8 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                         sv[j / 2][r] += dv[r];
                     }
                     if constexpr (WIDE) {
-                        pack(here, dg);
-                        pack(here + AREA, dv);
+                        pack_halves(here, dg);
+                        pack_halves(here + 2 * AREA, dv);
                     } else if (row < a.M && a.out[0]) {
                         store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.jpad - n, dg);
                         store4<T>(a.out[1] + row * a.os[1] + n * (long long)sizeof(T), a.jpad - n, dv);
@@ -480,7 +543,11 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
             if constexpr (WIDE) {
                 if (MODE == FORWARD || a.out[0]) {
                     flush(lane, area, a.out[0], a.os[0], row0, nw);
-                    if constexpr (MODE == GRAD) flush(lane, area + AREA, a.out[1], a.os[1], row0, nw);
+                    if constexpr (MODE == GRAD) {
+                        flush(lane, area + AREA, a.out[0] + a.plane, a.os[0], row0, nw);
+                        flush(lane, area + 2 * AREA, a.out[1], a.os[1], row0, nw);
+                        flush(lane, area + 3 * AREA, a.out[1] + a.plane, a.os[1], row0, nw);
+                    }
                 }
             }
         }
@@ -558,23 +625,24 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 }
             }
             const char *pl = lds[stage], *ql = pl + QAT;
-            if constexpr (SPLIT) {
-                u32x4 fq[NM][3];
+            if constexpr (QP > 1) {
+                static_assert(PER == 4);
+                u32x4 fq[NM][QP];
 #pragma unroll
                 for (int m = 0; m < NM; m++)
 #pragma unroll
-                    for (int k = 0; k < 3; k++) fq[m][k] = qf.read(ql + k * TM * 64, 0, m);
+                    for (int k = 0; k < QP; k++) fq[m][k] = qf.read(ql + k * QPLANE, 0, m);
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    u32x4 fp[3];
+                    u32x4 fp[PP];
 #pragma unroll
-                    for (int k = 0; k < 3; k++) fp[k] = pf.read(pl + k * TJ * 64, 0, j);
+                    for (int k = 0; k < PP; k++) fp[k] = pf.read(pl + k * PPLANE, 0, j);
 #pragma unroll
                     for (int m = 0; m < NM; m++) acc[j][m] = mma(fp, fq[m], acc[j][m]);
                 }
             } else {
 #pragma unroll
-                for (int kk = 0; kk < CH / 4; kk++) {
+                for (int kk = 0; kk < PER / 4; kk++) {
                     u32x4 fp[NJ], fq[NM];
 #pragma unroll
                     for (int j = 0; j < NJ; j++) fp[j] = pf.read(pl, kk, j);
@@ -731,36 +799,37 @@ constexpr long long kMaxWidth = 1 << 20, kMaxTokens = 1 << 30;   // of K and N; 
 constexpr int kCus = 256;                                         // of an MI355X: plans are made without a device at hand
 
 // How a product is run: its tile and the number of parts of its reduction, by the least estimated time.
-// A step (128 bytes of the reduction) of a tile takes time in proportion to its area, the larger
-// tiles' at a better rate (the measured ones of a long reduction); a part ends in an epilogue
-// and a fold. Measured, bf16, 48,060 tokens, K 384, N 1,536: FORWARD Large 143, Medium 156, Small 182 us (113
-// GFLOP: 790 TFLOP/s); GRAD Medium 250, Small 286; DX 170 and 182; DW 137 and 235, and 695 unsplit, whose 72
-// tiles leave most CUs idle. fp32, 1,344 tokens, K 512, N 2,048: DX Small 43 (split, with 6 of the fold) where
+// A step of a tile takes time in proportion to its area, the larger tiles' at a better rate (the
+// measured ones of a long reduction); a part ends in an epilogue and a fold. Measured, bf16, 48,060 tokens,
+// K 384, N 1,536: FORWARD Large 143, Medium 156, Small 182 us (113 GFLOP: 790 TFLOP/s); GRAD Medium 305; DX
+// Large 315, Medium 245 (290 with two blocks a CU), Small 270; DW Medium in 10 parts 215, in 7 on two blocks a CU
+// 235. fp32, 1,344 tokens, K 512, N 2,048: DX Small 43 (split, with 6 of the fold) where
 // Medium takes 48 and an unsplit one 157; DW 43 (and 6), 47 and 59.
 struct Plan {
     int tile, splits, part;              // 0 Large, 1 Medium, 2 Small; parts, steps of a part
 };
-long long steps_of(long long r, int size) { return std::max(1LL, (r * size + CH * 16 - 1) / (CH * 16)); }
-Plan plan_of(Mode mode, long long J, long long M, long long steps, int size) {
+long long steps_of(Mode mode, long long r, int size) { return std::max(1LL, (r + step_of(mode, size) - 1) / step_of(mode, size)); }
+Plan plan_of(Mode mode, long long J, long long M, long long steps, stx_type type) {
     struct Kind {
-        int tj, tm, slots;
-        double rate[2], alone[3];        // relative rate, 16-bit and fp32; and of 1, 2, 3 blocks on a CU
+        int tj, tm;
+        double rate[2];                  // relative rate, 16-bit and fp32
     };
-    static constexpr Kind kinds[] = {{256, 256, 1, {1.0, 1.0}, {1, 1, 1}},
-                                     {128, 128, 2, {0.86, 0.96}, {0.6, 1, 1}},
-                                     {128, 64, 3, {0.62, 0.85}, {0.4, 0.75, 1}}};
+    static constexpr Kind kinds[] = {{256, 256, {1.0, 1.0}}, {128, 128, {0.86, 0.96}}, {128, 64, {0.62, 0.85}}};
+    static constexpr double alone[3][3] = {{1, 1, 1}, {0.6, 1, 1}, {0.4, 0.75, 1}};   // of 1, 2, 3 blocks on a CU that holds 1, 2, 3
     const bool gated = mode == FORWARD || mode == GRAD;
+    const int size = type_size(type);
     const int w = mode == DW ? 2 : 1;
     Plan best{};
     double least = 0;
     for (int k = mode == GRAD || size == 4 ? 1 : 0; k < 3; k++) {    // Large has no registers for GRAD's epilogue: 460 us where Medium takes 250
         const Kind& c = kinds[k];
+        const int slots = slots_of(k, mode, type);
         const long long tiles = (J * (gated ? 2 : 1) + c.tj - 1) / c.tj * ((M + c.tm - 1) / c.tm) * w;
         const double area = c.tj * (double)c.tm / 65536, step = area / c.rate[size == 4] * (size == 4 ? 5.5 : 0.95);   // us on a whole CU
         for (int s = 1; s <= (gated ? 1 : 32) && (s == 1 || steps / s >= 4); s++) {
-            const long long part = (steps + s - 1) / s, items = tiles * ((steps + part - 1) / part), rest = items % (kCus * c.slots);
+            const long long part = (steps + s - 1) / s, items = tiles * ((steps + part - 1) / part), rest = items % (kCus * slots);
             const long long k_rest = (rest + kCus - 1) / kCus;
-            const double busy = (double)(items / (kCus * c.slots)) * c.slots + (rest ? k_rest / c.alone[k_rest - 1] : 0.0);
+            const double busy = (double)(items / (kCus * slots)) * slots + (rest ? k_rest / alone[slots - 1][k_rest - 1] : 0.0);
             double us = busy * (part * step + 4.0 * area) + 2.0;
             if (s > 1) us += 4.0 + 8.0 * s * J * M * w / 4e6;
             if (least == 0 || us < least) {
@@ -780,7 +849,8 @@ void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
     if (tiles * parts >= (1LL << 30)) fail(STX_STATUS_UNSUPPORTED, "gated_ff: too many tiles");
     a.tiles = (int)tiles;
     a.items = (int)(tiles * parts);
-    const long long blocks = std::min<long long>(a.items, (long long)device_cus() * C::SLOTS);
+    constexpr int slots = slots_of(C::TJ == 256 ? 0 : C::TM == 128 ? 1 : 2, (Mode)MODE, type_of<T>);
+    const long long blocks = std::min<long long>(a.items, (long long)device_cus() * slots);
     hipLaunchKernelGGL((ff_kernel<T, MODE, C, AL>), dim3(xcd_grid(blocks)), dim3(C::NT), 0, stream, a);
     launch_check("ff_kernel");
 }
@@ -788,7 +858,8 @@ void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
 // What goes through registers has no Large tile.
 template <class T, int MODE>
 void launch_ff(const FfArgs& a, bool aligned, int tile, int parts, hipStream_t stream) {
-    if constexpr (sizeof(T) == 4) return tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
+    constexpr bool held = sizeof(T) == 4 || (std::is_same_v<T, f16> && (MODE == DX || MODE == DW));
+    if constexpr (held) return tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
     else if (!aligned) tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
     else if (MODE != GRAD && tile == 0) launch_tiles<T, MODE == GRAD ? FORWARD : MODE, Large, true>(a, parts, stream);
     else if (tile == 1) launch_tiles<T, MODE, Medium, true>(a, parts, stream);
@@ -836,7 +907,7 @@ FfArgs products(const Block& b, const float* bg, const float* bv, stx_act act, i
     k.J = b.N;
     k.M = (int)b.M;
     k.RP = k.RQ = b.K;
-    k.steps = (int)steps_of(b.K, size);
+    k.steps = (int)steps_of(FORWARD, b.K, size);
     k.jpad = b.N;
     k.b[0] = bg;
     k.b[1] = bv;
@@ -847,8 +918,8 @@ bool products_aligned(const Block& b, int size) {
     return b.K % (16 / size) == 0 && aligned_rows(b.x.data, b.x.stride) && aligned_rows(b.wg.data, b.wg.stride) && aligned_rows(b.wv.data, b.wv.stride);
 }
 
-// Workspace of the backward pass: dg and dv with rows of a multiple of 64 elements, the parts of
-// split reductions, the biases' column sums (for the smallest tile's waves).
+// Workspace of the backward pass: dg and dv with rows of a multiple of 64 elements (of 16-bit data the
+// high parts and the low ones of each), the parts of split reductions, the biases' column sums (for the smallest tile's waves).
 struct BackPlan {
     long long Np;
     Plan grad, dx, dw;
@@ -857,19 +928,20 @@ struct BackPlan {
 // Rows of column sums that GRAD writes with a tile: one a wave along the tokens, of whole tiles.
 template <class C>
 long long sum_rows(long long M) { return (M + C::TM - 1) / C::TM * C::WM; }
-BackPlan back_plan(long long M, long long K, long long N, int size) {
+BackPlan back_plan(long long M, long long K, long long N, stx_type type) {
     BackPlan p{};
+    const int size = type_size(type);
     p.Np = pad64(N);
-    p.grad = plan_of(GRAD, N, M, steps_of(K, size), size);
-    p.dx = plan_of(DX, K, M, 2 * steps_of(N, size), size);
-    p.dw = plan_of(DW, K, N, steps_of(M, size), size);
+    p.grad = plan_of(GRAD, N, M, steps_of(GRAD, K, size), type);
+    p.dx = plan_of(DX, K, M, 2 * steps_of(DX, N, size), type);
+    p.dw = plan_of(DW, K, N, steps_of(DW, M, size), type);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += pad256(bytes);
         return here;
     };
-    p.dg = take(2 * (size_t)(M * p.Np) * size);
+    p.dg = take(2 * (size_t)(M * p.Np) * sizeof(float));
     // One after another, in the same place: the products run in one stream.
     const size_t dx = p.dx.splits > 1 ? (size_t)p.dx.splits * M * K : 0, dw = p.dw.splits > 1 ? (size_t)p.dw.splits * 2 * N * K : 0;
     p.part = take(std::max(dx, dw) * sizeof(float));
@@ -895,9 +967,10 @@ template <class T>
 void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, stx_act act, const Rows* dx, const Rows* dwg, const Rows* dwv,
               float* dbg, float* dbv, char* ws, hipStream_t stream) {
     constexpr int size = sizeof(T);
-    const BackPlan p = back_plan(b.M, b.K, b.N, size);
+    const BackPlan p = back_plan(b.M, b.K, b.N, type_of<T>);
     char* dg = ws + p.dg;
-    char* dv = dg + b.M * p.Np * size;
+    char* dv = dg + b.M * p.Np * (long long)sizeof(float);
+    const long long plane = b.M * p.Np * 2;
     float* part = reinterpret_cast<float*>(ws + p.part);
     float* db = reinterpret_cast<float*>(ws + p.db);
     const bool aligned = products_aligned(b, size);
@@ -909,6 +982,7 @@ void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, 
         k.out[1] = dv;
         k.os[0] = k.os[1] = p.Np * size;
         k.jpad = (int)p.Np;
+        k.plane = plane;
         k.part = dbg || dbv ? db : nullptr;
         launch_ff<T, GRAD>(k, aligned, p.grad.tile, 1, stream);
     }
@@ -930,7 +1004,8 @@ void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, 
         k.M = (int)b.M;
         k.RP = b.N;
         k.RQ = p.Np;
-        k.steps = (int)steps_of(b.N, size);
+        k.steps = (int)steps_of(DX, b.N, size);
+        k.plane = plane;
         k.chunk = p.dx.part;
         k.out[0] = dx->data;
         k.os[0] = dx->stride;
@@ -949,7 +1024,8 @@ void run_back(const Block& b, const Rows& dh, const float* bg, const float* bv, 
         k.M = b.N;
         k.qpad = (int)p.Np;
         k.RP = k.RQ = b.M;
-        k.steps = (int)steps_of(b.M, size);
+        k.steps = (int)steps_of(DW, b.M, size);
+        k.plane = plane;
         k.chunk = p.dw.part;
         k.out[0] = dwg->data;
         k.out[1] = dwv->data;
@@ -988,7 +1064,7 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
         with_type(type, [&](auto t) {
             using T = decltype(t);
             if (b.M > kFew)
-                return launch_ff<T, FORWARD>(k, products_aligned(b, size), plan_of(FORWARD, b.N, b.M, k.steps, size).tile, 1, as_stream(stream));
+                return launch_ff<T, FORWARD>(k, products_aligned(b, size), plan_of(FORWARD, b.N, b.M, k.steps, type).tile, 1, as_stream(stream));
             const dim3 grid((b.N + 15) / 16), block(512);
             if (b.M <= 16) hipLaunchKernelGGL((ff_few_kernel<T, 1>), grid, block, 0, as_stream(stream), k);
             else if (b.M <= 32) hipLaunchKernelGGL((ff_few_kernel<T, 2>), grid, block, 0, as_stream(stream), k);
@@ -1001,10 +1077,10 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
 STX_API size_t stx_gated_ff_back_workspace_size(int64_t n_tokens, int64_t n_in, int64_t n_hidden, stx_type type) {
     size_t bytes = 0;
     (void)guard([&] {
-        const int size = type_size(type);
+        (void)type_size(type);
         STX_REQUIRE(n_tokens >= 0 && n_tokens <= kMaxTokens && n_in > 0 && n_in <= kMaxWidth && n_hidden > 0 && n_hidden <= kMaxWidth,
                     "gated_ff_back_workspace_size: %lld tokens, K = %lld, N = %lld", (long long)n_tokens, (long long)n_in, (long long)n_hidden);
-        bytes = back_plan(n_tokens, n_in, n_hidden, size).total;
+        bytes = back_plan(n_tokens, n_in, n_hidden, type).total;
     });
     return bytes;
 }
@@ -1038,7 +1114,7 @@ STX_API stx_status stx_gated_ff_back(const stx_tensor* dh, const stx_tensor* x, 
         for (const stx_tensor* o : {dx, dw_gate, dw_value})
             for (const stx_tensor* i : {dh, x, w_gate, w_value})
                 STX_REQUIRE(!o || !overlap(span_of(o, size), span_of(i, size)), "gated_ff_back: an output overlaps an input");
-        check_workspace(workspace, workspace_bytes, back_plan(b.M, b.K, b.N, size).total, "gated_ff_back");
+        check_workspace(workspace, workspace_bytes, back_plan(b.M, b.K, b.N, type).total, "gated_ff_back");
         if (!dx && !dw_gate && !db_gate && !db_value) return;
         with_type(type, [&](auto t) {
             run_back<decltype(t)>(b, h, b_gate, b_value, act, dx ? &rx : nullptr, dw_gate ? &rg : nullptr, dw_value ? &rv : nullptr, db_gate,

@@ -20,6 +20,9 @@ inline int type_size(stx_type t) {
     }
 }
 
+template <class T>
+constexpr stx_type type_of = std::is_same_v<T, float> ? STX_TYPE_F32 : std::is_same_v<T, f16> ? STX_TYPE_F16 : STX_TYPE_BF16;
+
 // Calls f(T{}) with the device type of t.
 template <class F>
 void with_type(stx_type t, F&& f) {

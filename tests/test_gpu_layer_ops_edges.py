@@ -1,0 +1,74 @@
+"""The transformer-layer operators where ordinary data does not take them: intermediate values beyond the
+data type's range and precision, operands of one sign, means far from zero, tails, other streams,
+very many slices, offsets past 32 bits. References and bounds as in test_gpu_layer_ops."""
+import math
+
+import pytest
+
+import stx
+from test_gpu_layer_ops import ACTS, F64, TYPES, U, act_ref, close, ff_ref, half_step, norm_ref, randn, rope_ref  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ---------------------------------------------------------------------- gated block, backward
+def ff_back_bounds(x, wg, wv, act, dh):
+    """Gradients in 64 bits, bounded by the products' roundings alone: dg and dv, known to half a step of 16 bits
+    (2^-17), enter each sum with that and with their own error as ff_ref has it; products of two parts
+    leave out the two low ones (2^-17 once more). Three of them: 3 * 2^-17, less than an eighth of bf16's half step."""
+    ref = ff_ref(x, wg, wv, act, None, None, dh)
+    X, G, V, D = (t.to(F64) for t in (x, wg, wv, dh))
+    g, v = torch.mm(X, G.t().contiguous()), torch.mm(X, V.t().contiguous())
+    a, d = act_ref(g, act)
+    dg, dv = D * v * d, D * a
+    K, N, M = x.shape[1], wg.shape[0], x.shape[0]
+    walk = 4 * math.sqrt(K) * U
+    eg, ev = walk * torch.mm(X.abs(), G.abs().t().contiguous()) + U * g.abs(), walk * torch.mm(X.abs(), V.abs().t().contiguous()) + U * v.abs()
+    ed, ea = eg + 16 * U * (1 + g.abs()), 1.13 * eg + 16 * U * (1 + g * g) * a.abs() + 2 * U * g.abs()
+    part = 3 * 2.0 ** -17
+    fg = D.abs() * (ev * d.abs() + v.abs() * ed) + (part + 4 * U) * dg.abs()
+    fv = D.abs() * ea + (part + 4 * U) * dv.abs()
+    w2, w3 = 4 * math.sqrt(2 * N) * U, 4 * math.sqrt(max(1, M)) * U
+    e = {"dx": torch.mm(fg + w2 * dg.abs(), G.abs()) + torch.mm(fv + w2 * dv.abs(), V.abs()),
+         "dwg": torch.mm((fg + w3 * dg.abs()).t().contiguous(), X.abs()), "dwv": torch.mm((fv + w3 * dv.abs()).t().contiguous(), X.abs())}
+    return ref, e
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 64, 40), (40, 384, 96), (300, 333, 301), (777, 512, 130), (5000, 392, 1030)], ids=str)
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_gated_gradients_are_rounded_once(device, dtype, shape, act):
+    """dx and the weights' gradients of 16-bit data to half a step of it and the products' fp32 roundings: nothing on the way
+    is rounded to the data's type."""
+    M, K, N = shape
+    dt = TYPES[dtype]
+    x, dh = randn(device, (M, K), 501, dtype=dt), randn(device, (M, N), 502, dtype=dt)
+    wg, wv = (randn(device, (N, K), 503 + i, K ** -0.5, dtype=dt) for i in range(2))
+    ref, e = ff_back_bounds(x, wg, wv, act, dh)
+    for name, got in zip(("dx", "dwg", "dwv"), stx.gated_ff_back(dh, x, wg, wv, ACTS[act])):
+        close(got, ref[name], e[name], name)
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("small", [False, True])
+def test_gated_gradients_of_scaled_halves(device, small, aligned):
+    """fp16 with the loss scaled: gradients of the two products beyond 65,504 and below 2^-25, sums of them in range."""
+    M, K, N = 400, 72 if aligned else 71, 88
+    dt = torch.float16
+    if small:
+        x, dh = randn(device, (M, K), 511, 200.0, dtype=dt), randn(device, (M, N), 512, 2.0 ** -17, dtype=dt)
+        wg, wv = (randn(device, (N, K), 513 + i, 2.0 ** -22, dtype=dt) for i in range(2))
+    else:
+        x, dh = randn(device, (M, K), 515, 2.0 ** -6, dtype=dt), randn(device, (M, N), 516, 6000.0, dtype=dt)
+        wg, wv = randn(device, (N, K), 517, 2.0 ** -14, dtype=dt), randn(device, (N, K), 518, 100.0, dtype=dt)
+        wv[:, ::2] = 0
+    ref, e = ff_back_bounds(x, wg, wv, "none", dh)
+    X, G, V, D = (t.to(F64) for t in (x, wg, wv, dh))
+    dg = D * torch.mm(X, V.t().contiguous())
+    assert bool((dg.abs() < 2.0 ** -25).any() if small else (dg.abs() > 65504).any())
+    fits = {n: ref[n].abs() < 65000 for n in e}
+    assert float(fits["dwg"].double().mean()) > 0.9 and (small or float(fits["dx"][:, ::2].double().mean()) > 0.9)
+    for name, got in zip(("dx", "dwg", "dwv"), stx.gated_ff_back(dh, x, wg, wv, stx.ACT_NONE)):
+        keep = fits[name]
+        close(got[keep], ref[name][keep], e[name][keep], name)
