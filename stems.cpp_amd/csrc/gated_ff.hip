@@ -29,20 +29,31 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 acc, bf16) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
 
-// fp32 values as sums of three bf16 ones: x = h + m + l with h the upper half of x's bits, m that of
-// x - h, l the rest, all exact (8 bits each of the 24). A product of two such sums without its
-// three smallest terms, which are below 2^-23 of it together, is six bf16 products: 2.7 times the rate
-// of the fp32 matrix instruction, at its accuracy. An infinity's rest is inf - inf: NaN.
+// fp32 values as sums of three bf16 ones (Henry, Tang and Heinecke, "Leveraging the bfloat16 artificial
+// intelligence datatype for higher-precision computations", 2019): x = h + m + l with h = bf16(x), m =
+// bf16(x - h), l = x - h - m, all exact. Rounded to nearest, |m| <= 2^-8 |x| and |l| <= 2^-17 |x| have either
+// sign, and a product of two such sums without its three smallest terms (2 |m l| + |l l|: below 2^-24 of it)
+// is six bf16 products without bias: 2.7 times the rate of the fp32 matrix instruction, at its
+// accuracy. (Parts cut off instead drop up to 2^-21, always towards zero.) h is kept below infinity for
+// finite x; an infinity's rest is inf - inf: NaN.
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 struct Split {
     u32x2 part[3];                       // four values' h, m, l as bf16
-    __device__ __forceinline__ explicit Split(u32x4 x) {
+    __device__ __forceinline__ explicit Split(u32x4 bits) {
+        f32x4 x = __builtin_bit_cast(f32x4, bits);
 #pragma unroll
-        for (int k = 0; k < 3; k++) {
-            part[k] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+        for (int k = 0; k < 3; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(x[i] & 0xffff0000u));
-        }
+            for (int i = 0; i < 2; i++) {
+                f32x2 v = {x[2 * i], x[2 * i + 1]};
+                if (k == 0) v = f32x2{__builtin_amdgcn_fmed3f(v[0], -0x1.fep127f, 0x1.fep127f), __builtin_amdgcn_fmed3f(v[1], -0x1.fep127f, 0x1.fep127f)};
+                const unsigned pair = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+                part[k][i] = pair;
+                x[2 * i] -= __uint_as_float(pair << 16);
+                x[2 * i + 1] -= __uint_as_float(pair & 0xffff0000u);
+            }
     }
 };
 // x as a high and a low bf16 part; an infinity has a low part of 0.

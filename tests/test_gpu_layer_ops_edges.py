@@ -72,3 +72,47 @@ def test_gated_gradients_of_scaled_halves(device, small, aligned):
     for name, got in zip(("dx", "dwg", "dwv"), stx.gated_ff_back(dh, x, wg, wv, stx.ACT_NONE)):
         keep = fits[name]
         close(got[keep], ref[name][keep], e[name][keep], name)
+
+
+# ------------------------------------------------------------------- gated block, fp32 products
+def bits(device, *values):
+    return torch.tensor(values, dtype=torch.int32, device=device).view(torch.float32)
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 4])
+def test_gated_fp32_products_of_long_mantissas(device, K):
+    """Products of fp32 values whose low 16 bits are all ones, all alike in sign, with a value product of 1: the bf16
+    parts leave out less than u of each, its sums round it twice. 4 u in all."""
+    M, N = 130, 24
+    worst = bits(device, 0x3F80FFFF, 0x3F81FFFF, 0x3FFFFFFF, 0x3F80FFFD)
+    g = torch.Generator(device=device)
+    g.manual_seed(520)
+    pick = lambda *s: worst[torch.randint(0, 4, s, generator=g, device=device)]  # noqa: E731
+    x, w = pick(M, K), pick(N, K)
+    x[0], w[0] = worst[0], worst[0]
+    one = torch.ones(N, device=device)
+    h = stx.gated_ff(x, w, torch.zeros_like(w), stx.ACT_NONE, b_value=one)
+    want = torch.mm(x.to(F64), w.to(F64).t().contiguous())
+    assert float(((h.to(F64) - want).abs() / want).max()) <= 4 * U
+    # The largest finite values have no part beyond them.
+    top = bits(device, 0x7F7FFFFF).expand(M, K).contiguous()
+    h = stx.gated_ff(top, torch.full_like(w, 2.0 ** -4), torch.zeros_like(w), stx.ACT_NONE, b_value=one)
+    want = (top.to(F64).sum(1) * 2.0 ** -4)[:, None].expand(M, N)
+    assert float(((h.to(F64) - want).abs() / want).max()) <= 4 * U
+
+
+def test_gated_fp32_products_are_unbiased(device):
+    """Positive operands: the errors' mean lies within six standard errors of 0, taken over the 512 independent rows of
+    the weights (an error that is always towards zero lies at 0.7 u)."""
+    M, K, N = 640, 256, 512
+    g = torch.Generator(device=device)
+    g.manual_seed(521)
+    x, w = (torch.rand(s, generator=g, device=device) + 0.5 for s in ((M, K), (N, K)))
+    h = stx.gated_ff(x, w, torch.zeros_like(w), stx.ACT_NONE, b_value=torch.ones(N, device=device))
+    want = torch.mm(x.to(F64), w.to(F64).t().contiguous())
+    e = (h.to(F64) - want) / want
+    assert abs(float(e.mean())) <= 6 * float(e.square().mean().sqrt()) / math.sqrt(N)
+    dw = stx.gated_ff_back(torch.ones(M, N, device=device), x, w, torch.zeros_like(w), stx.ACT_NONE, b_value=torch.ones(N, device=device))[1]
+    want = x.to(F64).sum(0).expand(N, K)                      # one row for all n: 256 independent columns
+    e = ((dw.to(F64) - want) / want)[0]
+    assert abs(float(e.mean())) <= 6 * float(e.square().mean().sqrt()) / math.sqrt(K)
