@@ -1106,6 +1106,9 @@ def concat(tensors, dim, out=None, stream=None):
 
 
 # ----------------------------------------- transformer-layer operators (fp32, fp16, bf16)
+# stream: as everywhere, the torch stream that the call runs on (default: the current one). The
+# caller orders it after whatever fills the operands, and keeps them alive (or calls their
+# record_stream) until it is done; tensors that a call makes belong to it.
 TYPE_F32 = 0
 TYPE_F16 = 1
 TYPE_BF16 = 30
@@ -1187,10 +1190,22 @@ def _floats(t, like, count, what, dtype=None):
     return t.data_ptr()
 
 
+def _empty(shape, dtype, like, stream):
+    """A new tensor on like's device that belongs to the stream of the call: memory that its own stream may still be
+    using is not handed to the kernel, nor the kernel's to another stream once the tensor is dropped."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+
+
 def _launch(fn, like, stream, *args):
     """fn(*args, stream) with like's device current, on `stream` (default: that device's current stream)."""
     import torch
     index = like.device.index
+    if stream is not None and stream.device != like.device:
+        raise ValueError(f"the stream belongs to {stream.device}, the operands are on {like.device}")
     s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
     if index == torch._C._cuda_getDevice():
         status = fn(*args, s)
@@ -1202,15 +1217,10 @@ def _launch(fn, like, stream, *args):
 
 
 def _scratch(need, workspace, like, stream):
-    """(pointer, bytes) of the caller's workspace, or of a new one that belongs to `stream` (so that memory freed on
-    return is not handed to another stream while the call still uses it); and the tensor that owns it."""
+    """(pointer, bytes) of the caller's workspace, or of a new one; and the tensor that owns it."""
     if workspace is None:
         import torch
-        if stream is None:
-            workspace = torch.empty(max(256, need), dtype=torch.uint8, device=like.device)
-        else:
-            with torch.cuda.stream(stream):
-                workspace = torch.empty(max(256, need), dtype=torch.uint8, device=like.device)
+        workspace = _empty(max(256, need), torch.uint8, like, stream)
     elif not workspace.is_cuda or workspace.device != like.device or not workspace.is_contiguous():
         raise ValueError(f"workspace must be a contiguous CUDA (HIP) tensor on {like.device}, is on {workspace.device}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -1227,10 +1237,10 @@ def _rope_scaled(fn, q, pos, params, k, out, k_out, stream):
     factors = getattr(params, "factors", None)
     if factors is not None and factors.device != q.device:
         raise ValueError(f"freq_factors are on {factors.device}, q is on {q.device}")
-    out = q.new_empty(q.shape) if out is None else out
+    out = _empty(q.shape, q.dtype, q, stream) if out is None else out
     dk = dko = None
     if k is not None:
-        k_out = k.new_empty(k.shape) if k_out is None else k_out
+        k_out = _empty(k.shape, k.dtype, q, stream) if k_out is None else k_out
         dk, dko = _typed(k, q, "k"), _typed(k_out, q, "k_out")
     _launch(fn, q, stream, _typed(q, q, "q"), dk, _type(q), pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0,
             ctypes.byref(params), _typed(out, q, "out"), dko)
@@ -1257,13 +1267,15 @@ def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, o
                   stream=None):
     """act(GroupNorm(x) * weight + bias) with the channels last: x (B, T1, T2, C), (B, T, C) or (T, C), contiguous;
     weight and bias: float32 device (C,) or None. Returns (out, stats): stats is float64 (B, n_groups, 2), mean and
-    1 / sqrt(var + eps), for group_norm_cl_back. out may be x."""
+    1 / sqrt(var + eps), for group_norm_cl_back; with stats=False they are not kept (None). out may be x."""
     import torch
-    out = x.new_empty(x.shape) if out is None else out
+    out = _empty(x.shape, x.dtype, x, stream) if out is None else out
     dx, t, L = _typed(x, x, "x", True), _type(x), lib()
     C, B = x.shape[-1], x.shape[0] if x.dim() > 2 else 1
     if stats is None:
-        stats = torch.empty((B, n_groups, 2), dtype=torch.float64, device=x.device)
+        stats = _empty((B, n_groups, 2), torch.float64, x, stream)
+    elif stats is False:
+        stats = None
     ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(dx, t, int(n_groups)), workspace, x, stream)
     _launch(L.stx_group_norm_cl, x, stream, dx, t, int(n_groups), float(eps), _floats(weight, x, C, "weight"),
             _floats(bias, x, C, "bias"), int(act), _typed(out, x, "out", True),
@@ -1275,11 +1287,11 @@ def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_N
                        workspace=None, stream=None):
     """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy or x."""
     import torch
-    dx = x.new_empty(x.shape) if dx is None else dx
+    dx = _empty(x.shape, x.dtype, x, stream) if dx is None else dx
     da, t, L = _typed(x, x, "x", True), _type(x), lib()
     C, B = x.shape[-1], x.shape[0] if x.dim() > 2 else 1
-    dweight = torch.empty(C, dtype=torch.float32, device=x.device) if dweight is None else dweight
-    dbias = torch.empty(C, dtype=torch.float32, device=x.device) if dbias is None else dbias
+    dweight = _empty(C, torch.float32, x, stream) if dweight is None else dweight
+    dbias = _empty(C, torch.float32, x, stream) if dbias is None else dbias
     ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(da, t, int(n_groups)), workspace, x, stream)
     _launch(L.stx_group_norm_cl_back, x, stream, _typed(dy, x, "dy", True), da, t,
             _floats(stats, x, B * n_groups * 2, "stats", torch.float64), int(n_groups), _floats(weight, x, C, "weight"),
@@ -1293,7 +1305,7 @@ def gated_ff(x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=None, out
     float32 (N,) or None; out (..., N)."""
     N = w_gate.shape[0]
     if out is None:
-        out = x.new_empty((*x.shape[:-1], N))
+        out = _empty((*x.shape[:-1], N), x.dtype, x, stream)
     _launch(lib().stx_gated_ff, x, stream, _typed(x, x, "x"), _typed(w_gate, x, "w_gate"), _typed(w_value, x, "w_value"),
             _type(x), _floats(b_gate, x, N, "b_gate"), _floats(b_value, x, N, "b_value"), int(act), _typed(out, x, "out"))
     return out
@@ -1311,13 +1323,13 @@ def gated_ff_back(dh, x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=
     there is no such bias."""
     import torch
     N, K = w_gate.shape
-    dev = x.device
-    dx = _out(dx, x)
-    dw_gate, dw_value = _out(dw_gate, w_gate), _out(dw_value, w_value)
+    dx = _empty(x.shape, x.dtype, x, stream) if dx is None else dx
+    dw_gate = _empty(w_gate.shape, w_gate.dtype, x, stream) if dw_gate is None else dw_gate
+    dw_value = _empty(w_value.shape, w_value.dtype, x, stream) if dw_value is None else dw_value
     if db_gate is None and b_gate is not None:
-        db_gate = torch.empty(N, dtype=torch.float32, device=dev)
+        db_gate = _empty(N, torch.float32, x, stream)
     if db_value is None and b_value is not None:
-        db_value = torch.empty(N, dtype=torch.float32, device=dev)
+        db_value = _empty(N, torch.float32, x, stream)
     d = [_typed(t, x, n) for t, n in ((dh, "dh"), (x, "x"), (w_gate, "w_gate"), (w_value, "w_value"), (dx, "dx"),
                                       (dw_gate, "dw_gate"), (dw_value, "dw_value"))]
     L, t = lib(), _type(x)

@@ -116,3 +116,35 @@ def test_gated_fp32_products_are_unbiased(device):
     want = x.to(F64).sum(0).expand(N, K)                      # one row for all n: 256 independent columns
     e = ((dw.to(F64) - want) / want)[0]
     assert abs(float(e.mean())) <= 6 * float(e.square().mean().sqrt()) / math.sqrt(K)
+
+
+# ------------------------------------------------------------------------------- streams
+def test_outputs_belong_to_the_given_stream(device):
+    """With a stream that is not the current one, what a call makes comes from that stream's memory: dropped, it goes
+    back there and not to the current stream."""
+    s = torch.cuda.Stream()
+    x, w = randn(device, (300, 64), 531), randn(device, (96, 64), 532, 0.125)
+    s.wait_stream(torch.cuda.current_stream())
+    want = stx.gated_ff(x, w, w)
+    for make in (lambda: stx.gated_ff(x, w, w, stream=s), lambda: stx.group_norm_cl(x, 4, stream=s)[0],
+                 lambda: stx.gated_ff_back(want, x, w, w, stream=s)[0], lambda: stx.rope_scaled(x.view(1, 300, 1, 64), torch.arange(300, device=device, dtype=torch.int32),
+                                                                                               stx.rope_params(64), stream=s)):
+        t = make()
+        size, at = t.numel() * 4, t.data_ptr()
+        del t
+        here = [torch.empty(size, dtype=torch.uint8, device=device) for _ in range(8)]
+        assert at not in [t.data_ptr() for t in here]
+        with torch.cuda.stream(s):
+            there = [torch.empty(size, dtype=torch.uint8, device=device) for _ in range(8)]
+        assert at in [t.data_ptr() for t in there]
+        del here, there
+    s.synchronize()
+    y = stx.gated_ff(x, w, w, stream=s)
+    s.synchronize()
+    assert torch.equal(y, want)
+
+
+def test_norm_without_statistics(device):
+    x = randn(device, (2, 50, 24), 533)
+    y, stats = stx.group_norm_cl(x, 3, stats=False)
+    assert stats is None and torch.equal(y, stx.group_norm_cl(x, 3)[0])
