@@ -352,8 +352,8 @@ __global__ __launch_bounds__(kThreads) void gn_cl_fold_kernel(NormArgs a, long l
 
 __device__ __forceinline__ double2 moments(const NormArgs& a, double2 s, double n) {
     if (n == 0.0) return make_double2(0.0, 1.0 / sqrt(a.eps));
-    const double mean = s.x / n;
-    return make_double2(mean, 1.0 / sqrt(fmax(0.0, s.y / n - mean * mean) + a.eps));
+    const double mean = s.x / n, var = s.y / n - mean * mean;
+    return make_double2(mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps));   // NaN stays NaN
 }
 
 // dbias and dweight of kParamChannels channels: the slots' sums over slices, chunks and R.

@@ -148,3 +148,19 @@ def test_norm_without_statistics(device):
     x = randn(device, (2, 50, 24), 533)
     y, stats = stx.group_norm_cl(x, 3, stats=False)
     assert stats is None and torch.equal(y, stx.group_norm_cl(x, 3)[0])
+
+
+# ---------------------------------------------------------------------------- group norm
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("place", [0, 5])
+def test_group_norm_cl_statistics_of_nonfinite_groups(device, bad, place):
+    """1 / sqrt(var + eps) of a group with a NaN or an infinity is NaN, its mean the sum's. The other
+    groups' are what they are without it."""
+    x = randn(device, (2, 40, 12), 541)
+    clean = stx.group_norm_cl(x, 3, act=stx.ACT_SILU)[1]
+    x[0, place, 4] = float(bad)
+    y, stats = stx.group_norm_cl(x, 3, act=stx.ACT_SILU)
+    assert bool(y[0, :, 4:8].isnan().all())
+    assert bool(stats[0, 1, 1].isnan()) and torch.equal(stats[0, 1, 0], x[0, :, 4:8].to(F64).mean()) != (bad == "nan")
+    stats[0, 1] = clean[0, 1]
+    assert torch.equal(stats, clean)
