@@ -17,14 +17,16 @@ namespace {
 //
 // A block has a tile of `cols` vector columns x `rws` super-rows at a time, and one chunk of the
 // slice's super-rows. Two kernels, forward and backward alike:
-//   sums:  two sums of every slot (position in the super-row) over the chunk: x, x^2 or dz, dz xhat;
+//   sums:  two sums of every slot (position in the super-row) over the chunk: t, t^2 or dz, dz xhat;
 //          added up to groups (backward: times w), one pair a (slice, chunk, tile, group), and in the
 //          backward pass also kept per slot, for dweight and dbias;
 //   apply: each block adds the pairs of its slice's groups, then streams its elements, one fused
 //          multiply-add and the activation each. In the backward pass extra blocks add the
 //          slots' sums to dweight and dbias.
-// (slices with more than kDirect pairs have them added by a small kernel in between). x and x^2 are
-// summed in double, since E[x^2] - mean^2 cancels; the backward sums in float over kHeld rows
+// (slices with more than kDirect pairs have them added by a small kernel in between). t = x - the
+// group's first element, and t and t^2 are summed in double: E[t^2] - E[t]^2 loses at most 2^-53 times the
+// number of elements, wherever the mean lies (the element is within that number's root of deviations
+// from it); sums of x itself would lose 2^-53 mean^2 / var. The backward sums in float over kHeld rows
 // of a thread (64 terms drift by about 1e-7 of their sum), then in double. Both passes are bound by
 // memory: HBM in the first, in the second the last-level cache as far as it still holds the input.
 // Measured: fp32 4 x 85,995 x 48, one group, GELU (66 MB): 15.5 us (4.3 TB/s) and 25.4 us (5.2 TB/s read
@@ -92,6 +94,7 @@ struct NormArgs {
     double2* stats_out;
     double2* part;                       // [B][rows][G], rows = chunks x tiles
     double2* folded;                     // [B][G]
+    double* shift;                       // [B][G], forward: what the sums are taken from
     double2* slot;                       // backward: [B][chunks][slots]
     long long rows;                      // of `part`, or 1 where they are folded (0: no elements)
     unsigned first;                      // backward: apply blocks before this one add dweight and dbias
@@ -231,6 +234,12 @@ __device__ __forceinline__ void for_channels(const Geometry& g, int col, F&& f) 
     }
 }
 
+template <class T>
+__device__ __forceinline__ double group_shift(const T* x, int first) {
+    const float v = to_f32(x[first]);
+    return fabsf(v) <= 0x1.fffffep127f ? (double)v : 0.0;            // not of an infinity or NaN: those spoil the sums by themselves
+}
+
 template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
     constexpr int V = kVec;
@@ -247,12 +256,15 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
         const T* x = static_cast<const T*>(a.x) + p.slice * n;
         const T* dy = static_cast<const T*>(a.dy) + p.slice * n;
         Chan k[BACK ? V : 1];
-        if constexpr (BACK) {
-            for_channels<V>(a.g, p.col, [&](int e, int c, int g) {
+        double shift[BACK ? 1 : V];
+        for_channels<V>(a.g, p.col, [&](int e, int c, int g) {
+            if constexpr (BACK) {
                 const double2 st = a.stats_in[p.slice * a.g.G + g];
                 k[e].set(a, st.x, st.y, c);
-            });
-        }
+            } else {
+                shift[e] = group_shift(x, g * a.g.width);
+            }
+        });
         std::conditional_t<BACK, float, double> s1[V] = {}, s2[V] = {};
         int held = 0;
         auto flush = [&] {
@@ -292,8 +304,9 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
                         s1[e] += dz;
                         s2[e] = fmaf(dz, t, s2[e]);
                     } else {
-                        s1[e] += (double)xe;
-                        s2[e] = fma((double)xe, (double)xe, s2[e]);
+                        const double t = (double)xe - shift[e];
+                        s1[e] += t;
+                        s2[e] = fma(t, t, s2[e]);
                     }
                 }
             }
@@ -330,7 +343,9 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
             s.x = lane_sum<64>(s.x);
             s.y = lane_sum<64>(s.y);
         }
-        if (lane == 0) part[g] = s;
+        if (lane != 0) continue;
+        part[g] = s;
+        if (!BACK && p.chunk == 0 && p.tile == 0) a.shift[p.slice * a.g.G + g] = group_shift(static_cast<const T*>(a.x) + p.slice * a.g.T * a.g.C, g * a.g.width);
     }
 }
 
@@ -350,10 +365,10 @@ __global__ __launch_bounds__(kThreads) void gn_cl_fold_kernel(NormArgs a, long l
     if (threadIdx.x == 0) a.folded[blockIdx.x] = red[0];
 }
 
-__device__ __forceinline__ double2 moments(const NormArgs& a, double2 s, double n) {
+__device__ __forceinline__ double2 moments(const NormArgs& a, double2 s, double n, long long at) {
     if (n == 0.0) return make_double2(0.0, 1.0 / sqrt(a.eps));
     const double mean = s.x / n, var = s.y / n - mean * mean;
-    return make_double2(mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps));   // NaN stays NaN
+    return make_double2(a.shift[at] + mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps));   // NaN stays NaN
 }
 
 // dbias and dweight of kParamChannels channels: the slots' sums over slices, chunks and R.
@@ -402,7 +417,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
         for (int g = (int)threadIdx.x; g < G; g += kThreads) {
             const double n = (double)a.g.T * (min((g + 1) * a.g.width, a.g.C) - g * a.g.width);
             const double2 s = groups[g];
-            groups[g] = BACK ? make_double2(s.x / n, s.y / n) : moments(a, s, n);
+            groups[g] = BACK ? make_double2(s.x / n, s.y / n) : moments(a, s, n, p.slice * G + g);
             if (!BACK && a.stats_out && p.chunk == 0 && p.tile == 0) a.stats_out[p.slice * G + g] = groups[g];
         }
     }
@@ -457,13 +472,14 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
 long long pair_rows(const Geometry& g) { return g.srows ? (long long)g.chunks * g.tiles : 0; }
 bool folds(const Geometry& g) { return pair_rows(g) > 1 && (g.G > kThreads || pair_rows(g) * g.G > kDirect); }
 struct Spaces {
-    size_t folded, slot, total;          // `part` is at 0
+    size_t folded, shift, slot, total;   // `part` is at 0
 };
 Spaces spaces(const Geometry& g) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Spaces s{};
     s.folded = up((size_t)g.B * pair_rows(g) * g.G * sizeof(double2));
-    s.slot = s.folded + up(folds(g) ? (size_t)g.B * g.G * sizeof(double2) : 0);
+    s.shift = s.folded + up(folds(g) ? (size_t)g.B * g.G * sizeof(double2) : 0);
+    s.slot = s.shift + up((size_t)g.B * g.G * sizeof(double));
     s.total = s.slot + (size_t)g.B * g.chunks * g.slots * sizeof(double2);
     return s;
 }
@@ -493,6 +509,7 @@ void run_norm(NormArgs& a, stx_type type, void* ws, hipStream_t stream) {
     a.tiles = FastDiv((unsigned)g.tiles);
     a.part = static_cast<double2*>(ws);
     a.folded = reinterpret_cast<double2*>(static_cast<char*>(ws) + at.folded);
+    a.shift = reinterpret_cast<double*>(static_cast<char*>(ws) + at.shift);
     a.slot = reinterpret_cast<double2*>(static_cast<char*>(ws) + at.slot);
     a.rows = pair_rows(g);
     a.first = BACK && (a.dw || a.db) ? (unsigned)((g.C + kParamChannels - 1) / kParamChannels) : 0;

@@ -164,3 +164,22 @@ def test_group_norm_cl_statistics_of_nonfinite_groups(device, bad, place):
     assert bool(stats[0, 1, 1].isnan()) and torch.equal(stats[0, 1, 0], x[0, :, 4:8].to(F64).mean()) != (bad == "nan")
     stats[0, 1] = clean[0, 1]
     assert torch.equal(stats, clean)
+
+
+@pytest.mark.parametrize("shape", [(2, 400, 32, 2), (1, 3001, 48, 1), (3, 9, 33, 3), (1, 700, 2048, 512)], ids=str)
+@pytest.mark.parametrize("mean,std", [(1e6, 0.25), (-3e5, 0.1), (1e4, 1e-2)])
+def test_group_norm_cl_of_small_deviations(device, shape, mean, std):
+    """Means of 10^6 and more deviations: the statistics to 1e-10, as of any other data, and the output to the float
+    roundings of x - mean. The first token of one slice is 0, which the sums are then taken from."""
+    B, T, C, G = shape
+    x = randn(device, (B, T, C), 551, std, mean)
+    x[0, 0] = 0.0
+    w, b = randn(device, (C,), 552, 0.3, 1.0), randn(device, (C,), 553)
+    y, stats = stx.group_norm_cl(x, G, 1e-5, w, b)
+    ref = norm_ref(x, G, 1e-5, w, b, "none")
+    assert torch.allclose(stats, ref["stats"], rtol=1e-10, atol=1e-13)
+    close(y, ref["y"], ref["ey"], "y")
+    if B > 1:
+        ws = torch.empty(stx.group_norm_cl_workspace_size(x, G), dtype=torch.uint8, device=device)
+        again, s2 = stx.group_norm_cl(x, G, 1e-5, w, b, out=x, workspace=ws)      # in place: the first elements are overwritten
+        assert torch.equal(again, y) and torch.equal(s2, stats)
