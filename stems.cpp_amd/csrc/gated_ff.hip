@@ -524,7 +524,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
                 if constexpr (MODE == FORWARD) {
                     float h[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) h[r] = act_f32<act()>(acc[j][m][r]) * acc[j + 1][m][r];
+                    for (int r = 0; r < 4; r++) h[r] = act_f32<act(), T>(acc[j][m][r]) * acc[j + 1][m][r];
                     if constexpr (WIDE) pack(here, h);
                     else if (row < a.M) store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.J - n, h);
                 } else {
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         float d;
-                        const float g = act_f32<act()>(acc[j][m][r], d);
+                        const float g = act_f32<act(), T>(acc[j][m][r], d);
                         const bool in = whole() || (row < a.M && n + r < a.J);   // what lies past the edges may be anything, NaN too
                         dg[r] = in ? dh[r] * acc[j + 1][m][r] * d : 0.f;
                         dv[r] = in ? dh[r] * g : 0.f;
@@ -735,7 +735,7 @@ __global__ __launch_bounds__(512) void ff_few_kernel(FfArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const bool in = n + r < a.J;
-        h[r] = act_f32<act()>(g[r] + (a.b[0] && in ? a.b[0][n + r] : 0.f)) * (v[r] + (a.b[1] && in ? a.b[1][n + r] : 0.f));
+        h[r] = act_f32<act(), T>(g[r] + (a.b[0] && in ? a.b[0][n + r] : 0.f)) * (v[r] + (a.b[1] && in ? a.b[1][n + r] : 0.f));
     }
     });
     store4<T>(a.out[0] + row * a.os[0] + n * (long long)sizeof(T), a.J - n, h);

@@ -299,7 +299,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
                     if constexpr (BACK) {
                         const float t = xe - k[e].mh;
                         float d;
-                        (void)act_f32<ACT>(fmaf(t, k[e].A, k[e].B), d);
+                        (void)act_f32<ACT, T>(fmaf(t, k[e].A, k[e].B), d);
                         const float dz = to_f32(f.dy[i].v[e]) * d;
                         s1[e] += dz;
                         s2[e] = fmaf(dz, t, s2[e]);
@@ -458,10 +458,10 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
                 const float t = to_f32(f.x[i].v[e]) - k[e].mh, z = fmaf(t, k[e].A, k[e].B);
                 if constexpr (BACK) {
                     float d;
-                    (void)act_f32<ACT>(z, d);
+                    (void)act_f32<ACT, T>(z, d);
                     y[e] = fmaf(t, k[e].q, fmaf(to_f32(f.dy[i].v[e]) * d, k[e].A, k[e].p));
                 } else {
-                    y[e] = act_f32<ACT>(z);
+                    y[e] = act_f32<ACT, T>(z);
                 }
             }
             store_vec<T, V>(out + at, left, y);

@@ -111,17 +111,35 @@ __device__ __forceinline__ T from_f32(float x) {
     return (T)x;
 }
 
-// 1 / (1 + exp(-z)) on the hardware's 2^y and reciprocal (1 ulp each): the rounding of y = -z log2 e
-// costs |z| ulps of exp(-z), which the result meets only where exp(-z) dominates it, z < 0. Four
-// instructions; with a library exp the epilogue of the gated block took longer than its products.
-__device__ __forceinline__ float sigmoid_f32(float z) {
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+// exp(-z) on the hardware's 2^y (1 ulp), y = -z log2 e. Rounding y costs |z| / 2 ulps. FINE, for fp32
+// results, adds what was rounded off (two more ulps at any z, five instructions); for 16-bit
+// ones those ulps lie 2^12 below their own. The rest is held to [-1, 1] for infinite z.
+template <bool FINE>
+__device__ __forceinline__ float exp_neg(float z) {
+    constexpr float C1 = -0x1.715476p0f, C2 = -0x1.4ae0cp-26f;       // -log2 e
+    const float y = z * (FINE ? C1 : -1.44269504088896340736f), e = __builtin_amdgcn_exp2f(y);
+    if constexpr (!FINE) return e;
+    const float rest = __builtin_amdgcn_fmed3f(fmaf(z, C2, fmaf(z, C1, -y)), -1.f, 1.f);
+    return e * fmaf(rest, 0.69314718055994530942f, 1.f);
 }
 
-// Phi(z), the normal distribution, and phi = exp(-z^2/2): Phi(-|z|) = phi t P(t) / 2 with
-// t = 1 / (1 + |z| / (2 sqrt2)), P the polynomial of stx_gelu_erf (gelu_phi_neg in ops.hip).
-__device__ __forceinline__ float normal_cdf(float z, float& phi) {
-    phi = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f);   // z^2 / 2 ulps, in the tails
+// s = 1 / (1 + exp(-z)), and r = 1 - s, not by a subtraction where s is near 1.
+template <bool FINE>
+__device__ __forceinline__ float sigmoid_f32(float z) { return __builtin_amdgcn_rcpf(1.f + exp_neg<FINE>(z)); }
+template <bool FINE>
+__device__ __forceinline__ float sigmoid_f32(float z, float& r) {
+    const float e = exp_neg<FINE>(z), s = __builtin_amdgcn_rcpf(1.f + e);
+    r = z > 0.f ? e * s : 1.f - s;
+    return s;
+}
+
+// Phi(z), the normal distribution, and zphi = z exp(-z^2/2): Phi(-|z|) = exp(-z^2/2) t P(t) / 2 with
+// t = 1 / (1 + |z| / (2 sqrt2)), P the polynomial of stx_gelu_erf (gelu_phi_neg in ops.hip). Rounding the
+// exponent costs z^2 / 4 ulps, and 2^y ends at 2^-126. FINE, for fp32 results, forms q = exp(-z^2/4) from an
+// exponent in two parts, whose square neither loses them nor ends before fp32 does, seven
+// instructions more; |z| is taken as 18 at most there, where q^2 is 0.
+template <bool FINE>
+__device__ __forceinline__ float normal_cdf(float z, float& zphi) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.35355339059327376220f, fabsf(z), 1.f));
     float p = -1.5161373655e-02f;
     p = fmaf(p, t, 9.183117002e-02f);
@@ -136,29 +154,45 @@ __device__ __forceinline__ float normal_cdf(float z, float& phi) {
     p = fmaf(p, t, 1.234102100e-01f);
     p = fmaf(p, t, 1.4104762675e-01f);
     p = fmaf(p, t, 1.410473883e-01f);
-    const float q = phi * (t * p);
-    return z < 0.f ? q : 1.f - q;
+    float tail;
+    if constexpr (FINE) {
+        constexpr float C1 = -0x1.715476p-2f, C2 = -0x1.4ae0cp-28f;  // -log2 e / 4
+        const float c = __builtin_amdgcn_fmed3f(z, -18.f, 18.f), h = c * c, y = h * C1;
+        const float rest = fmaf(h, C2, fmaf(fmaf(c, c, -h), C1, fmaf(h, C1, -y)));
+        float q = __builtin_amdgcn_exp2f(y);
+        q = fmaf(q, rest * 0.69314718055994530942f, q);
+        tail = q * (q * (t * p));
+        zphi = c * q * q;
+    } else {
+        const float phi = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f);
+        tail = phi * (t * p);
+        zphi = z * phi;
+    }
+    return z < 0.f ? tail : 1.f - tail;
 }
 
-// act(z), and its derivative d.
-template <int ACT>
+// act(z), and its derivative d, for results of type T.
+template <int ACT, class T>
 __device__ __forceinline__ float act_f32(float z) {
-    float phi;
-    if constexpr (ACT == STX_ACT_GELU) return z * normal_cdf(z, phi);
-    if constexpr (ACT == STX_ACT_SILU) return z * sigmoid_f32(z);
-    if constexpr (ACT == STX_ACT_SIGMOID) return sigmoid_f32(z);
+    constexpr bool FINE = sizeof(T) == 4;
+    float zphi;
+    if constexpr (ACT == STX_ACT_GELU) return z * normal_cdf<FINE>(z, zphi);
+    if constexpr (ACT == STX_ACT_SILU) return z * sigmoid_f32<FINE>(z);
+    if constexpr (ACT == STX_ACT_SIGMOID) return sigmoid_f32<FINE>(z);
     return z;
 }
-template <int ACT>
+template <int ACT, class T>
 __device__ __forceinline__ float act_f32(float z, float& d) {
+    constexpr bool FINE = sizeof(T) == 4;
     if constexpr (ACT == STX_ACT_GELU) {
-        float phi;
-        const float c = normal_cdf(z, phi);
-        d = fmaf(z * phi, 0.39894228040143267794f, c);               // Phi + z phi / sqrt(2 pi)
+        float zphi;
+        const float c = normal_cdf<FINE>(z, zphi);
+        d = fmaf(zphi, 0.39894228040143267794f, c);                 // Phi + z phi / sqrt(2 pi)
         return z * c;
     } else if constexpr (ACT == STX_ACT_SILU || ACT == STX_ACT_SIGMOID) {
-        const float s = sigmoid_f32(z);
-        d = ACT == STX_ACT_SILU ? s * fmaf(z, 1.f - s, 1.f) : s * (1.f - s);
+        float r;
+        const float s = sigmoid_f32<FINE>(z, r);
+        d = ACT == STX_ACT_SILU ? s * fmaf(z, r, 1.f) : s * r;
         return ACT == STX_ACT_SILU ? z * s : s;
     } else {
         d = 1.f;

@@ -183,3 +183,58 @@ def test_group_norm_cl_of_small_deviations(device, shape, mean, std):
         ws = torch.empty(stx.group_norm_cl_workspace_size(x, G), dtype=torch.uint8, device=device)
         again, s2 = stx.group_norm_cl(x, G, 1e-5, w, b, out=x, workspace=ws)      # in place: the first elements are overwritten
         assert torch.equal(again, y) and torch.equal(s2, stats)
+
+
+# ---------------------------------------------------------------------------- activations
+# fp32, from the evaluations: 2^y and the reciprocal 1 ulp (2 u) each, the polynomial of GELU 2 u, products and sums u
+# each. GELU: q = exp(-z^2/4) within 5 u twice, the rest 6 u: 16 u. Sigmoid: exp(-z) within 5 u, and 4 u: 9 u; SiLU 10 u; 1 - s
+# within 16 u on either side. Results below 2^-126 come from subnormal factors, each rounded to 2^-150, times |z| < 16.
+TINY = 16 * 2.0 ** -149
+
+
+def grid(device, act, top=12.0):
+    z = torch.linspace(-14.3 if act == "gelu" else -86.0, top, 60000, dtype=F64, device=device).to(torch.float32)
+    return torch.cat([z, -torch.logspace(-30, 0, 500, device=device), torch.tensor([0.0, 1e30, -1e30, -200.0, 200.0], device=device)])
+
+
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("act,most", [("gelu", 16), ("silu", 10), ("sigmoid", 9)])
+def test_fp32_activations_in_the_tails(device, few, act, most):
+    """act(z) in fp32 to a few u of itself, wherever it is small: z as one token's gate products, or as many tokens'."""
+    z, one = grid(device, act), torch.ones(1, 1, device=device)
+    x, w = (one, z[:, None]) if few else (z[:, None], one)
+    h = stx.gated_ff(x, w, torch.zeros_like(w), ACTS[act], b_value=torch.ones_like(w[:, 0])).flatten()
+    want = act_ref(z.to(F64).clamp_min(-1000), act)[0]
+    off = ((h.to(F64) - want).abs() - TINY).clamp_min(0)
+    assert bool((off <= most * U * want.abs()).all()), (float((off / want.abs().clamp_min(TINY)).max()) / U, float(z[(off / want.abs().clamp_min(TINY)).argmax()]))
+
+
+@pytest.mark.parametrize("op", ["norm", "gated"])
+@pytest.mark.parametrize("act", ["gelu", "silu", "sigmoid"])
+def test_fp32_slopes_in_the_tails(device, op, act):
+    """act'(z) in fp32, as the bias's gradient of one token: the same bounds of its factors."""
+    z = grid(device, act, 40.0)
+    n = z.numel()
+    if op == "norm":
+        stats = torch.tensor([[[0.0, 1.0]]], dtype=F64, device=device)             # xhat is x
+        d = stx.group_norm_cl_back(torch.ones(1, n, device=device), z[None], stats, 1, act=ACTS[act])[2]
+    else:
+        d = stx.gated_ff_back(torch.ones(1, n, device=device), torch.ones(1, 1, device=device), z[:, None], torch.zeros(n, 1, device=device), ACTS[act],
+                              torch.zeros(n, device=device), torch.ones(n, device=device))[3]
+    y = z.to(F64).clamp(-1000, 1000)
+    want = act_ref(y, act)[1]
+    s, r = torch.sigmoid(y), torch.sigmoid(-y)
+    scale = {"gelu": 16 * (0.5 * torch.erfc(-y / math.sqrt(2.0)) + y.abs() * torch.exp(-y * y / 2) * 0.4), "sigmoid": 26 * s * r, "silu": 26 * s * (1 + y.abs() * r)}[act]
+    off = ((d.to(F64) - want).abs() - TINY).clamp_min(0)
+    assert bool((off <= U * scale).all()), (float((off / scale.clamp_min(TINY)).max()) / U, float(z[(off / scale.clamp_min(TINY)).argmax()]))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_half_slopes_of_open_gates(device, dtype):
+    """The slope of a sigmoid near 1 keeps its digits in 16-bit data too: 26 u and the exponent's |z| u."""
+    z = torch.linspace(-30, 30, 2001, device=device).to(TYPES[dtype])
+    n, dt = z.numel(), TYPES[dtype]
+    d = stx.gated_ff_back(torch.ones(1, n, device=device, dtype=dt), torch.ones(1, 1, device=device, dtype=dt), z[:, None], torch.zeros(n, 1, device=device, dtype=dt),
+                          stx.ACT_SIGMOID, torch.zeros(n, device=device), torch.ones(n, device=device))[3]
+    want = act_ref(z.to(F64), "sigmoid")[1]
+    assert bool(((d.to(F64) - want).abs() <= (26 + z.to(F64).abs()) * U * want).all())
