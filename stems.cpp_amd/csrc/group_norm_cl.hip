@@ -196,7 +196,8 @@ __device__ __forceinline__ void fold_rows(double2* red, int rows, int width) {
 // Per-channel constants, all of the centred t = x - mh, where mean = mh + a rest that joins the
 // additive constants (a float mean alone would cost |mean| 2^-24 / std; a product x r - mean r, which
 // would save the subtraction, costs as much):
-//   xhat = t r - d,  z = xhat w + b = t A + B,  dx = r (w dz - S1/n - xhat S2/n) = t q + (dz A + p).
+//   xhat = t r - d,  z = xhat w + b = t A + B,  dx = r (w dz - S1/n - xhat S2/n) = t r q + (dz A + p).
+// (r q as one constant would hold r^2, which leaves fp32 where the data's deviations pass 10^19.)
 struct Chan {
     float mh, r, d, A, B, p, q;
     __device__ __forceinline__ void set(const NormArgs& a, double mean, double rstd, int c) {
@@ -210,7 +211,7 @@ struct Chan {
     }
     __device__ __forceinline__ void set_back(double mean, double rstd, double s1, double s2) {   // S1 / n, S2 / n
         p = (float)(((mean - (double)mh) * rstd * s2 - s1) * rstd);
-        q = (float)(-rstd * rstd * s2);
+        q = (float)(-rstd * s2);
     }
 };
 
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
                 if constexpr (BACK) {
                     float d;
                     (void)act_f32<ACT, T>(z, d);
-                    y[e] = fmaf(t, k[e].q, fmaf(to_f32(f.dy[i].v[e]) * d, k[e].A, k[e].p));
+                    y[e] = fmaf(t * k[e].r, k[e].q, fmaf(to_f32(f.dy[i].v[e]) * d, k[e].A, k[e].p));
                 } else {
                     y[e] = act_f32<ACT, T>(z);
                 }

@@ -238,3 +238,19 @@ def test_half_slopes_of_open_gates(device, dtype):
                           stx.ACT_SIGMOID, torch.zeros(n, device=device), torch.ones(n, device=device))[3]
     want = act_ref(z.to(F64), "sigmoid")[1]
     assert bool(((d.to(F64) - want).abs() <= (26 + z.to(F64).abs()) * U * want).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [1e24, 1e-22])
+def test_group_norm_cl_gradient_at_the_ranges_ends(device, dtype, scale):
+    """Data whose variance lies beyond fp32 (and without eps below it): the gradients of the same data at scale 1, bound
+    and all, divided by the scale."""
+    dt = TYPES[dtype]
+    x, dy = (randn(device, (2, 60, 24), 561 + i, scale if i == 0 else 1.0, dtype=dt) for i in range(2))
+    w, b = randn(device, (24,), 563, 0.3, 1.0), randn(device, (24,), 564, 0.3)
+    ref = norm_ref(x, 3, 0.0, w, b, "silu", dy)
+    y, stats = stx.group_norm_cl(x, 3, 0.0, w, b, stx.ACT_SILU)
+    close(y, ref["y"], ref["ey"], "y")
+    dx, dw, db = stx.group_norm_cl_back(dy, x, stats, 3, w, b, stx.ACT_SILU)
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        close(got, ref[name], ref["e" + name], name)
