@@ -743,8 +743,9 @@ __global__ __launch_bounds__(512) void ff_few_kernel(FfArgs a) {
 
 // Sums of the parts of a split reduction, in order: part [splits][W][rows][cols] to out[w][rows][cols].
 template <class T, int V>
-__global__ __launch_bounds__(256) void ff_fold_kernel(const float* part, int splits, long long rows, int cols, int w, char* o0, char* o1, long long s0, long long s1) {
-    const long long n = rows * cols, i = (blockIdx.x * 256LL + threadIdx.x) * V;
+__global__ __launch_bounds__(256) void ff_fold_kernel(const float* part, int splits, long long rows, int cols, int w, char* o0, char* o1, long long s0, long long s1,
+                                                     unsigned base) {
+    const long long n = rows * cols, i = ((base + blockIdx.x) * 256LL + threadIdx.x) * V;
     if (i >= w * n) return;
     float s[V] = {};
 #pragma unroll 4
@@ -966,12 +967,14 @@ void fold(const float* part, int splits, long long rows, int cols, int w, char* 
     const long long n = rows * cols * w;
     auto launch = [&](auto v) {
         constexpr int V = v();
-        hipLaunchKernelGGL((ff_fold_kernel<T, V>), dim3((unsigned)((n / V + 255) / 256)), dim3(256), 0, stream, part, splits, rows, cols, w, o0, o1, s0, s1);
+        launch_all((n / V + 255) / 256, [&](dim3 grid, unsigned first) {
+            hipLaunchKernelGGL((ff_fold_kernel<T, V>), grid, dim3(256), 0, stream, part, splits, rows, cols, w, o0, o1, s0, s1, first);
+            launch_check("ff_fold_kernel");
+        });
     };
     STX_REQUIRE(n / 256 < (1LL << 31), "gated_ff_back: gradients too large");
     if (cols % 4 == 0) launch(std::integral_constant<int, 4>{});
     else launch(std::integral_constant<int, 1>{});
-    launch_check("ff_fold_kernel");
 }
 
 template <class T>

@@ -97,6 +97,7 @@ struct NormArgs {
     double* shift;                       // [B][G], forward: what the sums are taken from
     double2* slot;                       // backward: [B][chunks][slots]
     long long rows;                      // of `part`, or 1 where they are folded (0: no elements)
+    unsigned base;                       // blocks of the launches before this one
     unsigned first;                      // backward: apply blocks before this one add dweight and dbias
     float *dw, *db;
     double eps;
@@ -245,7 +246,7 @@ template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
     constexpr int V = kVec;
     __shared__ double2 red[kThreads * V];
-    const Place p = place(a, blockIdx.x);
+    const Place p = place(a, a.base + blockIdx.x);
     const int width = a.g.cols * V, first = p.tile * width, here = min(width, a.g.slots - first);
     double2* mine = red + p.row * width + (int)threadIdx.x % a.g.cols * V;
     if (p.row < a.g.rws) {
@@ -353,7 +354,8 @@ __global__ __launch_bounds__(kThreads) void gn_cl_sums_kernel(NormArgs a) {
 // The pairs of one group of one slice.
 __global__ __launch_bounds__(kThreads) void gn_cl_fold_kernel(NormArgs a, long long rows) {
     __shared__ double2 red[kThreads];
-    const long long b = blockIdx.x / (unsigned)a.g.G, g = blockIdx.x % (unsigned)a.g.G;
+    const unsigned bid = a.base + blockIdx.x;
+    const long long b = bid / (unsigned)a.g.G, g = bid % (unsigned)a.g.G;
     double2 s = make_double2(0.0, 0.0);
 #pragma unroll 4
     for (long long r = threadIdx.x; r < rows; r += kThreads) {
@@ -363,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_fold_kernel(NormArgs a, long l
     }
     red[threadIdx.x] = s;
     fold_rows(red, kThreads, 1);
-    if (threadIdx.x == 0) a.folded[blockIdx.x] = red[0];
+    if (threadIdx.x == 0) a.folded[bid] = red[0];
 }
 
 __device__ __forceinline__ double2 moments(const NormArgs& a, double2 s, double n, long long at) {
@@ -396,8 +398,9 @@ template <class T, bool BACK, int ACT>
 __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
     constexpr int V = kVec;
     extern __shared__ double2 groups[];                  // [max(G, kThreads)]
-    if (BACK && blockIdx.x < a.first) return add_params(a, groups, blockIdx.x);
-    const Place p = place(a, blockIdx.x - a.first);
+    const unsigned bid = a.base + blockIdx.x;
+    if (BACK && bid < a.first) return add_params(a, groups, bid);
+    const Place p = place(a, bid - a.first);
     {
         const int G = a.g.G, parts = max(1, kThreads / G);
         const double2* from = a.part + p.slice * a.rows * G;
@@ -518,21 +521,28 @@ void run_norm(NormArgs& a, stx_type type, void* ws, hipStream_t stream) {
     with_type(type, [&](auto t) {
         using T = decltype(t);
         if (g.srows && g.B) {
-            if constexpr (BACK) with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_sums_kernel<T, true, act()>), dim3(blocks), dim3(kThreads), 0, stream, a); });
-            else hipLaunchKernelGGL((gn_cl_sums_kernel<T, false, STX_ACT_NONE>), dim3(blocks), dim3(kThreads), 0, stream, a);
-            launch_check("gn_cl_sums_kernel");
+            launch_all(blocks, [&](dim3 grid, unsigned first) {
+                a.base = first;
+                if constexpr (BACK) with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_sums_kernel<T, true, act()>), grid, dim3(kThreads), 0, stream, a); });
+                else hipLaunchKernelGGL((gn_cl_sums_kernel<T, false, STX_ACT_NONE>), grid, dim3(kThreads), 0, stream, a);
+                launch_check("gn_cl_sums_kernel");
+            });
         }
         const bool apply = !BACK || a.out;
         if (folds(g) && g.B && apply) {
-            hipLaunchKernelGGL(gn_cl_fold_kernel, dim3((unsigned)(g.B * g.G)), dim3(kThreads), 0, stream, a, a.rows);
-            launch_check("gn_cl_fold_kernel");
+            launch_all(g.B * g.G, [&](dim3 grid, unsigned first) {
+                a.base = first;
+                hipLaunchKernelGGL(gn_cl_fold_kernel, grid, dim3(kThreads), 0, stream, a, a.rows);
+                launch_check("gn_cl_fold_kernel");
+            });
             a.part = a.folded;
             a.rows = 1;
         }
-        const unsigned grid = a.first + (apply ? blocks : 0);
-        if (grid == 0) return;
-        with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_apply_kernel<T, BACK, act()>), dim3(grid), dim3(kThreads), sizeof(double2) * std::max(g.G, kThreads), stream, a); });
-        launch_check("gn_cl_apply_kernel");
+        launch_all(a.first + (apply ? blocks : 0), [&](dim3 grid, unsigned first) {
+            a.base = first;
+            with_act(a.act, [&](auto act) { hipLaunchKernelGGL((gn_cl_apply_kernel<T, BACK, act()>), grid, dim3(kThreads), sizeof(double2) * std::max(g.G, kThreads), stream, a); });
+            launch_check("gn_cl_apply_kernel");
+        });
     });
 }
 

@@ -32,6 +32,7 @@ struct RopeScaledArgs {
     const float* factors;
     long long pos_stride;
     unsigned tokens, tile;               // all tokens, and of a block
+    unsigned base;                       // blocks of the launches before this one
     FastDiv n;                           // ne2: token -> (i3, i2)
     FastDiv rows, units;                 // rows of a token (q's, then k's); units of a row
     unsigned q_rows;
@@ -99,7 +100,7 @@ template <class T, int V, bool VEC, int MODE>
 __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(RopeScaledArgs a) {
     extern __shared__ float2 cs[];       // [tile][n_dims / 2]
     const int half = a.n_dims / 2;
-    const unsigned t0 = blockIdx.x * a.tile;
+    const unsigned t0 = (a.base + blockIdx.x) * a.tile;
     const unsigned nt = min(a.tile, a.tokens - t0);
     for (unsigned e = threadIdx.x; e < nt * (unsigned)half; e += kRopeThreads) {
         const unsigned t = t0 + e / (unsigned)half;
@@ -184,11 +185,14 @@ RopeSide side_of(const stx_tensor* s, const stx_tensor* d) {
 }
 
 template <class T, int V, bool VEC>
-void rope_launch(const RopeScaledArgs& a, int mode, size_t lds, hipStream_t stream) {
-    const dim3 grid((a.tokens + a.tile - 1) / a.tile), block(kRopeThreads);
-    if (mode == 0) hipLaunchKernelGGL((rope_scaled_kernel<T, VEC ? V : 2, VEC, 0>), grid, block, lds, stream, a);
-    else hipLaunchKernelGGL((rope_scaled_kernel<T, VEC ? V : 1, VEC, 2>), grid, block, lds, stream, a);
-    launch_check("rope_scaled_kernel");
+void rope_launch(RopeScaledArgs a, int mode, size_t lds, hipStream_t stream) {
+    launch_all((a.tokens + a.tile - 1) / a.tile, [&](dim3 grid, unsigned first) {
+        const dim3 block(kRopeThreads);
+        a.base = first;
+        if (mode == 0) hipLaunchKernelGGL((rope_scaled_kernel<T, VEC ? V : 2, VEC, 0>), grid, block, lds, stream, a);
+        else hipLaunchKernelGGL((rope_scaled_kernel<T, VEC ? V : 1, VEC, 2>), grid, block, lds, stream, a);
+        launch_check("rope_scaled_kernel");
+    });
 }
 
 void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos, int64_t pos_stride,

@@ -2,6 +2,7 @@
 // typed tensors on the host, conversions, vector access and activations on the device.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "tensor.hpp"
@@ -90,6 +91,15 @@ inline void check_workspace(const void* ws, size_t have, size_t need, const char
     if (need == 0) return;
     STX_REQUIRE(ws != nullptr && have >= need, "%s: workspace of %zu bytes needed, %zu given", what, need, ws ? have : (size_t)0);
     STX_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, "%s: the workspace must be 256-byte aligned", what);
+}
+
+// Calls launch(grid, first) for blocks in turn, `first` the number of those before: a launch has at
+// most 2^32 - 1 threads (here 2^31 of blocks of 256).
+template <class F>
+void launch_all(unsigned long long blocks, F&& launch) {
+    constexpr unsigned kMost = 1u << 23;
+    for (unsigned long long first = 0; first < blocks; first += kMost)
+        launch(dim3((unsigned)std::min<unsigned long long>(kMost, blocks - first)), (unsigned)first);
 }
 
 // ------------------------------------------------------------------------------- device

@@ -254,3 +254,43 @@ def test_group_norm_cl_gradient_at_the_ranges_ends(device, dtype, scale):
     dx, dw, db = stx.group_norm_cl_back(dy, x, stats, 3, w, b, stx.ACT_SILU)
     for name, got in (("dx", dx), ("dw", dw), ("db", db)):
         close(got, ref[name], ref["e" + name], name)
+
+
+# ------------------------------------------------------------------------------- large calls
+def test_group_norm_cl_of_more_slices_than_a_launch_has_blocks(device):
+    """2^24 slices and a few of one token: a workgroup each, more than a launch may have."""
+    B, C = (1 << 24) + 3, 8
+    x = randn(device, (B, 1, C), 571, dtype=torch.bfloat16)
+    y, stats = stx.group_norm_cl(x, 2, act=stx.ACT_SILU)
+    dx, dw, db = stx.group_norm_cl_back(x, x, stats, 2, act=stx.ACT_SILU)
+    sums = torch.zeros(2, C, dtype=F64, device=device)
+    bound = torch.zeros(2, C, dtype=F64, device=device)
+    for part in torch.arange(B, device=device).split(1 << 21):
+        s = slice(int(part[0]), int(part[-1]) + 1)
+        v = x[s].view(-1, 2, 4)                                                   # a group is a slice of its own
+        ref = norm_ref(v.reshape(-1, 4, 1), 1, 1e-5, None, None, "silu", v.reshape(-1, 4, 1))
+        close(y[s].view(-1, 4, 1), ref["y"], ref["ey"], "y")
+        close(dx[s].view(-1, 4, 1), ref["dx"], ref["edx"], "dx")
+        assert torch.allclose(stats[s].view(-1, 1, 2), ref["stats"], rtol=1e-10, atol=1e-13)
+        z = (v.to(F64) - ref["stats"][:, 0, 0].view(-1, 2, 1)) * ref["stats"][:, 0, 1].view(-1, 2, 1)
+        d = v.to(F64) * act_ref(z, "silu")[1]
+        e = (64 * U * (1 + z.abs()) * v.to(F64).abs()).flatten(1)
+        sums += torch.stack([(d * z).flatten(1).sum(0), d.flatten(1).sum(0)])
+        bound += torch.stack([(e * (1 + z.abs().flatten(1))).sum(0), e.sum(0)])
+    close(dw, sums[0], bound[0], "dw")
+    close(db, sums[1], bound[1], "db")
+
+
+def test_rope_of_more_tokens_than_a_launch_has_blocks(device):
+    """2^24 tokens and a few, a workgroup each (rows of odd halves, element by element), in place: the first and the last."""
+    N, H, D = (1 << 24) + 3, 2, 514
+    q = torch.zeros(1, N, H, D, dtype=torch.bfloat16, device=device)
+    at = [0, 1, (1 << 23) - 1, 1 << 23, (1 << 24) - 1, 1 << 24, N - 1]
+    x = randn(device, (1, len(at), H, D), 572, dtype=torch.bfloat16)
+    q[:, at] = x
+    pos = torch.arange(N, device=device, dtype=torch.int32)
+    stx.rope_scaled(q, pos, stx.rope_params(D, 2), out=q)
+    want, mag = rope_ref(x, pos[at], D, 2)
+    close(q[:, at], want, 4 * U * mag, "rope")
+    del q
+    torch.cuda.empty_cache()
