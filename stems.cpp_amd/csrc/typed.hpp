@@ -202,6 +202,7 @@ __device__ __forceinline__ float act_f32(float z, float& d) {
     } else if constexpr (ACT == STX_ACT_SILU || ACT == STX_ACT_SIGMOID) {
         float r;
         const float s = sigmoid_f32<FINE>(z, r);
+        if (ACT == STX_ACT_SILU && !FINE) r = 1.f - s;               // beside 1 its digits do not count in 16 bits (4 % of a gradient's time)
         d = ACT == STX_ACT_SILU ? s * fmaf(z, r, 1.f) : s * r;
         return ACT == STX_ACT_SILU ? z * s : s;
     } else {
