@@ -825,7 +825,9 @@ STX_API stx_status stx_rope_scaled_back(const stx_tensor* q, const stx_tensor* k
  * weight and bias: device float[C], either may be NULL (1 and 0). stats: device double
  * [B][n_groups][2], receives mean and 1 / sqrt(var + eps) for stx_group_norm_cl_back (NULL: not
  * kept); without elements (T1 or T2 0) they are 0 and 1 / sqrt(eps). dst may be a. workspace:
- * device, 256-byte aligned, no initialisation; calls that share one must not overlap. */
+ * device, 256-byte aligned, no initialisation; calls that share one must not overlap. Its size is
+ * enough for the gradients too; stx_group_norm_cl_forward_workspace_size (below) gives what this call needs,
+ * which for many short slices is a small part of it. Fewer than 2^30 slices. */
 STX_API size_t     stx_group_norm_cl_workspace_size(const stx_tensor* a, stx_type type, int n_groups);
 STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_groups, double eps, const float* weight,
                                      const float* bias, stx_act act, const stx_tensor* dst, double* stats,
@@ -867,6 +869,10 @@ STX_API stx_status stx_gated_ff_back(const stx_tensor* dh, const stx_tensor* x, 
                                      stx_act act, const stx_tensor* dx, const stx_tensor* dw_gate,
                                      const stx_tensor* dw_value, float* db_gate, float* db_value, void* workspace,
                                      size_t workspace_bytes, stx_stream stream);
+
+/* Workspace of stx_group_norm_cl alone: without the sums of a slice's positions that its gradients
+ * add up to dweight and dbias. */
+STX_API size_t     stx_group_norm_cl_forward_workspace_size(const stx_tensor* a, stx_type type, int n_groups);
 
 /* ------------------------------------------------------------------------------------------
  * Versioned function table (after libstems V1, src/libstems_v1.h:146-189). Every entry point
@@ -1087,6 +1093,7 @@ typedef struct stx_api_v1 {
                                 const stx_tensor* dw_gate, const stx_tensor* dw_value,
                                 float* db_gate, float* db_value, void* workspace,
                                 size_t workspace_bytes, stx_stream stream);
+    size_t (*group_norm_cl_forward_workspace_size)(const stx_tensor* a, stx_type type, int n_groups);
     void (*reserved[16])(void);
 } stx_api_v1;
 

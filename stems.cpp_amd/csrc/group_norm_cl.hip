@@ -476,7 +476,7 @@ __global__ __launch_bounds__(kThreads) void gn_cl_apply_kernel(NormArgs a) {
 long long pair_rows(const Geometry& g) { return g.srows ? (long long)g.chunks * g.tiles : 0; }
 bool folds(const Geometry& g) { return pair_rows(g) > 1 && (g.G > kThreads || pair_rows(g) * g.G > kDirect); }
 struct Spaces {
-    size_t folded, shift, slot, total;   // `part` is at 0
+    size_t folded, shift, slot, total;   // `part` is at 0; the forward call needs no slot
 };
 Spaces spaces(const Geometry& g) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -551,17 +551,27 @@ void run_norm(NormArgs& a, stx_type type, void* ws, hipStream_t stream) {
 
 using namespace stx;
 
-extern "C" {
-
-STX_API size_t stx_group_norm_cl_workspace_size(const stx_tensor* a, stx_type type, int n_groups) {
+namespace {
+size_t query(const stx_tensor* a, stx_type type, int n_groups, size_t Spaces::*size) {
     size_t bytes = 0;
     (void)guard([&] {
         STX_REQUIRE(a != nullptr, "group_norm_cl: a is NULL");
         stx_tensor t = *a;
         t.data = reinterpret_cast<void*>((uintptr_t)256);          // a query may have no data yet
-        bytes = spaces(check_norm(&t, type, n_groups)).total;
+        bytes = spaces(check_norm(&t, type, n_groups)).*size;
     });
     return bytes;
+}
+}  // namespace
+
+extern "C" {
+
+STX_API size_t stx_group_norm_cl_workspace_size(const stx_tensor* a, stx_type type, int n_groups) {
+    return query(a, type, n_groups, &Spaces::total);
+}
+
+STX_API size_t stx_group_norm_cl_forward_workspace_size(const stx_tensor* a, stx_type type, int n_groups) {
+    return query(a, type, n_groups, &Spaces::slot);
 }
 
 STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_groups, double eps, const float* weight,
@@ -577,7 +587,7 @@ STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_g
         STX_REQUIRE(contiguous_typed(dst, size), "group_norm_cl: dst must be contiguous");
         STX_REQUIRE(dst->data == a->data || !overlap(span_of(a, size), span_of(dst, size)), "group_norm_cl: dst overlaps a in part");
         STX_REQUIRE(eps >= 0.0, "group_norm_cl: negative eps");
-        check_workspace(workspace, workspace_bytes_, spaces(k.g).total, "group_norm_cl");
+        check_workspace(workspace, workspace_bytes_, spaces(k.g).slot, "group_norm_cl");
         k.x = a->data;
         k.dy = a->data;                  // not read
         k.out = dst->data;

@@ -125,6 +125,7 @@ _SIGNATURES = {
     "stx_rope_scaled": (_i, [_vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp]),
     "stx_rope_scaled_back": (_i, [_vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp]),
     "stx_group_norm_cl_workspace_size": (ctypes.c_size_t, [_vp, _i, _i]),
+    "stx_group_norm_cl_forward_workspace_size": (ctypes.c_size_t, [_vp, _i, _i]),
     "stx_group_norm_cl": (_i, [_vp, _i, _i, ctypes.c_double, _vp, _vp, _i, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "stx_group_norm_cl_back": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "stx_gated_ff": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp]),
@@ -1263,6 +1264,10 @@ def group_norm_cl_workspace_size(x, n_groups):
     return lib().stx_group_norm_cl_workspace_size(_typed(x, x, "x", True), _type(x), int(n_groups))
 
 
+def group_norm_cl_forward_workspace_size(x, n_groups):
+    return lib().stx_group_norm_cl_forward_workspace_size(_typed(x, x, "x", True), _type(x), int(n_groups))
+
+
 def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, out=None, stats=None, workspace=None,
                   stream=None):
     """act(GroupNorm(x) * weight + bias) with the channels last: x (B, T1, T2, C), (B, T, C) or (T, C), contiguous;
@@ -1276,7 +1281,7 @@ def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, o
         stats = _empty((B, n_groups, 2), torch.float64, x, stream)
     elif stats is False:
         stats = None
-    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(dx, t, int(n_groups)), workspace, x, stream)
+    ws, nbytes, keep = _scratch(L.stx_group_norm_cl_forward_workspace_size(dx, t, int(n_groups)), workspace, x, stream)
     _launch(L.stx_group_norm_cl, x, stream, dx, t, int(n_groups), float(eps), _floats(weight, x, C, "weight"),
             _floats(bias, x, C, "bias"), int(act), _typed(out, x, "out", True),
             _floats(stats, x, B * n_groups * 2, "stats", torch.float64), ws, nbytes)

@@ -294,3 +294,16 @@ def test_rope_of_more_tokens_than_a_launch_has_blocks(device):
     close(q[:, at], want, 4 * U * mag, "rope")
     del q
     torch.cuda.empty_cache()
+
+
+def test_group_norm_cl_in_its_smaller_workspace(device):
+    """The forward call in exactly what its own query asks for: the same bits, and nothing beyond written."""
+    for shape, G in (((700, 1, 24), 8), ((3, 4001, 48), 1), ((1, 2000, 1024), 512)):
+        x = randn(device, shape, 581, dtype=torch.bfloat16)
+        need = stx.group_norm_cl_forward_workspace_size(x, G)
+        room = torch.full((need + 4096,), 77, dtype=torch.uint8, device=device)
+        y, stats = stx.group_norm_cl(x, G, workspace=room[:need])
+        assert bool((room[need:] == 77).all())
+        full = torch.empty(stx.group_norm_cl_workspace_size(x, G), dtype=torch.uint8, device=device)
+        want, s2 = stx.group_norm_cl(x, G, workspace=full)
+        assert torch.equal(y, want) and torch.equal(stats, s2)
