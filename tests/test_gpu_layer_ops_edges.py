@@ -307,3 +307,49 @@ def test_group_norm_cl_in_its_smaller_workspace(device):
         full = torch.empty(stx.group_norm_cl_workspace_size(x, G), dtype=torch.uint8, device=device)
         want, s2 = stx.group_norm_cl(x, G, workspace=full)
         assert torch.equal(y, want) and torch.equal(stats, s2)
+
+
+def test_group_norm_cl_gradient_past_32_bits(device):
+    """Slices of 2^31 bytes and more: dx of the second one's first, last and other rows, dweight and dbias against 64 bits. All
+    but every thousandth row of x and dy are 0, so the sums are those rows'; rows between them have a gradient too."""
+    B, T, C, G, step, dt = 2, 1100000, 1024, 4, 1000, torch.bfloat16
+    x, dy = (torch.zeros(B, T, C, dtype=dt, device=device) for _ in range(2))
+    for i in range(B):
+        x[i, ::step] = randn(device, (T // step, C), 591 + i, 1.0, 0.5, dtype=dt)
+        dy[i, ::step] = randn(device, (T // step, C), 593 + i, 1.0, 1.0, dtype=dt)
+    w, b = randn(device, (C,), 595, 0.3, 1.0), randn(device, (C,), 596, 0.3)
+    stats = stx.group_norm_cl(x, G, 1e-5, w, b, stx.ACT_SILU)[1]
+    dx = torch.full_like(x, float("nan"))
+    dw, db = stx.group_norm_cl_back(dy, x, stats, G, w, b, stx.ACT_SILU, dx=dx)[1:]
+    W, bias, n = w.to(F64).view(G, C // G), b.to(F64).view(G, C // G), T * (C // G)
+    sums, bounds = torch.zeros(2, C, dtype=F64, device=device), torch.zeros(2, C, dtype=F64, device=device)
+    for i in range(B):
+        v, g = (t[i, ::step].to(F64).view(-1, G, C // G) for t in (x, dy))
+        mean = v.sum((0, 2), keepdim=True) / n
+        r = (v.square().sum((0, 2), keepdim=True) / n - mean * mean + 1e-5).rsqrt()
+        assert torch.allclose(stats[i], torch.cat([mean, r]).view(2, G).t(), rtol=1e-10, atol=1e-13)
+
+        def slope(v):
+            xh = (v - mean) * r
+            z = xh * W + bias
+            return xh, act_ref(z, "silu")[1], 8 * U * ((xh * W).abs() + bias.abs()) + 32 * U * (1 + z.abs())
+
+        xh, d, ed = slope(v)
+        dz, edz = g * d, g.abs() * ed
+        s1, s2 = (W * dz).sum((0, 2), keepdim=True) / n, (W * dz * xh).sum((0, 2), keepdim=True) / n
+        e1 = (W.abs() * edz).sum((0, 2), keepdim=True) / n
+        e2 = (W.abs() * (edz * xh.abs() + 8 * U * dz.abs() * (xh.abs() + 1))).sum((0, 2), keepdim=True) / n
+        for rows in (slice(0, T, step), slice(1, T, 99991), slice(T - 3, T)):
+            v, g = (t[i, rows].to(F64).view(-1, G, C // G) for t in (x, dy))
+            xr, dr, er = slope(v)
+            wdz = W * g * dr
+            want = r * (wdz - s1 - xr * s2)
+            bound = r * ((W * g).abs() * er + e1 + e2 * xr.abs() + 8 * U * (wdz.abs() + s1.abs() + (xr * s2).abs() + s2.abs()))
+            close(dx[i, rows].view(-1, G, C // G), want, bound, f"dx of slice {i}, rows {rows}")
+        sums += torch.stack([(dz * xh).sum(0).flatten(), dz.sum(0).flatten()])
+        bounds += torch.stack([(edz * xh.abs() + 8 * U * dz.abs() * (xh.abs() + 1)).sum(0).flatten(), (edz + 4 * U * dz.abs()).sum(0).flatten()])
+    close(dw, sums[0], bounds[0], "dw")
+    close(db, sums[1], bounds[1], "db")
+    assert not bool(dx[1].isnan().any())
+    del x, dy, dx
+    torch.cuda.empty_cache()
