@@ -163,12 +163,17 @@ __device__ __forceinline__ u32x4 load_chunk(const char* p, long long left) {
 __device__ __forceinline__ unsigned lds_address(const void* p) {
     return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)p);
 }
+// m0 is named as overwritten, so that no use of the compiler's own is placed across; it warns that it
+// never allocates that register.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds(const void* p, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 template <class T>
 __device__ __forceinline__ void load4(const char* p, int left, float (&f)[4]) {
