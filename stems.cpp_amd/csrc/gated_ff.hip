@@ -103,17 +103,19 @@ enum Mode { FORWARD, GRAD, DX, DW };
 // twice as much in flight, took 5 to 10 % longer: twice the barriers), and 32 elsewhere, where an
 // operand has two or three parts.
 constexpr int step_of(Mode mode, int size) { return size == 2 && (mode == FORWARD || mode == GRAD) ? 64 : 32; }
+// Blocks of a tile (0 Large, 1 Medium, 2 Small) that a CU holds: what LDS has room for, and the registers are held to.
+constexpr int slots_of(int tile, Mode mode, stx_type type) {
+    return tile == 0 ? 1 : tile == 1 && !(type == STX_TYPE_BF16 && (mode == DX || mode == DW)) ? 2 : 3;
+}
 template <int TJ_, int TM_, int WJ_, int WM_>
 struct Tile {
     static constexpr int TJ = TJ_, TM = TM_, WJ = WJ_, WM = WM_, NT = 64 * WJ * WM;
+    template <class T, int MODE>
+    static constexpr int slots = slots_of(TJ == 256 ? 0 : TM == 128 ? 1 : 2, (Mode)MODE, type_of<T>);
 };
 using Large = Tile<256, 256, 2, 4>;
 using Medium = Tile<128, 128, 2, 2>;
 using Small = Tile<128, 64, 2, 2>;
-// Blocks of a tile (0 Large, 1 Medium, 2 Small) that a CU holds: what its registers and LDS have room for.
-constexpr int slots_of(int tile, Mode mode, stx_type type) {
-    return tile == 0 ? 1 : tile == 1 && !(type == STX_TYPE_BF16 && (mode == DX || mode == DW)) ? 2 : 3;
-}
 
 struct FfArgs {
     const char* p[2];
@@ -288,7 +290,7 @@ struct Source {
 // longer than the products), and have one stage of three planes: two would leave room for one
 // block a CU. fp16's P of DX and DW is split there too.
 template <class T, int MODE, class C, bool ALIGNED>
-__global__ __launch_bounds__(C::NT, 2) void ff_kernel(FfArgs a) {
+__global__ __launch_bounds__(C::NT, (C::template slots<T, MODE> * C::NT / 256)) void ff_kernel(FfArgs a) {
     constexpr int NT = C::NT, E = 16 / sizeof(T), TJ = C::TJ, TM = C::TM;
     constexpr int NJ = TJ / C::WJ / 16, NM = TM / C::WM / 16;       // 16 x 16 tiles of a wave
     constexpr bool GATED = MODE == FORWARD || MODE == GRAD, PS = !GATED, QS = MODE == DW;
@@ -866,8 +868,7 @@ void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
     if (tiles * parts >= (1LL << 30)) fail(STX_STATUS_UNSUPPORTED, "gated_ff: too many tiles");
     a.tiles = (int)tiles;
     a.items = (int)(tiles * parts);
-    constexpr int slots = slots_of(C::TJ == 256 ? 0 : C::TM == 128 ? 1 : 2, (Mode)MODE, type_of<T>);
-    const long long blocks = std::min<long long>(a.items, (long long)device_cus() * slots);
+    const long long blocks = std::min<long long>(a.items, (long long)device_cus() * C::template slots<T, MODE>);
     hipLaunchKernelGGL((ff_kernel<T, MODE, C, AL>), dim3(xcd_grid(blocks)), dim3(C::NT), 0, stream, a);
     launch_check("ff_kernel");
 }
