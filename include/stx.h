@@ -756,7 +756,8 @@ STX_API stx_status stx_separate_audio(const stx_audio_view* input, int model_cha
  * statistics have the types given below whatever the data's. Sums and statistics are kept in
  * 32 bits or more and results rounded once. Results are deterministic. Nothing is allocated, and
  * every call may be captured into a graph. Tensors, workspace and stream belong to the current
- * device. Inputs of no elements are valid: outputs that are sums over them are zeros.
+ * device. What a call writes overlaps nothing else that it is given, but where an operator says so;
+ * slices whose rows alternate in one buffer do not overlap. Inputs of no elements are valid: outputs that are sums over them are zeros.
  * ---------------------------------------------------------------------------------------- */
 typedef int32_t stx_type;          /* ggml's numbers of these types */
 enum {
@@ -804,7 +805,8 @@ typedef struct {
  * pos[i3 * pos_stride + i2] (pos_stride 0: every sequence has the same positions). Angles are
  * formed in double (up to 2^40 in magnitude), the rotation in float. Rows are contiguous; any
  * other strides, so q and k may be slices of a projection's output. q_dst may be q and k_dst may
- * be k; outputs overlap nothing else. At most 2^31 - 1 tokens (N * batch), 2^24 - 1 rows and
+ * be k; outputs overlap nothing else, and their strides nest (each at least the extent of the smaller
+ * ones' dimensions). At most 2^31 - 1 tokens (N * batch), 2^24 - 1 rows and
  * fewer than 2^27 elements a token. */
 STX_API stx_status stx_rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
                                    int64_t pos_stride, const stx_rope_params* params, const stx_tensor* q_dst,

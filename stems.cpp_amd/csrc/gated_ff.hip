@@ -1075,8 +1075,9 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
         const Rows d = rows_of(dst, size, "gated_ff: dst");
         check_tokens(dst, x, b.N, "dst");
         check_output(dst, d, size, "dst");
-        for (const stx_tensor* t : {x, w_gate, w_value})
-            STX_REQUIRE(!overlap(span_of(t, size), span_of(dst, size)), "gated_ff: dst overlaps an input");
+        const size_t floats = (size_t)b.N * sizeof(float);
+        check_apart("gated_ff", {{"dst", dst, size}},
+                    {{"x", x, size}, {"w_gate", w_gate, size}, {"w_value", w_value, size}, {"b_gate", b_gate, floats}, {"b_value", b_value, floats}});
         if (b.M == 0) return;
         FfArgs k = products(b, b_gate, b_value, act, size);
         k.out[0] = d.data;
@@ -1129,12 +1130,13 @@ STX_API stx_status stx_gated_ff_back(const stx_tensor* dh, const stx_tensor* x, 
             for (const stx_tensor* t : {dw_gate, dw_value}) check_same_shape(w_gate, t, "gated_ff_back: weight gradients");
             check_output(dw_gate, rg, size, "dw_gate");
             check_output(dw_value, rv, size, "dw_value");
-            STX_REQUIRE(!overlap(span_of(dw_gate, size), span_of(dw_value, size)), "gated_ff_back: dw_gate overlaps dw_value");
         }
-        for (const stx_tensor* o : {dx, dw_gate, dw_value})
-            for (const stx_tensor* i : {dh, x, w_gate, w_value})
-                STX_REQUIRE(!o || !overlap(span_of(o, size), span_of(i, size)), "gated_ff_back: an output overlaps an input");
-        check_workspace(workspace, workspace_bytes, back_plan(b.M, b.K, b.N, type).total, "gated_ff_back");
+        const size_t need = back_plan(b.M, b.K, b.N, type).total, floats = (size_t)b.N * sizeof(float);
+        check_workspace(workspace, workspace_bytes, need, "gated_ff_back");
+        check_apart("gated_ff_back",
+                    {{"dx", dx, size}, {"dw_gate", dw_gate, size}, {"dw_value", dw_value, size}, {"db_gate", db_gate, floats}, {"db_value", db_value, floats},
+                     {"the workspace", workspace, need}},
+                    {{"dh", dh, size}, {"x", x, size}, {"w_gate", w_gate, size}, {"w_value", w_value, size}, {"b_gate", b_gate, floats}, {"b_value", b_value, floats}});
         if (!dx && !dw_gate && !db_gate && !db_value) return;
         with_type(type, [&](auto t) {
             run_back<decltype(t)>(b, h, b_gate, b_value, act, dx ? &rx : nullptr, dw_gate ? &rg : nullptr, dw_value ? &rv : nullptr, db_gate,

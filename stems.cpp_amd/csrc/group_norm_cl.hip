@@ -587,7 +587,11 @@ STX_API stx_status stx_group_norm_cl(const stx_tensor* a, stx_type type, int n_g
         STX_REQUIRE(contiguous_typed(dst, size), "group_norm_cl: dst must be contiguous");
         STX_REQUIRE(dst->data == a->data || !overlap(span_of(a, size), span_of(dst, size)), "group_norm_cl: dst overlaps a in part");
         STX_REQUIRE(eps >= 0.0, "group_norm_cl: negative eps");
-        check_workspace(workspace, workspace_bytes_, spaces(k.g).slot, "group_norm_cl");
+        const size_t need = spaces(k.g).slot, floats = (size_t)k.g.C * sizeof(float);
+        check_workspace(workspace, workspace_bytes_, need, "group_norm_cl");
+        const Operand w("weight", weight, floats), b("bias", bias, floats);
+        check_apart("group_norm_cl", {{"dst", dst, size}, {"stats", stats, (size_t)k.g.B * k.g.G * sizeof(double2)}, {"the workspace", workspace, need}}, {w, b});
+        check_apart("group_norm_cl", {{"stats", stats, (size_t)k.g.B * k.g.G * sizeof(double2)}, {"the workspace", workspace, need}}, {{"a", a, size}});
         k.x = a->data;
         k.dy = a->data;                  // not read
         k.out = dst->data;
@@ -620,7 +624,12 @@ STX_API stx_status stx_group_norm_cl_back(const stx_tensor* dy, const stx_tensor
             STX_REQUIRE(dx->data == dy->data || !overlap(span_of(dy, size), span_of(dx, size)), "group_norm_cl_back: dx overlaps dy in part");
         }
         STX_REQUIRE(stats != nullptr || k.g.B == 0, "group_norm_cl_back: stats is NULL");
-        check_workspace(workspace, workspace_bytes_, spaces(k.g).total, "group_norm_cl_back");
+        const size_t need = spaces(k.g).total, floats = (size_t)k.g.C * sizeof(float);
+        check_workspace(workspace, workspace_bytes_, need, "group_norm_cl_back");
+        const Operand dw("dweight", dweight, floats), db("dbias", dbias, floats), ws("the workspace", workspace, need);
+        const Operand s("stats", stats, (size_t)k.g.B * k.g.G * sizeof(double2)), w("weight", weight, floats), b("bias", bias, floats);
+        check_apart("group_norm_cl_back", {{"dx", dx, size}, dw, db, ws}, {s, w, b});
+        check_apart("group_norm_cl_back", {dw, db, ws}, {{"dy", dy, size}, {"a", a, size}});
         if (!dx && !dweight && !dbias) return;
         k.x = a->data;
         k.dy = dy->data;

@@ -175,8 +175,10 @@ void check_out(const stx_tensor* src, const stx_tensor* dst, int size, const cha
         STX_REQUIRE(dst->ne[i] <= 1 || dst->nb[i] > 0, "%s: output stride nb[%d] is 0", what, i);
         same = same && (dst->ne[i] <= 1 || dst->nb[i] == src->nb[i]);
     }
+    STX_REQUIRE(nelem(view(dst)) == 0 || nested(dst, size), "%s: rows of the output overlap", what);
     // In place with other strides, or in part over the input, rows would be read after they were written.
     STX_REQUIRE(same || src->data != dst->data || nelem(view(src)) == 0, "%s: in place with other strides", what);
+    STX_REQUIRE(same || shared(src, dst, size) != Shared::yes, "%s: the output overlaps the input in part", what);
 }
 
 RopeSide side_of(const stx_tensor* s, const stx_tensor* d) {
@@ -205,6 +207,8 @@ void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const 
         check_out(k, k_dst, size, "rope_scaled: k");
         STX_REQUIRE(k->ne[0] == q->ne[0] && k->ne[2] == q->ne[2] && k->ne[3] == q->ne[3],
                     "rope_scaled: q and k differ in head size, tokens or batch");
+        STX_REQUIRE(shared(q_dst, k_dst, size) != Shared::yes && shared(q_dst, k, size) != Shared::yes && shared(k_dst, q, size) != Shared::yes,
+                    "rope_scaled: an output overlaps the other side's tensors");
     }
     const long long dim = q->ne[0];
     if (p->mode != 0 && p->mode != 2) fail(STX_STATUS_UNSUPPORTED, "rope_scaled: mode %d (only 0 and 2)", p->mode);

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "tensor.hpp"
@@ -86,6 +87,70 @@ inline Span span_of(const void* p, size_t bytes) {
     return p && bytes ? Span{lo, lo + bytes} : Span{0, 0};
 }
 inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+// Whether the elements of tensors can be told apart by their strides: over the dimensions of more than
+// one element the strides agree, and each is at least the extent of the dimensions below it.
+enum class Shared { no, yes, unknown };
+struct Nest {
+    int n = 0;
+    long long stride[3], na[3], nb[3];   // ascending; elements of a and of b
+    bool ok = true;
+    Nest(const stx_tensor* a, const stx_tensor* b, int size) {
+        for (int i = 1; i < 4; i++) {
+            if (a->ne[i] <= 1 && b->ne[i] <= 1) continue;
+            ok = ok && (a->ne[i] <= 1 || b->ne[i] <= 1 || a->nb[i] == b->nb[i]);
+            const long long s = a->ne[i] > 1 ? a->nb[i] : b->nb[i];
+            int at = n++;
+            for (; at > 0 && stride[at - 1] > s; at--) stride[at] = stride[at - 1], na[at] = na[at - 1], nb[at] = nb[at - 1];
+            stride[at] = s, na[at] = a->ne[i], nb[at] = b->ne[i];
+        }
+        long long extent = std::max(a->ne[0], b->ne[0]) * size;
+        for (int i = 0; i < n; i++) {
+            ok = ok && stride[i] >= extent;
+            extent += (std::max(na[i], nb[i]) - 1) * stride[i];
+        }
+    }
+    // Whether rows of a and b fall together with b's data `delta` bytes behind a's; dimensions below `i`.
+    bool meet(int i, long long delta, long long ra, long long rb) const {
+        if (i == 0) return -rb < delta && delta < ra;
+        long long la = ra, lb = rb;      // what the lower dimensions reach
+        for (int k = 0; k < i - 1; k++) la += (na[k] - 1) * stride[k], lb += (nb[k] - 1) * stride[k];
+        const long long s = stride[i - 1];
+        auto ceil = [&](long long v) { return v >= 0 ? (v + s - 1) / s : -(-v / s); };
+        // delta + d s in (-lb, la) for steps d of b's less a's: three at most, the strides being nested
+        for (long long d = std::max(1 - na[i - 1], ceil(1 - lb - delta)), last = std::min(nb[i - 1] - 1, -ceil(1 - la + delta)); d <= last; d++)
+            if (meet(i - 1, delta + d * s, ra, rb)) return true;
+        return false;
+    }
+};
+inline bool nested(const stx_tensor* t, int size) { return Nest(t, t, size).ok; }
+inline Shared shared(const stx_tensor* a, const stx_tensor* b, int size) {
+    if (!overlap(span_of(a, size), span_of(b, size))) return Shared::no;
+    const Nest n(a, b, size);
+    if (!n.ok) return Shared::unknown;
+    const long long delta = static_cast<const char*>(b->data) - static_cast<const char*>(a->data);
+    return n.meet(n.n, delta, a->ne[0] * size, b->ne[0] * size) ? Shared::yes : Shared::no;
+}
+
+// Memory of a call, as a tensor or as so many bytes, and the check that what it writes is nothing else's.
+struct Operand {
+    const char* what;
+    Span span;
+    const stx_tensor* t;
+    int size;
+    Operand(const char* what, const stx_tensor* t, int size) : what(what), span(t ? span_of(t, size) : Span{0, 0}), t(t), size(size) {}
+    Operand(const char* what, const void* p, size_t bytes) : what(what), span(span_of(p, bytes)), t(nullptr), size(0) {}
+};
+inline void check_apart(const char* op, std::initializer_list<Operand> written, std::initializer_list<Operand> read) {
+    auto apart = [&](const Operand& a, const Operand& b) {
+        const bool same = overlap(a.span, b.span) && !(a.t && b.t && shared(a.t, b.t, a.size) == Shared::no);
+        STX_REQUIRE(!same, "%s: %s overlaps %s", op, a.what, b.what);
+    };
+    for (auto a = written.begin(); a != written.end(); a++) {
+        for (auto b = a + 1; b != written.end(); b++) apart(*a, *b);
+        for (const Operand& b : read) apart(*a, b);
+    }
+}
 
 inline void check_workspace(const void* ws, size_t have, size_t need, const char* what) {
     if (need == 0) return;

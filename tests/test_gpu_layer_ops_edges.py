@@ -353,3 +353,30 @@ def test_group_norm_cl_gradient_past_32_bits(device):
     assert not bool(dx[1].isnan().any())
     del x, dy, dx
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ slices of one buffer
+def test_outputs_beside_inputs_in_one_buffer(device):
+    """Slices whose rows alternate in memory share no element: taken, with the bits of separate tensors and the rest of the
+    buffer as it was."""
+    dt = torch.bfloat16
+    room = randn(device, (150, 100), 601, dtype=dt)
+    x, out = room[:, :40], room[:, 60:84]
+    wg, wv = (randn(device, (24, 40), 602 + i, 0.2, dtype=dt) for i in range(2))
+    before, want = room.clone(), stx.gated_ff(x.contiguous(), wg, wv)
+    stx.gated_ff(x, wg, wv, out=out)
+    assert torch.equal(out, want) and torch.equal(room[:, :60], before[:, :60]) and torch.equal(room[:, 84:], before[:, 84:])
+    dh = randn(device, (150, 24), 604, dtype=dt)
+    grads = stx.gated_ff_back(dh, x, wg, wv)
+    both = torch.zeros(24, 80, device=device, dtype=dt)
+    got = stx.gated_ff_back(dh, x, wg, wv, dw_gate=both[:, :40], dw_value=both[:, 40:])
+    assert all(torch.equal(a, b) for a, b in zip(got[:3], grads[:3]))
+    qkv = randn(device, (2, 30, 12, 16), 605, dtype=dt)
+    pos = torch.arange(30, device=device, dtype=torch.int32)
+    q, k = qkv[:, :, :4], qkv[:, :, 4:6]
+    yq, yk = stx.rope_scaled(q, pos, stx.rope_params(16), k)
+    copy = qkv.clone()
+    stx.rope_scaled(copy[:, :, :4], pos, stx.rope_params(16), copy[:, :, 4:6], out=copy[:, :, 6:10], k_out=copy[:, :, 10:])   # into the rows beside
+    assert torch.equal(copy[:, :, 6:10], yq) and torch.equal(copy[:, :, 10:], yk) and torch.equal(copy[:, :, :6], qkv[:, :, :6])
+    turned = torch.empty(4, 30, 2, 16, device=device, dtype=dt).permute(2, 1, 0, 3)                                           # heads outermost
+    assert torch.equal(stx.rope_scaled(q, pos, stx.rope_params(16), out=turned), yq)
