@@ -790,7 +790,7 @@ typedef struct {
     int32_t  n_dims;               /* even, 2 .. min(ne0, 8192) */
     int32_t  mode;                 /* 0 or 2 */
     int32_t  n_ctx_orig;           /* trained length; used when ext_factor != 0 */
-    float    freq_base;            /* > 0, and != 1 when ext_factor != 0 */
+    float    freq_base;            /* finite, as all of these; > 0, and != 1 when ext_factor != 0 */
     float    freq_scale;           /* > 0 */
     float    ext_factor;
     float    attn_factor;
@@ -861,7 +861,8 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
  * db_gate and db_value (device float[N]); any may be NULL, and the work for it is left out (both
  * weights' gradients or neither). Results are rounded once: the gradients of the two products are
  * held in fp32, for fp16 and bf16 in two bf16 parts (16 bits at any fp32 exponent), so they may pass
- * fp16's range where the results do not; an infinite x or weight gives NaN in the gradients it enters.
+ * fp16's range where the results do not; an infinite x or weight may give NaN in a gradient that it
+ * would have made infinite.
  * Outputs overlap no input. workspace: device, 256-byte aligned, no
  * initialisation; calls that share one must not overlap. The size is for n_tokens tokens, K =
  * n_in, N = n_hidden (0 for sizes that stx_gated_ff_back rejects). */

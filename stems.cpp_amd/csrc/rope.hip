@@ -215,6 +215,9 @@ void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const 
     STX_REQUIRE(p->n_dims > 0 && p->n_dims % 2 == 0 && p->n_dims <= dim, "rope_scaled: n_dims must be even, positive and <= ne0");
     if (p->n_dims > 2 * kRopeTable || dim > (1 << 20)) fail(STX_STATUS_UNSUPPORTED, "rope_scaled: rows of %lld with %d rotated", dim, p->n_dims);
     STX_REQUIRE(p->freq_base > 0.f && p->freq_scale > 0.f, "rope_scaled: freq_base and freq_scale must be positive");
+    for (float v : {p->freq_base, p->freq_scale, p->ext_factor, p->attn_factor})
+        STX_REQUIRE(std::isfinite(v), "rope_scaled: a parameter is not finite");
+    STX_REQUIRE(p->ext_factor == 0.f || (std::isfinite(p->beta_fast) && std::isfinite(p->beta_slow)), "rope_scaled: beta_fast or beta_slow is not finite");
     STX_REQUIRE(pos_stride >= 0, "rope_scaled: negative pos_stride");
     RopeScaledArgs a{};
     a.log2_base = std::log2((double)p->freq_base);

@@ -80,3 +80,9 @@ def test_ff_gradients_over_other_memory(change, word):
 def test_ff_output_over_a_bias():
     rc = L.stx_gated_ff(ref(desc([24, 10], GB)), ref(desc([24, 8], 2 * GB)), ref(desc([24, 8], 3 * GB)), F32, 4 * GB + 64, None, 2, ref(desc([8, 10], 4 * GB)), None)
     assert rc == INVALID and b"b_gate" in L.stx_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(freq_base=float("inf")), dict(freq_scale=float("inf")), dict(attn_factor=float("nan")), dict(ext_factor=float("nan")),
+                                dict(ext_factor=1.0, n_ctx_orig=10, beta_fast=float("inf")), dict(ext_factor=1.0, n_ctx_orig=10, beta_slow=float("inf"))])
+def test_rope_parameters_that_are_not_finite(kw):
+    assert rope(**kw) == INVALID and b"finite" in L.stx_last_error()
