@@ -1191,14 +1191,23 @@ def _floats(t, like, count, what, dtype=None):
     return t.data_ptr()
 
 
-def _empty(shape, dtype, like, stream):
+def _empty(shape, like, stream, dtype=None):
     """A new tensor on like's device that belongs to the stream of the call: memory that its own stream may still be
     using is not handed to the kernel, nor the kernel's to another stream once the tensor is dropped."""
+    if stream is None:
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
+    import torch
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _empty_like(t, stream):
+    """_empty of t's shape and type, contiguous."""
     import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _launch(fn, like, stream, *args):
@@ -1221,7 +1230,7 @@ def _scratch(need, workspace, like, stream):
     """(pointer, bytes) of the caller's workspace, or of a new one; and the tensor that owns it."""
     if workspace is None:
         import torch
-        workspace = _empty(max(256, need), torch.uint8, like, stream)
+        workspace = _empty(max(256, need), like, stream, torch.uint8)
     elif not workspace.is_cuda or workspace.device != like.device or not workspace.is_contiguous():
         raise ValueError(f"workspace must be a contiguous CUDA (HIP) tensor on {like.device}, is on {workspace.device}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -1238,10 +1247,10 @@ def _rope_scaled(fn, q, pos, params, k, out, k_out, stream):
     factors = getattr(params, "factors", None)
     if factors is not None and factors.device != q.device:
         raise ValueError(f"freq_factors are on {factors.device}, q is on {q.device}")
-    out = _empty(q.shape, q.dtype, q, stream) if out is None else out
+    out = _empty_like(q, stream) if out is None else out
     dk = dko = None
     if k is not None:
-        k_out = _empty(k.shape, k.dtype, q, stream) if k_out is None else k_out
+        k_out = _empty_like(k, stream) if k_out is None else k_out
         dk, dko = _typed(k, q, "k"), _typed(k_out, q, "k_out")
     _launch(fn, q, stream, _typed(q, q, "q"), dk, _type(q), pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0,
             ctypes.byref(params), _typed(out, q, "out"), dko)
@@ -1274,11 +1283,11 @@ def group_norm_cl(x, n_groups, eps=1e-5, weight=None, bias=None, act=ACT_NONE, o
     weight and bias: float32 device (C,) or None. Returns (out, stats): stats is float64 (B, n_groups, 2), mean and
     1 / sqrt(var + eps), for group_norm_cl_back; with stats=False they are not kept (None). out may be x."""
     import torch
-    out = _empty(x.shape, x.dtype, x, stream) if out is None else out
+    out = _empty_like(x, stream) if out is None else out
     dx, t, L = _typed(x, x, "x", True), _type(x), lib()
     C, B = x.shape[-1], x.shape[0] if x.dim() > 2 else 1
     if stats is None:
-        stats = _empty((B, n_groups, 2), torch.float64, x, stream)
+        stats = _empty((B, n_groups, 2), x, stream, torch.float64)
     elif stats is False:
         stats = None
     ws, nbytes, keep = _scratch(L.stx_group_norm_cl_forward_workspace_size(dx, t, int(n_groups)), workspace, x, stream)
@@ -1292,11 +1301,11 @@ def group_norm_cl_back(dy, x, stats, n_groups, weight=None, bias=None, act=ACT_N
                        workspace=None, stream=None):
     """Gradients (dx, dweight, dbias) of group_norm_cl from dy, its x and its stats; dx may be dy or x."""
     import torch
-    dx = _empty(x.shape, x.dtype, x, stream) if dx is None else dx
+    dx = _empty_like(x, stream) if dx is None else dx
     da, t, L = _typed(x, x, "x", True), _type(x), lib()
     C, B = x.shape[-1], x.shape[0] if x.dim() > 2 else 1
-    dweight = _empty(C, torch.float32, x, stream) if dweight is None else dweight
-    dbias = _empty(C, torch.float32, x, stream) if dbias is None else dbias
+    dweight = _empty(C, x, stream, torch.float32) if dweight is None else dweight
+    dbias = _empty(C, x, stream, torch.float32) if dbias is None else dbias
     ws, nbytes, keep = _scratch(L.stx_group_norm_cl_workspace_size(da, t, int(n_groups)), workspace, x, stream)
     _launch(L.stx_group_norm_cl_back, x, stream, _typed(dy, x, "dy", True), da, t,
             _floats(stats, x, B * n_groups * 2, "stats", torch.float64), int(n_groups), _floats(weight, x, C, "weight"),
@@ -1310,7 +1319,7 @@ def gated_ff(x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=None, out
     float32 (N,) or None; out (..., N)."""
     N = w_gate.shape[0]
     if out is None:
-        out = _empty((*x.shape[:-1], N), x.dtype, x, stream)
+        out = _empty((*x.shape[:-1], N), x, stream)
     _launch(lib().stx_gated_ff, x, stream, _typed(x, x, "x"), _typed(w_gate, x, "w_gate"), _typed(w_value, x, "w_value"),
             _type(x), _floats(b_gate, x, N, "b_gate"), _floats(b_value, x, N, "b_value"), int(act), _typed(out, x, "out"))
     return out
@@ -1328,13 +1337,13 @@ def gated_ff_back(dh, x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=
     there is no such bias."""
     import torch
     N, K = w_gate.shape
-    dx = _empty(x.shape, x.dtype, x, stream) if dx is None else dx
-    dw_gate = _empty(w_gate.shape, w_gate.dtype, x, stream) if dw_gate is None else dw_gate
-    dw_value = _empty(w_value.shape, w_value.dtype, x, stream) if dw_value is None else dw_value
+    dx = _empty_like(x, stream) if dx is None else dx
+    dw_gate = _empty_like(w_gate, stream) if dw_gate is None else dw_gate
+    dw_value = _empty_like(w_value, stream) if dw_value is None else dw_value
     if db_gate is None and b_gate is not None:
-        db_gate = _empty(N, torch.float32, x, stream)
+        db_gate = _empty(N, x, stream, torch.float32)
     if db_value is None and b_value is not None:
-        db_value = _empty(N, torch.float32, x, stream)
+        db_value = _empty(N, x, stream, torch.float32)
     d = [_typed(t, x, n) for t, n in ((dh, "dh"), (x, "x"), (w_gate, "w_gate"), (w_value, "w_value"), (dx, "dx"),
                                       (dw_gate, "dw_gate"), (dw_value, "dw_value"))]
     L, t = lib(), _type(x)
