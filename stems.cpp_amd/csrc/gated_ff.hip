@@ -820,9 +820,9 @@ constexpr int kCus = 256;                                         // of an MI355
 // How a product is run: its tile and the number of parts of its reduction, by the least estimated time.
 // A step of a tile takes time in proportion to its area, the larger tiles' at a better rate (the
 // measured ones of a long reduction); a part ends in an epilogue and a fold. Measured, bf16, 48,060 tokens,
-// K 384, N 1,536: FORWARD Large 143, Medium 156, Small 182 us (113 GFLOP: 790 TFLOP/s); GRAD Medium 305; DX
-// Large 315, Medium 245 (290 with two blocks a CU), Small 270; DW Medium in 10 parts 215, in 7 on two blocks a CU
-// 235. fp32, 1,344 tokens, K 512, N 2,048: DX Small 43 (split, with 6 of the fold) where
+// K 384, N 1,536: FORWARD Large 143, Medium 156, Small 182 us (113 GFLOP: 790 TFLOP/s); GRAD Medium 299; DX
+// Large 350, Medium 281 (328 with two blocks a CU), Small 305; DW Medium in 10 parts 227, in 7 on two blocks a CU
+// 249. fp32, 1,344 tokens, K 512, N 2,048: DX Small 44 (split, with 6 of the fold) where
 // Medium takes 48 and an unsplit one 157; DW 43 (and 6), 47 and 59.
 struct Plan {
     int tile, splits, part;              // 0 Large, 1 Medium, 2 Small; parts, steps of a part

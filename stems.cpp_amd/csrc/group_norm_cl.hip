@@ -27,11 +27,12 @@ namespace {
 // group's first element, and t and t^2 are summed in double: E[t^2] - E[t]^2 loses at most 2^-53 times the
 // number of elements, wherever the mean lies (the element is within that number's root of deviations
 // from it); sums of x itself would lose 2^-53 mean^2 / var. The backward sums in float over kHeld rows
-// of a thread (64 terms drift by about 1e-7 of their sum), then in double. Both passes are bound by
-// memory: HBM in the first, in the second the last-level cache as far as it still holds the input.
-// Measured: fp32 4 x 85,995 x 48, one group, GELU (66 MB): 15.5 us (4.3 TB/s) and 25.4 us (5.2 TB/s read
-// and written); gradients of fp32 4 x 21,499 x 96, four groups, GELU (33 MB a tensor): 17.5 and 21.6 us;
-// of bf16 60 x 801 x 384, 32 groups, SiLU (37 MB a tensor): 19.1 and 23.5 us. The gradients keep the vector units three quarters busy.
+// of a thread (64 terms drift by about 1e-7 of their sum), then in double. The first forward
+// pass is bound by HBM, the second, as far as the last-level cache still holds the input, by that or by the
+// activation: with GELU the vector units are busy 91 % of the time, in the gradients 72 to 82 %.
+// Measured: fp32 4 x 85,995 x 48, one group, GELU (66 MB): 15.3 us (4.3 TB/s) and 25.6 us (5.2 TB/s read
+// and written); gradients of fp32 4 x 21,499 x 96, four groups, GELU (33 MB a tensor): 19.4 and 22.4 us;
+// of bf16 60 x 801 x 384, 32 groups, SiLU (37 MB a tensor): 19.2 and 23.7 us.
 constexpr int kThreads = 256;
 constexpr int kVec = 4;                  // elements of a vector: with 8 of 16 bits a channel's constants leave four waves a SIMD
 constexpr int kBatch = 2;                // super-rows a thread has in flight

@@ -11,10 +11,11 @@ namespace {
 // Each block takes a tile of consecutive tokens (N x batch flattened, so short sequences of a
 // large batch fill tiles too): it forms cos and sin of the tile's angles once, in LDS, and rotates
 // all rows (heads of q, then of k) of those tokens with them. The operator reads and writes every
-// element once and is bound by HBM; the angles cost half / (rows * dim) of a double-precision
-// evaluation an element. 60 x 801 tokens of 16 rows of 64 fp32 values, slices of a projection (394 MB):
-// 73 us, 5.4 TB/s; the gradient of 2 x 16,384 tokens of 40 rows of 128 bf16 values, 96 of them rotated
-// (671 MB): 132 us, 5.1 TB/s, the rate of a large copy; one token of 16 rows: 2.5 us.
+// element once; the angles cost half / (rows * dim) of a double-precision evaluation an element.
+// With 16 rows a token or more it is bound by HBM: 60 x 801 tokens of 16 rows of 64 fp32 values, slices
+// of a projection (394 MB): 73 us, 5.4 TB/s; the gradient of 2 x 16,384 tokens of 40 rows of 128 bf16 values,
+// 96 of them rotated (671 MB): 131 us, 5.1 TB/s, the rate of a large copy. With fewer, by the angles:
+// 200,000 tokens of 2 rows of 64 bf16 values (102 MB, 20 us at that rate): 42 us. One token of 16 rows: 2.3 us.
 //
 // Angles are products of a position and a frequency in double (a float angle of 10^5 radians
 // would be off by 2^-8); cos and sin are reduced and evaluated in double and rounded to float
