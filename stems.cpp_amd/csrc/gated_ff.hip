@@ -56,11 +56,11 @@ struct Split {
             }
     }
 };
-// x as a high and a low bf16 part; an infinity has a low part of 0.
+// x as a high and a low bf16 part; the high one is finite, so that a finite x stays so and an infinity,
+// in the low part, meets no zero of another high part.
 __device__ __forceinline__ void halves(float x, bf16& hi, bf16& lo) {
-    hi = (bf16)x;
-    const float rest = x - (float)hi;
-    lo = (bf16)(rest == rest ? rest : 0.f);
+    hi = (bf16)__builtin_amdgcn_fmed3f(x, -0x1.fep127f, 0x1.fep127f);
+    lo = (bf16)(x - (float)hi);
 }
 __device__ __forceinline__ f32x4 mma(const u32x4 (&a)[1], const u32x4 (&b)[2], f32x4 acc) {   // smallest terms first
     acc = mma(a[0], b[1], acc, bf16{});
@@ -93,7 +93,7 @@ __device__ __forceinline__ f32x4 mma(const u32x4 (&a)[3], const u32x4 (&b)[3], f
 // results' own rounding (bf16, 48,060 tokens, K 384, N 1,536: 2.3e-3 where it is 1.65e-3), and fp16's would end
 // at 65,504 and 2^-24, where a sum that they enter need not. DX and DW multiply both parts, by
 // bf16's P as it is and by fp16's in two bf16 parts (without the product of the two low ones, below
-// 2^-17 of the whole). An infinity in P gives NaN there: infinity times a low part of 0.
+// 2^-17 of the whole). An infinity in P may give NaN there: infinity times a low part of 0.
 // In FORWARD and GRAD r is the fastest dimension of both operands, in DX of Q only and in DW of
 // neither; an operand whose r is not its fastest dimension is "strided" below.
 enum Mode { FORWARD, GRAD, DX, DW };

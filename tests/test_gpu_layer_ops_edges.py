@@ -380,3 +380,30 @@ def test_outputs_beside_inputs_in_one_buffer(device):
     assert torch.equal(copy[:, :, 6:10], yq) and torch.equal(copy[:, :, 10:], yk) and torch.equal(copy[:, :, :6], qkv[:, :, :6])
     turned = torch.empty(4, 30, 2, 16, device=device, dtype=dt).permute(2, 1, 0, 3)                                           # heads outermost
     assert torch.equal(stx.rope_scaled(q, pos, stx.rope_params(16), out=turned), yq)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("N", [8, 7])
+def test_gated_gradients_of_infinite_and_largest_gradients(device, dtype, N):
+    """An infinite dh makes infinite what it enters, by the sign of the weight or token that it meets, and no NaN; the largest
+    finite gradients of the products stay finite."""
+    M, K, dt = 70, 24, TYPES[dtype]
+    x = randn(device, (M, K), 611, dtype=dt).abs() + 0.5
+    wg = randn(device, (N, K), 612, 0.5, dtype=dt)
+    wg = torch.where(wg.abs() < 0.01, torch.full_like(wg, 0.25), wg)
+    dh = randn(device, (M, N), 613, dtype=dt)
+    dh[5, 3] = float("inf")
+    one = torch.ones(N, device=device)
+    dx, dwg, dwv, _, _ = stx.gated_ff_back(dh, x, wg, wg.clone(), stx.ACT_NONE)      # both products are g: dg = dv = dh g
+    g = torch.mm(x[5:6].to(F64), wg[3:4].to(F64).t().contiguous()).sign()
+    assert torch.equal(dx[5].to(F64), math.inf * g[0] * wg[3].to(F64).sign())
+    assert torch.equal(dwg[3].to(F64), math.inf * g.expand(1, K)[0]) and torch.equal(dwv[3], dwg[3])
+    keep = torch.arange(M, device=device) != 5
+    assert bool(dx[keep].isfinite().all()) and bool(dwg[[0, 1, 2, 4, 5, 6]].isfinite().all())
+    if dtype == "bf16":
+        dh = torch.zeros_like(dh)
+        dh[0, 0] = torch.finfo(dt).max
+        w = torch.full_like(wg, 2.0 ** -12)
+        dx = stx.gated_ff_back(dh, x, w, torch.zeros_like(w), stx.ACT_NONE, torch.zeros_like(one), one * 1.0039)[0]          # dg rounds to infinity as bf16
+        want = float(torch.finfo(dt).max) * float(one[0] * 1.0039) * 2.0 ** -12
+        assert bool(((dx[0].to(F64) - want).abs() <= half_step(dt) * 1.01 * want).all())
