@@ -850,9 +850,9 @@ STX_API stx_status stx_group_norm_cl_back(const stx_tensor* dy, const stx_tensor
  * rows are contiguous, row strides any. b_gate, b_value: device float[N], either may be NULL.
  * Products are accumulated in fp32, on the matrix cores: of fp16 and bf16 as they are; of fp32,
  * above 64 tokens and in the gradients, as the six larger products of three bf16 parts an element,
- * which hold all of a finite element above 2^-100 (smaller ones lose low bits; an infinity gives
- * NaN where a sum of products might have been infinite). dst overlaps no input. At most 2^30
- * tokens, K and N at most 2^20. */
+ * which hold all of an element above 2^-100 (smaller ones lose low bits); infinities and NaN give
+ * what they give in a sum of products. dst overlaps no input. At most 2^30 tokens, K and N at
+ * most 2^20. */
 STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, const stx_tensor* w_value, stx_type type,
                                 const float* b_gate, const float* b_value, stx_act act, const stx_tensor* dst,
                                 stx_stream stream);
@@ -861,8 +861,8 @@ STX_API stx_status stx_gated_ff(const stx_tensor* x, const stx_tensor* w_gate, c
  * db_gate and db_value (device float[N]); any may be NULL, and the work for it is left out (both
  * weights' gradients or neither). Results are rounded once: the gradients of the two products are
  * held in fp32, for fp16 and bf16 in two bf16 parts (16 bits at any fp32 exponent), so they may pass
- * fp16's range where the results do not; an infinite x or weight may give NaN in a gradient that it
- * would have made infinite.
+ * fp16's range where the results do not; there, an infinite x or weight may give NaN in a gradient
+ * that it would have made infinite.
  * Outputs overlap no input. workspace: device, 256-byte aligned, no
  * initialisation; calls that share one must not overlap. The size is for n_tokens tokens, K =
  * n_in, N = n_hidden (0 for sizes that stx_gated_ff_back rejects). */

@@ -34,21 +34,38 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 acc, bf16) {
 // bf16(x - h), l = x - h - m, all exact. Rounded to nearest, |m| <= 2^-8 |x| and |l| <= 2^-17 |x| have either
 // sign, and a product of two such sums without its three smallest terms (2 |m l| + |l l|: below 2^-24 of it)
 // is six bf16 products without bias: 2.7 times the rate of the fp32 matrix instruction, at its
-// accuracy. (Parts cut off instead drop up to 2^-21, always towards zero.) h is kept below infinity for
-// finite x; an infinity's rest is inf - inf: NaN.
+// accuracy. (Parts cut off instead drop up to 2^-21, always towards zero.) Values beyond the largest
+// bf16 are rare enough for a form of their own (EDGE): h stays finite where x is, and an infinity is
+// +-1 + 0 +- inf, so that in the six products it meets the other's h alone and gives what it gives there.
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+template <bool EDGE>
 struct Split {
+    static constexpr float most = 0x1.fep127f;
     u32x2 part[3];                       // four values' h, m, l as bf16
+    static __device__ __forceinline__ float largest(u32x4 bits, float v) {
+        const f32x4 x = __builtin_bit_cast(f32x4, bits);
+        return fmaxf(fmaxf(fmaxf(fmaxf(v, fabsf(x[0])), fabsf(x[1])), fabsf(x[2])), fabsf(x[3]));   // NaN is passed over
+    }
     __device__ __forceinline__ explicit Split(u32x4 bits) {
         f32x4 x = __builtin_bit_cast(f32x4, bits);
+        float beyond[4] = {};
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool inf = fabsf(x[i]) == __builtin_inff();
+                beyond[i] = inf ? x[i] : 0.f;
+                x[i] = inf ? copysignf(1.f, x[i]) : x[i];
+            }
+        }
 #pragma unroll
         for (int k = 0; k < 3; k++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 f32x2 v = {x[2 * i], x[2 * i + 1]};
-                if (k == 0) v = f32x2{__builtin_amdgcn_fmed3f(v[0], -0x1.fep127f, 0x1.fep127f), __builtin_amdgcn_fmed3f(v[1], -0x1.fep127f, 0x1.fep127f)};
+                if (EDGE && k == 0) v = f32x2{__builtin_amdgcn_fmed3f(v[0], -most, most), __builtin_amdgcn_fmed3f(v[1], -most, most)};
+                if (EDGE && k == 2) v += f32x2{beyond[2 * i], beyond[2 * i + 1]};
                 const unsigned pair = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
                 part[k][i] = pair;
                 x[2 * i] -= __uint_as_float(pair << 16);
@@ -421,13 +438,20 @@ __global__ __launch_bounds__(C::NT, (C::template slots<T, MODE> * C::NT / 256)) 
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         } else if constexpr (SPLIT) {
             __syncthreads();                             // the one stage is read
+            auto split = [&](auto edge) {
 #pragma unroll
-            for (int i = 0; i < PSource::N + QSource::N; i++) {
-                const Split v(hold[i]);
-                char* to = lds[0] + (i < PSource::N ? PSource::spot(i) : QAT + QSource::spot(i - PSource::N));
+                for (int i = 0; i < PSource::N + QSource::N; i++) {
+                    const Split<edge()> v(hold[i]);
+                    char* to = lds[0] + (i < PSource::N ? PSource::spot(i) : QAT + QSource::spot(i - PSource::N));
 #pragma unroll
-                for (int k = 0; k < 3; k++) *reinterpret_cast<u32x2*>(to + k * (i < PSource::N ? PPLANE : QPLANE)) = v.part[k];
-            }
+                    for (int k = 0; k < 3; k++) *reinterpret_cast<u32x2*>(to + k * (i < PSource::N ? PPLANE : QPLANE)) = v.part[k];
+                }
+            };
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < PSource::N + QSource::N; i++) v = Split<false>::largest(hold[i], v);
+            if (__builtin_amdgcn_ballot_w64(v > Split<false>::most)) split(std::true_type{});
+            else split(std::false_type{});
         } else {
 #pragma unroll
             for (int i = 0; i < HELD; i++) {

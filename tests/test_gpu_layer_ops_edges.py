@@ -407,3 +407,28 @@ def test_gated_gradients_of_infinite_and_largest_gradients(device, dtype, N):
         dx = stx.gated_ff_back(dh, x, w, torch.zeros_like(w), stx.ACT_NONE, torch.zeros_like(one), one * 1.0039)[0]          # dg rounds to infinity as bf16
         want = float(torch.finfo(dt).max) * float(one[0] * 1.0039) * 2.0 ** -12
         assert bool(((dx[0].to(F64) - want).abs() <= half_step(dt) * 1.01 * want).all())
+
+
+@pytest.mark.parametrize("M", [40, 70])
+@pytest.mark.parametrize("K", [24, 23])
+def test_gated_fp32_products_of_infinities(device, M, K):
+    """Infinite tokens and weights in fp32: what the sums of products are in floating point (an infinity, or NaN with a zero
+    or another sign), at 40 tokens as at 70, and the rows that meet none as they are without."""
+    N = 30
+    x, wg, wv = (randn(device, s, 621 + i) for i, s in enumerate(((M, K), (N, K), (N, K))))
+    wv = wv.abs() + 0.1
+    clean = stx.gated_ff(x, wg, wv, stx.ACT_NONE)
+    x[3, 2], x[5, 1], x[9, 0], x[9, 4], x[11, 7], x[M - 1, K - 1] = math.inf, -math.inf, math.inf, -math.inf, math.nan, math.inf
+    wg[1, 3], wg[2, 5], wg[4, 2], wv[6, 9] = math.inf, -math.inf, 0.0, math.inf
+    got = stx.gated_ff(x, wg, wv, stx.ACT_NONE)
+    want = (x.to(F64)[:, None] * wg.to(F64)).sum(-1) * (x.to(F64)[:, None] * wv.to(F64)).sum(-1)
+    assert torch.equal(got.isnan(), want.isnan()) and 5 * N > int(want.isnan().sum()) > N
+    assert torch.equal(got[want.isinf()].to(F64), want[want.isinf()]) and int(want.isinf().sum()) > 2 * M
+    rows = [m for m in range(M) if m not in (3, 5, 9, 11, M - 1)]
+    cols = [n for n in range(N) if n not in (1, 2, 4, 6)]
+    assert torch.equal(got[rows][:, cols], clean[rows][:, cols])
+
+
+def test_gated_fp32_gradients_of_infinite_gradients(device):
+    for N in (8, 7):
+        test_gated_gradients_of_infinite_and_largest_gradients(device, "f32", N)
