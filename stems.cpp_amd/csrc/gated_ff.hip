@@ -119,6 +119,7 @@ enum Mode { FORWARD, GRAD, DX, DW };
 // of every row in FORWARD and GRAD of 16-bit data, in two stages of LDS (five stages of 32, which keep
 // twice as much in flight, took 5 to 10 % longer: twice the barriers), and 32 elsewhere, where an
 // operand has two or three parts.
+constexpr bool splits(Mode mode, stx_type type) { return type == STX_TYPE_F32 || (type == STX_TYPE_F16 && (mode == DX || mode == DW)); }   // P, on its way to LDS
 constexpr int step_of(Mode mode, int size) { return size == 2 && (mode == FORWARD || mode == GRAD) ? 64 : 32; }
 // Blocks of a tile (0 Large, 1 Medium, 2 Small) that a CU holds: what LDS has room for, and the registers are held to.
 constexpr int slots_of(int tile, Mode mode, stx_type type) {
@@ -864,7 +865,8 @@ Plan plan_of(Mode mode, long long J, long long M, long long steps, stx_type type
     const int w = mode == DW ? 2 : 1;
     Plan best{};
     double least = 0;
-    for (int k = mode == GRAD || size == 4 ? 1 : 0; k < 3; k++) {    // Large has no registers for GRAD's epilogue: 460 us where Medium takes 250
+    // Large has no registers for GRAD's epilogue (460 us where Medium took 250), nor for operands that are split.
+    for (int k = mode == GRAD || splits(mode, type) ? 1 : 0; k < 3; k++) {
         const Kind& c = kinds[k];
         const int slots = slots_of(k, mode, type);
         const long long tiles = (J * (gated ? 2 : 1) + c.tj - 1) / c.tj * ((M + c.tm - 1) / c.tm) * w;
@@ -900,8 +902,7 @@ void launch_tiles(FfArgs a, int parts, hipStream_t stream) {
 // What goes through registers has no Large tile.
 template <class T, int MODE>
 void launch_ff(const FfArgs& a, bool aligned, int tile, int parts, hipStream_t stream) {
-    constexpr bool held = sizeof(T) == 4 || (std::is_same_v<T, f16> && (MODE == DX || MODE == DW));
-    if constexpr (held) return tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
+    if constexpr (splits((Mode)MODE, type_of<T>)) return tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
     else if (!aligned) tile == 2 ? launch_tiles<T, MODE, Small, false>(a, parts, stream) : launch_tiles<T, MODE, Medium, false>(a, parts, stream);
     else if (MODE != GRAD && tile == 0) launch_tiles<T, MODE == GRAD ? FORWARD : MODE, Large, true>(a, parts, stream);
     else if (tile == 1) launch_tiles<T, MODE, Medium, true>(a, parts, stream);
