@@ -301,9 +301,9 @@ def plain_rel(s):
 def diagonals(g):
     """Sums of [H][M][N] over equal column - row, [H][M + N - 1], from -(M - 1) on, in 64 bits."""
     H, M, N = g.shape
-    wide = torch.zeros(H, M, N + M, dtype=F32, device=g.device)
+    wide = torch.zeros(H, M, N + M, dtype=F64, device=g.device)
     wide[:, :, :N] = g.flip(1)
-    return wide.view(H, -1)[:, :M * (N + M - 1)].view(H, M, N + M - 1).sum(1, dtype=F64)
+    return wide.view(H, -1)[:, :M * (N + M - 1)].view(H, M, N + M - 1).sum(1)
 
 
 def plain_rel_back(s):
@@ -312,7 +312,8 @@ def plain_rel_back(s):
     table = torch.zeros(H, c["buckets"], dtype=F64, device=DEV)
     for b in range(c["batch"]):
         mask, _ = seen(s, b)
-        y, dy = s["y"][b].to(F32), s["dy"][b].to(F32)
+        # In 64 bits: a row's terms add up to 0, and where most of its keys share a bucket so does that bucket's sum.
+        y, dy = s["y"][b].to(F64), s["dy"][b].to(F64)
         g = torch.where(mask, y * (dy - (y * dy).sum(-1, keepdim=True)), 0.0)
         parts.append((s["scale"] * g).to(s["y"].dtype))
         rel = torch.arange(N + M - 1, device=DEV) - (M - 1) - (s["starts"][b] if s["starts"] is not None else 0)
