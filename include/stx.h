@@ -878,6 +878,35 @@ STX_API stx_status stx_gated_ff_back(const stx_tensor* dh, const stx_tensor* x, 
 STX_API size_t     stx_group_norm_cl_forward_workspace_size(const stx_tensor* a, stx_type type, int n_groups);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention operators over fp32, fp16 and bf16 tensors, with their gradients, under the rules of the
+ * transformer-layer operators above (one element type a call, deterministic, nothing allocated, capturable).
+ * ---------------------------------------------------------------------------------------- */
+
+/* RMS norms of the queries and keys of each head and stx_rope_scaled in one pass: every row x of q [dim, heads,
+ * N, batch] and, where k is not NULL, of k [dim, kv heads, N, batch] (stx_rms_norm_mul of each head, then the
+ * rotation of stx_qkv_rope_split) becomes
+ *   dst = R(pos) (w * x / sqrt(mean(x^2) + eps)).
+ * w_q and w_k: device float[dim], or with per_head != 0 float[heads][dim] and float[kv heads][dim]; either may be
+ * NULL (1). pos, pos_stride and params as in stx_rope_scaled; so are strides, limits and the outputs that may be the
+ * inputs. Mean squares are formed in double, the rest in float, rounded once. Rows of up to 1,024 elements; eps >= 0. */
+STX_API stx_status stx_qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
+                                    int64_t pos_stride, const stx_rope_params* params, const float* w_q,
+                                    const float* w_k, int per_head, double eps, const stx_tensor* q_dst,
+                                    const stx_tensor* k_dst, stx_stream stream);
+/* Its gradients, from dq_out and dk_out (of q_dst and k_dst) and the forward call's inputs: dq and dk (of q and k;
+ * each may be the gradient that it comes from, or its q or k), dw_q and dw_k (of the weights, in their layout, summed
+ * over tokens and batch and, where heads share them, over heads). Any may be NULL. workspace: device, 256-byte
+ * aligned, no initialisation; calls that share one must not overlap. None is needed without dw_q and dw_k. */
+STX_API size_t     stx_qk_norm_rope_back_workspace_size(const stx_tensor* q, const stx_tensor* k, stx_type type,
+                                                        int n_dims, int per_head);
+STX_API stx_status stx_qk_norm_rope_back(const stx_tensor* dq_out, const stx_tensor* dk_out, const stx_tensor* q,
+                                         const stx_tensor* k, stx_type type, const int32_t* pos, int64_t pos_stride,
+                                         const stx_rope_params* params, const float* w_q, const float* w_k,
+                                         int per_head, double eps, const stx_tensor* dq, const stx_tensor* dk,
+                                         float* dw_q, float* dw_k, void* workspace, size_t workspace_bytes,
+                                         stx_stream stream);
+
+/* ------------------------------------------------------------------------------------------
  * Versioned function table (after libstems V1, src/libstems_v1.h:146-189). Every entry point
  * above, in header order; a later revision of V1 may append entries (never reorder them), so
  * a consumer checks `size` against the prefix it needs.
@@ -1097,6 +1126,22 @@ typedef struct stx_api_v1 {
                                 float* db_gate, float* db_value, void* workspace,
                                 size_t workspace_bytes, stx_stream stream);
     size_t (*group_norm_cl_forward_workspace_size)(const stx_tensor* a, stx_type type, int n_groups);
+    /* Appended: the attention operators over typed tensors. */
+    stx_status (*qk_norm_rope)(const stx_tensor* q, const stx_tensor* k, stx_type type,
+                               const int32_t* pos, int64_t pos_stride,
+                               const stx_rope_params* params, const float* w_q, const float* w_k,
+                               int per_head, double eps, const stx_tensor* q_dst,
+                               const stx_tensor* k_dst, stx_stream stream);
+    size_t (*qk_norm_rope_back_workspace_size)(const stx_tensor* q, const stx_tensor* k,
+                                               stx_type type, int n_dims, int per_head);
+    stx_status (*qk_norm_rope_back)(const stx_tensor* dq_out, const stx_tensor* dk_out,
+                                    const stx_tensor* q, const stx_tensor* k, stx_type type,
+                                    const int32_t* pos, int64_t pos_stride,
+                                    const stx_rope_params* params, const float* w_q,
+                                    const float* w_k, int per_head, double eps,
+                                    const stx_tensor* dq, const stx_tensor* dk, float* dw_q,
+                                    float* dw_k, void* workspace, size_t workspace_bytes,
+                                    stx_stream stream);
     void (*reserved[16])(void);
 } stx_api_v1;
 

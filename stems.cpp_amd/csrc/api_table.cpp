@@ -104,6 +104,9 @@ const stx_api_v1 kApiV1 = {
     &stx_gated_ff_back_workspace_size,
     &stx_gated_ff_back,
     &stx_group_norm_cl_forward_workspace_size,
+    &stx_qk_norm_rope,
+    &stx_qk_norm_rope_back_workspace_size,
+    &stx_qk_norm_rope_back,
     {},
 };
 }  // namespace

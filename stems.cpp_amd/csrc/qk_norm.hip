@@ -1,0 +1,544 @@
+// qk_norm.hip — RMS norms of queries and keys per head with the rotation in the same pass, forward and
+// backward (stx_qk_norm_rope, stx_qk_norm_rope_back).
+#include <algorithm>
+
+#include "rope_angles.hpp"
+
+namespace stx {
+namespace {
+
+// A row x of one head (of q or k) gives y = R(pos) (w x r), r = 1 / sqrt(mean(x^2) + eps), R the rotation
+// of rope.hip. Its gradient: dz = R^T dy, dw = sum over the rows of dz x r, and with g = w dz
+//   dx = r (g - x r^2 mean(g x)).
+// Both read and write every element once (the gradient reads x again instead of r), so HBM bounds them.
+// A row is held by `lanes` lanes of a wave, V elements a unit and K units a lane, all of them loaded
+// before the first is stored: outputs may be inputs. A lane whose pair partner lies in another unit
+// (mode 2, or units of one element) loads it too, from the same lines: units stay dense for any
+// n_dims, where units of a pair of halves would leave 6 of 16 lanes idle at 128 elements, 96 rotated.
+// Sums of squares and of g x are held in double: data whose squares leave fp32 keeps its norm.
+struct QkSide {
+    const char *x, *dy;
+    char* out;
+    const float* w;
+    long long x1, x2, x3, y1, y2, y3, o1, o2, o3;    // byte strides of x, dy and out
+};
+
+struct QkArgs {
+    QkSide q, k;
+    RopeAngles at;
+    double eps;
+    unsigned tokens, tile;               // all tokens, and of a block
+    unsigned base;                       // blocks of the launches before this one
+    FastDiv rows;                        // rows of a token: q's, then k's
+    unsigned q_rows;
+    int dim, units, log_lanes, mode;
+    int w_stride;                        // from a head's weights to the next's: dim, or 0 where heads share them
+    float* part;                         // backward: sums of dz x r, [block][2 or rows][dim], or NULL
+};
+
+constexpr int kQkThreads = 256;
+constexpr int kQkDim = 1024;             // of a row: 64 lanes x 16 elements
+
+template <class T, int V>
+struct Row {
+    const QkSide* side;
+    unsigned h;                          // of the side
+    bool is_k;
+    long long i2, i3;
+    __device__ __forceinline__ Row(const QkArgs& a, unsigned t, unsigned row) {
+        const unsigned b = a.at.n.div(t);
+        i3 = b;
+        i2 = t - b * a.at.n.d;
+        is_k = row >= a.q_rows;
+        side = is_k ? &a.k : &a.q;
+        h = is_k ? row - a.q_rows : row;
+    }
+    __device__ __forceinline__ const T* x() const { return reinterpret_cast<const T*>(side->x + h * side->x1 + i2 * side->x2 + i3 * side->x3); }
+    __device__ __forceinline__ const T* dy() const { return reinterpret_cast<const T*>(side->dy + h * side->y1 + i2 * side->y2 + i3 * side->y3); }
+    __device__ __forceinline__ T* out() const { return reinterpret_cast<T*>(side->out + h * side->o1 + i2 * side->o2 + i3 * side->o3); }
+};
+
+// Where the partners of unit `at` start; `at` itself where they are in the unit or there are none.
+template <int V>
+__device__ __forceinline__ int partner(const QkArgs& a, int at) {
+    const int half = a.at.n_dims / 2;
+    if (at >= a.at.n_dims) return at;
+    if (a.mode == 0) return V == 1 ? at ^ 1 : at;
+    return at < half ? at + half : at - half;
+}
+
+// The rotation of unit `at` with values f and partners p, in place.
+template <int V>
+__device__ __forceinline__ void rotate(const QkArgs& a, int at, const float2* tab, float (&f)[V], const float (&p)[V]) {
+    const int half = a.at.n_dims / 2;
+    if (V > 1 && a.mode == 0) {
+#pragma unroll
+        for (int v = 0; v + 1 < V; v += 2) {
+            const int pair = (at + v) / 2;
+            if (pair >= half) continue;
+            const float2 r = tab[pair];
+            const float x0 = f[v], x1 = f[v + 1];
+            f[v] = fmaf(x0, r.x, -(x1 * r.y));
+            f[v + 1] = fmaf(x0, r.y, x1 * r.x);
+        }
+    } else if (at < a.at.n_dims) {
+        const bool first = a.mode == 0 ? at % 2 == 0 : at < half;
+        const int pair = a.mode == 0 ? at / 2 : first ? at : at - half;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float2 r = tab[pair + v];
+            f[v] = first ? fmaf(f[v], r.x, -(p[v] * r.y)) : fmaf(p[v], r.y, f[v] * r.x);
+        }
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void take(const T* p, float (&f)[V]) {
+    const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int v = 0; v < V; v++) f[v] = to_f32(x.v[v]);
+}
+template <class T, int V>
+__device__ __forceinline__ void give(T* p, const float (&f)[V]) {
+    Pack<T, V> x;
+#pragma unroll
+    for (int v = 0; v < V; v++) x.v[v] = from_f32<T>(f[v]);
+    *reinterpret_cast<Pack<T, V>*>(p) = x;
+}
+template <int V>
+__device__ __forceinline__ void weights(const float* w, int at, float (&f)[V]) {
+    if (w) {
+        __builtin_memcpy(f, w + at, sizeof f);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) f[v] = 1.f;
+    }
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
+    extern __shared__ float2 cs[];       // [tile][n_dims / 2]
+    const int half = a.at.n_dims / 2;
+    const unsigned t0 = (a.base + blockIdx.x) * a.tile, nt = min(a.tile, a.tokens - t0);
+    rope_table<kQkThreads>(a.at, t0, nt, cs);
+    __syncthreads();
+    const int lanes = 1 << a.log_lanes, lane = threadIdx.x & (lanes - 1);
+    const unsigned total = nt * a.rows.d, groups = kQkThreads >> a.log_lanes;
+    for (unsigned first = 0; first < total; first += groups) {
+        const unsigned row = first + (threadIdx.x >> a.log_lanes), at_row = min(row, total - 1);   // every lane takes part in the sums
+        const unsigned tk = a.rows.div(at_row);
+        const Row<T, V> r(a, t0 + tk, at_row - tk * a.rows.d);
+        const T* src = r.x();
+        float x[K][V], p[K][V];
+        double sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int u = lane + (k << a.log_lanes), at = u * V;
+#pragma unroll
+            for (int v = 0; v < V; v++) x[k][v] = p[k][v] = 0.f;
+            if (u >= a.units) continue;
+            take<T, V>(src + at, x[k]);
+            const int other = partner<V>(a, at);
+            if (other != at) take<T, V>(src + other, p[k]);
+#pragma unroll
+            for (int v = 0; v < V; v++) sum = fma((double)x[k][v], (double)x[k][v], sum);
+        }
+        const float rstd = (float)(1.0 / sqrt(lane_sum_dyn(sum, lanes) / a.dim + a.eps));
+        if (row >= total) continue;
+        T* out = r.out();
+        const float* w = r.side->w ? r.side->w + (long long)r.h * a.w_stride : nullptr;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int u = lane + (k << a.log_lanes), at = u * V;
+            if (u >= a.units) continue;
+            float f[V];
+            weights<V>(w, at, f);
+#pragma unroll
+            for (int v = 0; v < V; v++) x[k][v] = x[k][v] * rstd * f[v];
+            const int other = partner<V>(a, at);
+            if (other != at) {
+                weights<V>(w, other, f);
+#pragma unroll
+                for (int v = 0; v < V; v++) p[k][v] = p[k][v] * rstd * f[v];
+            }
+            rotate<V>(a, at, cs + tk * half, x[k], p[k]);
+            give<T, V>(out + at, x[k]);
+        }
+    }
+}
+
+// Sums over the rows of dz x r are kept by the lanes that hold the elements, over the tokens of a block:
+// where heads share weights, one for q and one for k and any row a group; where they do not (PER_HEAD),
+// a group of lanes keeps to a head, or takes its heads one after another. Added up in LDS in
+// order, and over the blocks by qk_fold_kernel.
+template <class T, int V, int K, bool PER_HEAD>
+__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a) {
+    extern __shared__ float2 cs[];       // [tile][n_dims / 2], then sums [1 or 2][groups][units * V]
+    const int half = a.at.n_dims / 2;
+    const unsigned block = a.base + blockIdx.x, t0 = block * a.tile, nt = min(a.tile, a.tokens - t0);
+    rope_table<kQkThreads>(a.at, t0, nt, cs);
+    __syncthreads();
+    const int lanes = 1 << a.log_lanes, lane = threadIdx.x & (lanes - 1);
+    const unsigned groups = kQkThreads >> a.log_lanes, group = threadIdx.x >> a.log_lanes, rows = a.rows.d;
+    float* red = reinterpret_cast<float*>(cs + a.tile * half);
+    const int width = a.units * V;
+    float acc[PER_HEAD ? 1 : 2][K][V] = {};
+    // One row: dx is written where `valid`.
+    auto row_of = [&](unsigned tk, unsigned row, bool valid) {
+        const Row<T, V> r(a, t0 + tk, row);
+        const T *src = r.x(), *dsrc = r.dy();
+        const float* w = r.side->w ? r.side->w + (long long)r.h * a.w_stride : nullptr;
+        float x[K][V], z[K][V], p[K][V], f[K][V];
+        double sxx = 0.0, sgx = 0.0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int u = lane + (k << a.log_lanes), at = u * V;
+#pragma unroll
+            for (int v = 0; v < V; v++) x[k][v] = z[k][v] = p[k][v] = f[k][v] = 0.f;
+            if (u >= a.units) continue;
+            take<T, V>(src + at, x[k]);
+            take<T, V>(dsrc + at, z[k]);
+            const int other = partner<V>(a, at);
+            if (other != at) take<T, V>(dsrc + other, p[k]);
+            weights<V>(w, at, f[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int u = lane + (k << a.log_lanes), at = u * V;
+            if (u >= a.units) continue;
+            rotate<V>(a, at, cs + tk * half, z[k], p[k]);
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                sxx = fma((double)x[k][v], (double)x[k][v], sxx);
+                sgx = fma((double)(f[k][v] * z[k][v]), (double)x[k][v], sgx);
+            }
+        }
+        const double r2 = 1.0 / (lane_sum_dyn(sxx, lanes) / a.dim + a.eps), rd = sqrt(r2);
+        const float rstd = (float)rd, mean = (float)(lane_sum_dyn(sgx, lanes) / a.dim * rd);
+        if (!valid) return;
+        T* out = r.side->out ? r.out() : nullptr;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int u = lane + (k << a.log_lanes), at = u * V;
+            if (u >= a.units) continue;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const float xh = x[k][v] * rstd, dw = z[k][v] * xh;
+                if constexpr (PER_HEAD) {
+                    acc[0][k][v] += dw;
+                } else {
+                    acc[0][k][v] += r.is_k ? 0.f : dw;
+                    acc[1][k][v] += r.is_k ? dw : 0.f;
+                }
+                x[k][v] = rstd * fmaf(f[k][v], z[k][v], -(xh * mean));
+            }
+            if (out) give<T, V>(out + at, x[k]);
+        }
+    };
+    auto lay = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int u = lane + (k << a.log_lanes);
+            if (u >= a.units) continue;
+#pragma unroll
+            for (int v = 0; v < V; v++) red[(i * groups + group) * width + u * V + v] = acc[i][k][v];
+        }
+    };
+    if constexpr (PER_HEAD) {
+        const unsigned slices = groups >= rows ? groups / rows : 1, heads = groups >= rows ? rows : groups;
+        const unsigned slice = group / heads;
+        for (unsigned h0 = 0; h0 < rows; h0 += heads) {
+            const unsigned h = h0 + group % heads;
+            for (unsigned tk0 = 0; tk0 < nt; tk0 += slices) {
+                const unsigned tk = tk0 + slice;
+                row_of(min(tk, nt - 1), min(h, rows - 1), tk < nt && slice < slices && h < rows);
+            }
+            if (!a.part) continue;
+            lay(0);
+            __syncthreads();
+            const unsigned here = min(heads, rows - h0);
+            for (unsigned e = threadIdx.x; e < here * a.dim; e += kQkThreads) {
+                const unsigned i = e / a.dim, d = e - i * a.dim;
+                float s = 0.f;
+                for (unsigned j = 0; j < slices; j++) s += red[(j * heads + i) * width + d];
+                a.part[((long long)block * rows + h0 + i) * a.dim + d] = s;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) acc[0][k][v] = 0.f;
+        }
+    } else {
+        const unsigned total = nt * rows;
+        for (unsigned first = 0; first < total; first += groups) {
+            const unsigned row = first + group, at_row = min(row, total - 1), tk = a.rows.div(at_row);
+            row_of(tk, at_row - tk * rows, row < total);
+        }
+        if (!a.part) return;
+        lay(0);
+        lay(1);
+        __syncthreads();
+        for (unsigned e = threadIdx.x; e < 2 * a.dim; e += kQkThreads) {
+            const unsigned i = e / a.dim, d = e - i * a.dim;
+            float s = 0.f;
+            for (unsigned g = 0; g < groups; g++) s += red[(i * groups + g) * width + d];
+            a.part[((long long)block * 2 + i) * a.dim + d] = s;
+        }
+    }
+}
+
+// The weights' gradients: column sums of part [rows][cols], 32 columns x 32 lanes a block; the first
+// q_cols of them are q's.
+__global__ __launch_bounds__(1024) void qk_fold_kernel(const float* part, long long rows, unsigned cols, unsigned q_cols, float* dwq, float* dwk) {
+    __shared__ double red[32][33];
+    const unsigned c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
+    double s = 0.0;
+    if (c < cols) {
+#pragma unroll 8
+        for (long long r = lane; r < rows; r += 32) s += (double)part[r * cols + c];
+    }
+    red[lane][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (lane || c >= cols) return;
+    for (int i = 1; i < 32; i++) s += red[i][threadIdx.x];
+    float* d = c < q_cols ? dwq : dwk;
+    if (d) d[c < q_cols ? c : c - q_cols] = (float)s;
+}
+
+// --------------------------------------------------------------------------------- host
+// The widest access (16, then 8 bytes, then an element) that every row's start, its length and, in mode 2, both halves allow.
+int width_of(std::initializer_list<const stx_tensor*> all, long long dim, const stx_rope_params* p, int size) {
+    for (int bytes : {16, 8}) {
+        const int w = bytes / size;
+        bool ok = dim % w == 0 && (p->mode == 0 || p->n_dims / 2 % w == 0);
+        for (const stx_tensor* t : all) ok = ok && rows_aligned(t, bytes);
+        if (ok) return w;
+    }
+    return 1;
+}
+
+struct Shape {
+    long long q_rows, k_rows, tokens, dim;
+    long long rows() const { return q_rows + k_rows; }
+    bool empty() const { return tokens == 0 || rows() == 0; }
+};
+
+Shape shape_of(const stx_tensor* q, const stx_tensor* k, const char* op) {
+    const long long n = q->ne[2], b = q->ne[3], dim = q->ne[0];
+    if (k)
+        STX_REQUIRE(k->ne[0] == dim && k->ne[2] == n && k->ne[3] == b, "%s: q and k differ in head size, tokens or batch", op);
+    const Shape s{q->ne[1], k ? k->ne[1] : 0, n * b, dim};
+    STX_REQUIRE(dim > 0, "%s: rows of no elements", op);
+    if (dim > kQkDim) fail(STX_STATUS_UNSUPPORTED, "%s: rows of %lld elements (%d at most)", op, dim, kQkDim);
+    if (s.empty()) return s;
+    STX_REQUIRE(n < (1LL << 31) && b < (1LL << 31) && n * b < (1LL << 31), "%s: more than 2^31 - 1 tokens", op);
+    STX_REQUIRE(s.rows() < (1LL << 24) && s.rows() * dim < (1LL << 27), "%s: too many rows a token", op);
+    return s;
+}
+
+// Tokens of a block of the backward pass: 64 at most, so that its sums are a small part of its traffic, and
+// four blocks a CU as long as there are tokens.
+constexpr long long kQkBlocks = 4 * 256;
+long long back_tile(long long tokens, int n_dims) {
+    return std::max(1LL, std::min({64LL, tokens / kQkBlocks, (long long)kRopeTable / (n_dims / 2)}));
+}
+// Blocks of the backward pass for any rotation of rows of `dim` elements.
+size_t back_part(const Shape& s, long long tile, int per_head) {
+    return (size_t)((s.tokens + tile - 1) / tile) * (per_head ? s.rows() : 2) * s.dim * sizeof(float);
+}
+
+QkArgs args_of(const stx_tensor* q, const Shape& s, const RopeAngles& at, const stx_rope_params* p, const int32_t* pos, double eps, int per_head, int w) {
+    QkArgs a{};
+    a.at = at;
+    a.at.pos = pos;
+    a.at.n = FastDiv((unsigned)q->ne[2]);
+    a.eps = eps;
+    a.tokens = (unsigned)s.tokens;
+    a.rows = FastDiv((unsigned)s.rows());
+    a.q_rows = (unsigned)s.q_rows;
+    a.dim = (int)s.dim;
+    a.units = (int)(s.dim / w);
+    while (a.log_lanes < 6 && (1 << a.log_lanes) < a.units) a.log_lanes++;
+    a.mode = p->mode;
+    a.w_stride = per_head ? a.dim : 0;
+    return a;
+}
+
+QkSide side(const stx_tensor* x, const stx_tensor* dy, const stx_tensor* out, const float* w) {
+    QkSide s{};
+    s.x = static_cast<const char*>(x->data);
+    s.x1 = x->nb[1], s.x2 = x->nb[2], s.x3 = x->nb[3];
+    if (dy) s.dy = static_cast<const char*>(dy->data), s.y1 = dy->nb[1], s.y2 = dy->nb[2], s.y3 = dy->nb[3];
+    if (out) s.out = static_cast<char*>(out->data), s.o1 = out->nb[1], s.o2 = out->nb[2], s.o3 = out->nb[3];
+    s.w = w;
+    return s;
+}
+
+// Calls f(V, K) as constants: units of w elements, as many a lane as a row of them needs.
+template <class T, class F>
+void with_units(int w, int units, F&& f) {
+    constexpr int W = 16 / sizeof(T);
+    auto lanes = [&](auto v) {
+        constexpr int V = v();
+        if (units <= 64) f(v, std::integral_constant<int, 1>{});
+        else f(v, std::integral_constant<int, kQkDim / 64 / V>{});
+    };
+    if (w == W) lanes(std::integral_constant<int, W>{});
+    else if (w == W / 2) lanes(std::integral_constant<int, W / 2>{});
+    else lanes(std::integral_constant<int, 1>{});
+}
+
+void check_eps(double eps, const char* op) { STX_REQUIRE(eps >= 0.0 && std::isfinite(eps), "%s: eps must be finite and not negative", op); }
+
+size_t weight_bytes(const stx_tensor* t, int per_head) { return t ? (size_t)t->ne[0] * (per_head ? t->ne[1] : 1) * sizeof(float) : 0; }
+
+void qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos, int64_t pos_stride, const stx_rope_params* p,
+                  const float* w_q, const float* w_k, int per_head, double eps, const stx_tensor* q_dst, const stx_tensor* k_dst, stx_stream stream) {
+    const char* op = "qk_norm_rope";
+    const int size = type_size(type);
+    check_row_output(q, q_dst, size, "qk_norm_rope: q");
+    STX_REQUIRE((k == nullptr) == (k_dst == nullptr), "%s: k and k_dst go together", op);
+    if (k) {
+        check_row_output(k, k_dst, size, "qk_norm_rope: k");
+        STX_REQUIRE(shared(q_dst, k_dst, size) != Shared::yes && shared(q_dst, k, size) != Shared::yes && shared(k_dst, q, size) != Shared::yes,
+                    "%s: an output overlaps the other side's tensors", op);
+    }
+    const Shape s = shape_of(q, k, op);
+    const RopeAngles at = rope_angles(p, s.dim, pos_stride, 1.f, op);
+    check_eps(eps, op);
+    for (const stx_tensor* d : {q_dst, k_dst})
+        if (d) check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, weight_bytes(q, per_head)}, {"w_k", w_k, weight_bytes(k, per_head)}});
+    if (s.empty()) return;
+    STX_REQUIRE(pos != nullptr, "%s: pos is NULL", op);
+    const int w = width_of({q, k, q_dst, k_dst}, s.dim, p, size);
+    QkArgs a = args_of(q, s, at, p, pos, eps, per_head, w);
+    a.q = side(q, nullptr, q_dst, w_q);
+    if (k) a.k = side(k, nullptr, k_dst, w_k);
+    // Tokens a block: four rounds of rows, as long as two blocks a CU remain.
+    const long long round = kQkThreads >> a.log_lanes;
+    const long long tile = std::max(1LL, std::min({16LL, 4 * round / s.rows(), s.tokens / 512, (long long)kRopeTable / (a.at.n_dims / 2)}));
+    a.tile = (unsigned)tile;
+    const size_t lds = sizeof(float2) * tile * (a.at.n_dims / 2);
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        with_units<T>(w, a.units, [&](auto v, auto n) {
+            launch_all((s.tokens + tile - 1) / tile, [&](dim3 grid, unsigned first) {
+                a.base = first;
+                hipLaunchKernelGGL((qk_norm_rope_kernel<T, v(), n()>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
+                launch_check("qk_norm_rope_kernel");
+            });
+        });
+    });
+}
+
+void qk_norm_rope_back(const stx_tensor* dyq, const stx_tensor* dyk, const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
+                       int64_t pos_stride, const stx_rope_params* p, const float* w_q, const float* w_k, int per_head, double eps, const stx_tensor* dq,
+                       const stx_tensor* dk, float* dw_q, float* dw_k, void* ws, size_t ws_bytes, stx_stream stream) {
+    const char* op = "qk_norm_rope_back";
+    const int size = type_size(type);
+    check_typed(q, size, "qk_norm_rope_back: q");
+    check_typed(dyq, size, "qk_norm_rope_back: dq_out");
+    check_same_shape(q, dyq, "qk_norm_rope_back: dq_out");
+    if (dq) {
+        check_row_output(q, dq, size, "qk_norm_rope_back: dq");
+        check_row_output(dyq, dq, size, "qk_norm_rope_back: dq");
+    }
+    STX_REQUIRE((k == nullptr) == (dyk == nullptr) && (k || (!dk && !dw_k)), "%s: k, dk_out and k's gradients go together", op);
+    if (k) {
+        check_typed(k, size, "qk_norm_rope_back: k");
+        check_typed(dyk, size, "qk_norm_rope_back: dk_out");
+        check_same_shape(k, dyk, "qk_norm_rope_back: dk_out");
+        if (dk) {
+            check_row_output(k, dk, size, "qk_norm_rope_back: dk");
+            check_row_output(dyk, dk, size, "qk_norm_rope_back: dk");
+        }
+        auto apart = [&](const stx_tensor* a, const stx_tensor* b) {
+            STX_REQUIRE(!a || !b || shared(a, b, size) != Shared::yes, "%s: an output overlaps the other side's tensors", op);
+        };
+        for (const stx_tensor* t : {k, dyk, dk}) apart(dq, t);
+        for (const stx_tensor* t : {q, dyq}) apart(dk, t);
+    }
+    const Shape s = shape_of(q, k, op);
+    const RopeAngles at = rope_angles(p, s.dim, pos_stride, -1.f, op);
+    check_eps(eps, op);
+    const bool sums = dw_q || dw_k;
+    const long long tile = s.empty() ? 1 : back_tile(s.tokens, p->n_dims);
+    const size_t need = sums && !s.empty() ? back_part(s, tile, per_head) : 0, wq = weight_bytes(q, per_head), wk = weight_bytes(k, per_head);
+    check_workspace(ws, ws_bytes, need, op);
+    check_apart(op, {{"dw_q", dw_q, wq}, {"dw_k", dw_k, wk}, {"the workspace", need ? ws : nullptr, need}},
+                {{"q", q, size}, {"k", k, size}, {"dq_out", dyq, size}, {"dk_out", dyk, size}, {"dq", dq, size}, {"dk", dk, size}, {"w_q", w_q, wq}, {"w_k", w_k, wk}});
+    for (const stx_tensor* d : {dq, dk})
+        if (d) check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, wq}, {"w_k", w_k, wk}});
+    if (!dq && !dk && !sums) return;
+    float* part = sums ? static_cast<float*>(ws) : nullptr;
+    long long blocks = 0;
+    if (!s.empty()) {
+        STX_REQUIRE(pos != nullptr, "%s: pos is NULL", op);
+        const int w = width_of({q, k, dyq, dyk, dq, dk}, s.dim, p, size);
+        QkArgs a = args_of(q, s, at, p, pos, eps, per_head, w);
+        a.q = side(q, dyq, dq, w_q);
+        if (k) a.k = side(k, dyk, dk, w_k);
+        a.tile = (unsigned)tile;
+        a.part = part;
+        blocks = (s.tokens + tile - 1) / tile;
+        const size_t lds = sizeof(float2) * tile * (p->n_dims / 2) + (sums ? sizeof(float) * (per_head ? 1 : 2) * (kQkThreads >> a.log_lanes) * a.units * w : 0);
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            with_units<T>(w, a.units, [&](auto v, auto n) {
+                launch_all(blocks, [&](dim3 grid, unsigned first) {
+                    a.base = first;
+                    if (per_head) hipLaunchKernelGGL((qk_norm_rope_back_kernel<T, v(), n(), true>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
+                    else hipLaunchKernelGGL((qk_norm_rope_back_kernel<T, v(), n(), false>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
+                    launch_check("qk_norm_rope_back_kernel");
+                });
+            });
+        });
+    }
+    if (!sums) return;
+    const unsigned cols = (unsigned)((per_head ? s.rows() : 2) * s.dim), q_cols = (unsigned)((per_head ? s.q_rows : 1) * s.dim);
+    if (cols == 0) return;
+    hipLaunchKernelGGL(qk_fold_kernel, dim3((cols + 31) / 32), dim3(1024), 0, as_stream(stream), part, blocks, cols, q_cols, dw_q, dw_k);
+    launch_check("qk_fold_kernel");
+}
+
+}  // namespace
+}  // namespace stx
+
+using namespace stx;
+
+extern "C" {
+
+STX_API stx_status stx_qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos, int64_t pos_stride,
+                                    const stx_rope_params* params, const float* w_q, const float* w_k, int per_head, double eps,
+                                    const stx_tensor* q_dst, const stx_tensor* k_dst, stx_stream stream) {
+    return guard([&] { qk_norm_rope(q, k, type, pos, pos_stride, params, w_q, w_k, per_head, eps, q_dst, k_dst, stream); });
+}
+
+STX_API size_t stx_qk_norm_rope_back_workspace_size(const stx_tensor* q, const stx_tensor* k, stx_type type, int n_dims, int per_head) {
+    size_t bytes = 0;
+    (void)guard([&] {
+        const int size = type_size(type);
+        STX_REQUIRE(q != nullptr, "qk_norm_rope_back_workspace_size: q is NULL");
+        for (const stx_tensor* t : {q, k})
+            for (int i = 0; t && i < 4; i++) STX_REQUIRE(t->ne[i] >= 0, "qk_norm_rope_back_workspace_size: negative ne[%d]", i);
+        (void)size;
+        const Shape s = shape_of(q, k, "qk_norm_rope_back_workspace_size");
+        STX_REQUIRE(n_dims > 0 && n_dims % 2 == 0 && n_dims <= s.dim, "qk_norm_rope_back_workspace_size: n_dims = %d", n_dims);
+        if (!s.empty()) bytes = back_part(s, back_tile(s.tokens, n_dims), per_head);
+    });
+    return bytes;
+}
+
+STX_API stx_status stx_qk_norm_rope_back(const stx_tensor* dq_out, const stx_tensor* dk_out, const stx_tensor* q, const stx_tensor* k,
+                                         stx_type type, const int32_t* pos, int64_t pos_stride, const stx_rope_params* params,
+                                         const float* w_q, const float* w_k, int per_head, double eps, const stx_tensor* dq,
+                                         const stx_tensor* dk, float* dw_q, float* dw_k, void* workspace, size_t workspace_bytes,
+                                         stx_stream stream) {
+    return guard([&] {
+        qk_norm_rope_back(dq_out, dk_out, q, k, type, pos, pos_stride, params, w_q, w_k, per_head, eps, dq, dk, dw_q, dw_k, workspace,
+                          workspace_bytes, stream);
+    });
+}
+
+}  // extern "C"

@@ -1,9 +1,8 @@
 // rope.hip — rotary positions over typed tensors with scaled angles, forward and backward
 // (stx_rope_scaled, stx_rope_scaled_back).
 #include <algorithm>
-#include <cmath>
 
-#include "typed.hpp"
+#include "rope_angles.hpp"
 
 namespace stx {
 namespace {
@@ -29,44 +28,13 @@ struct RopeSide {
 
 struct RopeScaledArgs {
     RopeSide q, k;
-    const int* pos;
-    const float* factors;
-    long long pos_stride;
+    RopeAngles at;
     unsigned tokens, tile;               // all tokens, and of a block
     unsigned base;                       // blocks of the launches before this one
-    FastDiv n;                           // ne2: token -> (i3, i2)
     FastDiv rows, units;                 // rows of a token (q's, then k's); units of a row
     unsigned q_rows;
-    int dim, n_dims;
-    double log2_base, scale, ext, lo, inv_range, m;
-    float sign;                          // -1: the gradient
+    int dim;
 };
-
-// cos and sin of a finite angle |theta| < 2^40: theta - n pi/2 with pi/2 in two doubles (the fma
-// makes the first product exact), then Taylor polynomials on |r| <= pi/4, cut below 2^-33.
-__device__ __forceinline__ void cos_sin(double theta, double& c, double& s) {
-    const double n = rint(theta * 0.63661977236758134308);
-    const double r = fma(-n, 6.123233995736765886e-17, fma(-n, 1.57079632679489661923, theta));
-    const double z = r * r;
-    double ps = -2.50521083854417187751e-08;               // -1/11!
-    ps = fma(ps, z, 2.75573192239858906526e-06);
-    ps = fma(ps, z, -1.98412698412698412698e-04);
-    ps = fma(ps, z, 8.33333333333333333333e-03);
-    ps = fma(ps, z, -1.66666666666666666667e-01);
-    const double sn = fma(ps * z, r, r);
-    double pc = 2.08767569878680989792e-09;                // 1/12!
-    pc = fma(pc, z, -2.75573192239858906526e-07);
-    pc = fma(pc, z, 2.48015873015873015873e-05);
-    pc = fma(pc, z, -1.38888888888888888889e-03);
-    pc = fma(pc, z, 4.16666666666666666667e-02);
-    pc = fma(pc, z, -5.00000000000000000000e-01);
-    const double cn = fma(pc, z, 1.0);
-    const int quad = (int)(long long)n & 3;
-    c = quad & 1 ? sn : cn;
-    s = quad & 1 ? cn : sn;
-    if (quad == 1 || quad == 2) c = -c;
-    if (quad >= 2) s = -s;
-}
 
 // What a thread moves at once. MODE 0: V elements, V/2 adjacent pairs. MODE 2: V elements of the
 // first half and V of the second, or V elements past n_dims. VEC: as vectors of V; otherwise
@@ -94,33 +62,21 @@ constexpr int kRopeThreads = 256;
 // Units a thread of a tile, one after another. The two calls above by it: 1: 81, 134 us; 2: 72, 136; 4: 73, 132;
 // 8: 77, 149. Four loaded before the first is stored: 76, 150 (the waves' registers, hence fewer waves).
 constexpr int kRopeUnits = 4;
-constexpr int kRopeTable = 4096;         // pairs in LDS: 32 KB
 constexpr int kRopeTile = 16;
 
 template <class T, int V, bool VEC, int MODE>
 __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(RopeScaledArgs a) {
     extern __shared__ float2 cs[];       // [tile][n_dims / 2]
-    const int half = a.n_dims / 2;
+    const int half = a.at.n_dims / 2;
     const unsigned t0 = (a.base + blockIdx.x) * a.tile;
     const unsigned nt = min(a.tile, a.tokens - t0);
-    for (unsigned e = threadIdx.x; e < nt * (unsigned)half; e += kRopeThreads) {
-        const unsigned t = t0 + e / (unsigned)half;
-        const int i = (int)(e % (unsigned)half);
-        const unsigned i3 = a.n.div(t);
-        const double p = (double)a.pos[(long long)i3 * a.pos_stride + (t - i3 * a.n.d)];
-        double far = exp2(-2.0 * i / a.n_dims * a.log2_base);
-        if (a.factors) far /= (double)a.factors[i];
-        const double mix = a.ext * (1.0 - fmin(1.0, fmax(0.0, ((double)i - a.lo) * a.inv_range)));
-        double c, s;
-        cos_sin(p * (a.ext != 0.0 ? a.scale * far * (1.0 - mix) + far * mix : a.scale * far), c, s);
-        cs[e] = make_float2((float)(c * a.m), a.sign * (float)(s * a.m));
-    }
+    rope_table<kRopeThreads>(a.at, t0, nt, cs);
     __syncthreads();
     const unsigned total = nt * a.rows.d * a.units.d;
     for (unsigned e = threadIdx.x; e < total; e += kRopeThreads) {
         const unsigned row = a.units.div(e), u = e - row * a.units.d;
         const unsigned tk = a.rows.div(row), h = row - tk * a.rows.d;
-        const unsigned t = t0 + tk, i3 = a.n.div(t), i2 = t - i3 * a.n.d;
+        const unsigned t = t0 + tk, i3 = a.at.n.div(t), i2 = t - i3 * a.at.n.d;
         const bool is_k = h >= a.q_rows;
         const RopeSide& side = is_k ? a.k : a.q;
         const long long i1 = is_k ? h - a.q_rows : h;
@@ -141,7 +97,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(RopeScaledArg
             }
             rope_store<T, V, VEC>(out + at, x, a.dim - at);
         } else {
-            const int pairs = half / V, at = (int)u < pairs ? (int)u * V : a.n_dims + ((int)u - pairs) * V;
+            const int pairs = half / V, at = (int)u < pairs ? (int)u * V : a.at.n_dims + ((int)u - pairs) * V;
             Pack<T, V> x = rope_load<T, V, VEC>(src + at, V);
             if (at < half) {
                 Pack<T, V> y = rope_load<T, V, VEC>(src + at + half, V);
@@ -157,29 +113,6 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(RopeScaledArg
             rope_store<T, V, VEC>(out + at, x, V);
         }
     }
-}
-
-// Whether every row of src and dst starts at a multiple of `bytes`.
-bool rows_aligned(const stx_tensor* t, int bytes) {
-    if (!t) return true;
-    bool ok = reinterpret_cast<uintptr_t>(t->data) % bytes == 0;
-    for (int i = 1; i < 4; i++) ok = ok && (t->ne[i] <= 1 || t->nb[i] % bytes == 0);
-    return ok;
-}
-
-void check_out(const stx_tensor* src, const stx_tensor* dst, int size, const char* what) {
-    check_typed(src, size, what);
-    check_typed(dst, size, what);
-    check_same_shape(src, dst, what);
-    bool same = src->data == dst->data;
-    for (int i = 1; i < 4; i++) {
-        STX_REQUIRE(dst->ne[i] <= 1 || dst->nb[i] > 0, "%s: output stride nb[%d] is 0", what, i);
-        same = same && (dst->ne[i] <= 1 || dst->nb[i] == src->nb[i]);
-    }
-    STX_REQUIRE(nelem(view(dst)) == 0 || nested(dst, size), "%s: rows of the output overlap", what);
-    // In place with other strides, or in part over the input, rows would be read after they were written.
-    STX_REQUIRE(same || src->data != dst->data || nelem(view(src)) == 0, "%s: in place with other strides", what);
-    STX_REQUIRE(same || shared(src, dst, size) != Shared::yes, "%s: the output overlaps the input in part", what);
 }
 
 RopeSide side_of(const stx_tensor* s, const stx_tensor* d) {
@@ -201,39 +134,18 @@ void rope_launch(RopeScaledArgs a, int mode, size_t lds, hipStream_t stream) {
 void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos, int64_t pos_stride,
                  const stx_rope_params* p, const stx_tensor* q_dst, const stx_tensor* k_dst, float sign, stx_stream stream) {
     const int size = type_size(type);
-    STX_REQUIRE(p != nullptr && p->size >= sizeof(stx_rope_params), "rope_scaled: params are NULL or their size is too small");
-    check_out(q, q_dst, size, "rope_scaled: q");
+    check_row_output(q, q_dst, size, "rope_scaled: q");
     STX_REQUIRE((k == nullptr) == (k_dst == nullptr), "rope_scaled: k and k_dst go together");
     if (k) {
-        check_out(k, k_dst, size, "rope_scaled: k");
+        check_row_output(k, k_dst, size, "rope_scaled: k");
         STX_REQUIRE(k->ne[0] == q->ne[0] && k->ne[2] == q->ne[2] && k->ne[3] == q->ne[3],
                     "rope_scaled: q and k differ in head size, tokens or batch");
         STX_REQUIRE(shared(q_dst, k_dst, size) != Shared::yes && shared(q_dst, k, size) != Shared::yes && shared(k_dst, q, size) != Shared::yes,
                     "rope_scaled: an output overlaps the other side's tensors");
     }
     const long long dim = q->ne[0];
-    if (p->mode != 0 && p->mode != 2) fail(STX_STATUS_UNSUPPORTED, "rope_scaled: mode %d (only 0 and 2)", p->mode);
-    STX_REQUIRE(p->n_dims > 0 && p->n_dims % 2 == 0 && p->n_dims <= dim, "rope_scaled: n_dims must be even, positive and <= ne0");
-    if (p->n_dims > 2 * kRopeTable || dim > (1 << 20)) fail(STX_STATUS_UNSUPPORTED, "rope_scaled: rows of %lld with %d rotated", dim, p->n_dims);
-    STX_REQUIRE(p->freq_base > 0.f && p->freq_scale > 0.f, "rope_scaled: freq_base and freq_scale must be positive");
-    for (float v : {p->freq_base, p->freq_scale, p->ext_factor, p->attn_factor})
-        STX_REQUIRE(std::isfinite(v), "rope_scaled: a parameter is not finite");
-    STX_REQUIRE(p->ext_factor == 0.f || (std::isfinite(p->beta_fast) && std::isfinite(p->beta_slow)), "rope_scaled: beta_fast or beta_slow is not finite");
-    STX_REQUIRE(pos_stride >= 0, "rope_scaled: negative pos_stride");
     RopeScaledArgs a{};
-    a.log2_base = std::log2((double)p->freq_base);
-    a.scale = p->freq_scale;
-    a.ext = p->ext_factor;
-    a.m = p->attn_factor;
-    if (p->ext_factor != 0.f) {
-        STX_REQUIRE(p->n_ctx_orig > 0 && p->beta_fast > 0.f && p->beta_slow > 0.f && p->freq_base != 1.f,
-                    "rope_scaled: ext_factor needs n_ctx_orig, beta_fast and beta_slow above 0 and freq_base != 1");
-        const double pi = 3.14159265358979323846;
-        auto turns = [&](double r) { return p->n_dims * std::log(p->n_ctx_orig / (r * 2 * pi)) / (2 * std::log((double)p->freq_base)); };
-        a.lo = std::fmax(0.0, std::floor(turns(p->beta_fast)));
-        a.inv_range = 1.0 / std::fmax(0.001, std::fmin(p->n_dims - 1.0, std::ceil(turns(p->beta_slow))) - a.lo);
-        a.m *= 1.0 + 0.1 * std::log(1.0 / (double)p->freq_scale);
-    }
+    a.at = rope_angles(p, dim, pos_stride, sign, "rope_scaled");
     const long long q_rows = q->ne[1], k_rows = k ? k->ne[1] : 0, n = q->ne[2];
     if (n == 0 || q->ne[3] == 0 || q_rows + k_rows == 0) return;
     STX_REQUIRE(n < (1LL << 31) && q->ne[3] < (1LL << 31) && n * q->ne[3] < (1LL << 31), "rope_scaled: more than 2^31 - 1 tokens");
@@ -241,18 +153,14 @@ void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const 
     STX_REQUIRE(pos != nullptr, "rope_scaled: pos is NULL");
     a.q = side_of(q, q_dst);
     a.k = side_of(k, k_dst);
-    a.pos = pos;
-    a.pos_stride = pos_stride;
-    a.factors = p->freq_factors;
+    a.at.pos = pos;
     a.tokens = (unsigned)(n * q->ne[3]);
-    a.n = FastDiv((unsigned)n);
+    a.at.n = FastDiv((unsigned)n);
     a.rows = FastDiv((unsigned)(q_rows + k_rows));
     a.q_rows = (unsigned)q_rows;
     a.dim = (int)dim;
-    a.n_dims = p->n_dims;
-    a.sign = sign;
     // The widest access (16, then 8 bytes) that every row's start and, in mode 2, both halves allow.
-    const int half = a.n_dims / 2;
+    const int half = p->n_dims / 2;
     int v = 0;
     for (int bytes : {16, 8}) {
         const int w = bytes / size;
@@ -260,7 +168,7 @@ void rope_scaled(const stx_tensor* q, const stx_tensor* k, stx_type type, const 
         if (v == 0 && fits && rows_aligned(q, bytes) && rows_aligned(q_dst, bytes) && rows_aligned(k, bytes) && rows_aligned(k_dst, bytes)) v = w;
     }
     const int w = v ? v : p->mode == 0 ? 2 : 1;
-    a.units = FastDiv((unsigned)(p->mode == 0 ? (dim + w - 1) / w : half / w + (dim - a.n_dims + w - 1) / w));
+    a.units = FastDiv((unsigned)(p->mode == 0 ? (dim + w - 1) / w : half / w + (dim - p->n_dims + w - 1) / w));
     // Tokens a block: kRopeUnits units a thread, as long as two blocks a CU remain.
     const long long items = (long long)a.rows.d * a.units.d;
     long long tile = std::max(1LL, std::min<long long>(kRopeTile, kRopeThreads * kRopeUnits / items));

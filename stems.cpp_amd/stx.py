@@ -132,6 +132,10 @@ _SIGNATURES = {
     "stx_gated_ff_back_workspace_size": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _i]),
     "stx_gated_ff_back": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
                                _vp]),
+    "stx_qk_norm_rope": (_i, [_vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _i, ctypes.c_double, _vp, _vp, _vp]),
+    "stx_qk_norm_rope_back_workspace_size": (ctypes.c_size_t, [_vp, _vp, _i, _i, _i]),
+    "stx_qk_norm_rope_back": (_i, [_vp, _vp, _vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _i, ctypes.c_double, _vp, _vp,
+                                   _vp, _vp, _vp, ctypes.c_size_t, _vp]),
 }
 
 
@@ -1237,16 +1241,7 @@ def _scratch(need, workspace, like, stream):
 
 
 def _rope_scaled(fn, q, pos, params, k, out, k_out, stream):
-    import torch
-    shape = q.shape
-    if len(shape) not in (3, 4):
-        raise ValueError("q must be (batch, tokens, heads, head size) or (tokens, heads, head size)")
-    batch, n = (shape[0] if len(shape) == 4 else 1), shape[-3]
-    if pos.dtype is not torch.int32 or pos.device != q.device or tuple(pos.shape) not in ((n,), (batch, n)) or (n > 1 and pos.stride(-1) != 1):
-        raise ValueError(f"pos must be ({n},) or ({batch}, {n}) int32 with contiguous rows on {q.device}, is {tuple(pos.shape)} {pos.dtype}")
-    factors = getattr(params, "factors", None)
-    if factors is not None and factors.device != q.device:
-        raise ValueError(f"freq_factors are on {factors.device}, q is on {q.device}")
+    _positions(q, pos, params)
     out = _empty_like(q, stream) if out is None else out
     dk = dko = None
     if k is not None:
@@ -1353,3 +1348,84 @@ def gated_ff_back(dh, x, w_gate, w_value, act=ACT_SIGMOID, b_gate=None, b_value=
             _floats(b_value, x, N, "b_value"), int(act), d[4], d[5], d[6], _floats(db_gate, x, N, "db_gate"),
             _floats(db_value, x, N, "db_value"), ws, nbytes)
     return dx, dw_gate, dw_value, db_gate, db_value
+
+
+# ------------------------------------------------------ attention operators (fp32, fp16, bf16)
+def _positions(q, pos, params):
+    """(batch, tokens) of q (batch, tokens, heads, head size) or (tokens, heads, head size), its positions checked."""
+    import torch
+    shape = q.shape
+    if len(shape) not in (3, 4):
+        raise ValueError("q must be (batch, tokens, heads, head size) or (tokens, heads, head size)")
+    batch, n = (shape[0] if len(shape) == 4 else 1), shape[-3]
+    if pos.dtype is not torch.int32 or pos.device != q.device or tuple(pos.shape) not in ((n,), (batch, n)) or (n > 1 and pos.stride(-1) != 1):
+        raise ValueError(f"pos must be ({n},) or ({batch}, {n}) int32 with contiguous rows on {q.device}, is {tuple(pos.shape)} {pos.dtype}")
+    factors = getattr(params, "factors", None)
+    if factors is not None and factors.device != q.device:
+        raise ValueError(f"freq_factors are on {factors.device}, q is on {q.device}")
+    return batch, n
+
+
+def _head_weights(q, k, w_q, w_k):
+    """Whether the norms' weights are (heads, head size), one for each head, instead of (head size,)."""
+    dims = {w.dim() for w in (w_q, w_k) if w is not None}
+    if len(dims) > 1 or not dims <= {1, 2}:
+        raise ValueError("w_q and w_k must both be (head size,), or (heads, head size) and (kv heads, head size)")
+    per_head = dims == {2}
+    for w, x, what in ((w_q, q, "w_q"), (w_k, k, "w_k")):
+        if w is not None and (x is None or tuple(w.shape) != (tuple(x.shape[-2:]) if per_head else (x.shape[-1],))):
+            raise ValueError(f"{what} has shape {tuple(w.shape)}, which is not its side's")
+    return per_head
+
+
+def _weight(w, x, what):
+    return None if w is None else _floats(w, x, w.numel(), what)
+
+
+def qk_norm_rope(q, pos, params, w_q=None, k=None, w_k=None, eps=1e-6, out=None, k_out=None, stream=None):
+    """Rotary positions of w * x / sqrt(mean(x^2) + eps) for every row x of q (batch, tokens, heads, head size) and, in
+    the same launch, of k (batch, tokens, kv heads, head size): out, or (out, k_out). w_q, w_k: float32 device (head
+    size,), or one for each head, (heads, head size) and (kv heads, head size); None: 1. pos, params, strides and
+    outputs that may be the inputs as in rope_scaled."""
+    _positions(q, pos, params)
+    per_head = _head_weights(q, k, w_q, w_k)
+    out = _empty_like(q, stream) if out is None else out
+    dk = dko = None
+    if k is not None:
+        k_out = _empty_like(k, stream) if k_out is None else k_out
+        dk, dko = _typed(k, q, "k"), _typed(k_out, q, "k_out")
+    _launch(lib().stx_qk_norm_rope, q, stream, _typed(q, q, "q"), dk, _type(q), pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0,
+            ctypes.byref(params), _weight(w_q, q, "w_q"), _weight(w_k, q, "w_k"), per_head, float(eps), _typed(out, q, "out"), dko)
+    return out if k is None else (out, k_out)
+
+
+def qk_norm_rope_back(dy, q, pos, params, w_q=None, dy_k=None, k=None, w_k=None, eps=1e-6, dq=None, dk=None, dw_q=None, dw_k=None,
+                      workspace=None, stream=None):
+    """Gradients (dq, dw_q, dk, dw_k) of qk_norm_rope from dy and dy_k (of its outputs) and its inputs; dw_q and dw_k are
+    float32 in their weights' layout, None where there are no such weights, and dk and dw_k None without k. dq may be dy
+    or q, dk may be dy_k or k."""
+    import torch
+    _positions(q, pos, params)
+    per_head = _head_weights(q, k, w_q, w_k)
+    dq = _empty_like(q, stream) if dq is None else dq
+    if k is not None and dk is None:
+        dk = _empty_like(k, stream)
+    if w_q is not None and dw_q is None:
+        dw_q = _empty(w_q.shape, q, stream, torch.float32)
+    if w_k is not None and dw_k is None:
+        dw_k = _empty(w_k.shape, q, stream, torch.float32)
+    L, t, a = lib(), _type(q), _typed(q, q, "q")
+    b = None if k is None else _typed(k, q, "k")
+    ws, nbytes, keep = _scratch(L.stx_qk_norm_rope_back_workspace_size(a, b, t, params.n_dims, per_head), workspace, q, stream)
+    _launch(L.stx_qk_norm_rope_back, q, stream, _typed(dy, q, "dy"), None if dy_k is None else _typed(dy_k, q, "dy_k"), a, b, t,
+            pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, ctypes.byref(params), _weight(w_q, q, "w_q"),
+            _weight(w_k, q, "w_k"), per_head, float(eps), _typed(dq, q, "dq"), None if dk is None else _typed(dk, q, "dk"),
+            _floats_like(dw_q, w_q, q, "dw_q"), _floats_like(dw_k, w_k, q, "dw_k"), ws, nbytes)
+    return dq, dw_q, dk, dw_k
+
+
+def _floats_like(t, w, like, what):
+    """_floats of a gradient of w's shape."""
+    if t is not None and w is None:
+        raise ValueError(f"{what} without its weights")
+    return None if t is None else _floats(t, like, w.numel(), what)
