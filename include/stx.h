@@ -906,6 +906,42 @@ STX_API stx_status stx_qk_norm_rope_back(const stx_tensor* dq_out, const stx_ten
                                          float* dw_q, float* dw_k, void* workspace, size_t workspace_bytes,
                                          stx_stream stream);
 
+/* Buckets of key positions relative to a query's, rel = key - query: with n buckets on a side (n_buckets, or half of
+ * them when bidirectional, the first half for rel <= 0 and the second for rel > 0), near = n / 2 and d = |rel|
+ * (not bidirectional: max(-rel, 0), so later keys are in bucket 0),
+ *   d                                                                                  for d < near
+ *   min(n - 1, near + floor((n - near) * ln(d / near) / ln(max_distance / near)))      otherwise
+ * (Raffel et al., "Exploring the limits of transfer learning", 2020, section 2.1). A distance on a border belongs to the
+ * bucket above: borders are found in whole numbers. Size tagged: set size to the struct's. */
+typedef struct {
+    uint32_t size;
+    int32_t  n_buckets;            /* 2 (bidirectional: 4, and even) .. 256 */
+    int32_t  max_distance;         /* near < max_distance <= 2048 */
+    int32_t  bidirectional;        /* buckets of their own for keys after the query */
+    int32_t  causal;               /* a query sees no key after its own position */
+} stx_rel_params;
+
+/* stx_soft_max_ext with a learned position bias and masks, which that op refuses, over scores x [keys, queries, heads,
+ * batch] of any of the types:
+ *   dst = softmax over the keys of scale * x + table[bucket(key - (query + start))][head].
+ * table: device float [n_buckets][heads] (ggml [heads, n_buckets]). lengths: device int32[batch], keys of each sequence,
+ * taken as 0 .. keys (NULL: all); starts: device int32[batch], the position of its first query (NULL: 0). Masked scores
+ * are not read into the result whatever they hold, NaN among it, and get zeros; a row that sees no key, or only scores of
+ * -infinity, is zeros. Sums are float. Rows are contiguous; any other strides. dst may be x, and overlaps nothing else. Fewer than 2^30 keys and
+ * queries, 2^24 heads and sequences. */
+STX_API stx_status stx_soft_max_rel(const stx_tensor* x, stx_type type, const float* table,
+                                    const stx_rel_params* params, float scale, const int32_t* lengths,
+                                    const int32_t* starts, const stx_tensor* dst, stx_stream stream);
+/* Its gradients, from dy (of dst), y (dst as the forward call left it) and the same masks: dx (of x) and dtable (device
+ * float [n_buckets][heads], summed over the batch); either may be NULL. Row dots and the table's sums are formed in
+ * double. dx overlaps no input. At most 65,535 heads. workspace: device, 256-byte aligned, no initialisation; calls that share one must not
+ * overlap. None is needed without dtable. */
+STX_API size_t     stx_soft_max_rel_back_workspace_size(const stx_tensor* y, stx_type type, int n_buckets);
+STX_API stx_status stx_soft_max_rel_back(const stx_tensor* dy, const stx_tensor* y, stx_type type,
+                                         const stx_rel_params* params, float scale, const int32_t* lengths,
+                                         const int32_t* starts, const stx_tensor* dx, float* dtable, void* workspace,
+                                         size_t workspace_bytes, stx_stream stream);
+
 /* ------------------------------------------------------------------------------------------
  * Versioned function table (after libstems V1, src/libstems_v1.h:146-189). Every entry point
  * above, in header order; a later revision of V1 may append entries (never reorder them), so
@@ -1142,6 +1178,15 @@ typedef struct stx_api_v1 {
                                     const stx_tensor* dq, const stx_tensor* dk, float* dw_q,
                                     float* dw_k, void* workspace, size_t workspace_bytes,
                                     stx_stream stream);
+    stx_status (*soft_max_rel)(const stx_tensor* x, stx_type type, const float* table,
+                               const stx_rel_params* params, float scale, const int32_t* lengths,
+                               const int32_t* starts, const stx_tensor* dst, stx_stream stream);
+    size_t (*soft_max_rel_back_workspace_size)(const stx_tensor* y, stx_type type, int n_buckets);
+    stx_status (*soft_max_rel_back)(const stx_tensor* dy, const stx_tensor* y, stx_type type,
+                                    const stx_rel_params* params, float scale,
+                                    const int32_t* lengths, const int32_t* starts,
+                                    const stx_tensor* dx, float* dtable, void* workspace,
+                                    size_t workspace_bytes, stx_stream stream);
     void (*reserved[16])(void);
 } stx_api_v1;
 

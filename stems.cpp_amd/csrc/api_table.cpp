@@ -107,6 +107,9 @@ const stx_api_v1 kApiV1 = {
     &stx_qk_norm_rope,
     &stx_qk_norm_rope_back_workspace_size,
     &stx_qk_norm_rope_back,
+    &stx_soft_max_rel,
+    &stx_soft_max_rel_back_workspace_size,
+    &stx_soft_max_rel_back,
     {},
 };
 }  // namespace

@@ -136,6 +136,9 @@ _SIGNATURES = {
     "stx_qk_norm_rope_back_workspace_size": (ctypes.c_size_t, [_vp, _vp, _i, _i, _i]),
     "stx_qk_norm_rope_back": (_i, [_vp, _vp, _vp, _vp, _i, _vp, ctypes.c_int64, _vp, _vp, _vp, _i, ctypes.c_double, _vp, _vp,
                                    _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "stx_soft_max_rel": (_i, [_vp, _i, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "stx_soft_max_rel_back_workspace_size": (ctypes.c_size_t, [_vp, _i, _i]),
+    "stx_soft_max_rel_back": (_i, [_vp, _vp, _i, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
 }
 
 
@@ -1429,3 +1432,62 @@ def _floats_like(t, w, like, what):
     if t is not None and w is None:
         raise ValueError(f"{what} without its weights")
     return None if t is None else _floats(t, like, w.numel(), what)
+
+
+class RelParams(ctypes.Structure):
+    """stx_rel_params: buckets of relative positions."""
+    _fields_ = [("size", ctypes.c_uint32), ("n_buckets", ctypes.c_int32), ("max_distance", ctypes.c_int32),
+                ("bidirectional", ctypes.c_int32), ("causal", ctypes.c_int32)]
+
+
+def rel_params(n_buckets=32, max_distance=128, bidirectional=True, causal=False):
+    """The buckets of soft_max_rel, and whether a query sees later keys."""
+    return RelParams(ctypes.sizeof(RelParams), int(n_buckets), int(max_distance), int(bool(bidirectional)), int(bool(causal)))
+
+
+def _per_sequence(t, like, count, what):
+    """Pointer of an int32 vector with a value for each sequence, or None."""
+    if t is None:
+        return None
+    import torch
+    return _floats(t, like, count, what, torch.int32)
+
+
+def _scores(x, what):
+    if x.dim() != 4:
+        raise ValueError(f"{what} must be (batch, heads, queries, keys), is {tuple(x.shape)}")
+    return x.shape
+
+
+def soft_max_rel(x, table, params, scale=1.0, lengths=None, starts=None, out=None, stream=None):
+    """softmax(scale * x + table[bucket]) over the keys of scores x (batch, heads, queries, keys), bucket that of the key's
+    position less the query's (rel_params). table: float32 device (n_buckets, heads); lengths: int32 device (batch,), keys
+    of each sequence (None: all); starts: int32 device (batch,), position of its first query (None: 0). Masked places, and
+    rows that see no key, are 0. Rows are contiguous, other strides any; out may be x."""
+    B, H = _scores(x, "x")[:2]
+    out = _empty_like(x, stream) if out is None else out
+    if tuple(table.shape) != (params.n_buckets, H):
+        raise ValueError(f"table must be ({params.n_buckets}, {H}), is {tuple(table.shape)}")
+    _launch(lib().stx_soft_max_rel, x, stream, _typed(x, x, "x"), _type(x), _floats(table, x, params.n_buckets * H, "table"),
+            ctypes.byref(params), float(scale), _per_sequence(lengths, x, B, "lengths"), _per_sequence(starts, x, B, "starts"),
+            _typed(out, x, "out"))
+    return out
+
+
+def soft_max_rel_back(dy, y, params, scale=1.0, lengths=None, starts=None, dx=None, dtable=None, workspace=None, stream=None):
+    """Gradients (dx, dtable) of soft_max_rel from dy, its result y and the same masks; dtable is float32 (n_buckets, heads).
+    dtable=False: not computed (None)."""
+    import torch
+    B, H = _scores(y, "y")[:2]
+    dx = _empty_like(y, stream) if dx is None else dx
+    if dtable is None:
+        dtable = _empty((params.n_buckets, H), y, stream, torch.float32)
+    elif dtable is False:
+        dtable = None
+    L, t, a = lib(), _type(y), _typed(y, y, "y")
+    need = 0 if dtable is None else L.stx_soft_max_rel_back_workspace_size(a, t, params.n_buckets)
+    ws, nbytes, keep = _scratch(need, workspace, y, stream)
+    _launch(L.stx_soft_max_rel_back, y, stream, _typed(dy, y, "dy"), a, t, ctypes.byref(params), float(scale),
+            _per_sequence(lengths, y, B, "lengths"), _per_sequence(starts, y, B, "starts"), _typed(dx, y, "dx"),
+            _floats(dtable, y, params.n_buckets * H, "dtable"), ws, nbytes)
+    return dx, dtable

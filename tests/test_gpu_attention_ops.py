@@ -8,6 +8,11 @@ result's type relative to the value, plus half the smallest subnormal step of fp
           g = w dz, dx = r (g - xh mean(g xh)): each term's roundings, 8 u r (|w| D + |xh| mean(|w| D |xh|)).
           dw: sums of dz xh over n rows in float of at most n / 4 + 64 terms: each partial sum is at most S = sum |D xh|,
           a random walk of sqrt(n) roundings u S / ... bounded by (8 + 4 sqrt(n)) u S.
+  rel     an exponent in units of log2 has the roundings of scale log2e, of the fused product and bias, of the bias and of
+          the difference to the row's largest: 5 u (|scale x| + |bias|) of the natural one; at most 5 u Z relative to
+          each exponential, Z the row's largest |scale x| + |bias|, as much of their sum, 2 u of the hardware's 2^y each,
+          and of the sum a rounding for each of a lane's terms and 16 of the tree. Backward: products and sums are in
+          double, so one rounding to float and one to the type; the table's sums one.
 """
 import math
 
@@ -173,3 +178,208 @@ def test_qk_empty(device):
     assert stx.qk_norm_rope(x, pos, p, w).shape == x.shape
     dx, dw, _, _ = stx.qk_norm_rope_back(x, x, pos, p, w)
     assert dx.shape == x.shape and torch.equal(dw, torch.zeros(8, device=device))
+
+
+# ------------------------------------------------------------------ softmax with a position bias
+def edges_of(n_buckets, distance, both):
+    """(buckets of a side, exact ones, first distance of each of the others), in whole numbers."""
+    n = n_buckets // 2 if both else n_buckets
+    near = n // 2
+    m = n - near
+    first = []
+    for k in range(m):
+        d = near
+        while d ** m < near ** (m - k) * distance ** k:
+            d += 1
+        first.append(d)
+    return n, near, first
+
+
+def buckets_ref(rel, n_buckets, distance, both):
+    n, near, first = edges_of(n_buckets, distance, both)
+    d = rel.abs() if both else (-rel).clamp(min=0)
+    k = d.clamp(max=near)
+    for i, edge in enumerate(first):
+        k = torch.where(d >= edge, near + i, k)
+    return torch.where((rel > 0) & both, k + n, k)
+
+
+def seen_ref(B, M, N, lengths, starts, causal, device):
+    """Which keys each query sees, and key less query position, (B, M, N)."""
+    start = torch.zeros(B, device=device, dtype=torch.int64) if starts is None else starts.long()
+    end = torch.full((B,), N, device=device) if lengths is None else lengths.long()
+    j = torch.arange(N, device=device)
+    rel = j - (torch.arange(M, device=device)[:, None] + start[:, None, None])
+    mask = (j < end[:, None, None]).expand(B, M, N)
+    return (mask & (rel <= 0) if causal else mask), rel
+
+
+REL = [
+    # B, H, M, N, n_buckets, max_distance, both, causal, masks
+    (1, 1, 1, 1, 32, 128, True, False, None),
+    (8, 8, 1, 801, 32, 128, False, True, "ragged"),
+    (2, 3, 60, 60, 32, 128, True, False, None),               # several rows a wave
+    (2, 3, 61, 7, 8, 20, True, True, "ragged"),
+    (2, 2, 130, 131, 4, 3, True, False, "ragged"),
+    (3, 2, 77, 513, 16, 50, False, False, "ragged"),          # later keys all in bucket 0
+    (1, 2, 801, 801, 32, 128, True, False, None),
+    (2, 1, 90, 1100, 64, 1000, True, False, "ragged"),        # reach beyond most keys
+    (1, 2, 40, 2049, 32, 128, False, True, None),
+    (1, 1, 9, 4100, 256, 2048, True, False, None),
+    (1, 1, 5, 8200, 32, 128, True, False, "ragged"),
+    (1, 2, 3, 17001, 32, 128, True, True, "ragged"),          # rows read twice
+    (1, 1, 300, 33, 2, 2, False, True, None),
+]
+
+
+def rel_inputs(device, dt, shape):
+    B, H, M, N, nb, dist, both, causal, masks = shape
+    x = randn(device, (B, H, M, N), 1, 6.0, dtype=dt)
+    table = randn(device, (nb, H), 2, 0.7)
+    lengths = starts = None
+    if masks:
+        lengths = torch.tensor([max(1, N - 7 * b - N // 3 * (b % 2)) for b in range(B)], device=device, dtype=torch.int32)
+    if causal:
+        starts = torch.tensor([max(0, (N if lengths is None else int(lengths[b])) - M) for b in range(B)], device=device, dtype=torch.int32)
+    return x, table, lengths, starts, stx.rel_params(nb, dist, both, causal)
+
+
+def rel_ref(x, table, mask, bucket, scale):
+    """y and the largest |scale x| + |bias| of each row; rows without keys are zeros."""
+    bias = table.to(F64)[bucket].permute(0, 3, 1, 2)
+    z = (x.to(F64) * scale + bias).masked_fill(~mask[:, None], -math.inf)
+    top = z.amax(-1, keepdim=True)
+    e = torch.exp(z - torch.where(top.isinf(), 0.0, top))
+    s = e.sum(-1, keepdim=True)
+    size = ((x.to(F64) * scale).abs() + bias.abs()).masked_fill(~mask[:, None], 0.0).amax(-1, keepdim=True)
+    return torch.where(s > 0, e / s, 0.0), size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", REL, ids=lambda s: "-".join(str(v) for v in s))
+def test_soft_max_rel(device, dtype, shape):
+    B, H, M, N, nb, dist, both, causal, _ = shape
+    x, table, lengths, starts, p = rel_inputs(device, TYPES[dtype], shape)
+    mask, rel = seen_ref(B, M, N, lengths, starts, causal, device)
+    want, size = rel_ref(x, table, mask, buckets_ref(rel, nb, dist, both), 0.25)
+    x.masked_fill_(~mask[:, None], math.nan)                     # what is masked is not looked at
+    got = stx.soft_max_rel(x, table, p, 0.25, lengths, starts)
+    per_lane = N / 64 if N <= 1024 else N / 256 + 16
+    close(got, want, want * (10 * size + 8 + 2 * (per_lane + 16)) * U, "y")
+    assert bool((got[~mask[:, None].expand_as(got)] == 0).all())
+    stx.soft_max_rel(x, table, p, 0.25, lengths, starts, out=x)
+    assert torch.equal(x, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", REL, ids=lambda s: "-".join(str(v) for v in s))
+def test_soft_max_rel_back(device, dtype, shape):
+    B, H, M, N, nb, dist, both, causal, _ = shape
+    x, table, lengths, starts, p = rel_inputs(device, TYPES[dtype], shape)
+    mask, rel = seen_ref(B, M, N, lengths, starts, causal, device)
+    bucket = buckets_ref(rel, nb, dist, both)
+    y = rel_ref(x, table, mask, bucket, 0.25)[0].to(x.dtype)
+    dy = randn(device, x.shape, 3, dtype=x.dtype)
+    g = y.to(F64) * (dy.to(F64) - (y.to(F64) * dy.to(F64)).sum(-1, keepdim=True))
+    dtable = torch.zeros(nb, H, dtype=F64, device=device)
+    size = torch.zeros_like(dtable)
+    for k in range(nb):
+        here = (bucket == k)[:, None]
+        dtable[k], size[k] = (torch.where(here, v, 0.0).sum((0, 2, 3)) for v in (g, g.abs()))
+    for t in (y, dy):
+        t.masked_fill_(~mask[:, None], math.nan)
+    dx, dt = stx.soft_max_rel_back(dy, y, p, 0.25, lengths, starts)
+    close(dx, g * 0.25, 2 * U * (g * 0.25).abs(), "dx")
+    close(dt, dtable, 2.0 ** -45 * size, "dtable")
+    again = stx.soft_max_rel_back(dy, y, p, 0.25, lengths, starts)
+    assert torch.equal(again[0], dx) and torch.equal(again[1], dt)
+    assert torch.equal(stx.soft_max_rel_back(dy, y, p, 0.25, lengths, starts, dtable=False)[0], dx)
+
+
+@pytest.mark.parametrize("nb,dist,both", [(32, 128, True), (32, 128, False), (256, 2048, True), (256, 2048, False), (8, 27, False), (4, 2, True), (2, 2, False),
+                                          (16, 81, False), (128, 33, True)])
+def test_rel_buckets(device, nb, dist, both):
+    """Every distance's bucket, borders that are whole numbers among them: a table that lets one bucket a head through."""
+    N = 2 * dist + 9
+    table = torch.full((nb, nb), -math.inf, device=device)
+    table.fill_diagonal_(0.0)
+    x = torch.zeros((1, nb, 1, N), device=device)
+    start = torch.tensor([N // 2], dtype=torch.int32, device=device)
+    y = stx.soft_max_rel(x, table, stx.rel_params(nb, dist, both), starts=start)
+    want = buckets_ref(torch.arange(N, device=device) - N // 2, nb, dist, both)
+    assert torch.equal(y[0, :, 0] > 0, want == torch.arange(nb, device=device)[:, None])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_rel_masks_at_their_limits(device, causal):
+    """Lengths of zero, below zero and past the keys; starts far before, past the keys and at the type's limits."""
+    lengths = torch.tensor([0, -5, 1, 40, 1000, 2 ** 31 - 1, -2 ** 31, 17], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, 3, -1, -9, 100, 2 ** 31 - 1, -2 ** 31, -2 ** 31], dtype=torch.int32, device=device)
+    B, H, M, N = 8, 2, 12, 40
+    x, table = randn(device, (B, H, M, N), 1), randn(device, (32, H), 2)
+    p = stx.rel_params(causal=causal)
+    mask, rel = seen_ref(B, M, N, lengths, starts, causal, device)
+    want, size = rel_ref(x, table, mask, buckets_ref(rel, 32, 128, True), 1.0)
+    got = stx.soft_max_rel(x, table, p, 1.0, lengths, starts)
+    close(got, want, want * (10 * size + 50) * U, "y")
+    dy = randn(device, x.shape, 3)
+    dx, dt = stx.soft_max_rel_back(dy, got, p, 1.0, lengths, starts)
+    assert bool((dx[~mask[:, None].expand_as(dx)] == 0).all()) and bool(dt.isfinite().all())
+
+
+def test_rel_infinite_scores(device):
+    """Scores of -infinity are keys left out; a row of them alone is zeros; the type's lowest value is a score as any."""
+    x = torch.zeros((1, 1, 4, 70), device=device)
+    x[0, 0, 0, 5:] = -math.inf
+    x[0, 0, 1] = -math.inf
+    x[0, 0, 2] = torch.finfo(torch.float32).min
+    x[0, 0, 3, 0] = math.nan
+    table = torch.zeros((32, 1), device=device)
+    y = stx.soft_max_rel(x, table, stx.rel_params(), 0.25)
+    assert torch.allclose(y[0, 0, 0, :5], torch.full((5,), 0.2, device=device)) and bool((y[0, 0, 0, 5:] == 0).all())
+    assert bool((y[0, 0, 1] == 0).all()) and torch.allclose(y[0, 0, 2], torch.full((70,), 1 / 70, device=device))
+    assert bool(y[0, 0, 3].isnan().all())
+
+
+def test_rel_strides_and_empty(device):
+    """Rows of a wider buffer at odd offsets, its other elements as they were; calls of no elements."""
+    B, H, M, N = 2, 3, 33, 45
+    p = stx.rel_params(16, 30)
+    table = randn(device, (16, H), 2)
+    for dt in TYPES.values():
+        wide = randn(device, (H, B, M, N + 5), 1, dtype=dt)
+        x = wide.transpose(0, 1)[..., 3:3 + N]
+        want = stx.soft_max_rel(x.contiguous(), table, p)
+        out = torch.full((B, H, M + 1, N + 3), 7.0, device=device, dtype=dt)
+        stx.soft_max_rel(x, table, p, out=out[:, :, 1:, 1:1 + N])
+        assert torch.equal(out[:, :, 1:, 1:1 + N], want)
+        out[:, :, 1:, 1:1 + N] = 7.0
+        assert bool((out == 7.0).all())
+        dwide = randn(device, (B, H, M, N + 1), 4, dtype=dt)
+        dx, dt_ = stx.soft_max_rel_back(dwide[..., 1:], want, p)
+        dx2, dt2 = stx.soft_max_rel_back(dwide[..., 1:].contiguous(), want, p)
+        assert torch.equal(dx, dx2) and torch.equal(dt_, dt2)
+    for shape in ((0, H, M, N), (B, H, 0, N), (B, H, M, 0)):
+        x = torch.empty(shape, device=device)
+        assert stx.soft_max_rel(x, table, p).shape == x.shape
+        dx, dt_ = stx.soft_max_rel_back(x, x, p)
+        assert dx.shape == x.shape and torch.equal(dt_, torch.zeros(16, H, device=device))
+
+
+def test_rel_gradient_against_differences(device):
+    B, H, M, N = 1, 2, 5, 9
+    x, table, dy = randn(device, (B, H, M, N), 1), randn(device, (8, H), 2), randn(device, (B, H, M, N), 3)
+    p = stx.rel_params(8, 6, True, True)
+    starts = torch.tensor([3], dtype=torch.int32, device=device)
+    mask, rel = seen_ref(B, M, N, None, starts, True, device)
+    bucket = buckets_ref(rel, 8, 6, True)
+    dx, dt = stx.soft_max_rel_back(dy, stx.soft_max_rel(x, table, p, 0.5, None, starts), p, 0.5, None, starts)
+    f = lambda x, w: float((rel_ref(x, w, mask, bucket, 0.5)[0] * dy.to(F64)).sum())  # noqa: E731
+    step = 1e-5
+    for t, got in ((x, dx), (table, dt)):
+        for i in range(0, t.numel(), 3):
+            d = torch.zeros_like(t, dtype=F64).view(-1)
+            d[i] = step
+            d, t64 = d.view_as(t), t.to(F64)
+            diff = (f(t64 + d, table) - f(t64 - d, table) if t is x else f(x, t64 + d) - f(x, t64 - d)) / (2 * step)
+            assert abs(float(got.reshape(-1)[i]) - diff) < 1e-5 * max(1.0, abs(diff))
