@@ -942,6 +942,26 @@ STX_API stx_status stx_soft_max_rel_back(const stx_tensor* dy, const stx_tensor*
                                          const int32_t* starts, const stx_tensor* dx, float* dtable, void* workspace,
                                          size_t workspace_bytes, stx_stream stream);
 
+/* Differential attention (Ye et al., "Differential Transformer", 2024): the difference of two softmax maps over the
+ * same values, so that what both attend to cancels. For head h of H, over the keys that a query sees,
+ *   dst_h = softmax(scale * q_2h k_2g^T) v_g - lambda_h * softmax(scale * q_2h+1 k_2g+1^T) v_g,  g = h / (H / kv heads).
+ * q [D, 2 H, queries, batch], k [D, 2 kv heads, keys, batch], v [V, kv heads, keys, batch], dst [V, H, queries, batch]; kv
+ * heads divide H, D is at most 128 and V at most 256. lambda: device float[H]. lengths: device int32[batch], keys of each
+ * sequence, taken as 0 .. keys (NULL: all); causal: query i of sequence b sees keys up to starts[b] + i (starts: device
+ * int32[batch], NULL: 0). A query that sees no key gets zeros. Keys from a sequence's length on are not looked at,
+ * whatever they hold; values of keys before it are finite, also where causality hides them. For the gradients, second (as dst, the second map's output, before
+ * lambda) and lse (device float [batch][H][2][queries], each map's ln sum exp of the scaled scores, -infinity for a query without
+ * keys) receive what stx_diff_attention_back takes; NULL otherwise. Scores, sums and products are float, the maps
+ * rounded to the type for their product with v (16-bit types). Rows are contiguous, other strides any; 16-byte aligned rows of k and v are
+ * faster. Outputs overlap nothing else and their strides nest. workspace: device, 256-byte aligned, no initialisation (0
+ * bytes where the call does not split the keys); calls that share one must not overlap. scale > 0. */
+STX_API size_t     stx_diff_attention_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
+                                                     stx_type type);
+STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v, stx_type type,
+                                      const float* lambda, float scale, int causal, const int32_t* lengths,
+                                      const int32_t* starts, const stx_tensor* dst, const stx_tensor* second, float* lse,
+                                      void* workspace, size_t workspace_bytes, stx_stream stream);
+
 /* ------------------------------------------------------------------------------------------
  * Versioned function table (after libstems V1, src/libstems_v1.h:146-189). Every entry point
  * above, in header order; a later revision of V1 may append entries (never reorder them), so
@@ -1187,6 +1207,13 @@ typedef struct stx_api_v1 {
                                     const int32_t* lengths, const int32_t* starts,
                                     const stx_tensor* dx, float* dtable, void* workspace,
                                     size_t workspace_bytes, stx_stream stream);
+    size_t (*diff_attention_workspace_size)(const stx_tensor* q, const stx_tensor* k,
+                                            const stx_tensor* v, stx_type type);
+    stx_status (*diff_attention)(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
+                                 stx_type type, const float* lambda, float scale, int causal,
+                                 const int32_t* lengths, const int32_t* starts,
+                                 const stx_tensor* dst, const stx_tensor* second, float* lse,
+                                 void* workspace, size_t workspace_bytes, stx_stream stream);
     void (*reserved[16])(void);
 } stx_api_v1;
 

@@ -110,6 +110,8 @@ const stx_api_v1 kApiV1 = {
     &stx_soft_max_rel,
     &stx_soft_max_rel_back_workspace_size,
     &stx_soft_max_rel_back,
+    &stx_diff_attention_workspace_size,
+    &stx_diff_attention,
     {},
 };
 }  // namespace

@@ -139,6 +139,8 @@ _SIGNATURES = {
     "stx_soft_max_rel": (_i, [_vp, _i, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "stx_soft_max_rel_back_workspace_size": (ctypes.c_size_t, [_vp, _i, _i]),
     "stx_soft_max_rel_back": (_i, [_vp, _vp, _i, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "stx_diff_attention_workspace_size": (ctypes.c_size_t, [_vp, _vp, _vp, _i]),
+    "stx_diff_attention": (_i, [_vp, _vp, _vp, _i, _vp, ctypes.c_float, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
 }
 
 
@@ -1491,3 +1493,40 @@ def soft_max_rel_back(dy, y, params, scale=1.0, lengths=None, starts=None, dx=No
             _per_sequence(lengths, y, B, "lengths"), _per_sequence(starts, y, B, "starts"), _typed(dx, y, "dx"),
             _floats(dtable, y, params.n_buckets * H, "dtable"), ws, nbytes)
     return dx, dtable
+
+
+def _heads(q, k, v):
+    """(batch, queries, heads, head size of v) of differential attention's operands."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or q.shape[2] % 2:
+        raise ValueError("q must be (batch, queries, 2 heads, D), k (batch, keys, 2 kv heads, D), v (batch, keys, kv heads, V)")
+    return q.shape[0], q.shape[1], q.shape[2] // 2, v.shape[3]
+
+
+def diff_attention(q, k, v, lam, scale=None, causal=False, lengths=None, starts=None, keep=False, out=None, second=None, lse=None,
+                   workspace=None, stream=None):
+    """softmax(scale q1 k1') v - lam softmax(scale q2 k2') v: q (batch, queries, 2 heads, D) with a head's two maps side by
+    side, k (batch, keys, 2 kv heads, D), v (batch, keys, kv heads, V), lam float32 device (heads,); scale defaults to
+    1 / sqrt(D). lengths: int32 device (batch,), keys of each sequence (None: all); causal: query i sees keys up to
+    starts[b] + i, starts int32 device (batch,) (None: 0). Returns (out, second, lse): out (batch, queries, heads, V), and
+    with keep=True what diff_attention_back takes, the second map's output and both maps' ln sum exp, float32 (batch, heads,
+    2, queries) (None otherwise)."""
+    import torch
+    B, M, H, V = _heads(q, k, v)
+    out = _empty((B, M, H, V), q, stream) if out is None else out
+    if keep:
+        second = _empty((B, M, H, V), q, stream) if second is None else second
+        lse = _empty((B, H, 2, M), q, stream, torch.float32) if lse is None else lse
+    L, t = lib(), _type(q)
+    a, b, c = _typed(q, q, "q"), _typed(k, q, "k"), _typed(v, q, "v")
+    need = L.stx_diff_attention_workspace_size(a, b, c, t)
+    ws, nbytes = None, 0
+    if need:
+        ws, nbytes, owner = _scratch(need, workspace, q, stream)
+    _launch(L.stx_diff_attention, q, stream, a, b, c, t, _floats(lam, q, H, "lam"), _scale(scale, q), bool(causal),
+            _per_sequence(lengths, q, B, "lengths"), _per_sequence(starts, q, B, "starts"), _typed(out, q, "out"),
+            None if second is None else _typed(second, q, "second"), _floats(lse, q, B * H * 2 * M, "lse"), ws, nbytes)
+    return out, second, lse
+
+
+def _scale(scale, q):
+    return float(max(1, q.shape[-1]) ** -0.5 if scale is None else scale)

@@ -13,13 +13,16 @@ result's type relative to the value, plus half the smallest subnormal step of fp
           each exponential, Z the row's largest |scale x| + |bias|, as much of their sum, 2 u of the hardware's 2^y each,
           and of the sum a rounding for each of a lane's terms and 16 of the tree. Backward: products and sums are in
           double, so one rounding to float and one to the type; the table's sums one.
+  diff    a score is a sum of D float products, off by at most (D + 8) u Z with Z = scale sum |q k|, and so, relative to
+          itself, is each exponential, as is their sum: 2 (D + 8) u Z; P is rounded to the type (h) and multiplied by v
+          in float, a random walk of 4 sqrt(N) u; in all, of A = sum P |v|, for each map. Backward: see the test.
 """
 import math
 
 import pytest
 
 import stx
-from test_gpu_layer_ops import F64, TYPES, U, YARN, close, randn, rope_ref
+from test_gpu_layer_ops import F64, TYPES, U, YARN, close, half_step, norm_close, randn, rope_ref
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -383,3 +386,151 @@ def test_rel_gradient_against_differences(device):
             d, t64 = d.view_as(t), t.to(F64)
             diff = (f(t64 + d, table) - f(t64 - d, table) if t is x else f(x, t64 + d) - f(x, t64 - d)) / (2 * step)
             assert abs(float(got.reshape(-1)[i]) - diff) < 1e-5 * max(1.0, abs(diff))
+
+
+# ------------------------------------------------------------------------ differential attention
+DIFF = [
+    # B, M, N, H, Hk, D, V, causal, masks
+    (1, 1, 1, 1, 1, 64, 128, False, None),
+    (2, 1, 300, 8, 2, 64, 128, True, "ragged"),               # single tokens: waves and blocks split the keys
+    (3, 1, 5000, 4, 4, 64, 128, True, "ragged"),
+    (2, 3, 700, 8, 2, 128, 256, True, "ragged"),
+    (1, 16, 1000, 1, 1, 128, 128, False, None),
+    (2, 4, 400, 4, 1, 32, 64, False, "ragged"),
+    (1, 2, 130, 2, 1, 64, 64, True, None),
+    (2, 60, 60, 4, 4, 64, 128, False, None),
+    (1, 801, 801, 4, 4, 64, 128, False, "ragged"),
+    (2, 131, 260, 8, 2, 64, 128, True, "ragged"),
+    (1, 200, 200, 4, 2, 64, 64, True, None),
+    (1, 129, 333, 4, 2, 128, 256, True, "ragged"),
+    (1, 70, 190, 2, 2, 96, 96, False, None),                   # rows padded in LDS
+    (1, 150, 150, 6, 2, 40, 80, True, None),
+    (2, 90, 77, 3, 3, 32, 32, True, None),                     # more queries than keys
+    (1, 65, 100, 2, 1, 33, 47, True, "ragged"),                # rows that are not whole chunks
+    (1, 9, 50, 2, 1, 1, 1, False, None),
+]
+
+
+def diff_inputs(device, dt, shape, pad=None):
+    B, M, N, H, Hk, D, V, causal, masks = shape
+    q, k, v = (randn(device, s, 1 + i, dtype=dt) for i, s in enumerate(((B, M, 2 * H, D), (B, N, 2 * Hk, D), (B, N, Hk, V))))
+    lam = randn(device, (H,), 4, 0.2, 0.5)
+    lengths = starts = None
+    if masks:
+        lengths = torch.tensor([max(1, N - 7 * b - N // 3 * (b % 2)) for b in range(B)], device=device, dtype=torch.int32)
+    if causal:
+        starts = torch.tensor([max(0, (N if lengths is None else int(lengths[b])) - M) for b in range(B)], device=device, dtype=torch.int32)
+    return q, k, v, lam, lengths, starts
+
+
+def diff_maps(q, k, v, mask, scale):
+    """Both maps P (2, B, H, M, N), ln sum exp (B, H, 2, M), Z and the operands repeated for each head, in 64 bits."""
+    B, M, H2, D = q.shape
+    H, Hk = H2 // 2, v.shape[2]
+    q = q.to(F64).view(B, M, H, 2, D).permute(3, 0, 2, 1, 4).contiguous()
+    k = k.to(F64).view(B, -1, Hk, 2, D).permute(3, 0, 2, 1, 4).repeat_interleave(H // Hk, 2).contiguous()
+    v = v.to(F64).permute(0, 2, 1, 3).repeat_interleave(H // Hk, 1).contiguous()
+    kt = k.transpose(3, 4).contiguous()
+    z = (torch.matmul(q, kt) * scale).masked_fill(~mask[:, None], -math.inf)
+    size = (torch.matmul(q.abs(), kt.abs()) * scale).masked_fill(~mask[:, None], 0.0).amax(-1, keepdim=True)
+    top = z.amax(-1, keepdim=True)
+    top = torch.where(top.isinf(), 0.0, top)
+    e = torch.exp(z - top)
+    s = e.sum(-1, keepdim=True)
+    lse = (top + torch.log(s)).squeeze(-1).permute(1, 2, 0, 3)
+    return torch.where(s > 0, e / s, 0.0), lse, size, q, k, v
+
+
+def spoil(k, v, lengths):
+    """Keys from a sequence's length on hold NaN."""
+    if lengths is not None:
+        for b, n in enumerate(lengths.tolist()):
+            k[b, n:] = math.nan
+            v[b, n:] = math.nan
+
+
+def check_diff(got, q, k, v, lam, mask, scale, what, norms=True):
+    out, second, lse = got
+    p, want_lse, size, _, _, v64 = diff_maps(q, k, v, mask, scale)
+    D, N = q.shape[3], k.shape[1]
+    o = [torch.matmul(m, v64) for m in p]
+    h = half_step(q.dtype) if q.dtype != torch.float32 else 0.0
+    off = [(2 * (D + 8) * U * size[m] + h + (8 + 4 * math.sqrt(N)) * U) * torch.matmul(p[m], v64.abs()) for m in range(2)]
+    lam = lam.to(F64)[:, None, None]
+    want = (o[0] - lam * o[1]).transpose(1, 2)
+    close(out, want, (off[0] + lam.abs() * off[1]).transpose(1, 2), what + " out")
+    if norms and N >= 64:
+        norm_close(out, want, 2, what + " out")
+    if second is not None:
+        close(second, o[1].transpose(1, 2), off[1].transpose(1, 2), what + " second")
+        seen = want_lse > -math.inf
+        assert bool((lse[~seen] == -math.inf).all())
+        bound = ((D + 8) * U * size.squeeze(-1).permute(1, 2, 0, 3) + (16 + math.sqrt(N)) * U) + 4 * U * want_lse.abs()
+        assert bool(((lse.to(F64) - want_lse).abs() <= bound)[seen].all()), what + " lse"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", DIFF, ids=lambda s: "-".join(str(v) for v in s))
+def test_diff_attention(device, dtype, shape):
+    B, M, N, H, Hk, D, V, causal, _ = shape
+    q, k, v, lam, lengths, starts = diff_inputs(device, TYPES[dtype], shape)
+    mask, _ = seen_ref(B, M, N, lengths, starts, causal, device)
+    kept, v_kept = k.clone(), v.clone()
+    spoil(k, v, lengths)
+    got = stx.diff_attention(q, k, v, lam, causal=causal, lengths=lengths, starts=starts, keep=True)
+    check_diff(got, q, kept, v_kept, lam, mask, D ** -0.5, "diff")
+    alone = stx.diff_attention(q, k, v, lam, causal=causal, lengths=lengths, starts=starts)
+    assert torch.equal(alone[0], got[0]) and alone[1] is None and alone[2] is None
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 20, 70])
+@pytest.mark.parametrize("causal", [False, True])
+def test_diff_masks_at_their_limits(device, dtype, M, causal):
+    """Rows that see no key; lengths and starts at and past their limits."""
+    lengths = torch.tensor([0, -5, 1, 40, 1000, 2 ** 31 - 1, -2 ** 31, 17], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, 3, -1, -9, 100, 2 ** 31 - 1, -2 ** 31, -2 ** 31], dtype=torch.int32, device=device)
+    B, N, H, Hk, D, V = 8, 90, 4, 2, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    mask, _ = seen_ref(B, M, N, lengths, starts, causal, device)
+    got = stx.diff_attention(q, k, v, lam, causal=causal, lengths=lengths, starts=starts, keep=True)
+    check_diff(got, q, k, v, lam, mask, D ** -0.5, "limits", norms=False)
+    nothing = ~mask.any(-1)
+    for t in got[:2]:
+        assert bool((t[nothing] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_diff_strides_and_neighbours(device, dtype):
+    """q, k and v as slices of projections, at unaligned offsets too, a cache longer than its keys, outputs into wider
+    buffers whose other elements stay."""
+    B, M, N, H, Hk, D, V = 2, 37, 90, 4, 2, 64, 128
+    dt = TYPES[dtype]
+    for shift in (0, 3):
+        wide = randn(device, (B, M, 2 * H * D + 13), 1, dtype=dt)
+        q = wide[..., shift:shift + 2 * H * D].unflatten(-1, (2 * H, D))
+        cache = randn(device, (B, N + 30, Hk, 2 * D + V + 16), 2, dtype=dt)
+        k = cache[:, 5:5 + N, :, shift:shift + 2 * D]
+        k = k.reshape(B, N, 2 * Hk, D)
+        v = cache[:, 5:5 + N, :, 2 * D + shift:2 * D + shift + V]
+        lam = randn(device, (H,), 4, 0.2, 0.5)
+        mask, _ = seen_ref(B, M, N, None, None, False, device)
+        want = stx.diff_attention(q.contiguous(), k.contiguous(), v.contiguous(), lam, keep=True)
+        buffers = [torch.full((B, M + 2, H, V + 5), 7.0, device=device, dtype=dt) for _ in range(2)]
+        out, second = (t[:, 1:M + 1, :, shift:shift + V] for t in buffers)
+        got = stx.diff_attention(q, k, v, lam, keep=True, out=out, second=second)
+        if shift == 0:
+            assert torch.equal(out, want[0]) and torch.equal(second, want[1]) and torch.equal(got[2], want[2])
+        check_diff(got, q, k, v, lam, mask, D ** -0.5, "strides")
+        for t, s in zip(buffers, (out, second)):
+            s.fill_(7.0)
+            assert bool((t == 7.0).all())
+
+
+def test_diff_empty(device):
+    lam = torch.ones(2, device=device)
+    make = lambda B, M, N: (torch.empty(B, M, 4, 8, device=device), torch.empty(B, N, 2, 8, device=device), torch.empty(B, N, 1, 8, device=device))  # noqa: E731
+    for B, M, N in ((0, 3, 3), (2, 0, 3)):
+        assert stx.diff_attention(*make(B, M, N), lam, keep=True)[0].shape == (B, M, 2, 8)
+    out, second, lse = stx.diff_attention(*make(2, 3, 0), lam, keep=True)
+    assert bool((out == 0).all()) and bool((second == 0).all()) and bool((lse == -math.inf).all())
