@@ -961,6 +961,20 @@ STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, 
                                       const float* lambda, float scale, int causal, const int32_t* lengths,
                                       const int32_t* starts, const stx_tensor* dst, const stx_tensor* second, float* lse,
                                       void* workspace, size_t workspace_bytes, stx_stream stream);
+/* Its gradients, from dy (of dst), the forward call's inputs and masks and what it kept: out (its dst), second and lse. dq
+ * (of q), dk and dv (of k and v, together or neither; summed over the heads that share a key head; zeros for keys from a
+ * sequence's length on), dlambda (device float[H]); any may be NULL. Scores are formed again; sums are float
+ * (dlambda's over rows double), the maps' gradients rounded to the type for their products (16-bit types; fp16's scaled by
+ * powers of two, so that they keep its range). dlambda comes from the maps themselves, not from the rounded second. The
+ * same rules for masked keys, strides and workspace; outputs overlap nothing else. */
+STX_API size_t     stx_diff_attention_back_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
+                                                          stx_type type);
+STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tensor* q, const stx_tensor* k,
+                                           const stx_tensor* v, stx_type type, const float* lambda, float scale,
+                                           int causal, const int32_t* lengths, const int32_t* starts,
+                                           const stx_tensor* out, const stx_tensor* second, const float* lse,
+                                           const stx_tensor* dq, const stx_tensor* dk, const stx_tensor* dv,
+                                           float* dlambda, void* workspace, size_t workspace_bytes, stx_stream stream);
 
 /* ------------------------------------------------------------------------------------------
  * Versioned function table (after libstems V1, src/libstems_v1.h:146-189). Every entry point
@@ -1214,6 +1228,16 @@ typedef struct stx_api_v1 {
                                  const int32_t* lengths, const int32_t* starts,
                                  const stx_tensor* dst, const stx_tensor* second, float* lse,
                                  void* workspace, size_t workspace_bytes, stx_stream stream);
+    size_t (*diff_attention_back_workspace_size)(const stx_tensor* q, const stx_tensor* k,
+                                                 const stx_tensor* v, stx_type type);
+    stx_status (*diff_attention_back)(const stx_tensor* dy, const stx_tensor* q,
+                                      const stx_tensor* k, const stx_tensor* v, stx_type type,
+                                      const float* lambda, float scale, int causal,
+                                      const int32_t* lengths, const int32_t* starts,
+                                      const stx_tensor* out, const stx_tensor* second,
+                                      const float* lse, const stx_tensor* dq,
+                                      const stx_tensor* dk, const stx_tensor* dv, float* dlambda,
+                                      void* workspace, size_t workspace_bytes, stx_stream stream);
     void (*reserved[16])(void);
 } stx_api_v1;
 

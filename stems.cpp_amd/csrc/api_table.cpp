@@ -112,6 +112,8 @@ const stx_api_v1 kApiV1 = {
     &stx_soft_max_rel_back,
     &stx_diff_attention_workspace_size,
     &stx_diff_attention,
+    &stx_diff_attention_back_workspace_size,
+    &stx_diff_attention_back,
     {},
 };
 }  // namespace

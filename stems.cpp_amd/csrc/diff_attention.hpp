@@ -200,7 +200,7 @@ inline DiffShape diff_shape(const stx_tensor* q, const stx_tensor* k, const stx_
     STX_REQUIRE(q->ne[0] > 0 && v->ne[0] > 0, "%s: rows of no elements", op);
     if (q->ne[0] > kDiffDim || v->ne[0] > kDiffValue)
         fail(STX_STATUS_UNSUPPORTED, "%s: heads of %lld and %lld elements (%d and %d at most)", op, (long long)q->ne[0], (long long)v->ne[0], kDiffDim, kDiffValue);
-    STX_REQUIRE(Hk > 0 ? H % Hk == 0 : H == 0, "%s: %lld heads do not share %lld key heads evenly", op, H, Hk);
+    STX_REQUIRE(Hk > 0 ? H > 0 && H % Hk == 0 : H == 0, "%s: %lld heads do not share %lld key heads evenly", op, H, Hk);
     STX_REQUIRE(q->ne[2] < (1LL << 28) && k->ne[2] < (1LL << 28) && q->ne[3] < (1LL << 20) && H < (1 << 16), "%s: more than 2^28 queries or keys, 2^20 sequences or 2^16 heads", op);
     STX_REQUIRE(Hk == 0 || q->ne[2] * (H / Hk) < (1LL << 30), "%s: more than 2^30 queries to a key head", op);
     return {q->ne[3], q->ne[2], k->ne[2], (int)H, (int)Hk, (int)q->ne[0], (int)v->ne[0]};

@@ -1,0 +1,596 @@
+// diff_attention_back.hip — the gradients of differential attention (stx_diff_attention_back).
+#include "diff_attention.hpp"
+
+namespace stx {
+namespace {
+
+// With P_m = exp(z_m - lse_m), O_m = P_m v and dP = dy v^T, D_m = rowsum(dy O_m):
+//   dS_1 = P_1 (dP - D_1),  dS_2 = -lambda P_2 (dP - D_2),  dq_m = s dS_m k_m,  dk_m = s dS_m^T q_m,
+//   dv = (P_1 - lambda P_2)^T dy,  dlambda = -sum P_2 dP.
+// Two kernels form the scores again, 14 D products where one that adds to dq from every block of keys would have 10 D, and need no
+// atomics: results are the same each time. The first has rows in registers and goes over the keys (dq, dlambda,
+// and D, from dy and the kept outputs, for the second); the second has keys in registers and goes over the rows of
+// its key head, so that gradients of shared heads add up in the accumulators. As in the forward kernel the accumulators of
+// one product are, where they stand, the operand of the next, whose other operand is read transposed from the tile.
+//
+// dS and P are rounded to 16 bits for their products (16-bit data). fp16's range would cut them: P is
+// scaled by 2^8, and dP - D by a power of two of the row (first kernel) or the call (second) that keeps
+// 2^8 P (dP - D) max(1, |lambda|) below 2^15, from |dP - D| <= 2 V max|v| max|dy|.
+template <class T>
+constexpr float kShift = std::is_same_v<T, f16> ? 8.f : 0.f;
+
+__device__ __forceinline__ float range_scale(const DiffArgs& a, float dy, float lam) {
+    const float bound = 2.f * a.vdim * __uint_as_float(a.most[0]) * dy * fmaxf(1.f, fabsf(lam));
+    if (!(bound > 0.f && bound < 0x1p120f)) return 1.f;
+    return __builtin_amdgcn_exp2f(fminf(fmaxf(7.f - ceilf(__builtin_amdgcn_logf(bound)), -100.f), 100.f));
+}
+
+template <class T, int DP, int VP, int NQ, bool ALIGNED>
+__global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
+    constexpr int NT = 256, KG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, ROWS = 64 * NQ;
+    constexpr int FIT = 32768 / ((2 * DP + VP) * (int)sizeof(T)), BK = FIT >= 64 ? 64 : FIT >= 32 ? 32 : 16;
+    using KL = Loader<T, DP, BK, 2, NT, ALIGNED>;
+    using VL = Loader<T, VP, BK, 1, NT, ALIGNED>;
+    constexpr int STAGE = KL::BYTES + VL::BYTES;
+    __shared__ __align__(128) char lds[2 * STAGE];
+
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, s = lane % 16;
+    const unsigned per = a.tile_div.div(blockIdx.x);
+    int tile = (int)(blockIdx.x - per * a.tile_div.d);
+    if (a.causal) tile = a.tiles - 1 - tile;                          // the longest first
+    const int b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
+    const Mask mask(a, b);
+    const int r0 = tile * ROWS, last = min(r0 + ROWS, a.rows) - 1;
+    const int end = mask.limit((int)a.group_div.div((unsigned)last)), least = mask.limit((int)a.group_div.div((unsigned)r0));
+    const char* kb = a.k.p + 2LL * kvh * a.k.s1 + b * a.k.s3;
+    const char* vb = a.v.p + (long long)kvh * a.v.s1 + b * a.v.s3;
+    KL kl;
+    VL vl;
+    auto fetch = [&](int key0, int stage) {
+        kl.fetch(lds + stage * STAGE, a.dim, [&](int map, int r) { return key0 + r < mask.length ? kb + map * a.k.s1 + (key0 + r) * a.k.s2 : nullptr; });
+        vl.fetch(lds + stage * STAGE + KL::BYTES, a.vdim, [&](int, int r) { return key0 + r < mask.length ? vb + (key0 + r) * a.v.s2 : nullptr; });
+    };
+    if (end > 0) fetch(0, 0);
+
+    u32x4 qf[2][NQ][GD], yf[NQ][GV];
+    int limit[NQ];
+    float base[2][NQ], dot[2][NQ], lam[NQ], unit[NQ], share[NQ];      // lse in units of log2; D; of the row
+    const float c = a.scale * kLog2e;
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int r = r0 + (wave * NQ + n) * 16 + s;
+        const RowAt row(a, kvh, min(r, a.rows - 1));
+        limit[n] = mask.limit(row.query);
+        lam[n] = a.lam[row.head];
+        unit[n] = 1.f, share[n] = 0.f;
+#pragma unroll
+        for (int m = 0; m < 2; m++) load_fragments<T, DP>(qf[m][n], row.at(a.q, b, 2, m), a.dim, lane);
+        load_fragments<T, VP>(yf[n], row.at(a.dy, b, 1, 0), a.vdim, lane);
+        const char *out = row.at(a.out, b, 1, 0), *second = row.at(a.second, b, 1, 0);
+        float d1 = 0.f, d2 = 0.f, most = 0.f;
+#pragma unroll
+        for (int g = 0; g < GV; g++) {
+            constexpr int E = 16 / sizeof(T);
+            const int at = g * 4 + lane / 16;
+            float y[E], o[E], o2[E];
+            unpack<T>(yf[n][g], y);
+            unpack<T>(load_chunk<T>(out + at * 16, a.vdim - at * E), o);
+            unpack<T>(load_chunk<T>(second + at * 16, a.vdim - at * E), o2);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                d1 = fmaf(y[e], fmaf(lam[n], o2[e], o[e]), d1);
+                d2 = fmaf(y[e], o2[e], d2);
+                most = fmaxf(most, fabsf(y[e]));
+            }
+        }
+        dot[0][n] = column_sum(d1), dot[1][n] = column_sum(d2);
+        most = column_max(most);
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const long long at = row.stat(a, b, m);
+            base[m][n] = fmaf(a.lse[at], kLog2e, -kShift<T>);
+            if (lane < 16 && r < a.rows) a.dots[at] = dot[m][n];
+        }
+        if constexpr (std::is_same_v<T, f16>) {
+            unit[n] = range_scale(a, most, lam[n]);
+            dot[0][n] *= unit[n], dot[1][n] *= unit[n];
+        }
+    }
+    f32x4 acc[2][NQ][ND] = {};
+    constexpr int KS = KG;
+    int stage = 0;
+    for (int key0 = 0; key0 < end; key0 += BK) {
+        kl.settle(lds + stage * STAGE);
+        vl.settle(lds + stage * STAGE + KL::BYTES);
+        arrived<ALIGNED>();
+        if (key0 + BK < end) fetch(key0 + BK, stage ^ 1);
+        const char *ks = lds + stage * STAGE, *vs = ks + KL::BYTES;
+        const bool whole = key0 + BK <= least;
+#pragma unroll
+        for (int k0 = 0; k0 < BK; k0 += KS) {
+            f32x4 z[2][NQ][KS / 16], dp[NQ][KS / 16];
+#pragma unroll
+            for (int t = 0; t < KS / 16; t++) {
+#pragma unroll
+                for (int n = 0; n < NQ; n++) z[0][n][t] = z[1][n][t] = dp[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int g = 0; g < GD; g++) {
+                        const u32x4 kf = Tile<T, DP>::plain(ks + m * BK * Tile<T, DP>::BYTES, k0 + t * 16, g, lane);
+#pragma unroll
+                        for (int n = 0; n < NQ; n++) z[m][n][t] = mma(kf, qf[m][n][g], z[m][n][t], T{});
+                    }
+#pragma unroll
+                for (int g = 0; g < GV; g++) {
+                    const u32x4 vf = Tile<T, VP>::plain(vs, k0 + t * 16, g, lane);
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) dp[n][t] = mma(vf, yf[n][g], dp[n][t], T{});
+                }
+            }
+            u32x4 ds[2][NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                const int left = whole ? KS : limit[n] - (key0 + k0 + lane / 16 * 4);
+#pragma unroll
+                for (int t = 0; t < KS / 16; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float p1 = __builtin_amdgcn_exp2f(fmaf(z[0][n][t][e], c, -base[0][n])), p2 = __builtin_amdgcn_exp2f(fmaf(z[1][n][t][e], c, -base[1][n]));
+                        if (!whole) {
+                            p1 = t * 16 + e < left ? p1 : 0.f;
+                            p2 = t * 16 + e < left ? p2 : 0.f;
+                        }
+                        const float d = dp[n][t][e];
+                        share[n] = fmaf(p2, d, share[n]);
+                        z[0][n][t][e] = p1 * fmaf(d, unit[n], -dot[0][n]);
+                        z[1][n][t][e] = p2 * -lam[n] * fmaf(d, unit[n], -dot[1][n]);
+                    }
+#pragma unroll
+                for (int m = 0; m < 2; m++) ds[m][n] = chunk_of<T>(z[m][n]);
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int i = 0; i < ND; i++) {
+                    const u32x4 kf = Tile<T, DP>::columns(ks + m * BK * Tile<T, DP>::BYTES, k0, i, lane);
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) acc[m][n][i] = mma(kf, ds[m][n], acc[m][n][i], T{});
+                }
+        }
+        stage ^= 1;
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int r = r0 + (wave * NQ + n) * 16 + s;
+        const float sum = column_sum(share[n]);
+        if (r >= a.rows) continue;
+        const RowAt row(a, kvh, r);
+        if (lane < 16) a.rows_lam[((long long)b * a.heads + row.head) * a.queries + row.query] = sum * __builtin_amdgcn_exp2f(-kShift<T>);
+        if (!a.dq.p) continue;
+        const float f = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / unit[n];
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            char* out = const_cast<char*>(row.at(a.dq, b, 2, m));
+#pragma unroll
+            for (int i = 0; i < ND; i++) {
+                const int at = i * 16 + lane / 16 * 4;
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = acc[m][n][i][e] * f;
+                store4<T>(out + at * sizeof(T), a.dim - at, o);
+            }
+        }
+    }
+}
+
+// Rows of a tile, and what the kernel takes of each: both maps' lse, D, -lambda, and the keys that it sees.
+constexpr int kRows = 32;
+struct RowStats {
+    float base[2][kRows], dot[2][kRows], lam[kRows];
+    int limit[kRows];
+};
+
+template <class T, int DP, int VP, int NK, bool ALIGNED>
+__global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
+    constexpr int NT = 256, RG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, NV = VP / 16, KEYS = 64 * NK;
+    using QL = Loader<T, DP, kRows, 2, NT, ALIGNED>;
+    using YL = Loader<T, VP, kRows, 1, NT, ALIGNED>;
+    constexpr int STAGE = QL::BYTES + YL::BYTES;
+    __shared__ __align__(128) char lds[2 * STAGE];
+    __shared__ RowStats stats[2];
+
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, s = lane % 16;
+    const unsigned per = a.tile_div.div(blockIdx.x);
+    const int index = (int)(blockIdx.x - per * a.tile_div.d), tile = index / a.splits, part = index - tile * a.splits;
+    const int b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
+    const Mask mask(a, b);
+    const int key0 = tile * KEYS, key_end = min(key0 + KEYS, a.keys);
+    // Rows from the first that sees a key of the tile on, in parts of whole tiles.
+    const int first = key0 >= mask.length ? a.rows : !a.causal ? 0 : (int)min((long long)a.rows, max(0LL, key0 - mask.start) * a.group);
+    const int each = ((a.rows - first + kRows - 1) / kRows + a.splits - 1) / a.splits * kRows;
+    const int begin = (int)min((long long)first + (long long)part * each, (long long)a.rows), end = (int)min((long long)begin + each, (long long)a.rows);
+    QL ql;
+    YL yl;
+    float held[6];                       // a row's stats on their way
+    float unit = 1.f;
+    if constexpr (std::is_same_v<T, f16>) {
+        float lam = 0.f;
+        for (int g = 0; g < a.group; g++) lam = fmaxf(lam, fabsf(a.lam[kvh * a.group + g]));
+        unit = range_scale(a, __uint_as_float(a.most[1]), lam);
+    }
+    auto fetch = [&](int r0, int stage) {
+        ql.fetch(lds + stage * STAGE, a.dim, [&](int map, int r) -> const char* { return r0 + r < end ? RowAt(a, kvh, r0 + r).at(a.q, b, 2, map) : nullptr; });
+        yl.fetch(lds + stage * STAGE + QL::BYTES, a.vdim, [&](int, int r) -> const char* { return r0 + r < end ? RowAt(a, kvh, r0 + r).at(a.dy, b, 1, 0) : nullptr; });
+        if (tid < kRows) {
+            const RowAt row(a, kvh, min(r0 + tid, a.rows - 1));
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const long long at = row.stat(a, b, m);
+                held[m] = fmaf(a.lse[at], kLog2e, -kShift<T>);
+                held[2 + m] = a.dots[at] * unit;
+            }
+            held[4] = -a.lam[row.head];
+            held[5] = __int_as_float(r0 + tid < end ? mask.limit(row.query) : 0);
+        }
+    };
+    auto settle = [&](int stage) {
+        ql.settle(lds + stage * STAGE);
+        yl.settle(lds + stage * STAGE + QL::BYTES);
+        if (tid < kRows) {
+            RowStats& st = stats[stage];
+            st.base[0][tid] = held[0], st.base[1][tid] = held[1], st.dot[0][tid] = held[2], st.dot[1][tid] = held[3];
+            st.lam[tid] = held[4];
+            st.limit[tid] = __float_as_int(held[5]);
+        }
+        arrived<ALIGNED>();
+    };
+    if (begin < end) fetch(begin, 0);
+
+    u32x4 kf[2][NK][GD], vf[NK][GV];
+#pragma unroll
+    for (int n = 0; n < NK; n++) {
+        const int key = key0 + (wave * NK + n) * 16 + s;
+        const bool in = key < mask.length;
+#pragma unroll
+        for (int m = 0; m < 2; m++) load_fragments<T, DP>(kf[m][n], in ? a.k.p + (2LL * kvh + m) * a.k.s1 + key * a.k.s2 + b * a.k.s3 : nullptr, a.dim, lane);
+        load_fragments<T, VP>(vf[n], in ? a.v.p + (long long)kvh * a.v.s1 + key * a.v.s2 + b * a.v.s3 : nullptr, a.vdim, lane);
+    }
+    f32x4 dk[2][NK][ND] = {}, dv[NK][NV] = {};
+    const float c = a.scale * kLog2e;
+    int stage = 0;
+    for (int r0 = begin; r0 < end; r0 += kRows) {
+        settle(stage);
+        if (r0 + kRows < end) fetch(r0 + kRows, stage ^ 1);
+        const char *qs = lds + stage * STAGE, *ys = qs + QL::BYTES;
+        const RowStats& st = stats[stage];
+        // limits never fall, and rows past the end see nothing
+        const bool whole = r0 + kRows <= end && __builtin_amdgcn_readfirstlane(st.limit[0]) >= key_end && key0 + KEYS <= a.keys;
+#pragma unroll
+        for (int k0 = 0; k0 < kRows; k0 += RG) {
+            f32x4 z[2][NK][RG / 16], dp[NK][RG / 16];
+#pragma unroll
+            for (int t = 0; t < RG / 16; t++) {
+#pragma unroll
+                for (int n = 0; n < NK; n++) z[0][n][t] = z[1][n][t] = dp[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int g = 0; g < GD; g++) {
+                        const u32x4 qf = Tile<T, DP>::plain(qs + m * kRows * Tile<T, DP>::BYTES, k0 + t * 16, g, lane);
+#pragma unroll
+                        for (int n = 0; n < NK; n++) z[m][n][t] = mma(qf, kf[m][n][g], z[m][n][t], T{});
+                    }
+#pragma unroll
+                for (int g = 0; g < GV; g++) {
+                    const u32x4 yf = Tile<T, VP>::plain(ys, k0 + t * 16, g, lane);
+#pragma unroll
+                    for (int n = 0; n < NK; n++) dp[n][t] = mma(yf, vf[n][g], dp[n][t], T{});
+                }
+            }
+            u32x4 mix[NK], ds[2][NK];
+            f32x4 pm[NK][RG / 16];
+#pragma unroll
+            for (int t = 0; t < RG / 16; t++) {
+                const int at = k0 + t * 16 + lane / 16 * 4;
+                const f32x4 base1 = *reinterpret_cast<const f32x4*>(&st.base[0][at]), base2 = *reinterpret_cast<const f32x4*>(&st.base[1][at]);
+                const f32x4 dot1 = *reinterpret_cast<const f32x4*>(&st.dot[0][at]), dot2 = *reinterpret_cast<const f32x4*>(&st.dot[1][at]);
+                const f32x4 lam = *reinterpret_cast<const f32x4*>(&st.lam[at]);
+#pragma unroll
+                for (int n = 0; n < NK; n++) {
+                    const int key = key0 + (wave * NK + n) * 16 + s;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float p1 = __builtin_amdgcn_exp2f(fmaf(z[0][n][t][e], c, -base1[e])), p2 = lam[e] * __builtin_amdgcn_exp2f(fmaf(z[1][n][t][e], c, -base2[e]));
+                        if (!whole) {
+                            const bool in = key < st.limit[at + e];
+                            p1 = in ? p1 : 0.f;
+                            p2 = in ? p2 : 0.f;
+                        }
+                        pm[n][t][e] = p1 + p2;
+                        z[0][n][t][e] = p1 * fmaf(dp[n][t][e], unit, -dot1[e]);
+                        z[1][n][t][e] = p2 * fmaf(dp[n][t][e], unit, -dot2[e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NK; n++) {
+                mix[n] = chunk_of<T>(pm[n]);
+#pragma unroll
+                for (int m = 0; m < 2; m++) ds[m][n] = chunk_of<T>(z[m][n]);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const u32x4 yf = Tile<T, VP>::columns(ys, k0, i, lane);
+#pragma unroll
+                for (int n = 0; n < NK; n++) dv[n][i] = mma(yf, mix[n], dv[n][i], T{});
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int i = 0; i < ND; i++) {
+                    const u32x4 qf = Tile<T, DP>::columns(qs + m * kRows * Tile<T, DP>::BYTES, k0, i, lane);
+#pragma unroll
+                    for (int n = 0; n < NK; n++) dk[m][n][i] = mma(qf, ds[m][n], dk[m][n][i], T{});
+                }
+        }
+        stage ^= 1;
+    }
+    const float fk = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / unit, fv = __builtin_amdgcn_exp2f(-kShift<T>);
+#pragma unroll
+    for (int n = 0; n < NK; n++) {
+        const int key = key0 + (wave * NK + n) * 16 + s;
+        if (key >= a.keys) continue;
+        float* to = a.part ? a.part + (((long long)part * (gridDim.x / a.tile_div.d) + per) * a.keys + key) * (2 * DP + VP) : nullptr;
+#pragma unroll
+        for (int m = 0; m < 3; m++) {    // dk of both maps, dv
+            const Strided& d = m < 2 ? a.dk : a.dv;
+            char* out = const_cast<char*>(d.p) + (m < 2 ? 2LL * kvh + m : (long long)kvh) * d.s1 + key * d.s2 + b * d.s3;
+            const int width = m < 2 ? a.dim : a.vdim;
+            const float f = m < 2 ? fk : fv;
+#pragma unroll
+            for (int i = 0; i < (m < 2 ? ND : NV); i++) {
+                const int at = i * 16 + lane / 16 * 4;
+                const f32x4 v = (m < 2 ? dk[m < 2 ? m : 0][n][m < 2 ? i : 0] : dv[n][i]) * f;
+                if (to) {
+                    *reinterpret_cast<f32x4*>(to + m * DP + at) = v;
+                } else if (d.p) {
+                    const float o[4] = {v[0], v[1], v[2], v[3]};
+                    store4<T>(out + at * sizeof(T), width - at, o);
+                }
+            }
+        }
+    }
+}
+
+// Sums of the parts of the rows, in order, for a key: four elements a thread.
+template <class T>
+__global__ __launch_bounds__(256) void diff_fold_kernel(DiffArgs a, int dp, int vp, long long keys) {
+    const int width = 2 * dp + vp, quads = width / 4;
+    const long long e = blockIdx.x * 256LL + threadIdx.x, index = e / quads;   // of (sequence, key head), key
+    if (index >= keys) return;
+    const int at = (int)(e - index * quads) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < a.splits; i++) v += *reinterpret_cast<const f32x4*>(a.part + (i * keys + index) * width + at);
+    const unsigned per = (unsigned)(index / a.keys);
+    const int key = (int)(index - (long long)per * a.keys), b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
+    const int m = at < dp ? 0 : at < 2 * dp ? 1 : 2, col = at - m * dp;
+    const Strided& d = m < 2 ? a.dk : a.dv;
+    if (!d.p) return;
+    const float o[4] = {v[0], v[1], v[2], v[3]};
+    char* out = const_cast<char*>(d.p) + (m < 2 ? 2LL * kvh + m : (long long)kvh) * d.s1 + key * d.s2 + b * d.s3;
+    store4<T>(out + col * (long long)sizeof(T), (m < 2 ? a.dim : a.vdim) - col, o);
+}
+
+// lambda's gradient: less the sum of its head's rows.
+__global__ __launch_bounds__(1024) void diff_lambda_kernel(const float* rows, long long batch, int heads, int queries, float* dlam) {
+    __shared__ double red[16];
+    const int h = blockIdx.x;
+    double s = 0.0;
+    const long long n = batch * queries;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < n; i += 1024) {
+        const long long b = i / queries;
+        s += (double)rows[(b * heads + h) * queries + (i - b * queries)];
+    }
+    s = lane_sum<64>(s);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; i++) s += red[i];
+    dlam[h] = (float)-s;
+}
+
+// fp16: the largest |v| and |dy| of the call, as bits (0 before it; the order of maxima does not matter).
+__global__ void diff_clear_kernel(unsigned* most) { most[threadIdx.x] = 0; }
+struct MostArgs {
+    Strided t[2];
+    long long rows[2];
+    FastDiv d1[2], d2[2];                // row -> (heads), (tokens)
+    int width[2];
+    const int* lengths;
+    unsigned* most;
+};
+__global__ __launch_bounds__(256) void diff_most_kernel(MostArgs a) {
+    const int which = blockIdx.y;
+    float most = 0.f;
+    const int lane = threadIdx.x % 64;
+    for (long long r = blockIdx.x * 4LL + threadIdx.x / 64; r < a.rows[which]; r += gridDim.x * 4LL) {
+        const unsigned i = a.d1[which].div((unsigned)r), h = (unsigned)r - i * a.d1[which].d, b = a.d2[which].div(i), n = i - b * a.d2[which].d;
+        if (which == 0 && a.lengths && (int)n >= a.lengths[b]) continue;          // keys that are not there
+        const f16* p = reinterpret_cast<const f16*>(a.t[which].p + h * a.t[which].s1 + n * a.t[which].s2 + b * a.t[which].s3);
+        for (int d = lane; d < a.width[which]; d += 64) most = fmaxf(most, fabsf((float)p[d]));
+    }
+    most = lane_max<64>(most);
+    if (lane == 0 && most > 0.f) atomicMax(a.most + which, __float_as_uint(most));
+}
+
+// --------------------------------------------------------------------------------- host
+constexpr int kCus = 256;
+size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+struct BackPlan {
+    int nq, nk, dp, vp, splits;
+    long long q_tiles, k_tiles;
+    size_t dots, rows_lam, most, part, total;
+};
+BackPlan back_plan(const DiffShape& s, int size) {
+    BackPlan p{};
+    const long long group = s.H / s.Hk, rows = s.M * group, pairs = s.B * s.Hk;
+    const bool small = s.D <= 64 && s.V <= 128 && size == 2;
+    with_dims(s.D, s.V, [&](auto d, auto v) { p.dp = d(), p.vp = v(); });
+    p.nq = small && rows > 64 ? 2 : 1;
+    p.nk = 1;
+    p.q_tiles = (rows + 64 * p.nq - 1) / (64 * p.nq);
+    p.k_tiles = (s.N + 64 * p.nk - 1) / (64 * p.nk);
+    // Parts of the rows: as many as give two blocks a CU, of 8 tiles at least.
+    p.splits = (int)std::max(1LL, std::min({2LL * kCus / std::max(1LL, p.k_tiles * pairs), rows / (8 * kRows), 64LL}));
+    auto take = [&](size_t bytes) {
+        const size_t at = p.total;
+        p.total += pad256(bytes);
+        return at;
+    };
+    p.dots = take((size_t)s.B * s.H * 2 * s.M * sizeof(float));
+    p.rows_lam = take((size_t)s.B * s.H * s.M * sizeof(float));
+    p.most = take(2 * sizeof(unsigned));
+    p.part = take(p.splits > 1 ? (size_t)p.splits * pairs * s.N * (2 * p.dp + p.vp) * sizeof(float) : 0);
+    return p;
+}
+
+template <class T, int DP, int VP>
+void launch_dq(const DiffArgs& a, const BackPlan& p, bool aligned, unsigned blocks, hipStream_t stream) {
+    if (!aligned) hipLaunchKernelGGL((diff_dq_kernel<T, DP, VP, 1, false>), dim3(blocks), dim3(256), 0, stream, a);
+    else if (p.nq == 1) hipLaunchKernelGGL((diff_dq_kernel<T, DP, VP, 1, true>), dim3(blocks), dim3(256), 0, stream, a);
+    else if constexpr (sizeof(T) == 2 && DP <= 64) hipLaunchKernelGGL((diff_dq_kernel<T, DP, VP, 2, true>), dim3(blocks), dim3(256), 0, stream, a);
+    launch_check("diff_dq_kernel");
+}
+template <class T, int DP, int VP>
+void launch_dkv(const DiffArgs& a, bool aligned, unsigned blocks, hipStream_t stream) {
+    if (aligned) hipLaunchKernelGGL((diff_dkv_kernel<T, DP, VP, 1, true>), dim3(blocks), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((diff_dkv_kernel<T, DP, VP, 1, false>), dim3(blocks), dim3(256), 0, stream, a);
+    launch_check("diff_dkv_kernel");
+}
+
+void check_like(const stx_tensor* t, const stx_tensor* like, int size, const char* what) {
+    check_out_rows(t, like->ne[0], like->ne[1], like->ne[2], like->ne[3], size, what);
+    check_nested(t, size, what);
+}
+
+}  // namespace
+}  // namespace stx
+
+using namespace stx;
+
+extern "C" {
+
+STX_API size_t stx_diff_attention_back_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v, stx_type type) {
+    size_t bytes = 0;
+    (void)guard([&] {
+        const char* op = "diff_attention_back_workspace_size";
+        const int size = type_size(type);
+        for (const stx_tensor* t : {q, k, v}) {
+            STX_REQUIRE(t != nullptr, "%s: a tensor is NULL", op);
+            for (int i = 0; i < 4; i++) STX_REQUIRE(t->ne[i] >= 0, "%s: negative ne[%d]", op, i);
+        }
+        const DiffShape s = diff_shape(q, k, v, op);
+        if (s.B > 0 && s.H > 0) bytes = back_plan(s, size).total;
+    });
+    return bytes;
+}
+
+STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
+                                           stx_type type, const float* lambda, float scale, int causal, const int32_t* lengths,
+                                           const int32_t* starts, const stx_tensor* out, const stx_tensor* second, const float* lse,
+                                           const stx_tensor* dq, const stx_tensor* dk, const stx_tensor* dv, float* dlambda,
+                                           void* workspace, size_t workspace_bytes, stx_stream stream) {
+    return guard([&] {
+        const char* op = "diff_attention_back";
+        const int size = type_size(type);
+        check_typed(q, size, "diff_attention_back: q");
+        check_typed(k, size, "diff_attention_back: k");
+        check_typed(v, size, "diff_attention_back: v");
+        const DiffShape s = diff_shape(q, k, v, op);
+        check_out_rows(dy, s.V, s.H, s.M, s.B, size, "diff_attention_back: dy");
+        check_out_rows(out, s.V, s.H, s.M, s.B, size, "diff_attention_back: out");
+        check_out_rows(second, s.V, s.H, s.M, s.B, size, "diff_attention_back: second");
+        if (dq) check_like(dq, q, size, "diff_attention_back: dq");
+        STX_REQUIRE((dk == nullptr) == (dv == nullptr), "%s: dk and dv go together", op);
+        if (dk) {
+            check_like(dk, k, size, "diff_attention_back: dk");
+            check_like(dv, v, size, "diff_attention_back: dv");
+        }
+        check_scale(scale, op);
+        if (s.B == 0 || s.H == 0) {
+            if (dlambda && s.H > 0) {
+                hipLaunchKernelGGL(diff_lambda_kernel, dim3(s.H), dim3(1024), 0, as_stream(stream), nullptr, 0, s.H, 1, dlambda);
+                launch_check("diff_lambda_kernel");
+            }
+            return;
+        }
+        BackPlan p = back_plan(s, size);
+        check_workspace(workspace, workspace_bytes, p.total, op);
+        const size_t per = (size_t)s.B * sizeof(int32_t), kept = (size_t)s.B * s.H * 2 * s.M * sizeof(float), heads = s.H * sizeof(float);
+        check_apart(op, {{"dq", dq, size}, {"dk", dk, size}, {"dv", dv, size}, {"dlambda", dlambda, heads}, {"the workspace", workspace, p.total}},
+                    {{"dy", dy, size}, {"q", q, size}, {"k", k, size}, {"v", v, size}, {"lambda", lambda, heads}, {"lengths", lengths, per},
+                     {"starts", starts, per}, {"out", out, size}, {"second", second, size}, {"lse", lse, kept}});
+        STX_REQUIRE(lambda != nullptr && (s.M == 0 || lse != nullptr), "%s: lambda or lse is NULL", op);
+        if (!dq && !dk && !dlambda) return;
+        DiffArgs a = diff_args(s, q, k, v, lambda, scale, causal, lengths, starts);
+        a.out = strided(out), a.second = strided(second), a.dy = strided(dy);
+        a.dq = strided(dq), a.dk = strided(dk), a.dv = strided(dv);
+        a.lse = const_cast<float*>(lse);
+        char* ws = static_cast<char*>(workspace);
+        a.dots = reinterpret_cast<float*>(ws + p.dots);
+        a.rows_lam = reinterpret_cast<float*>(ws + p.rows_lam);
+        unsigned* most = reinterpret_cast<unsigned*>(ws + p.most);
+        a.most = most;
+        const hipStream_t st = as_stream(stream);
+        const long long pairs = s.B * s.Hk;
+        const bool keys_aligned = rows_in_chunks(k, size) && rows_in_chunks(v, size), rows_aligned = rows_in_chunks(q, size) && rows_in_chunks(dy, size);
+        if (!keys_aligned && p.nq > 1) p.nq = 1, p.q_tiles = (a.rows + 63) / 64;
+        STX_REQUIRE(p.q_tiles * pairs < (1LL << 22) && p.k_tiles * p.splits * pairs < (1LL << 22), "%s: too many tiles", op);
+        const long long quads = pairs * s.N * ((2 * p.dp + p.vp) / 4);
+        STX_REQUIRE(quads / 256 < (1LL << 23), "%s: k and v too large", op);
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            with_dims(s.D, s.V, [&](auto d, auto vd) {
+                if constexpr (std::is_same_v<T, f16>) {
+                    MostArgs m{};
+                    m.t[0] = a.v, m.t[1] = a.dy;
+                    m.rows[0] = s.B * s.N * s.Hk, m.rows[1] = s.B * s.M * s.H;
+                    m.d1[0] = FastDiv((unsigned)s.Hk), m.d1[1] = FastDiv((unsigned)s.H);
+                    m.d2[0] = FastDiv((unsigned)std::max(1LL, s.N)), m.d2[1] = FastDiv((unsigned)std::max(1LL, s.M));
+                    m.width[0] = m.width[1] = s.V;
+                    m.lengths = lengths;
+                    m.most = most;
+                    STX_REQUIRE(m.rows[0] < (1LL << 32) && m.rows[1] < (1LL << 32), "%s: 2^32 rows or more", op);
+                    hipLaunchKernelGGL(diff_clear_kernel, dim3(1), dim3(2), 0, st, most);
+                    const long long blocks = std::max(1LL, std::min(2LL * kCus, (std::max(m.rows[0], m.rows[1]) + 15) / 16));
+                    hipLaunchKernelGGL(diff_most_kernel, dim3((unsigned)blocks, 2), dim3(256), 0, st, m);
+                    launch_check("diff_most_kernel");
+                }
+                if (s.M > 0) {
+                    a.tiles = (int)p.q_tiles;
+                    a.tile_div = FastDiv((unsigned)p.q_tiles);
+                    launch_dq<T, d(), vd()>(a, p, keys_aligned, (unsigned)(p.q_tiles * pairs), st);
+                }
+                if (dk && s.N > 0) {
+                    a.tiles = (int)p.k_tiles, a.splits = p.splits;
+                    a.tile_div = FastDiv((unsigned)(p.k_tiles * p.splits));
+                    a.part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
+                    launch_dkv<T, d(), vd()>(a, rows_aligned, (unsigned)(p.k_tiles * p.splits * pairs), st);
+                    if (p.splits > 1) {
+                        hipLaunchKernelGGL((diff_fold_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a, p.dp, p.vp, pairs * s.N);
+                        launch_check("diff_fold_kernel");
+                    }
+                }
+            });
+        });
+        if (dlambda) {
+            hipLaunchKernelGGL(diff_lambda_kernel, dim3(s.H), dim3(1024), 0, st, a.rows_lam, s.M > 0 ? s.B : 0, s.H, std::max(1, a.queries), dlambda);
+            launch_check("diff_lambda_kernel");
+        }
+    });
+}
+
+}  // extern "C"

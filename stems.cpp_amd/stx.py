@@ -141,6 +141,9 @@ _SIGNATURES = {
     "stx_soft_max_rel_back": (_i, [_vp, _vp, _i, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "stx_diff_attention_workspace_size": (ctypes.c_size_t, [_vp, _vp, _vp, _i]),
     "stx_diff_attention": (_i, [_vp, _vp, _vp, _i, _vp, ctypes.c_float, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "stx_diff_attention_back_workspace_size": (ctypes.c_size_t, [_vp, _vp, _vp, _i]),
+    "stx_diff_attention_back": (_i, [_vp, _vp, _vp, _vp, _i, _vp, ctypes.c_float, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                     _vp, ctypes.c_size_t, _vp]),
 }
 
 
@@ -1530,3 +1533,23 @@ def diff_attention(q, k, v, lam, scale=None, causal=False, lengths=None, starts=
 
 def _scale(scale, q):
     return float(max(1, q.shape[-1]) ** -0.5 if scale is None else scale)
+
+
+def diff_attention_back(dy, q, k, v, lam, out, second, lse, scale=None, causal=False, lengths=None, starts=None, dq=None, dk=None,
+                        dv=None, dlam=None, workspace=None, stream=None):
+    """Gradients (dq, dk, dv, dlam) of diff_attention from dy (of out), its inputs and masks and what it kept (out, second,
+    lse); dlam is float32 (heads,)."""
+    import torch
+    B, M, H, V = _heads(q, k, v)
+    dq = _empty_like(q, stream) if dq is None else dq
+    dk = _empty_like(k, stream) if dk is None else dk
+    dv = _empty_like(v, stream) if dv is None else dv
+    dlam = _empty(H, q, stream, torch.float32) if dlam is None else dlam
+    L, t = lib(), _type(q)
+    d = [_typed(x, q, n) for x, n in ((dy, "dy"), (q, "q"), (k, "k"), (v, "v"), (out, "out"), (second, "second"), (dq, "dq"),
+                                      (dk, "dk"), (dv, "dv"))]
+    ws, nbytes, owner = _scratch(L.stx_diff_attention_back_workspace_size(d[1], d[2], d[3], t), workspace, q, stream)
+    _launch(L.stx_diff_attention_back, q, stream, d[0], d[1], d[2], d[3], t, _floats(lam, q, H, "lam"), _scale(scale, q),
+            bool(causal), _per_sequence(lengths, q, B, "lengths"), _per_sequence(starts, q, B, "starts"), d[4], d[5],
+            _floats(lse, q, B * H * 2 * M, "lse"), d[6], d[7], d[8], _floats(dlam, q, H, "dlam"), ws, nbytes)
+    return dq, dk, dv, dlam

@@ -534,3 +534,156 @@ def test_diff_empty(device):
         assert stx.diff_attention(*make(B, M, N), lam, keep=True)[0].shape == (B, M, 2, 8)
     out, second, lse = stx.diff_attention(*make(2, 3, 0), lam, keep=True)
     assert bool((out == 0).all()) and bool((second == 0).all()) and bool((lse == -math.inf).all())
+
+
+def diff_back_ref(dy, q, k, v, lam, out, second, lse, mask, scale):
+    """(gradient, bound of its error before rounding) of each, from what the forward call kept, in 64 bits. With E = (2 (D + 8) Z
+    + 8 |lse| + 16) u relative to P, dP off by (V + 8) u Y (Y = |dy| |v|^T) and D by (V + 8) u sum |dy| (|out| + 2 |lam
+    second|), dS = f P (dP - D) is off by |f| (E P |dP - D| + P (both)) and, rounded, by h |dS| more; sums drift by 4 sqrt(n) u."""
+    B, M, H2, D = q.shape
+    H, Hk, V, N = H2 // 2, v.shape[2], v.shape[3], k.shape[1]
+    g = H // Hk
+    h = half_step(q.dtype) if q.dtype != torch.float32 else 0.0
+    p, _, size, q64, k64, v64 = diff_maps(q, k, v, mask, scale)
+    z = torch.matmul(q64, k64.transpose(3, 4).contiguous()) * scale
+    ls = lse.to(F64).permute(2, 0, 1, 3)[..., None]
+    p = torch.where(mask[:, None], torch.exp(z - ls), 0.0)
+    E = (2 * (D + 8) * size + 8 * torch.where(ls.isinf(), 0.0, ls.abs()) + 16) * U
+    y, o, o2 = (t.to(F64).transpose(1, 2).contiguous() for t in (dy, out, second))
+    la = lam.to(F64)[:, None, None]
+    vt = v64.transpose(2, 3).contiguous()
+    dp, Y = torch.matmul(y, vt), torch.matmul(y.abs(), vt.abs())
+    dots = ((y * (o + la * o2)).sum(-1, keepdim=True), (y * o2).sum(-1, keepdim=True))
+    ddot = (V + 8) * U * (y.abs() * (o.abs() + 2 * (la * o2).abs())).sum(-1, keepdim=True)
+    dq, bq = (torch.zeros(2, B, H, M, D, dtype=F64, device=q.device) for _ in range(2))
+    dk, bk = (torch.zeros(2, B, H, N, D, dtype=F64, device=q.device) for _ in range(2))
+    tiny = 2.0 ** -38 * V * float(v64[~v64.isnan()].abs().max()) * float(y.abs().max()) * max(1.0, float(la.abs().max())) if q.dtype == torch.float16 else 0.0
+    for m, f in ((0, torch.ones_like(la)), (1, -la)):
+        ds = f * p[m] * (dp - dots[m])
+        e = f.abs() * p[m] * (E[m] * (dp - dots[m]).abs() + (V + 8) * U * Y + ddot) + h * ds.abs() + tiny * mask[:, None]
+        dq[m], dk[m] = torch.matmul(ds, k64[m]) * scale, torch.matmul(ds.transpose(2, 3).contiguous(), q64[m]) * scale
+        bq[m] = torch.matmul(e + 4 * math.sqrt(N) * U * ds.abs(), k64[m].abs()) * scale
+        bk[m] = torch.matmul((e + 4 * math.sqrt(M * g) * U * ds.abs()).transpose(2, 3).contiguous(), q64[m].abs()) * scale
+    mix = (p[0] - la * p[1]).transpose(2, 3).contiguous()
+    both = (p[0] * (E[0] + h + 4 * math.sqrt(M * g) * U) + la.abs() * p[1] * (E[1] + h + 4 * math.sqrt(M * g) * U)).transpose(2, 3).contiguous()
+    dv, bv = torch.matmul(mix, y), torch.matmul(both, y.abs())
+    dlam = -(p[1] * dp).sum((0, 2, 3))
+    bl = (p[1] * (E[1] * dp.abs() + (V + 8) * U * Y) + (math.sqrt(N) + 16) * U * (p[1] * dp).abs()).sum((0, 2, 3))
+    heads = lambda t: t.unflatten(1, (Hk, g)).sum(2)  # noqa: E731
+    rows = lambda t: t.permute(1, 3, 2, 0, 4).reshape(B, M, 2 * H, D)  # noqa: E731
+    keys = lambda t: torch.stack([heads(x) for x in t]).permute(1, 3, 2, 0, 4).reshape(B, N, 2 * Hk, D)  # noqa: E731
+    return (rows(dq), rows(bq)), (keys(dk), keys(bk)), (heads(dv).transpose(1, 2), heads(bv).transpose(1, 2)), (dlam, bl)
+
+
+def check_diff_back(got, dy, q, k, v, lam, kept, mask, scale, what, norms=True):
+    want = diff_back_ref(dy, q, k, v, lam, *kept, mask, scale)
+    for g, (w, bound), name in zip(got, want, ("dq", "dk", "dv", "dlam")):
+        close(g, w, bound, f"{what} {name}")
+        if norms and name != "dlam" and min(q.shape[1], k.shape[1]) >= 64:
+            norm_close(g, w, 2, f"{what} {name}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", DIFF, ids=lambda s: "-".join(str(v) for v in s))
+def test_diff_attention_back(device, dtype, shape):
+    B, M, N, H, Hk, D, V, causal, _ = shape
+    q, k, v, lam, lengths, starts = diff_inputs(device, TYPES[dtype], shape)
+    dy = randn(device, (B, M, H, V), 7, dtype=q.dtype)
+    mask, _ = seen_ref(B, M, N, lengths, starts, causal, device)
+    kc, vc = k.clone(), v.clone()
+    spoil(k, v, lengths)
+    masks = dict(causal=causal, lengths=lengths, starts=starts)
+    kept = stx.diff_attention(q, k, v, lam, keep=True, **masks)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept, **masks)
+    check_diff_back(got, dy, q, kc, vc, lam, kept, mask, D ** -0.5, "back")
+    if lengths is not None:
+        for b, n in enumerate(lengths.tolist()):
+            assert bool((got[1][b, n:] == 0).all()) and bool((got[2][b, n:] == 0).all())
+    again = stx.diff_attention_back(dy, q, k, v, lam, *kept, **masks)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 70])
+@pytest.mark.parametrize("causal", [False, True])
+def test_diff_back_masks_at_their_limits(device, dtype, M, causal):
+    lengths = torch.tensor([0, -5, 1, 40, 1000, 2 ** 31 - 1, -2 ** 31, 17], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, 3, -1, -9, 100, 2 ** 31 - 1, -2 ** 31, -2 ** 31], dtype=torch.int32, device=device)
+    B, N, H, Hk, D, V = 8, 90, 4, 2, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    dy = randn(device, (B, M, H, V), 7, dtype=q.dtype)
+    mask, _ = seen_ref(B, M, N, lengths, starts, causal, device)
+    masks = dict(causal=causal, lengths=lengths, starts=starts)
+    kept = stx.diff_attention(q, k, v, lam, keep=True, **masks)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept, **masks)
+    check_diff_back(got, dy, q, k, v, lam, kept, mask, D ** -0.5, "limits", norms=False)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-6, 1.0, 3e3])
+def test_diff_back_range(device, dtype, size):
+    """Gradients far from 1, and rows whose gradient is a small part of the largest: fp16 keeps its bits."""
+    B, M, N, H, Hk, D, V = 1, 80, 150, 2, 1, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    dy = (randn(device, (B, M, H, V), 7) * (size if size > 1e-3 else 1e-2))
+    dy[:, ::3] *= 1e-2
+    dy, mask = dy.to(q.dtype), torch.ones(B, M, N, dtype=torch.bool, device=device)
+    kept = stx.diff_attention(q, k, v, lam, keep=True)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept)
+    check_diff_back(got, dy, q, k, v, lam, kept, mask, D ** -0.5, "range", norms=size >= 1.0)
+
+
+def test_diff_gradient_against_differences(device):
+    """The whole way, forward and backward in fp32, against central differences of the definition in 64 bits."""
+    B, M, N, H, Hk, D, V = 1, 5, 7, 2, 1, 16, 16
+    q, k, v, lam, _, _ = diff_inputs(device, torch.float32, (B, M, N, H, Hk, D, V, False, None))
+    starts = torch.tensor([2], dtype=torch.int32, device=device)
+    mask, _ = seen_ref(B, M, N, None, starts, True, device)
+    dy = randn(device, (B, M, H, V), 7)
+    kept = stx.diff_attention(q, k, v, lam, causal=True, starts=starts, keep=True)
+    grads = stx.diff_attention_back(dy, q, k, v, lam, *kept, causal=True, starts=starts)
+
+    def f(q, k, v, lam):
+        p, _, _, _, _, v64 = diff_maps(q, k, v, mask, D ** -0.5)
+        o = torch.matmul(p[0], v64) - lam.to(F64)[:, None, None] * torch.matmul(p[1], v64)
+        return float((o.transpose(1, 2) * dy.to(F64)).sum())
+
+    args = [t.to(F64) for t in (q, k, v, lam)]
+    step = 1e-5
+    for a, grad in enumerate(grads):
+        for i in range(0, args[a].numel(), 5 if args[a].numel() > 2 else 1):
+            ends = []
+            for sign in (1, -1):
+                moved = [t.clone() for t in args]
+                moved[a].view(-1)[i] += sign * step
+                ends.append(f(*moved))
+            diff = (ends[0] - ends[1]) / (2 * step)
+            assert abs(float(grad.reshape(-1)[i]) - diff) < 2e-5 * max(1.0, abs(diff)), (a, i)
+
+
+def test_diff_back_strides_and_empty(device):
+    """Gradients into slices of wider buffers, from operands at unaligned offsets; calls without queries or keys."""
+    B, M, N, H, Hk, D, V = 2, 37, 90, 4, 2, 64, 128
+    for dt in TYPES.values():
+        q, k, v, lam, _, _ = diff_inputs(device, dt, (B, M, N, H, Hk, D, V, False, None))
+        dy = randn(device, (B, M, H, V), 7, dtype=dt)
+        kept = stx.diff_attention(q, k, v, lam, keep=True)
+        mask = torch.ones(B, M, N, dtype=torch.bool, device=device)
+        shifted = []
+        for t in (q, k, v, dy):
+            w = torch.zeros((*t.shape[:2], t.shape[2] + 1, t.shape[3] + 3), device=device, dtype=dt)
+            w[:, :, 1:, 3:] = t
+            shifted.append(w[:, :, 1:, 3:])
+        outs = [torch.full((t.shape[0], t.shape[1] + 1, t.shape[2], t.shape[3] + 5), 7.0, device=device, dtype=dt) for t in (q, k, v)]
+        into = [t[:, 1:, :, 2:2 + n] for t, n in zip(outs, (D, D, V))]
+        got = stx.diff_attention_back(shifted[3], *shifted[:3], lam, *kept, dq=into[0], dk=into[1], dv=into[2])
+        check_diff_back(got, dy, q, k, v, lam, kept, mask, D ** -0.5, "strides")
+        for t, s in zip(outs, into):
+            s.fill_(7.0)
+            assert bool((t == 7.0).all())
+    lam = torch.ones(2, device=device)
+    for b, m, n in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        q, k, v = torch.ones(b, m, 4, 8, device=device), torch.ones(b, n, 2, 8, device=device), torch.ones(b, n, 1, 8, device=device)
+        kept = stx.diff_attention(q, k, v, lam, keep=True)
+        got = stx.diff_attention_back(torch.ones(b, m, 2, 8, device=device), q, k, v, lam, *kept)
+        assert all(bool((t == 0).all()) for t in got) and got[3].shape == (2,)
