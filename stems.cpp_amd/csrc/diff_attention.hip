@@ -11,10 +11,14 @@ namespace {
 // the exponentials are, where they stand, the operand of O^T = V^T P^T. v is read transposed from its tile.
 // WK waves share rows and split a tile's keys between them (few rows: single tokens); others have rows of their own.
 //
-// m is raised only where a score passes it by 2^8, as a first tile always does: a sum scaled by any power is as good, and
-// the products of P then need no scaling in most tiles. P is rounded to 16 bits for its product (16-bit data): its
-// errors are independent and average out to about those of rounding the result. fp16's is
-// scaled by 2^6 so that shares of 2^-20 keep all their bits.
+// m is raised only where an exponential passes 2^14, as a first tile's do against -inf: a sum scaled by any power is as
+// good, most tiles then need neither the row's maximum nor a scaling of the sums, and the check is on
+// exponentials, which the compiler knows to be canonical (maxima of the products take an instruction more each).
+//
+// P is rounded to 16 bits for its product (16-bit data). Rounding both maps once leaves the difference 1.54 times the error
+// that rounding the result alone has (60 x 801 frames, lambda about 0.5: 2.5e-3 in bf16 where it is 1.65e-3), for the maps cancel and
+// their errors do not. The first map, which weighs more, is taken in two parts, 1.06 times; 204 -> 232 us.
+// fp16's P is scaled by 2^6 so that shares of 2^-20 keep all their bits.
 template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 6.f : 0.f;
 
@@ -27,14 +31,16 @@ constexpr int tile_keys() {
 }
 
 template <class T, int DP, int VP, int NQ, int WAVES, int WK, bool ALIGNED>
-__global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) {
-    constexpr int NT = 64 * WAVES, BK = tile_keys<T, DP, VP, WK>(), KW = BK / WK, KG = Tile<T, DP>::KEYS, KS = KW < 64 ? KW : 64;
+__global__ __launch_bounds__(64 * WAVES, WK == 1 ? 2 : 1) void diff_attention_kernel(DiffArgs a) {
+    constexpr int NT = 64 * WAVES, BK = tile_keys<T, DP, VP, WK>(), KW = BK / WK, KG = Tile<T, DP>::KEYS, KS = KW < 64 / NQ ? KW : 64 / NQ;
+    constexpr bool SPLIT = sizeof(T) == 2;
     constexpr int ROWS = 16 * NQ * (WAVES / WK), GD = Tile<T, DP>::GROUPS, NV = VP / 16;
     using KL = Loader<T, DP, BK, 2, NT, ALIGNED>;
     using VL = Loader<T, VP, BK, 1, NT, ALIGNED>;
     constexpr int STAGE = KL::BYTES + VL::BYTES, JOIN = WK > 1 ? WK * 2 * NV * 64 * 16 : 0, LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
     static_assert(KW % KS == 0 && KS % KG == 0 && LDS <= 160 * 1024);
     __shared__ __align__(128) char lds[LDS];
+    const unsigned lds0 = lds_address(lds);
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wk = wave % WK, s = lane % 16;
     const unsigned item = blockIdx.x, per = a.tile_div.div(item);
@@ -57,9 +63,16 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
     const char* vb = a.v.p + (long long)kvh * a.v.s1 + b * a.v.s3;
     KL kl;
     VL vl;
+    kl.space(a.k.s2, a.k.s1);
+    vl.space(a.v.s2, 0);
     auto fetch = [&](int key0, int stage) {
-        kl.fetch(lds + stage * STAGE, a.dim, [&](int map, int r) { return key0 + r < mask.length ? kb + map * a.k.s1 + (key0 + r) * a.k.s2 : nullptr; });
-        vl.fetch(lds + stage * STAGE + KL::BYTES, a.vdim, [&](int, int r) { return key0 + r < mask.length ? vb + (key0 + r) * a.v.s2 : nullptr; });
+        if (ALIGNED && key0 + BK <= mask.length && a.dim == DP && a.vdim == VP) {
+            kl.fetch_whole(lds0 + stage * STAGE, kb + key0 * a.k.s2, a.k.s2, a.k.s1);
+            vl.fetch_whole(lds0 + stage * STAGE + KL::BYTES, vb + key0 * a.v.s2, a.v.s2, 0);
+            return;
+        }
+        kl.fetch(lds0 + stage * STAGE, a.dim, [&](int map, int r) { return key0 + r < mask.length ? kb + map * a.k.s1 + (key0 + r) * a.k.s2 : nullptr; });
+        vl.fetch(lds0 + stage * STAGE + KL::BYTES, a.vdim, [&](int, int r) { return key0 + r < mask.length ? vb + (key0 + r) * a.v.s2 : nullptr; });
     };
     if (begin < end) fetch(begin, 0);
 
@@ -89,7 +102,7 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
         if (key0 + BK < end) fetch(key0 + BK, stage ^ 1);
         const char *ks = lds + stage * STAGE, *vs = ks + KL::BYTES;
         const bool whole = key0 + BK <= least && key0 + BK <= end;
-#pragma unroll
+#pragma unroll 1
         for (int k0 = 0; k0 < KW; k0 += KS) {
             const int at = wk * KW + k0;
             f32x4 z[2][NQ][KS / 16];
@@ -107,7 +120,9 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             if (!whole) {
+                asm volatile("");
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
                     const int left = min(limit[n], end) - (key0 + at + lane / 16 * 4);
@@ -120,33 +135,48 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
                 }
             }
             u32x4 p[2][NQ][KS / KG];
+            u32x4 low[SPLIT ? NQ : 1][KS / KG];
 #pragma unroll
             for (int m = 0; m < 2; m++) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
-                    float high = -__builtin_inff();
+                    f32x4 e[KS / 16];
+                    float high = 0.f;
+                    auto raise = [&](float base) {
 #pragma unroll
-                    for (int t = 0; t < KS / 16; t++) high = fmaxf(fmaxf(fmaxf(high, z[m][n][t][0]), fmaxf(z[m][n][t][1], z[m][n][t][2])), z[m][n][t][3]);
-                    high = column_max(high) * c;
-                    if (__builtin_amdgcn_ballot_w64(high - kShift<T> > top[m][n] + 8.f)) {
-                        const float up = fmaxf(top[m][n], high - kShift<T>), f = __builtin_amdgcn_exp2f(top[m][n] - (up == -__builtin_inff() ? 0.f : up));
+                        for (int t = 0; t < KS / 16; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) e[t][i] = __builtin_amdgcn_exp2f(fmaf(z[m][n][t][i], c, -base));
+                    };
+                    raise(top[m][n]);
+#pragma unroll
+                    for (int t = 0; t < KS / 16; t++) high = fmaxf(fmaxf(fmaxf(high, e[t][0]), e[t][1]), fmaxf(e[t][2], e[t][3]));
+                    if (__builtin_amdgcn_ballot_w64(!(high <= 0x1p14f && top[m][n] > -__builtin_inff()))) {   // -inf: no key yet
+                        float most = -__builtin_inff();
+#pragma unroll
+                        for (int t = 0; t < KS / 16; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) most = fmaxf(most, z[m][n][t][i]);
+                        const float up = fmaxf(top[m][n], column_max(most) * c - kShift<T>), base = up == -__builtin_inff() ? 0.f : up;
+                        const float f = __builtin_amdgcn_exp2f(top[m][n] - base);
                         top[m][n] = up;
                         sum[m][n] *= f;
 #pragma unroll
                         for (int i = 0; i < NV; i++) acc[m][n][i] *= f;
+                        raise(base);
                     }
-                    const float base = top[m][n] == -__builtin_inff() ? 0.f : top[m][n];
 #pragma unroll
                     for (int t = 0; t < KS / 16; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            z[m][n][t][e] = __builtin_amdgcn_exp2f(fmaf(z[m][n][t][e], c, -base));
-                            sum[m][n] += z[m][n][t][e];
-                        }
+                        for (int i = 0; i < 4; i++) sum[m][n] += e[t][i];
 #pragma unroll
-                    for (int g = 0; g < KS / KG; g++) p[m][n][g] = chunk_of<T>(&z[m][n][g * KG / 16]);
+                    for (int g = 0; g < KS / KG; g++) {
+                        p[m][n][g] = chunk_of<T>(&e[g * KG / 16]);
+                        if (SPLIT && m == 0) low[n][g] = rest_of<T>(&e[g * KG / 16], p[m][n][g]);
+                    }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g = 0; g < KS / KG; g++)
 #pragma unroll
@@ -156,6 +186,10 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
                     for (int m = 0; m < 2; m++)
 #pragma unroll
                         for (int n = 0; n < NQ; n++) acc[m][n][i] = mma(vf, p[m][n][g], acc[m][n][i], T{});
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int n = 0; n < NQ; n++) acc[0][n][i] = mma(vf, low[n][g], acc[0][n][i], T{});
+                    }
                 }
         }
         stage ^= 1;
@@ -163,7 +197,9 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int n = 0; n < NQ; n++) sum[m][n] = column_sum(sum[m][n]);
+        for (int n = 0; n < NQ; n++) {
+            sum[m][n] = column_sum(sum[m][n]);
+        }
 
     if constexpr (WK > 1) {              // the waves' sums, at the largest of their maxima
         static_assert(NQ == 1);
@@ -248,40 +284,36 @@ __global__ __launch_bounds__(64 * WAVES) void diff_attention_kernel(DiffArgs a) 
     }
 }
 
-// Rows whose keys were split: a wave a row, its parts in order.
+// Rows whose keys were split: a wave a row. A lane has a part (64 at most), its share of the row then goes to all.
 template <class T>
-__global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, int vp, long long all) {
-    const long long index = blockIdx.x * 4LL + threadIdx.x / 64;     // of (sequence, key head), row
-    if (index >= all) return;
-    const int lane = threadIdx.x % 64;
+__global__ __launch_bounds__(64) void diff_join_kernel(DiffArgs a, int vp, long long all) {
+    __shared__ float share[2][64];
+    const long long index = blockIdx.x;                              // of (sequence, key head), row
+    const int lane = threadIdx.x;
     const unsigned per = (unsigned)(index / a.rows);
     const int r = (int)(index - (long long)per * a.rows), b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
     const RowAt row(a, kvh, r);
-    float base[2], inv[2];
+    const float lam = a.lam[row.head];
 #pragma unroll
     for (int m = 0; m < 2; m++) {
-        float up = -__builtin_inff(), sum = 0.f;
-        for (int i = 0; i < a.splits; i++) up = fmaxf(up, a.part_stat[(i * all + index) * 4 + m * 2]);
-        base[m] = up == -__builtin_inff() ? 0.f : up;
-        for (int i = 0; i < a.splits; i++) sum = fmaf(a.part_stat[(i * all + index) * 4 + m * 2 + 1], __builtin_amdgcn_exp2f(a.part_stat[(i * all + index) * 4 + m * 2] - base[m]), sum);
-        inv[m] = sum == 0.f ? 0.f : 1.f / sum;
-        if (a.lse && lane == 0) a.lse[row.stat(a, b, m)] = sum == 0.f ? -__builtin_inff() : (up + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+        const float* stat = a.part_stat + ((long long)min(lane, a.splits - 1) * all + index) * 4 + m * 2;
+        const float top = lane < a.splits ? stat[0] : -__builtin_inff(), sum = lane < a.splits ? stat[1] : 0.f;
+        const float up = lane_max<64>(top), base = up == -__builtin_inff() ? 0.f : up, f = __builtin_amdgcn_exp2f(top - base);
+        const float total = (float)lane_sum<64>((double)(sum * f));
+        share[m][lane] = total == 0.f ? 0.f : f / total;
+        if (a.lse && lane == 0) a.lse[row.stat(a, b, m)] = total == 0.f ? -__builtin_inff() : (up + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
     }
-    const float lam = a.lam[row.head];
+    __syncthreads();
     T* out = reinterpret_cast<T*>(const_cast<char*>(row.at(a.out, b, 1, 0)));
     T* second = a.second.p ? reinterpret_cast<T*>(const_cast<char*>(row.at(a.second, b, 1, 0))) : nullptr;
     for (int d = lane; d < a.vdim; d += 64) {
         float o[2] = {};
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < a.splits; i++)
 #pragma unroll
-            for (int m = 0; m < 2; m++) {
-                const long long at = i * all + index;
-                o[m] = fmaf(a.part[(at * 2 + m) * vp + d], __builtin_amdgcn_exp2f(a.part_stat[at * 4 + m * 2] - base[m]), o[m]);
-            }
-        const float o2 = o[1] * inv[1];
-        out[d] = from_f32<T>(fmaf(-lam, o2, o[0] * inv[0]));
-        if (second) second[d] = from_f32<T>(o2);
+            for (int m = 0; m < 2; m++) o[m] = fmaf(a.part[((i * all + index) * 2 + m) * vp + d], share[m][i], o[m]);
+        out[d] = from_f32<T>(fmaf(-lam, o[1], o[0]));
+        if (second) second[d] = from_f32<T>(o[1]);
     }
 }
 
@@ -397,7 +429,7 @@ STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, 
             with_dims(s.D, s.V, [&](auto d, auto v) { launch_forward<T, d(), v()>(a, p, aligned, as_stream(stream)); });
             if (p.splits == 1) return;
             const long long all = s.B * s.Hk * a.rows;
-            hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, as_stream(stream), a, p.vp, all);
+            hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)all), dim3(64), 0, as_stream(stream), a, p.vp, all);
             launch_check("diff_join_kernel");
         });
     });

@@ -24,7 +24,7 @@ struct DiffArgs {
     const float* lam;                    // [heads]
     float* lse;                          // [sequence][head][map][query]
     float* dots;                         // backward: dy . o of each map, laid out as lse
-    float* rows_lam;                     // backward: a row's share of lambda's gradient, [sequence][head][query]
+    double* tiles_lam;                   // backward: a block's shares of lambda's gradient, [block][group]
     const unsigned* most;                // fp16's backward: largest |v| and |dy| of the call, as bits
     float* part;                         // split keys (forward) or rows (keys' gradients)
     float* part_stat;
@@ -90,18 +90,45 @@ struct Tile {
     }
 };
 
-// The chunks that a thread brings of MAPS tiles of ROWS rows, straight to LDS (ALIGNED) or through registers.
+// The chunks that a thread brings of MAPS tiles of ROWS rows, straight to LDS (ALIGNED; `lds` is an address there) or
+// through registers.
 template <class T, int W, int ROWS, int MAPS, int NT, bool ALIGNED>
 struct Loader {
     using L = Tile<T, W>;
     static constexpr int N = MAPS * ROWS * L::CHUNKS / NT, BYTES = MAPS * ROWS * L::BYTES;
     static_assert(MAPS * ROWS * L::CHUNKS % NT == 0);
+    static constexpr int STEP = NT / L::CHUNKS, PERIOD = STEP % 16 == 0 ? 1 : 16 / STEP;   // rows from a chunk to the thread's next; chunks until turn() repeats
+    static_assert(NT % L::CHUNKS == 0);
     u32x4 hold[ALIGNED ? 1 : N];
+    unsigned off[ALIGNED ? PERIOD : 1];  // of the thread's first chunks in a tile of evenly spaced rows
+    static __device__ __forceinline__ unsigned wave_start() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64 * 1024); }
+    __device__ __forceinline__ void space(long long stride, long long map) {
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int i = 0; i < PERIOD; i++) {
+                const int r = i * STEP + (int)threadIdx.x / L::CHUNKS;
+                off[i] = (unsigned)(r / ROWS * map + r % ROWS * stride) + (((int)threadIdx.x % L::CHUNKS) ^ L::turn(r)) * 16;
+            }
+        }
+    }
+    // The whole tile that starts at p, rows `stride` apart, maps `map` apart: a scalar base and one offset a load (with
+    // rows one by one, the addresses took a sixth of the forward kernel's instructions). Rows have W elements.
+    __device__ __forceinline__ void fetch_whole(unsigned lds, const char* p, long long stride, long long map) {
+        if constexpr (ALIGNED) {
+            const unsigned to = lds + wave_start();
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int r = i / PERIOD * PERIOD * STEP;
+                load_to_lds(p + r / ROWS * map + r % ROWS * stride, off[i % PERIOD], to + i * NT * 16);
+            }
+        }
+    }
     // row(map, r): a row's start, or NULL for one of zeros. `width` elements exist.
+    // (Tiles in a sequence's end, and rows that LDS pads.)
     template <class F>
-    __device__ __forceinline__ void fetch(char* lds, int width, F&& row) {
+    __device__ __forceinline__ void fetch(unsigned lds, int width, F&& row) {
         const int tid = threadIdx.x;
-        const unsigned to = ALIGNED ? lds_address(lds + tid / 64 * 1024) : 0;
+        const unsigned to = lds + wave_start();
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int e = i * NT + tid, r = e / L::CHUNKS, c = (e % L::CHUNKS) ^ L::turn(r % ROWS);
@@ -152,6 +179,24 @@ __device__ __forceinline__ u32x4 chunk_of(const f32x4* acc) {
     return f;
 }
 
+template <class T>
+__device__ __forceinline__ void unpack(u32x4 f, float (&v)[16 / sizeof(T)]) {
+    T t[16 / sizeof(T)];
+    __builtin_memcpy(t, &f, 16);
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(T); e++) v[e] = to_f32(t[e]);
+}
+// What rounding to chunk f (16-bit data) left of them, rounded.
+template <class T>
+__device__ __forceinline__ u32x4 rest_of(const f32x4* acc, u32x4 f) {
+    float v[16 / sizeof(T)];
+    unpack<T>(f, v);
+    f32x4 r[2];
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(T); e++) r[e / 4][e % 4] = acc[e / 4][e % 4] - v[e];
+    return chunk_of<T>(r);
+}
+
 // A row's chunks as a fragment in registers: lane l's row, chunk (l / 16) + 4 group.
 template <class T, int W>
 __device__ __forceinline__ void load_fragments(u32x4* f, const char* p, int width, int lane) {
@@ -160,13 +205,6 @@ __device__ __forceinline__ void load_fragments(u32x4* f, const char* p, int widt
         const int c = g * 4 + lane / 16;
         f[g] = load_chunk<T>(p + c * 16, p ? width - c * Tile<T, W>::E : 0);
     }
-}
-template <class T>
-__device__ __forceinline__ void unpack(u32x4 f, float (&v)[16 / sizeof(T)]) {
-    T t[16 / sizeof(T)];
-    __builtin_memcpy(t, &f, 16);
-#pragma unroll
-    for (int e = 0; e < 16 / (int)sizeof(T); e++) v[e] = to_f32(t[e]);
 }
 
 // Row r of (sequence b, key head kvh).
@@ -221,7 +259,7 @@ inline Strided strided(const stx_tensor* t) {
 inline bool rows_in_chunks(const stx_tensor* t, int size) {
     bool ok = reinterpret_cast<uintptr_t>(t->data) % 16 == 0 && t->ne[0] * size % 16 == 0;
     for (int i = 1; i < 4; i++) ok = ok && (t->ne[i] <= 1 || t->nb[i] % 16 == 0);
-    return ok;
+    return ok && (t->ne[1] <= 1 || t->nb[1] < (1 << 23)) && (t->ne[2] <= 1 || t->nb[2] < (1 << 23));   // offsets in a tile fit 31 bits
 }
 
 inline DiffArgs diff_args(const DiffShape& s, const stx_tensor* q, const stx_tensor* k, const stx_tensor* v, const float* lam, float scale, int causal,

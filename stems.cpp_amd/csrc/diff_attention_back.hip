@@ -26,35 +26,46 @@ __device__ __forceinline__ float range_scale(const DiffArgs& a, float dy, float 
 }
 
 template <class T, int DP, int VP, int NQ, bool ALIGNED>
-__global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_dq_kernel(DiffArgs a) {
     constexpr int NT = 256, KG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, ROWS = 64 * NQ;
     constexpr int FIT = 32768 / ((2 * DP + VP) * (int)sizeof(T)), BK = FIT >= 64 ? 64 : FIT >= 32 ? 32 : 16;
     using KL = Loader<T, DP, BK, 2, NT, ALIGNED>;
     using VL = Loader<T, VP, BK, 1, NT, ALIGNED>;
     constexpr int STAGE = KL::BYTES + VL::BYTES;
     __shared__ __align__(128) char lds[2 * STAGE];
+    const unsigned lds0 = lds_address(lds);
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, s = lane % 16;
     const unsigned per = a.tile_div.div(blockIdx.x);
-    int tile = (int)(blockIdx.x - per * a.tile_div.d);
-    if (a.causal) tile = a.tiles - 1 - tile;                          // the longest first
+    const int index = (int)(blockIdx.x - per * a.tile_div.d), part = index % a.splits;
+    const int tile = a.causal ? a.tiles - 1 - index / a.splits : index / a.splits;   // the longest first
     const int b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
     const Mask mask(a, b);
     const int r0 = tile * ROWS, last = min(r0 + ROWS, a.rows) - 1;
-    const int end = mask.limit((int)a.group_div.div((unsigned)last)), least = mask.limit((int)a.group_div.div((unsigned)r0));
+    const int most = mask.limit((int)a.group_div.div((unsigned)last)), least = mask.limit((int)a.group_div.div((unsigned)r0));
+    const int each = ((most + BK - 1) / BK + a.splits - 1) / a.splits * BK;   // keys of a part
+    const int begin = (int)min((long long)part * each, (long long)most), end = (int)min((long long)begin + each, (long long)most);
     const char* kb = a.k.p + 2LL * kvh * a.k.s1 + b * a.k.s3;
     const char* vb = a.v.p + (long long)kvh * a.v.s1 + b * a.v.s3;
     KL kl;
     VL vl;
+    kl.space(a.k.s2, a.k.s1);
+    vl.space(a.v.s2, 0);
     auto fetch = [&](int key0, int stage) {
-        kl.fetch(lds + stage * STAGE, a.dim, [&](int map, int r) { return key0 + r < mask.length ? kb + map * a.k.s1 + (key0 + r) * a.k.s2 : nullptr; });
-        vl.fetch(lds + stage * STAGE + KL::BYTES, a.vdim, [&](int, int r) { return key0 + r < mask.length ? vb + (key0 + r) * a.v.s2 : nullptr; });
+        if (ALIGNED && key0 + BK <= mask.length && a.dim == DP && a.vdim == VP) {
+            kl.fetch_whole(lds0 + stage * STAGE, kb + key0 * a.k.s2, a.k.s2, a.k.s1);
+            vl.fetch_whole(lds0 + stage * STAGE + KL::BYTES, vb + key0 * a.v.s2, a.v.s2, 0);
+            return;
+        }
+        kl.fetch(lds0 + stage * STAGE, a.dim, [&](int map, int r) { return key0 + r < mask.length ? kb + map * a.k.s1 + (key0 + r) * a.k.s2 : nullptr; });
+        vl.fetch(lds0 + stage * STAGE + KL::BYTES, a.vdim, [&](int, int r) { return key0 + r < mask.length ? vb + (key0 + r) * a.v.s2 : nullptr; });
     };
-    if (end > 0) fetch(0, 0);
+    if (begin < end) fetch(begin, 0);
 
     u32x4 qf[2][NQ][GD], yf[NQ][GV];
     int limit[NQ];
-    float base[2][NQ], dot[2][NQ], lam[NQ], unit[NQ], share[NQ];      // lse in units of log2; D; of the row
+    float base[2][NQ], dot[2][NQ], lam[NQ], unit[NQ];                 // lse in units of log2; D; of the row
+    float share[NQ], rest[NQ];           // of lambda's gradient; what rounding left of it
     const float c = a.scale * kLog2e;
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
@@ -62,7 +73,7 @@ __global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
         const RowAt row(a, kvh, min(r, a.rows - 1));
         limit[n] = mask.limit(row.query);
         lam[n] = a.lam[row.head];
-        unit[n] = 1.f, share[n] = 0.f;
+        unit[n] = 1.f, share[n] = rest[n] = 0.f;
 #pragma unroll
         for (int m = 0; m < 2; m++) load_fragments<T, DP>(qf[m][n], row.at(a.q, b, 2, m), a.dim, lane);
         load_fragments<T, VP>(yf[n], row.at(a.dy, b, 1, 0), a.vdim, lane);
@@ -89,7 +100,7 @@ __global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
         for (int m = 0; m < 2; m++) {
             const long long at = row.stat(a, b, m);
             base[m][n] = fmaf(a.lse[at], kLog2e, -kShift<T>);
-            if (lane < 16 && r < a.rows) a.dots[at] = dot[m][n];
+            if (lane < 16 && r < a.rows && part == 0) a.dots[at] = dot[m][n];
         }
         if constexpr (std::is_same_v<T, f16>) {
             unit[n] = range_scale(a, most, lam[n]);
@@ -99,14 +110,15 @@ __global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
     f32x4 acc[2][NQ][ND] = {};
     constexpr int KS = KG;
     int stage = 0;
-    for (int key0 = 0; key0 < end; key0 += BK) {
+    for (int key0 = begin; key0 < end; key0 += BK) {
         kl.settle(lds + stage * STAGE);
         vl.settle(lds + stage * STAGE + KL::BYTES);
         arrived<ALIGNED>();
         if (key0 + BK < end) fetch(key0 + BK, stage ^ 1);
         const char *ks = lds + stage * STAGE, *vs = ks + KL::BYTES;
-        const bool whole = key0 + BK <= least;
-#pragma unroll
+        const bool whole = key0 + BK <= least && key0 + BK <= end;
+        float sum[NQ] = {};
+#pragma unroll 1
         for (int k0 = 0; k0 < BK; k0 += KS) {
             f32x4 z[2][NQ][KS / 16], dp[NQ][KS / 16];
 #pragma unroll
@@ -128,10 +140,11 @@ __global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
                     for (int n = 0; n < NQ; n++) dp[n][t] = mma(vf, yf[n][g], dp[n][t], T{});
                 }
             }
+            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
             u32x4 ds[2][NQ];
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
-                const int left = whole ? KS : limit[n] - (key0 + k0 + lane / 16 * 4);
+                const int left = whole ? KS : min(limit[n], end) - (key0 + k0 + lane / 16 * 4);
 #pragma unroll
                 for (int t = 0; t < KS / 16; t++)
 #pragma unroll
@@ -142,13 +155,14 @@ __global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
                             p2 = t * 16 + e < left ? p2 : 0.f;
                         }
                         const float d = dp[n][t][e];
-                        share[n] = fmaf(p2, d, share[n]);
+                        sum[n] = fmaf(p2, d, sum[n]);
                         z[0][n][t][e] = p1 * fmaf(d, unit[n], -dot[0][n]);
                         z[1][n][t][e] = p2 * -lam[n] * fmaf(d, unit[n], -dot[1][n]);
                     }
 #pragma unroll
                 for (int m = 0; m < 2; m++) ds[m][n] = chunk_of<T>(z[m][n]);
             }
+            if constexpr (DP <= 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
@@ -158,47 +172,71 @@ __global__ __launch_bounds__(256) void diff_dq_kernel(DiffArgs a) {
                     for (int n = 0; n < NQ; n++) acc[m][n][i] = mma(kf, ds[m][n], acc[m][n][i], T{});
                 }
         }
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {   // dlambda is a sum of both signs over rows and keys: a tile's share is added without loss
+            const float y = sum[n] - rest[n], up = share[n] + y;
+            rest[n] = (up - share[n]) - y;
+            share[n] = up;
+        }
         stage ^= 1;
     }
+    // lambda's shares of the tile's rows, added up by head.
+    __syncthreads();
+    float* shares = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int at = (wave * NQ + n) * 16 + s;
+        const float sum = column_sum(share[n]);
+        if (lane < 16) shares[at] = r0 + at < a.rows ? sum * __builtin_amdgcn_exp2f(-kShift<T>) : 0.f;
+    }
+    __syncthreads();
+    for (int g = tid; g < a.group; g += NT) {
+        double sum = 0.0;
+        for (int at = (g + a.group - r0 % a.group) % a.group; at < ROWS; at += a.group) sum += (double)shares[at];
+        a.tiles_lam[((long long)blockIdx.x) * a.group + g] = sum;
+    }
+    if (!a.dq.p) return;
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int r = r0 + (wave * NQ + n) * 16 + s;
-        const float sum = column_sum(share[n]);
         if (r >= a.rows) continue;
         const RowAt row(a, kvh, r);
-        if (lane < 16) a.rows_lam[((long long)b * a.heads + row.head) * a.queries + row.query] = sum * __builtin_amdgcn_exp2f(-kShift<T>);
-        if (!a.dq.p) continue;
         const float f = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / unit[n];
+        float* to = a.part ? a.part + (((long long)part * (gridDim.x / a.tile_div.d) + per) * a.rows + r) * (2 * DP) : nullptr;
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             char* out = const_cast<char*>(row.at(a.dq, b, 2, m));
 #pragma unroll
             for (int i = 0; i < ND; i++) {
                 const int at = i * 16 + lane / 16 * 4;
-                float o[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = acc[m][n][i][e] * f;
-                store4<T>(out + at * sizeof(T), a.dim - at, o);
+                const f32x4 v = acc[m][n][i] * f;
+                if (to) {
+                    *reinterpret_cast<f32x4*>(to + m * DP + at) = v;
+                } else {
+                    const float o[4] = {v[0], v[1], v[2], v[3]};
+                    store4<T>(out + at * sizeof(T), a.dim - at, o);
+                }
             }
         }
     }
 }
 
-// Rows of a tile, and what the kernel takes of each: both maps' lse, D, -lambda, and the keys that it sees.
+// Rows of a tile (of one head), and what the kernel takes of each: both maps' lse and D, and the keys that it sees.
 constexpr int kRows = 32;
 struct RowStats {
-    float base[2][kRows], dot[2][kRows], lam[kRows];
+    float base[2][kRows], dot[2][kRows];
     int limit[kRows];
 };
 
 template <class T, int DP, int VP, int NK, bool ALIGNED>
-__global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_dkv_kernel(DiffArgs a) {
     constexpr int NT = 256, RG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, NV = VP / 16, KEYS = 64 * NK;
     using QL = Loader<T, DP, kRows, 2, NT, ALIGNED>;
     using YL = Loader<T, VP, kRows, 1, NT, ALIGNED>;
     constexpr int STAGE = QL::BYTES + YL::BYTES;
     __shared__ __align__(128) char lds[2 * STAGE];
     __shared__ RowStats stats[2];
+    const unsigned lds0 = lds_address(lds);
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, s = lane % 16;
     const unsigned per = a.tile_div.div(blockIdx.x);
@@ -206,32 +244,41 @@ __global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
     const int b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
     const Mask mask(a, b);
     const int key0 = tile * KEYS, key_end = min(key0 + KEYS, a.keys);
-    // Rows from the first that sees a key of the tile on, in parts of whole tiles.
-    const int first = key0 >= mask.length ? a.rows : !a.causal ? 0 : (int)min((long long)a.rows, max(0LL, key0 - mask.start) * a.group);
-    const int each = ((a.rows - first + kRows - 1) / kRows + a.splits - 1) / a.splits * kRows;
-    const int begin = (int)min((long long)first + (long long)part * each, (long long)a.rows), end = (int)min((long long)begin + each, (long long)a.rows);
+    // Of each head that shares the key head, the tiles from the first query that sees a key of this one on; in parts.
+    const int first = key0 >= mask.length ? a.queries : !a.causal ? 0 : (int)min((long long)a.queries, max(0LL, key0 - mask.start));
+    const int tiles = (a.queries - first + kRows - 1) / kRows;
+    const long long all = (long long)tiles * a.group, each = (all + a.splits - 1) / a.splits;
+    const long long begin = min(part * each, all), end = min(begin + each, all);
     QL ql;
     YL yl;
-    float held[6];                       // a row's stats on their way
+    ql.space(a.q.s2, a.q.s1);
+    yl.space(a.dy.s2, 0);
+    float held[5];                       // a row's stats on their way
     float unit = 1.f;
     if constexpr (std::is_same_v<T, f16>) {
         float lam = 0.f;
         for (int g = 0; g < a.group; g++) lam = fmaxf(lam, fabsf(a.lam[kvh * a.group + g]));
         unit = range_scale(a, __uint_as_float(a.most[1]), lam);
     }
-    auto fetch = [&](int r0, int stage) {
-        ql.fetch(lds + stage * STAGE, a.dim, [&](int map, int r) -> const char* { return r0 + r < end ? RowAt(a, kvh, r0 + r).at(a.q, b, 2, map) : nullptr; });
-        yl.fetch(lds + stage * STAGE + QL::BYTES, a.vdim, [&](int, int r) -> const char* { return r0 + r < end ? RowAt(a, kvh, r0 + r).at(a.dy, b, 1, 0) : nullptr; });
+    auto fetch = [&](int head, int i0, int stage) {
+        const char* q = a.q.p + 2LL * head * a.q.s1 + i0 * a.q.s2 + b * a.q.s3;
+        const char* y = a.dy.p + (long long)head * a.dy.s1 + i0 * a.dy.s2 + b * a.dy.s3;
+        if (ALIGNED && i0 + kRows <= a.queries && a.dim == DP && a.vdim == VP) {
+            ql.fetch_whole(lds0 + stage * STAGE, q, a.q.s2, a.q.s1);
+            yl.fetch_whole(lds0 + stage * STAGE + QL::BYTES, y, a.dy.s2, 0);
+        } else {
+            ql.fetch(lds0 + stage * STAGE, a.dim, [&](int map, int r) { return i0 + r < a.queries ? q + map * a.q.s1 + r * a.q.s2 : nullptr; });
+            yl.fetch(lds0 + stage * STAGE + QL::BYTES, a.vdim, [&](int, int r) { return i0 + r < a.queries ? y + r * a.dy.s2 : nullptr; });
+        }
         if (tid < kRows) {
-            const RowAt row(a, kvh, min(r0 + tid, a.rows - 1));
+            const int i = min(i0 + tid, a.queries - 1);
+            const long long at = ((long long)b * a.heads + head) * 2 * a.queries + i;
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                const long long at = row.stat(a, b, m);
-                held[m] = fmaf(a.lse[at], kLog2e, -kShift<T>);
-                held[2 + m] = a.dots[at] * unit;
+                held[m] = fmaf(a.lse[at + m * a.queries], kLog2e, -kShift<T>);
+                held[2 + m] = a.dots[at + m * a.queries] * unit;
             }
-            held[4] = -a.lam[row.head];
-            held[5] = __int_as_float(r0 + tid < end ? mask.limit(row.query) : 0);
+            held[4] = __int_as_float(i0 + tid < a.queries ? mask.limit(i) : 0);
         }
     };
     auto settle = [&](int stage) {
@@ -240,12 +287,17 @@ __global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
         if (tid < kRows) {
             RowStats& st = stats[stage];
             st.base[0][tid] = held[0], st.base[1][tid] = held[1], st.dot[0][tid] = held[2], st.dot[1][tid] = held[3];
-            st.lam[tid] = held[4];
-            st.limit[tid] = __float_as_int(held[5]);
+            st.limit[tid] = __float_as_int(held[4]);
         }
         arrived<ALIGNED>();
     };
-    if (begin < end) fetch(begin, 0);
+    // The next tile: of the same head, or the next head's first.
+    int head = kvh * a.group + (tiles ? (int)(begin / tiles) : 0), i0 = first + (tiles ? (int)(begin % tiles) : 0) * kRows;
+    auto step = [&](int& head, int& i0) {
+        i0 += kRows;
+        if (i0 >= a.queries) head++, i0 = first;
+    };
+    if (begin < end) fetch(head, i0, 0);
 
     u32x4 kf[2][NK][GD], vf[NK][GV];
 #pragma unroll
@@ -259,14 +311,15 @@ __global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
     f32x4 dk[2][NK][ND] = {}, dv[NK][NV] = {};
     const float c = a.scale * kLog2e;
     int stage = 0;
-    for (int r0 = begin; r0 < end; r0 += kRows) {
+    for (long long t = begin; t < end; t++) {
         settle(stage);
-        if (r0 + kRows < end) fetch(r0 + kRows, stage ^ 1);
+        const float lam = -a.lam[head];
+        const bool whole = i0 + kRows <= a.queries && mask.limit(i0) >= key_end && key0 + KEYS <= a.keys;   // limits never fall
+        step(head, i0);
+        if (t + 1 < end) fetch(head, i0, stage ^ 1);
         const char *qs = lds + stage * STAGE, *ys = qs + QL::BYTES;
         const RowStats& st = stats[stage];
-        // limits never fall, and rows past the end see nothing
-        const bool whole = r0 + kRows <= end && __builtin_amdgcn_readfirstlane(st.limit[0]) >= key_end && key0 + KEYS <= a.keys;
-#pragma unroll
+#pragma unroll 1
         for (int k0 = 0; k0 < kRows; k0 += RG) {
             f32x4 z[2][NK][RG / 16], dp[NK][RG / 16];
 #pragma unroll
@@ -288,6 +341,7 @@ __global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
                     for (int n = 0; n < NK; n++) dp[n][t] = mma(yf, vf[n][g], dp[n][t], T{});
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             u32x4 mix[NK], ds[2][NK];
             f32x4 pm[NK][RG / 16];
 #pragma unroll
@@ -295,13 +349,12 @@ __global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
                 const int at = k0 + t * 16 + lane / 16 * 4;
                 const f32x4 base1 = *reinterpret_cast<const f32x4*>(&st.base[0][at]), base2 = *reinterpret_cast<const f32x4*>(&st.base[1][at]);
                 const f32x4 dot1 = *reinterpret_cast<const f32x4*>(&st.dot[0][at]), dot2 = *reinterpret_cast<const f32x4*>(&st.dot[1][at]);
-                const f32x4 lam = *reinterpret_cast<const f32x4*>(&st.lam[at]);
 #pragma unroll
                 for (int n = 0; n < NK; n++) {
                     const int key = key0 + (wave * NK + n) * 16 + s;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        float p1 = __builtin_amdgcn_exp2f(fmaf(z[0][n][t][e], c, -base1[e])), p2 = lam[e] * __builtin_amdgcn_exp2f(fmaf(z[1][n][t][e], c, -base2[e]));
+                        float p1 = __builtin_amdgcn_exp2f(fmaf(z[0][n][t][e], c, -base1[e])), p2 = lam * __builtin_amdgcn_exp2f(fmaf(z[1][n][t][e], c, -base2[e]));
                         if (!whole) {
                             const bool in = key < st.limit[at + e];
                             p1 = in ? p1 : 0.f;
@@ -363,43 +416,44 @@ __global__ __launch_bounds__(256) void diff_dkv_kernel(DiffArgs a) {
     }
 }
 
-// Sums of the parts of the rows, in order, for a key: four elements a thread.
-template <class T>
-__global__ __launch_bounds__(256) void diff_fold_kernel(DiffArgs a, int dp, int vp, long long keys) {
-    const int width = 2 * dp + vp, quads = width / 4;
-    const long long e = blockIdx.x * 256LL + threadIdx.x, index = e / quads;   // of (sequence, key head), key
-    if (index >= keys) return;
+// Sums of the parts, in order: of a row's dq, or (KEYS) of a key's dk and dv; four elements a thread.
+template <class T, bool KEYS>
+__global__ __launch_bounds__(256) void diff_fold_kernel(DiffArgs a, int dp, int vp, long long all) {
+    const int width = KEYS ? 2 * dp + vp : 2 * dp, quads = width / 4, each = KEYS ? a.keys : a.rows;
+    const long long e = blockIdx.x * 256LL + threadIdx.x, index = e / quads;   // of (sequence, key head), row or key
+    if (index >= all) return;
     const int at = (int)(e - index * quads) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = 0; i < a.splits; i++) v += *reinterpret_cast<const f32x4*>(a.part + (i * keys + index) * width + at);
-    const unsigned per = (unsigned)(index / a.keys);
-    const int key = (int)(index - (long long)per * a.keys), b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
+    for (int i = 0; i < a.splits; i++) v += *reinterpret_cast<const f32x4*>(a.part + (i * all + index) * width + at);
+    const unsigned per = (unsigned)(index / each);
+    const int at_row = (int)(index - (long long)per * each), b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
     const int m = at < dp ? 0 : at < 2 * dp ? 1 : 2, col = at - m * dp;
-    const Strided& d = m < 2 ? a.dk : a.dv;
-    if (!d.p) return;
     const float o[4] = {v[0], v[1], v[2], v[3]};
-    char* out = const_cast<char*>(d.p) + (m < 2 ? 2LL * kvh + m : (long long)kvh) * d.s1 + key * d.s2 + b * d.s3;
-    store4<T>(out + col * (long long)sizeof(T), (m < 2 ? a.dim : a.vdim) - col, o);
+    if constexpr (KEYS) {
+        const Strided& d = m < 2 ? a.dk : a.dv;
+        char* out = const_cast<char*>(d.p) + (m < 2 ? 2LL * kvh + m : (long long)kvh) * d.s1 + at_row * d.s2 + b * d.s3;
+        store4<T>(out + col * (long long)sizeof(T), (m < 2 ? a.dim : a.vdim) - col, o);
+    } else {
+        store4<T>(const_cast<char*>(RowAt(a, kvh, at_row).at(a.dq, b, 2, m)) + col * (long long)sizeof(T), a.dim - col, o);
+    }
 }
 
-// lambda's gradient: less the sum of its head's rows.
-__global__ __launch_bounds__(1024) void diff_lambda_kernel(const float* rows, long long batch, int heads, int queries, float* dlam) {
-    __shared__ double red[16];
-    const int h = blockIdx.x;
+// lambda's gradient: less the sum of its head's shares, which lie [sequence][key head][tile and part][group].
+__global__ __launch_bounds__(256) void diff_lambda_kernel(const double* shares, long long batch, int kv_heads, int group, int tiles, float* dlam) {
+    __shared__ double red[4];
+    const int kvh = blockIdx.x / group, g = blockIdx.x % group;
     double s = 0.0;
-    const long long n = batch * queries;
+    const long long n = batch * tiles;
 #pragma unroll 4
-    for (long long i = threadIdx.x; i < n; i += 1024) {
-        const long long b = i / queries;
-        s += (double)rows[(b * heads + h) * queries + (i - b * queries)];
+    for (long long i = threadIdx.x; i < n; i += 256) {
+        const long long b = i / tiles;
+        s += shares[((b * kv_heads + kvh) * tiles + (i - b * tiles)) * group + g];
     }
     s = lane_sum<64>(s);
     if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = s;
     __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < 16; i++) s += red[i];
-    dlam[h] = (float)-s;
+    if (threadIdx.x == 0) dlam[blockIdx.x] = (float)-((red[0] + red[1]) + (red[2] + red[3]));
 }
 
 // fp16: the largest |v| and |dy| of the call, as bits (0 before it; the order of maxima does not matter).
@@ -430,11 +484,11 @@ __global__ __launch_bounds__(256) void diff_most_kernel(MostArgs a) {
 constexpr int kCus = 256;
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 struct BackPlan {
-    int nq, nk, dp, vp, splits;
+    int nq, nk, dp, vp, q_splits, k_splits;
     long long q_tiles, k_tiles;
-    size_t dots, rows_lam, most, part, total;
+    size_t dots, tiles_lam, most, part, total;
 };
-BackPlan back_plan(const DiffShape& s, int size) {
+BackPlan back_plan(const DiffShape& s, int size, bool causal) {
     BackPlan p{};
     const long long group = s.H / s.Hk, rows = s.M * group, pairs = s.B * s.Hk;
     const bool small = s.D <= 64 && s.V <= 128 && size == 2;
@@ -443,17 +497,22 @@ BackPlan back_plan(const DiffShape& s, int size) {
     p.nk = 1;
     p.q_tiles = (rows + 64 * p.nq - 1) / (64 * p.nq);
     p.k_tiles = (s.N + 64 * p.nk - 1) / (64 * p.nk);
-    // Parts of the rows: as many as give two blocks a CU, of 8 tiles at least.
-    p.splits = (int)std::max(1LL, std::min({2LL * kCus / std::max(1LL, p.k_tiles * pairs), rows / (8 * kRows), 64LL}));
+    // Parts of the keys or rows: as many as give two blocks a CU, or eight where causality makes tiles differ in length,
+    // of 256 keys or rows at least.
+    const long long want = (causal ? 8LL : 4LL) * kCus;
+    p.q_splits = (int)std::max(1LL, std::min({2LL * kCus / std::max(1LL, p.q_tiles * pairs), s.N / 256, 64LL}));
+    p.k_splits = (int)std::max(1LL, std::min({want / std::max(1LL, p.k_tiles * pairs), rows / 256, 64LL}));
     auto take = [&](size_t bytes) {
         const size_t at = p.total;
         p.total += pad256(bytes);
         return at;
     };
     p.dots = take((size_t)s.B * s.H * 2 * s.M * sizeof(float));
-    p.rows_lam = take((size_t)s.B * s.H * s.M * sizeof(float));
+    p.tiles_lam = take((size_t)((rows + 63) / 64) * p.q_splits * s.B * s.H * sizeof(double));   // of the smallest tiles
     p.most = take(2 * sizeof(unsigned));
-    p.part = take(p.splits > 1 ? (size_t)p.splits * pairs * s.N * (2 * p.dp + p.vp) * sizeof(float) : 0);
+    const size_t q_part = p.q_splits > 1 ? (size_t)p.q_splits * pairs * rows * 2 * p.dp : 0;
+    const size_t k_part = p.k_splits > 1 ? (size_t)p.k_splits * pairs * s.N * (2 * p.dp + p.vp) : 0;
+    p.part = take(std::max(q_part, k_part) * sizeof(float));         // one after the other
     return p;
 }
 
@@ -493,7 +552,7 @@ STX_API size_t stx_diff_attention_back_workspace_size(const stx_tensor* q, const
             for (int i = 0; i < 4; i++) STX_REQUIRE(t->ne[i] >= 0, "%s: negative ne[%d]", op, i);
         }
         const DiffShape s = diff_shape(q, k, v, op);
-        if (s.B > 0 && s.H > 0) bytes = back_plan(s, size).total;
+        if (s.B > 0 && s.H > 0) bytes = std::max(back_plan(s, size, false).total, back_plan(s, size, true).total);
     });
     return bytes;
 }
@@ -522,12 +581,12 @@ STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tenso
         check_scale(scale, op);
         if (s.B == 0 || s.H == 0) {
             if (dlambda && s.H > 0) {
-                hipLaunchKernelGGL(diff_lambda_kernel, dim3(s.H), dim3(1024), 0, as_stream(stream), nullptr, 0, s.H, 1, dlambda);
+                hipLaunchKernelGGL(diff_lambda_kernel, dim3(s.H), dim3(256), 0, as_stream(stream), nullptr, 0, 1, s.H, 1, dlambda);
                 launch_check("diff_lambda_kernel");
             }
             return;
         }
-        BackPlan p = back_plan(s, size);
+        BackPlan p = back_plan(s, size, causal != 0);
         check_workspace(workspace, workspace_bytes, p.total, op);
         const size_t per = (size_t)s.B * sizeof(int32_t), kept = (size_t)s.B * s.H * 2 * s.M * sizeof(float), heads = s.H * sizeof(float);
         check_apart(op, {{"dq", dq, size}, {"dk", dk, size}, {"dv", dv, size}, {"dlambda", dlambda, heads}, {"the workspace", workspace, p.total}},
@@ -541,16 +600,15 @@ STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tenso
         a.lse = const_cast<float*>(lse);
         char* ws = static_cast<char*>(workspace);
         a.dots = reinterpret_cast<float*>(ws + p.dots);
-        a.rows_lam = reinterpret_cast<float*>(ws + p.rows_lam);
+        a.tiles_lam = reinterpret_cast<double*>(ws + p.tiles_lam);
         unsigned* most = reinterpret_cast<unsigned*>(ws + p.most);
         a.most = most;
         const hipStream_t st = as_stream(stream);
         const long long pairs = s.B * s.Hk;
         const bool keys_aligned = rows_in_chunks(k, size) && rows_in_chunks(v, size), rows_aligned = rows_in_chunks(q, size) && rows_in_chunks(dy, size);
         if (!keys_aligned && p.nq > 1) p.nq = 1, p.q_tiles = (a.rows + 63) / 64;
-        STX_REQUIRE(p.q_tiles * pairs < (1LL << 22) && p.k_tiles * p.splits * pairs < (1LL << 22), "%s: too many tiles", op);
-        const long long quads = pairs * s.N * ((2 * p.dp + p.vp) / 4);
-        STX_REQUIRE(quads / 256 < (1LL << 23), "%s: k and v too large", op);
+        STX_REQUIRE(p.q_tiles * p.q_splits * pairs < (1LL << 22) && p.k_tiles * p.k_splits * pairs < (1LL << 22), "%s: too many tiles", op);
+        auto fold_blocks = [&](long long quads) { return dim3((unsigned)((quads + 255) / 256)); };   // split calls have few tiles
         with_type(type, [&](auto t) {
             using T = decltype(t);
             with_dims(s.D, s.V, [&](auto d, auto vd) {
@@ -569,25 +627,31 @@ STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tenso
                     hipLaunchKernelGGL(diff_most_kernel, dim3((unsigned)blocks, 2), dim3(256), 0, st, m);
                     launch_check("diff_most_kernel");
                 }
+                float* part = reinterpret_cast<float*>(ws + p.part);
                 if (s.M > 0) {
-                    a.tiles = (int)p.q_tiles;
-                    a.tile_div = FastDiv((unsigned)p.q_tiles);
-                    launch_dq<T, d(), vd()>(a, p, keys_aligned, (unsigned)(p.q_tiles * pairs), st);
+                    a.tiles = (int)p.q_tiles, a.splits = p.q_splits;
+                    a.tile_div = FastDiv((unsigned)(p.q_tiles * p.q_splits));
+                    a.part = p.q_splits > 1 ? part : nullptr;
+                    launch_dq<T, d(), vd()>(a, p, keys_aligned, (unsigned)(p.q_tiles * p.q_splits * pairs), st);
+                    if (dq && a.part) {
+                        hipLaunchKernelGGL((diff_fold_kernel<T, false>), fold_blocks(pairs * a.rows * (p.dp / 2)), dim3(256), 0, st, a, p.dp, p.vp, pairs * a.rows);
+                        launch_check("diff_fold_kernel");
+                    }
                 }
                 if (dk && s.N > 0) {
-                    a.tiles = (int)p.k_tiles, a.splits = p.splits;
-                    a.tile_div = FastDiv((unsigned)(p.k_tiles * p.splits));
-                    a.part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.part) : nullptr;
-                    launch_dkv<T, d(), vd()>(a, rows_aligned, (unsigned)(p.k_tiles * p.splits * pairs), st);
-                    if (p.splits > 1) {
-                        hipLaunchKernelGGL((diff_fold_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a, p.dp, p.vp, pairs * s.N);
+                    a.tiles = (int)p.k_tiles, a.splits = p.k_splits;
+                    a.tile_div = FastDiv((unsigned)(p.k_tiles * p.k_splits));
+                    a.part = p.k_splits > 1 ? part : nullptr;
+                    launch_dkv<T, d(), vd()>(a, rows_aligned, (unsigned)(p.k_tiles * p.k_splits * pairs), st);
+                    if (a.part) {
+                        hipLaunchKernelGGL((diff_fold_kernel<T, true>), fold_blocks(pairs * s.N * ((2 * p.dp + p.vp) / 4)), dim3(256), 0, st, a, p.dp, p.vp, pairs * s.N);
                         launch_check("diff_fold_kernel");
                     }
                 }
             });
         });
         if (dlambda) {
-            hipLaunchKernelGGL(diff_lambda_kernel, dim3(s.H), dim3(1024), 0, st, a.rows_lam, s.M > 0 ? s.B : 0, s.H, std::max(1, a.queries), dlambda);
+            hipLaunchKernelGGL(diff_lambda_kernel, dim3(s.H), dim3(256), 0, st, a.tiles_lam, s.M > 0 ? s.B : 0, s.Hk, a.group, (int)std::max(1LL, p.q_tiles * p.q_splits), dlambda);
             launch_check("diff_lambda_kernel");
         }
     });
