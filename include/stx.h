@@ -928,13 +928,13 @@ typedef struct {
  * taken as 0 .. keys (NULL: all); starts: device int32[batch], the position of its first query (NULL: 0). Masked scores
  * are not read into the result whatever they hold, NaN among it, and get zeros; a row that sees no key, or only scores of
  * -infinity, is zeros. Sums are float. Rows are contiguous; any other strides. dst may be x, and overlaps nothing else. Fewer than 2^30 keys and
- * queries, 2^24 heads and sequences. */
+ * queries, at most 65,535 heads and 2^24 - 1 sequences. */
 STX_API stx_status stx_soft_max_rel(const stx_tensor* x, stx_type type, const float* table,
                                     const stx_rel_params* params, float scale, const int32_t* lengths,
                                     const int32_t* starts, const stx_tensor* dst, stx_stream stream);
 /* Its gradients, from dy (of dst), y (dst as the forward call left it) and the same masks: dx (of x) and dtable (device
  * float [n_buckets][heads], summed over the batch); either may be NULL. Row dots and the table's sums are formed in
- * double. dx overlaps no input. At most 65,535 heads. workspace: device, 256-byte aligned, no initialisation; calls that share one must not
+ * double. dx overlaps no input. workspace: device, 256-byte aligned, no initialisation; calls that share one must not
  * overlap. None is needed without dtable. */
 STX_API size_t     stx_soft_max_rel_back_workspace_size(const stx_tensor* y, stx_type type, int n_buckets);
 STX_API stx_status stx_soft_max_rel_back(const stx_tensor* dy, const stx_tensor* y, stx_type type,

@@ -15,7 +15,10 @@ namespace {
 // before the first is stored: outputs may be inputs. A lane whose pair partner lies in another unit
 // (mode 2, or units of one element) loads it too, from the same lines: units stay dense for any
 // n_dims, where units of a pair of halves would leave 6 of 16 lanes idle at 128 elements, 96 rotated.
-// Sums of squares and of g x are held in double: data whose squares leave fp32 keeps its norm.
+// A lane's squares and products g x are added in float, by halves (three roundings at V 8), the lanes' in double; a wave that
+// meets a row whose squares leave fp32 forms them again in double, so data of any size keeps its norm. (In
+// double throughout, with a double division and root, these took more time than the memory's: the gradient of 2 x
+// 16,384 tokens of 40 rows of 128 bf16 values 297 us.)
 struct QkSide {
     const char *x, *dy;
     char* out;
@@ -26,11 +29,10 @@ struct QkSide {
 struct QkArgs {
     QkSide q, k;
     RopeAngles at;
-    double eps;
+    double eps, per_dim;                 // per_dim: 1 / dim
     unsigned tokens, tile;               // all tokens, and of a block
     unsigned base;                       // blocks of the launches before this one
-    FastDiv rows;                        // rows of a token: q's, then k's
-    unsigned q_rows;
+    FastDiv q_rows, k_rows;              // rows of a token
     int dim, units, log_lanes, mode;
     int w_stride;                        // from a head's weights to the next's: dim, or 0 where heads share them
     float* part;                         // backward: sums of dz x r, [block][2 or rows][dim], or NULL
@@ -39,23 +41,38 @@ struct QkArgs {
 constexpr int kQkThreads = 256;
 constexpr int kQkDim = 1024;             // of a row: 64 lanes x 16 elements
 
-template <class T, int V>
-struct Row {
-    const QkSide* side;
-    unsigned h;                          // of the side
-    bool is_k;
-    long long i2, i3;
-    __device__ __forceinline__ Row(const QkArgs& a, unsigned t, unsigned row) {
-        const unsigned b = a.at.n.div(t);
-        i3 = b;
-        i2 = t - b * a.at.n.d;
-        is_k = row >= a.q_rows;
-        side = is_k ? &a.k : &a.q;
-        h = is_k ? row - a.q_rows : row;
+// A tensor's rows as a group of lanes goes over them, `heads` and `tokens` a step: pointers move by what is uniform over the
+// launch, without a product an address (kernels that formed each row's addresses, and chose q's or k's strides by lane, ran
+// 62 vector instructions an element, and as long as those took).
+template <class P>
+struct Walk {
+    P* p;
+    long long step, carry, wrap;         // a step; a head past the last one, which is the next token; a token past the last
+    __device__ __forceinline__ Walk(P* base, long long s1, long long s2, long long s3, unsigned h, unsigned i2, unsigned b, unsigned heads, unsigned tokens,
+                                    unsigned rows, unsigned n)
+        : p(base + h * s1 + i2 * s2 + b * s3), step(heads * s1 + tokens * s2), carry(s2 - rows * s1), wrap(s3 - n * s2) {}
+};
+// Where a group is: its head, and its token in the sequence and in the block.
+struct Spot {
+    unsigned h, i2, b, tk;
+    __device__ __forceinline__ Spot(const QkArgs& a, unsigned t0, unsigned tk, unsigned h) : h(h), tk(tk) {
+        b = a.at.n.div(t0 + tk);
+        i2 = t0 + tk - b * a.at.n.d;
     }
-    __device__ __forceinline__ const T* x() const { return reinterpret_cast<const T*>(side->x + h * side->x1 + i2 * side->x2 + i3 * side->x3); }
-    __device__ __forceinline__ const T* dy() const { return reinterpret_cast<const T*>(side->dy + h * side->y1 + i2 * side->y2 + i3 * side->y3); }
-    __device__ __forceinline__ T* out() const { return reinterpret_cast<T*>(side->out + h * side->o1 + i2 * side->o2 + i3 * side->o3); }
+    template <class... W>
+    __device__ __forceinline__ void next(const QkArgs& a, unsigned rows, unsigned heads, unsigned tokens, W&... w) {
+        ((w.p += w.step), ...);
+        h += heads, i2 += tokens, tk += tokens;
+        if (h >= rows) {
+            h -= rows, i2++, tk++;
+            ((w.p += w.carry), ...);
+        }
+        if (i2 >= a.at.n.d) {
+            const unsigned turns = a.at.n.div(i2);
+            i2 -= turns * a.at.n.d;
+            ((w.p += turns * w.wrap), ...);
+        }
+    }
 };
 
 // Where the partners of unit `at` start; `at` itself where they are in the unit or there are none.
@@ -115,177 +132,246 @@ __device__ __forceinline__ void weights(const float* w, int at, float (&f)[V]) {
     }
 }
 
-template <class T, int V, int K>
-__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
-    extern __shared__ float2 cs[];       // [tile][n_dims / 2]
+// The table of a block's tokens; where they are several, from frequencies formed once, in LDS behind it (a frequency takes
+// as long as the angle's cos and sin).
+__device__ __forceinline__ void table(const QkArgs& a, unsigned t0, unsigned nt, float2* cs) {
     const int half = a.at.n_dims / 2;
-    const unsigned t0 = (a.base + blockIdx.x) * a.tile, nt = min(a.tile, a.tokens - t0);
-    rope_table<kQkThreads>(a.at, t0, nt, cs);
-    __syncthreads();
-    const int lanes = 1 << a.log_lanes, lane = threadIdx.x & (lanes - 1);
-    const unsigned total = nt * a.rows.d, groups = kQkThreads >> a.log_lanes;
-    for (unsigned first = 0; first < total; first += groups) {
-        const unsigned row = first + (threadIdx.x >> a.log_lanes), at_row = min(row, total - 1);   // every lane takes part in the sums
-        const unsigned tk = a.rows.div(at_row);
-        const Row<T, V> r(a, t0 + tk, at_row - tk * a.rows.d);
-        const T* src = r.x();
-        float x[K][V], p[K][V];
-        double sum = 0.0;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int u = lane + (k << a.log_lanes), at = u * V;
-#pragma unroll
-            for (int v = 0; v < V; v++) x[k][v] = p[k][v] = 0.f;
-            if (u >= a.units) continue;
-            take<T, V>(src + at, x[k]);
-            const int other = partner<V>(a, at);
-            if (other != at) take<T, V>(src + other, p[k]);
-#pragma unroll
-            for (int v = 0; v < V; v++) sum = fma((double)x[k][v], (double)x[k][v], sum);
-        }
-        const float rstd = (float)(1.0 / sqrt(lane_sum_dyn(sum, lanes) / a.dim + a.eps));
-        if (row >= total) continue;
-        T* out = r.out();
-        const float* w = r.side->w ? r.side->w + (long long)r.h * a.w_stride : nullptr;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int u = lane + (k << a.log_lanes), at = u * V;
-            if (u >= a.units) continue;
-            float f[V];
-            weights<V>(w, at, f);
-#pragma unroll
-            for (int v = 0; v < V; v++) x[k][v] = x[k][v] * rstd * f[v];
-            const int other = partner<V>(a, at);
-            if (other != at) {
-                weights<V>(w, other, f);
-#pragma unroll
-                for (int v = 0; v < V; v++) p[k][v] = p[k][v] * rstd * f[v];
-            }
-            rotate<V>(a, at, cs + tk * half, x[k], p[k]);
-            give<T, V>(out + at, x[k]);
-        }
+    if (a.tile > 1) {
+        double* frequency = reinterpret_cast<double*>(cs + a.tile * half);
+        for (int i = threadIdx.x; i < half; i += kQkThreads) frequency[i] = rope_frequency(a.at, i);
+        __syncthreads();
+        rope_table<kQkThreads>(a.at, t0, nt, cs, [&](int i) { return frequency[i]; });
+    } else {
+        rope_table<kQkThreads>(a.at, t0, nt, cs);
     }
+    __syncthreads();
 }
 
-// Sums over the rows of dz x r are kept by the lanes that hold the elements, over the tokens of a block:
-// where heads share weights, one for q and one for k and any row a group; where they do not (PER_HEAD),
-// a group of lanes keeps to a head, or takes its heads one after another. Added up in LDS in
-// order, and over the blocks by qk_fold_kernel.
-template <class T, int V, int K, bool PER_HEAD>
-__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a) {
-    extern __shared__ float2 cs[];       // [tile][n_dims / 2], then sums [1 or 2][groups][units * V]
-    const int half = a.at.n_dims / 2;
-    const unsigned block = a.base + blockIdx.x, t0 = block * a.tile, nt = min(a.tile, a.tokens - t0);
-    rope_table<kQkThreads>(a.at, t0, nt, cs);
-    __syncthreads();
-    const int lanes = 1 << a.log_lanes, lane = threadIdx.x & (lanes - 1);
-    const unsigned groups = kQkThreads >> a.log_lanes, group = threadIdx.x >> a.log_lanes, rows = a.rows.d;
-    float* red = reinterpret_cast<float*>(cs + a.tile * half);
-    const int width = a.units * V;
-    float acc[PER_HEAD ? 1 : 2][K][V] = {};
-    // One row: dx is written where `valid`.
-    auto row_of = [&](unsigned tk, unsigned row, bool valid) {
-        const Row<T, V> r(a, t0 + tk, row);
-        const T *src = r.x(), *dsrc = r.dy();
-        const float* w = r.side->w ? r.side->w + (long long)r.h * a.w_stride : nullptr;
-        float x[K][V], z[K][V], p[K][V], f[K][V];
-        double sxx = 0.0, sgx = 0.0;
+template <int V>
+__device__ __forceinline__ float by_halves(const float* f) {
+    if constexpr (V == 1) return f[0];
+    else return by_halves<V / 2>(f) + by_halves<V / 2>(f + V / 2);
+}
+// 1 / sqrt(m): the hardware's (1 ulp) and a Newton step, whose error is that of rounding m and the result; in double where m
+// is not a float's.
+__device__ __forceinline__ float inverse_root(double m) {
+    const float f = (float)m;
+    if (__builtin_amdgcn_ballot_w64(!(f > 1e-30f && f < 1e30f))) return (float)(1.0 / sqrt(m));
+    const float r = __builtin_amdgcn_rsqf(f), e = fmaf(-f * r, r, 1.f);
+    return fmaf(0.5f * r, e, r);
+}
+// Whether a lane's sum of squares may have left fp32 (a mean that eps outweighs may be too small).
+__device__ __forceinline__ bool outside(const QkArgs& a, float sum) {
+    return __builtin_amdgcn_ballot_w64(!(sum < 1e30f) || (sum < 1e-25f && a.eps < 1e-20));
+}
+
+// The weights of a lane's units and of their partners.
+template <int V, int K, bool PARTNERS>
+struct Weights {
+    float f[K][V], p[PARTNERS ? K : 1][V];
+    __device__ __forceinline__ void load(const QkArgs& a, const float* w, int lane) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int u = lane + (k << a.log_lanes), at = u * V;
-#pragma unroll
-            for (int v = 0; v < V; v++) x[k][v] = z[k][v] = p[k][v] = f[k][v] = 0.f;
-            if (u >= a.units) continue;
-            take<T, V>(src + at, x[k]);
-            take<T, V>(dsrc + at, z[k]);
-            const int other = partner<V>(a, at);
-            if (other != at) take<T, V>(dsrc + other, p[k]);
+            const int u = lane + (k << a.log_lanes), at = min(u, a.units - 1) * V;
             weights<V>(w, at, f[k]);
+            if constexpr (PARTNERS) weights<V>(w, partner<V>(a, at), p[k]);
         }
+    }
+};
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
+    extern __shared__ float2 cs[];       // [tile][n_dims / 2], then frequencies
+    const int half = a.at.n_dims / 2;
+    const unsigned t0 = (a.base + blockIdx.x) * a.tile, nt = min(a.tile, a.tokens - t0);
+    table(a, t0, nt, cs);
+    const int lanes = 1 << a.log_lanes, lane = threadIdx.x & (lanes - 1);
+    const unsigned groups = kQkThreads >> a.log_lanes, group = threadIdx.x >> a.log_lanes;
+    auto rows_of = [&](const QkSide& side, FastDiv rows) {
+        const unsigned heads = groups % rows.d, tokens = groups / rows.d, total = nt * rows.d;
+        const unsigned tk0 = rows.div(min(group, total - 1));
+        Spot s(a, t0, tk0, min(group, total - 1) - tk0 * rows.d);
+        Walk<const char> x(side.x, side.x1, side.x2, side.x3, s.h, s.i2, s.b, heads, tokens, rows.d, a.at.n.d);
+        Walk<char> out(side.out, side.o1, side.o2, side.o3, s.h, s.i2, s.b, heads, tokens, rows.d, a.at.n.d);
+        Weights<V, K, true> w;
+        if (a.w_stride == 0) w.load(a, side.w, lane);
+        for (unsigned row = group; row - group < total; row += groups, s.next(a, rows.d, heads, tokens, x, out)) {
+            const bool valid = row < total;                          // every lane takes part in the sums
+            float f[K][V], p[K][V], squares = 0.f;
+            const T* src = reinterpret_cast<const T*>(x.p);
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int u = lane + (k << a.log_lanes), at = u * V;
-            if (u >= a.units) continue;
-            rotate<V>(a, at, cs + tk * half, z[k], p[k]);
+            for (int k = 0; k < K; k++) {
+                const int u = lane + (k << a.log_lanes), at = u * V;
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                sxx = fma((double)x[k][v], (double)x[k][v], sxx);
-                sgx = fma((double)(f[k][v] * z[k][v]), (double)x[k][v], sgx);
+                for (int v = 0; v < V; v++) f[k][v] = p[k][v] = 0.f;
+                if (!valid || u >= a.units) continue;
+                take<T, V>(src + at, f[k]);
+                const int other = partner<V>(a, at);
+                if (other != at) take<T, V>(src + other, p[k]);
             }
-        }
-        const double r2 = 1.0 / (lane_sum_dyn(sxx, lanes) / a.dim + a.eps), rd = sqrt(r2);
-        const float rstd = (float)rd, mean = (float)(lane_sum_dyn(sgx, lanes) / a.dim * rd);
-        if (!valid) return;
-        T* out = r.side->out ? r.out() : nullptr;
+            if (a.w_stride != 0) w.load(a, side.w ? side.w + (long long)s.h * a.w_stride : nullptr, lane);
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int u = lane + (k << a.log_lanes), at = u * V;
-            if (u >= a.units) continue;
+            for (int k = 0; k < K; k++) {
+                float xx[V];
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const float xh = x[k][v] * rstd, dw = z[k][v] * xh;
-                if constexpr (PER_HEAD) {
-                    acc[0][k][v] += dw;
-                } else {
-                    acc[0][k][v] += r.is_k ? 0.f : dw;
-                    acc[1][k][v] += r.is_k ? dw : 0.f;
+                for (int v = 0; v < V; v++) xx[v] = f[k][v] * f[k][v];
+                squares += by_halves<V>(xx);
+            }
+            double sum = squares;
+            if (outside(a, squares)) {
+                sum = 0.0;
+#pragma unroll
+                for (int k = 0; k < K; k++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) sum = fma((double)f[k][v], (double)f[k][v], sum);
+            }
+            const float rstd = inverse_root(fma(lane_sum_dyn(sum, lanes), a.per_dim, a.eps));
+            if (!valid) continue;
+            T* to = reinterpret_cast<T*>(out.p);
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int u = lane + (k << a.log_lanes), at = u * V;
+                if (u >= a.units) continue;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    f[k][v] = f[k][v] * rstd * w.f[k][v];
+                    p[k][v] = p[k][v] * rstd * w.p[k][v];
                 }
-                x[k][v] = rstd * fmaf(f[k][v], z[k][v], -(xh * mean));
+                rotate<V>(a, at, cs + s.tk * half, f[k], p[k]);
+                give<T, V>(to + at, f[k]);
             }
-            if (out) give<T, V>(out + at, x[k]);
         }
     };
-    auto lay = [&](int i) {
+    if (a.q_rows.d) rows_of(a.q, a.q_rows);
+    if (a.k_rows.d) rows_of(a.k, a.k_rows);
+}
+
+// Sums over the rows of dz x r are kept by the lanes that hold the elements, over the tokens of a block, of q and then of k:
+// where heads share weights, a group takes any row; where they do not (PER_HEAD), it keeps to a head, or takes its
+// heads one after another. Added up in LDS in order, and over the blocks by qk_fold_kernel.
+template <class T, int V, int K, bool PER_HEAD>
+__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a) {
+    extern __shared__ float2 cs[];       // [tile][n_dims / 2], frequencies, then sums [groups][units * V]
+    const int half = a.at.n_dims / 2;
+    const unsigned block = a.base + blockIdx.x, t0 = block * a.tile, nt = min(a.tile, a.tokens - t0);
+    table(a, t0, nt, cs);
+    const int lanes = 1 << a.log_lanes, lane = threadIdx.x & (lanes - 1), width = a.units * V;
+    const unsigned groups = kQkThreads >> a.log_lanes, group = threadIdx.x >> a.log_lanes;
+    float* red = reinterpret_cast<float*>(cs + (a.tile + 1) * half);
+    // Rows from (tk, h) on, `heads` and `tokens` a step, `rounds` of them, those in the tile.
+    auto rows_of = [&](const QkSide& side, unsigned rows, unsigned tk0, unsigned h0, bool some, unsigned heads, unsigned tokens, unsigned rounds, float (&acc)[K][V]) {
+        Spot s(a, t0, min(tk0, nt - 1), h0);
+        Walk<const char> x(side.x, side.x1, side.x2, side.x3, s.h, s.i2, s.b, heads, tokens, rows, a.at.n.d);
+        Walk<const char> dy(side.dy, side.y1, side.y2, side.y3, s.h, s.i2, s.b, heads, tokens, rows, a.at.n.d);
+        Walk<char> out(side.out, side.o1, side.o2, side.o3, s.h, s.i2, s.b, heads, tokens, rows, a.at.n.d);
+        Weights<V, K, false> w;
+        w.load(a, side.w ? side.w + (long long)s.h * a.w_stride : nullptr, lane);
+        s.tk = tk0;
+        for (unsigned round = 0; round < rounds; round++, s.next(a, rows, heads, tokens, x, dy, out)) {
+            const bool valid = some && s.tk < nt;
+            float f[K][V], z[K][V], p[K][V], squares = 0.f, products = 0.f;
+            const T *src = reinterpret_cast<const T*>(x.p), *dsrc = reinterpret_cast<const T*>(dy.p);
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int u = lane + (k << a.log_lanes), at = u * V;
+#pragma unroll
+                for (int v = 0; v < V; v++) f[k][v] = z[k][v] = p[k][v] = 0.f;
+                if (!valid || u >= a.units) continue;
+                take<T, V>(src + at, f[k]);
+                take<T, V>(dsrc + at, z[k]);
+                const int other = partner<V>(a, at);
+                if (other != at) take<T, V>(dsrc + other, p[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int u = lane + (k << a.log_lanes), at = u * V;
+                if (valid && u < a.units) rotate<V>(a, at, cs + s.tk * half, z[k], p[k]);
+                float xx[V], gx[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    xx[v] = f[k][v] * f[k][v];
+                    p[k][v] = w.f[k][v] * z[k][v];
+                    gx[v] = p[k][v] * f[k][v];
+                }
+                squares += by_halves<V>(xx);
+                products += by_halves<V>(gx);
+            }
+            double sxx = squares, sgx = products;
+            if (outside(a, squares)) {
+                sxx = sgx = 0.0;
+#pragma unroll
+                for (int k = 0; k < K; k++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        sxx = fma((double)f[k][v], (double)f[k][v], sxx);
+                        sgx = fma((double)p[k][v], (double)f[k][v], sgx);
+                    }
+            }
+            const float rstd = inverse_root(fma(lane_sum_dyn(sxx, lanes), a.per_dim, a.eps));
+            const float mean = (float)(lane_sum_dyn(sgx, lanes) * a.per_dim * (double)rstd);
+            if (!valid) continue;
+            T* to = reinterpret_cast<T*>(out.p);
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int u = lane + (k << a.log_lanes), at = u * V;
+                if (u >= a.units) continue;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const float xh = f[k][v] * rstd;
+                    acc[k][v] = fmaf(z[k][v], xh, acc[k][v]);
+                    f[k][v] = rstd * fmaf(-xh, mean, p[k][v]);
+                }
+                if (side.out) give<T, V>(to + at, f[k]);
+            }
+        }
+    };
+    auto lay = [&](const float (&acc)[K][V]) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int u = lane + (k << a.log_lanes);
             if (u >= a.units) continue;
 #pragma unroll
-            for (int v = 0; v < V; v++) red[(i * groups + group) * width + u * V + v] = acc[i][k][v];
+            for (int v = 0; v < V; v++) red[group * width + u * V + v] = acc[k][v];
+        }
+        __syncthreads();
+    };
+    auto side_of = [&](const QkSide& side, FastDiv by, unsigned first) {       // first: its row of the sums
+        const unsigned rows = by.d;
+        if constexpr (PER_HEAD) {
+            const unsigned slices = groups >= rows ? groups / rows : 1, heads = groups >= rows ? rows : groups, slice = group / heads;
+            for (unsigned h0 = 0; h0 < rows; h0 += heads) {
+                float acc[K][V] = {};
+                const unsigned h = h0 + group % heads;
+                rows_of(side, rows, slice, min(h, rows - 1), slice < slices && h < rows, 0, slices, (nt + slices - 1) / slices, acc);
+                if (!a.part) continue;
+                lay(acc);
+                const unsigned here = min(heads, rows - h0);
+                for (unsigned e = threadIdx.x; e < here * a.dim; e += kQkThreads) {
+                    const unsigned i = e / a.dim, d = e - i * a.dim;
+                    float s = 0.f;
+                    for (unsigned j = 0; j < slices; j++) s += red[(j * heads + i) * width + d];
+                    a.part[((long long)block * (a.q_rows.d + a.k_rows.d) + first + h0 + i) * a.dim + d] = s;
+                }
+                __syncthreads();
+            }
+        } else {
+            float acc[K][V] = {};
+            const unsigned tk = by.div(group);
+            rows_of(side, rows, tk, group - tk * rows, true, groups % rows, groups / rows, (nt * rows + groups - 1) / groups, acc);
+            if (!a.part) return;
+            lay(acc);
+            for (unsigned d = threadIdx.x; d < (unsigned)a.dim; d += kQkThreads) {
+                float s = 0.f;
+                for (unsigned g = 0; g < groups; g++) s += red[g * width + d];
+                a.part[((long long)block * 2 + (first ? 1 : 0)) * a.dim + d] = s;
+            }
+            __syncthreads();
         }
     };
-    if constexpr (PER_HEAD) {
-        const unsigned slices = groups >= rows ? groups / rows : 1, heads = groups >= rows ? rows : groups;
-        const unsigned slice = group / heads;
-        for (unsigned h0 = 0; h0 < rows; h0 += heads) {
-            const unsigned h = h0 + group % heads;
-            for (unsigned tk0 = 0; tk0 < nt; tk0 += slices) {
-                const unsigned tk = tk0 + slice;
-                row_of(min(tk, nt - 1), min(h, rows - 1), tk < nt && slice < slices && h < rows);
-            }
-            if (!a.part) continue;
-            lay(0);
-            __syncthreads();
-            const unsigned here = min(heads, rows - h0);
-            for (unsigned e = threadIdx.x; e < here * a.dim; e += kQkThreads) {
-                const unsigned i = e / a.dim, d = e - i * a.dim;
-                float s = 0.f;
-                for (unsigned j = 0; j < slices; j++) s += red[(j * heads + i) * width + d];
-                a.part[((long long)block * rows + h0 + i) * a.dim + d] = s;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int v = 0; v < V; v++) acc[0][k][v] = 0.f;
-        }
-    } else {
-        const unsigned total = nt * rows;
-        for (unsigned first = 0; first < total; first += groups) {
-            const unsigned row = first + group, at_row = min(row, total - 1), tk = a.rows.div(at_row);
-            row_of(tk, at_row - tk * rows, row < total);
-        }
-        if (!a.part) return;
-        lay(0);
-        lay(1);
-        __syncthreads();
-        for (unsigned e = threadIdx.x; e < 2 * a.dim; e += kQkThreads) {
-            const unsigned i = e / a.dim, d = e - i * a.dim;
-            float s = 0.f;
-            for (unsigned g = 0; g < groups; g++) s += red[(i * groups + g) * width + d];
-            a.part[((long long)block * 2 + i) * a.dim + d] = s;
-        }
-    }
+    if (a.q_rows.d) side_of(a.q, a.q_rows, 0);
+    if (a.k_rows.d) side_of(a.k, a.k_rows, a.q_rows.d);
+    else if (!PER_HEAD && a.part)        // no rows: a sum of none
+        for (unsigned d = threadIdx.x; d < (unsigned)a.dim; d += kQkThreads) a.part[((long long)block * 2 + 1) * a.dim + d] = 0.f;
 }
 
 // The weights' gradients: column sums of part [rows][cols], 32 columns x 32 lanes a block; the first
@@ -330,6 +416,7 @@ Shape shape_of(const stx_tensor* q, const stx_tensor* k, const char* op) {
         STX_REQUIRE(k->ne[0] == dim && k->ne[2] == n && k->ne[3] == b, "%s: q and k differ in head size, tokens or batch", op);
     const Shape s{q->ne[1], k ? k->ne[1] : 0, n * b, dim};
     STX_REQUIRE(dim > 0, "%s: rows of no elements", op);
+    STX_REQUIRE(s.q_rows > 0 || s.k_rows == 0, "%s: k without heads of q", op);
     if (dim > kQkDim) fail(STX_STATUS_UNSUPPORTED, "%s: rows of %lld elements (%d at most)", op, dim, kQkDim);
     if (s.empty()) return s;
     STX_REQUIRE(n < (1LL << 31) && b < (1LL << 31) && n * b < (1LL << 31), "%s: more than 2^31 - 1 tokens", op);
@@ -354,9 +441,11 @@ QkArgs args_of(const stx_tensor* q, const Shape& s, const RopeAngles& at, const 
     a.at.pos = pos;
     a.at.n = FastDiv((unsigned)q->ne[2]);
     a.eps = eps;
+    a.per_dim = 1.0 / (double)s.dim;
     a.tokens = (unsigned)s.tokens;
-    a.rows = FastDiv((unsigned)s.rows());
-    a.q_rows = (unsigned)s.q_rows;
+    a.q_rows.d = a.k_rows.d = 0;
+    if (s.q_rows) a.q_rows = FastDiv((unsigned)s.q_rows);
+    if (s.k_rows) a.k_rows = FastDiv((unsigned)s.k_rows);
     a.dim = (int)s.dim;
     a.units = (int)(s.dim / w);
     while (a.log_lanes < 6 && (1 << a.log_lanes) < a.units) a.log_lanes++;
@@ -419,7 +508,7 @@ void qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const
     const long long round = kQkThreads >> a.log_lanes;
     const long long tile = std::max(1LL, std::min({16LL, 4 * round / s.rows(), s.tokens / 512, (long long)kRopeTable / (a.at.n_dims / 2)}));
     a.tile = (unsigned)tile;
-    const size_t lds = sizeof(float2) * tile * (a.at.n_dims / 2);
+    const size_t lds = sizeof(float2) * (tile + 1) * (a.at.n_dims / 2);
     with_type(type, [&](auto t) {
         using T = decltype(t);
         with_units<T>(w, a.units, [&](auto v, auto n) {
@@ -482,7 +571,7 @@ void qk_norm_rope_back(const stx_tensor* dyq, const stx_tensor* dyk, const stx_t
         a.tile = (unsigned)tile;
         a.part = part;
         blocks = (s.tokens + tile - 1) / tile;
-        const size_t lds = sizeof(float2) * tile * (p->n_dims / 2) + (sums ? sizeof(float) * (per_head ? 1 : 2) * (kQkThreads >> a.log_lanes) * a.units * w : 0);
+        const size_t lds = sizeof(float2) * (tile + 1) * (p->n_dims / 2) + (sums ? sizeof(float) * (kQkThreads >> a.log_lanes) * a.units * w : 0);
         with_type(type, [&](auto t) {
             using T = decltype(t);
             with_units<T>(w, a.units, [&](auto v, auto n) {

@@ -46,22 +46,30 @@ __device__ __forceinline__ void cos_sin(double theta, double& c, double& s) {
     if (quad >= 2) s = -s;
 }
 
-// cos and sin of the pairs of `nt` tokens from t0 on, by a block of THREADS: cs[token][n_dims / 2].
-template <int THREADS>
-__device__ __forceinline__ void rope_table(const RopeAngles& a, unsigned t0, unsigned nt, float2* cs) {
+// Pair i's angle a position.
+__device__ __forceinline__ double rope_frequency(const RopeAngles& a, int i) {
+    double far = exp2(-2.0 * i / a.n_dims * a.log2_base);
+    if (a.factors) far /= (double)a.factors[i];
+    const double mix = a.ext * (1.0 - fmin(1.0, fmax(0.0, ((double)i - a.lo) * a.inv_range)));
+    return a.ext != 0.0 ? a.scale * far * (1.0 - mix) + far * mix : a.scale * far;
+}
+// cos and sin of the pairs of `nt` tokens from t0 on, by a block of THREADS: cs[token][n_dims / 2]. frequency(i): pair i's.
+template <int THREADS, class F>
+__device__ __forceinline__ void rope_table(const RopeAngles& a, unsigned t0, unsigned nt, float2* cs, F&& frequency) {
     const int half = a.n_dims / 2;
     for (unsigned e = threadIdx.x; e < nt * (unsigned)half; e += THREADS) {
         const unsigned t = t0 + e / (unsigned)half;
         const int i = (int)(e % (unsigned)half);
         const unsigned i3 = a.n.div(t);
         const double p = (double)a.pos[(long long)i3 * a.pos_stride + (t - i3 * a.n.d)];
-        double far = exp2(-2.0 * i / a.n_dims * a.log2_base);
-        if (a.factors) far /= (double)a.factors[i];
-        const double mix = a.ext * (1.0 - fmin(1.0, fmax(0.0, ((double)i - a.lo) * a.inv_range)));
         double c, s;
-        cos_sin(p * (a.ext != 0.0 ? a.scale * far * (1.0 - mix) + far * mix : a.scale * far), c, s);
+        cos_sin(p * frequency(i), c, s);
         cs[e] = make_float2((float)(c * a.m), a.sign * (float)(s * a.m));
     }
+}
+template <int THREADS>
+__device__ __forceinline__ void rope_table(const RopeAngles& a, unsigned t0, unsigned nt, float2* cs) {
+    rope_table<THREADS>(a, t0, nt, cs, [&](int i) { return rope_frequency(a, i); });
 }
 
 // Checks of the parameters and positions for rows of `dim` elements; the rotation without pos and n.
