@@ -949,12 +949,13 @@ STX_API stx_status stx_soft_max_rel_back(const stx_tensor* dy, const stx_tensor*
  * heads divide H, D is at most 128 and V at most 256. lambda: device float[H]. lengths: device int32[batch], keys of each
  * sequence, taken as 0 .. keys (NULL: all); causal: query i of sequence b sees keys up to starts[b] + i (starts: device
  * int32[batch], NULL: 0). A query that sees no key gets zeros. Keys from a sequence's length on are not looked at,
- * whatever they hold; values of keys before it are finite, also where causality hides them. For the gradients, second (as dst, the second map's output, before
+ * whatever they hold; k and v before it are finite, also where causality hides them. For the gradients, second (as dst, the second map's output, before
  * lambda) and lse (device float [batch][H][2][queries], each map's ln sum exp of the scaled scores, -infinity for a query without
  * keys) receive what stx_diff_attention_back takes; NULL otherwise. Scores, sums and products are float, the maps
  * rounded to the type for their product with v (16-bit types). Rows are contiguous, other strides any; 16-byte aligned rows of k and v are
  * faster. Outputs overlap nothing else and their strides nest. workspace: device, 256-byte aligned, no initialisation (0
- * bytes where the call does not split the keys); calls that share one must not overlap. scale > 0. */
+ * bytes where the call does not split the keys); calls that share one must not overlap. scale > 0. Fewer than 2^28 queries and keys, 2^30 queries to a key head, 2^16 heads,
+ * 2^20 sequences, and 2^22 tiles: sequences * kv heads * ceil(queries * heads / kv heads / 64). */
 STX_API size_t     stx_diff_attention_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
                                                      stx_type type);
 STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v, stx_type type,
@@ -966,7 +967,7 @@ STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, 
  * sequence's length on), dlambda (device float[H]); any may be NULL. Scores are formed again; sums are float
  * (dlambda's over rows double), the maps' gradients rounded to the type for their products (16-bit types; fp16's scaled by
  * powers of two, so that they keep its range). dlambda comes from the maps themselves, not from the rounded second. The
- * same rules for masked keys, strides and workspace; outputs overlap nothing else. */
+ * same rules for masked keys, strides and workspace; dy is finite; outputs overlap nothing else. */
 STX_API size_t     stx_diff_attention_back_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
                                                           stx_type type);
 STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tensor* q, const stx_tensor* k,

@@ -218,7 +218,7 @@ struct RowAt {
         return t.p + (long long)(head * per_head + map) * t.s1 + query * t.s2 + b * t.s3;
     }
     __device__ __forceinline__ long long stat(const DiffArgs& a, int b, int map) const {
-        return ((long long)(b * a.heads + head) * 2 + map) * a.queries + query;
+        return (((long long)b * a.heads + head) * 2 + map) * a.queries + query;
     }
 };
 

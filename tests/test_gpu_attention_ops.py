@@ -687,3 +687,193 @@ def test_diff_back_strides_and_empty(device):
         kept = stx.diff_attention(q, k, v, lam, keep=True)
         got = stx.diff_attention_back(torch.ones(b, m, 2, 8, device=device), q, k, v, lam, *kept)
         assert all(bool((t == 0).all()) for t in got) and got[3].shape == (2,)
+
+
+# ----------------------------------------------------------------------- together, graphs, streams
+def attention_layer(x, w, pos, rope, lam, p, table, masks, keep):
+    """Differential attention over normed and rotated q and k, plus a pass of ordinary attention with a position bias."""
+    B, N, D = x.shape
+    H, dh = 4, 32
+    qkv = (x @ w.t()).view(B, N, 3 * H, dh)
+    q, k = stx.qk_norm_rope(qkv[:, :, :H], pos, rope, p["wq"], qkv[:, :, H:2 * H], p["wk"])
+    v = qkv[:, :, 2 * H:].reshape(B, N, H // 2, 2 * dh)
+    out, second, lse = stx.diff_attention(q, k, v, lam, keep=True, **masks)
+    score = torch.matmul(q.transpose(1, 2).float().contiguous(), k.permute(0, 2, 3, 1).float().contiguous()).to(x.dtype)
+    y = stx.soft_max_rel(score, table, p["rel"], dh ** -0.5, masks["lengths"], masks["starts"])
+    keep.update(qkv=qkv, q=q, k=k, v=v, out=out, second=second, lse=lse, y=y)
+    return out, y
+
+
+def layer_inputs(device, dt, seed=0):
+    B, N, D, H, dh = 2, 77, 96, 4, 32
+    r = lambda *s, seed, scale=1.0, t=dt: randn(device, s, seed, scale, dtype=t)  # noqa: E731
+    x, w = r(B, N, D, seed=seed + 1), r(3 * H * dh, D, seed=2, scale=D ** -0.5)
+    p = {"wq": r(H, dh, seed=3, scale=0.3, t=torch.float32) + 1, "wk": r(H, dh, seed=4, scale=0.3, t=torch.float32) + 1,
+         "rel": stx.rel_params(16, 40, False, True)}
+    lam, table = r(H // 2, seed=5, scale=0.2, t=torch.float32) + 0.5, r(16, H, seed=6, t=torch.float32)
+    masks = dict(causal=True, lengths=torch.tensor([N, N - 20], dtype=torch.int32, device=device), starts=torch.zeros(2, dtype=torch.int32, device=device))
+    return x, w, torch.arange(N, device=device, dtype=torch.int32), stx.rope_params(dh, 2), lam, p, table, masks
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_together(device, dtype):
+    """The operators one after another, forward and backward, against the layer in 64 bits and its gradients by autograd. The
+    roundings of qkv, q and k, the maps and the results (and of their gradients on the way back) lie one after another, each
+    relative to values that pass on with a gain of about 1 (scores: of their size, 6 at most here, so 6 h each): 24 h in
+    the 2-norm forward, twice that backward."""
+    dt = TYPES[dtype]
+    x, w, pos, rope, lam, p, table, masks = layer_inputs(device, dt)
+    B, N, D = x.shape
+    H, dh = 4, 32
+    kept = {}
+    out, y = attention_layer(x, w, pos, rope, lam, p, table, masks, kept)
+    dout, dy = randn(device, out.shape, 11, dtype=dt), randn(device, y.shape, 12, dtype=dt)
+    dq, dk, dv, dlam = stx.diff_attention_back(dout, kept["q"], kept["k"], kept["v"], lam, out, kept["second"], kept["lse"], **masks)
+    dscore, dtable = stx.soft_max_rel_back(dy, y, p["rel"], dh ** -0.5, masks["lengths"], masks["starts"])
+    dq = dq + torch.matmul(dscore.float(), kept["k"].transpose(1, 2).float().contiguous()).transpose(1, 2).to(dt)
+    dk = dk + torch.matmul(dscore.transpose(2, 3).float().contiguous(), kept["q"].transpose(1, 2).float().contiguous()).transpose(1, 2).to(dt)
+    qkv = kept["qkv"]
+    dqp, dwq, dkp, dwk = stx.qk_norm_rope_back(dq, qkv[:, :, :H], pos, rope, p["wq"], dk, qkv[:, :, H:2 * H], p["wk"])
+    dqkv = torch.cat([dqp, dkp, dv.reshape(B, N, H, dh)], 2).view(B, N, -1)
+    got = {"out": out, "y": y, "dx": dqkv @ w, "dlam": dlam, "dtable": dtable, "dwq": dwq, "dwk": dwk}
+
+    # in 64 bits, on the CPU (batched products of transposed views)
+    leaf = lambda t: t.to(F64).cpu().requires_grad_()  # noqa: E731
+    x6, wq6, wk6, lam6, table6 = (leaf(t) for t in (x, p["wq"], p["wk"], lam, table))
+    qkv6 = (x6 @ w.to(F64).cpu().t()).view(B, N, 3 * H, dh)
+    theta = pos.to(F64).cpu()[:, None, None] * 10000.0 ** (-2.0 * torch.arange(dh // 2, dtype=F64) / dh)
+
+    def turned(t, wt):
+        z = t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * wt
+        a, b = z[..., :dh // 2], z[..., dh // 2:]
+        return torch.cat([a * theta.cos() - b * theta.sin(), a * theta.sin() + b * theta.cos()], -1)
+
+    q6, k6 = turned(qkv6[:, :, :H], wq6), turned(qkv6[:, :, H:2 * H], wk6)
+    v6 = qkv6[:, :, 2 * H:].reshape(B, N, H // 2, 2 * dh)
+    mask, rel = (t.cpu() for t in seen_ref(B, N, N, masks["lengths"], masks["starts"], True, device))
+    z = torch.einsum("bihd,bjhd->bhij", q6, k6) * dh ** -0.5
+    maps = torch.softmax(z.masked_fill(~mask[:, None], -math.inf), -1)
+    out6 = torch.einsum("bhij,bjhd->bihd", maps[:, 0::2] - lam6[:, None, None] * maps[:, 1::2], v6)
+    y6 = torch.softmax((z + table6[buckets_ref(rel, 16, 40, False)].permute(0, 3, 1, 2)).masked_fill(~mask[:, None], -math.inf), -1)
+    ((out6 * dout.to(F64).cpu()).sum() + (y6 * dy.to(F64).cpu()).sum()).backward()
+    want = {"out": out6, "y": y6, "dx": x6.grad, "dlam": lam6.grad, "dtable": table6.grad, "dwq": wq6.grad, "dwk": wk6.grad}
+    h = half_step(dt)
+    for name, t in got.items():
+        ref = want[name].detach()
+        off = float((t.to(F64).cpu() - ref).norm() / ref.norm())
+        assert off <= (24 if name in ("out", "y") else 48) * h, (name, off)
+
+
+def test_graph_replays_and_streams(device):
+    """A captured forward and backward run of the operators, single tokens and split keys among it, replayed on new data with
+    eager calls between, on a stream of its own: the eager results each time."""
+    dt = torch.float16                                          # with the kernels that only fp16 has
+    x, w, pos, rope, lam, p, table, masks = layer_inputs(device, dt)
+    dout = randn(device, (2, 77, 2, 64), 21, dtype=dt)
+    token, cache_k, cache_v = (randn(device, s, 22 + i, dtype=dt) for i, s in enumerate(((2, 1, 4, 32), (2, 3000, 4, 32), (2, 3000, 2, 64))))
+
+    def step(s=None):
+        qkv = x @ w.t()
+        qkv = qkv.view(2, 77, 12, 32)
+        q, k = stx.qk_norm_rope(qkv[:, :, :4], pos, rope, p["wq"], qkv[:, :, 4:8], p["wk"], stream=s)
+        v = qkv[:, :, 8:].reshape(2, 77, 2, 64)
+        kept = stx.diff_attention(q, k, v, lam, keep=True, stream=s, **masks)
+        g = stx.diff_attention_back(dout, q, k, v, lam, *kept, stream=s, **masks)
+        n = stx.qk_norm_rope_back(g[0], qkv[:, :, :4], pos, rope, p["wq"], g[1], qkv[:, :, 4:8], p["wk"], stream=s)
+        score = qkv.view(2, 4, 77, 96)[..., :77]
+        y = stx.soft_max_rel(score, table, p["rel"], 0.2, masks["lengths"], masks["starts"], stream=s)
+        d = stx.soft_max_rel_back(score, y, p["rel"], 0.2, masks["lengths"], masks["starts"], stream=s)
+        t = stx.diff_attention(token, cache_k, cache_v, lam, stream=s)[0]
+        return [*kept, *g, *n, y, *d, t]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(s)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = step(s)
+    torch.cuda.synchronize()
+    for rep in range(4):
+        x.copy_(randn(device, x.shape, 100 + rep, 1.0 + rep, dtype=dt))
+        dout.copy_(randn(device, dout.shape, 200 + rep, 10.0 ** (rep - 2), dtype=dt))
+        cache_k.copy_(randn(device, cache_k.shape, 300 + rep, dtype=dt))
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), rep
+
+
+def test_two_streams_at_once(device):
+    """Two calls of each operator side by side give what they give alone."""
+    sets = []
+    for seed in (0, 50):
+        q, k, v, lam, _, _ = diff_inputs(device, torch.bfloat16, (2, 200, 600, 4, 2, 64, 128, False, None))
+        q = q * (1 + seed / 50)
+        x, table = randn(device, (2, 4, 150, 300), seed, dtype=torch.bfloat16), randn(device, (32, 4), seed + 1)
+        sets.append((q, k, v, lam, x, table))
+
+    def run(a, s=None):
+        q, k, v, lam, x, table = a
+        kept = stx.diff_attention(q, k, v, lam, keep=True, stream=s)
+        g = stx.diff_attention_back(kept[0], q, k, v, lam, *kept, stream=s)
+        y = stx.soft_max_rel(x, table, stx.rel_params(), stream=s)
+        return [*kept, *g, y, *stx.soft_max_rel_back(x, y, stx.rel_params(), stream=s)]
+
+    want = [run(a) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = [run(a, s) for a, s in zip(sets, streams)]
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            assert all(torch.equal(a, b) for a, b in zip(w, g))
+
+
+def test_offsets_past_32_bits(device):
+    """The last sequence of a cache of more than 2^32 bytes, rows of q and scores that far apart, and outputs there."""
+    B, N, Hk, D, V, H = 3, 1500, 2, 64, 128, 4
+    dt = torch.bfloat16
+    far = (1 << 31) + 64                                          # elements from a sequence to the next
+    cache = torch.empty(2 * far + N * Hk * (2 * D + V), device=device, dtype=dt)
+    k = torch.as_strided(cache, (B, N, 2 * Hk, D), (far, Hk * (2 * D + V), D, 1))
+    v = torch.as_strided(cache, (B, N, Hk, V), (far, Hk * (2 * D + V), V, 1), 2 * Hk * D)
+    kc, vc = randn(device, (B, N, 2 * Hk, D), 1, dtype=dt), randn(device, (B, N, Hk, V), 2, dtype=dt)
+    k.copy_(kc)
+    v.copy_(vc)
+    lam = randn(device, (H,), 4, 0.2, 0.5)
+    for M in (1, 90):
+        q, dy = randn(device, (B, M, 2 * H, D), 3, dtype=dt), randn(device, (B, M, H, V), 5, dtype=dt)
+        kept = stx.diff_attention(q, kc, vc, lam, keep=True)
+        got = stx.diff_attention(q, k, v, lam, keep=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, kept))
+        want = stx.diff_attention_back(dy, q, kc, vc, lam, *kept)
+        assert all(torch.equal(a, b) for a, b in zip(stx.diff_attention_back(dy, q, k, v, lam, *kept), want))
+    x = torch.as_strided(cache, (B, 1, 20, 300), (far, 0, 1000, 1))
+    table, p = randn(device, (32, 1), 6), stx.rel_params()
+    xc = randn(device, (B, 1, 20, 300), 7, dtype=dt)
+    x.copy_(xc)
+    want = stx.soft_max_rel(xc, table, p)
+    back = stx.soft_max_rel_back(xc, want, p)
+    assert torch.equal(stx.soft_max_rel(x, table, p, out=x), want) and torch.equal(x, want)
+    assert all(torch.equal(a, b) for a, b in zip(stx.soft_max_rel_back(xc, x, p), back))
+    t = torch.as_strided(cache, (B, 20, 2, 64), (far, 128, 64, 1))
+    tc = randn(device, (B, 20, 2, 64), 8, dtype=dt)
+    t.copy_(tc)
+    pos, r, w = torch.arange(20, device=device, dtype=torch.int32), stx.rope_params(64), torch.ones(64, device=device)
+    want = stx.qk_norm_rope(tc, pos, r, w)
+    assert torch.equal(stx.qk_norm_rope_back(tc, t, pos, r, w)[0], stx.qk_norm_rope_back(tc, tc, pos, r, w)[0])
+    stx.qk_norm_rope(t, pos, r, w, out=t)
+    assert torch.equal(t, want)
+
+
+def test_outputs_belong_to_the_given_stream(device):
+    """What a call allocates is on the stream that it runs on, the caller's being another."""
+    s = torch.cuda.Stream()
+    q, k, v, lam, _, _ = diff_inputs(device, torch.float32, (1, 3, 5, 2, 1, 16, 16, False, None))
+    s.wait_stream(torch.cuda.current_stream())
+    out, second, lse = stx.diff_attention(q, k, v, lam, keep=True, stream=s)
+    s.synchronize()
+    check_diff((out, second, lse), q, k, v, lam, torch.ones(1, 3, 5, dtype=torch.bool, device=device), 0.25, "stream")
