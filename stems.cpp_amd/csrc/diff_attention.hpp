@@ -25,7 +25,7 @@ struct DiffArgs {
     float* lse;                          // [sequence][head][map][query]
     float* dots;                         // backward: dy . o of each map, laid out as lse
     double* tiles_lam;                   // backward: a block's shares of lambda's gradient, [block][group]
-    const unsigned* most;                // fp16's backward: largest |v| and |dy| of the call, as bits
+    const float* most;                   // fp16's backward: largest |v| and |dy| of the call
     float* part;                         // split keys (forward) or rows (keys' gradients)
     float* part_stat;
     const int *lengths, *starts;
@@ -171,10 +171,10 @@ __device__ __forceinline__ u32x4 chunk_of(const f32x4* acc) {
     if constexpr (sizeof(T) == 4) {
         f = __builtin_bit_cast(u32x4, acc[0]);
     } else {
-        T v[8];
+        typedef T Pair __attribute__((ext_vector_type(2)));           // converted together, to nearest even
+        typedef float Floats __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = from_f32<T>(acc[e / 4][e % 4]);
-        __builtin_memcpy(&f, v, 16);
+        for (int e = 0; e < 4; e++) f[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((Floats{acc[e / 2][e % 2 * 2], acc[e / 2][e % 2 * 2 + 1]}), Pair));
     }
     return f;
 }

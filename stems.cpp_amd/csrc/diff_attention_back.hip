@@ -20,7 +20,7 @@ template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 8.f : 0.f;
 
 __device__ __forceinline__ float range_scale(const DiffArgs& a, float dy, float lam) {
-    const float bound = 2.f * a.vdim * __uint_as_float(a.most[0]) * dy * fmaxf(1.f, fabsf(lam));
+    const float bound = 2.f * a.vdim * a.most[0] * dy * fmaxf(1.f, fabsf(lam));
     if (!(bound > 0.f && bound < 0x1p120f)) return 1.f;
     return __builtin_amdgcn_exp2f(fminf(fmaxf(7.f - ceilf(__builtin_amdgcn_logf(bound)), -100.f), 100.f));
 }
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
     if constexpr (std::is_same_v<T, f16>) {
         float lam = 0.f;
         for (int g = 0; g < a.group; g++) lam = fmaxf(lam, fabsf(a.lam[kvh * a.group + g]));
-        unit = range_scale(a, __uint_as_float(a.most[1]), lam);
+        unit = range_scale(a, a.most[1], lam);
     }
     auto fetch = [&](int head, int i0, int stage) {
         const char* q = a.q.p + 2LL * head * a.q.s1 + i0 * a.q.s2 + b * a.q.s3;
@@ -456,28 +456,41 @@ __global__ __launch_bounds__(256) void diff_lambda_kernel(const double* shares, 
     if (threadIdx.x == 0) dlam[blockIdx.x] = (float)-((red[0] + red[1]) + (red[2] + red[3]));
 }
 
-// fp16: the largest |v| and |dy| of the call, as bits (0 before it; the order of maxima does not matter).
-__global__ void diff_clear_kernel(unsigned* most) { most[threadIdx.x] = 0; }
+// fp16: the largest |v| and |dy| of the call, of each block and then of all (8,192 waves' atomics on two words took 196 us).
+constexpr int kMostBlocks = 1024;
 struct MostArgs {
     Strided t[2];
     long long rows[2];
     FastDiv d1[2], d2[2];                // row -> (heads), (tokens)
-    int width[2];
+    int width, log_lanes;                // elements of a row, and lanes that hold 8 each of one
     const int* lengths;
-    unsigned* most;
+    float* most;                         // [2], then [2][kMostBlocks]
 };
 __global__ __launch_bounds__(256) void diff_most_kernel(MostArgs a) {
-    const int which = blockIdx.y;
+    const int which = blockIdx.y, lane = threadIdx.x % 64, chunk = lane & ((1 << a.log_lanes) - 1), left = a.width - chunk * 8;
     float most = 0.f;
-    const int lane = threadIdx.x % 64;
-    for (long long r = blockIdx.x * 4LL + threadIdx.x / 64; r < a.rows[which]; r += gridDim.x * 4LL) {
+    const long long step = (long long)gridDim.x * (256 >> a.log_lanes);
+#pragma unroll 4
+    for (long long r = blockIdx.x * (256LL >> a.log_lanes) + (threadIdx.x >> a.log_lanes); r < a.rows[which]; r += step) {
         const unsigned i = a.d1[which].div((unsigned)r), h = (unsigned)r - i * a.d1[which].d, b = a.d2[which].div(i), n = i - b * a.d2[which].d;
-        if (which == 0 && a.lengths && (int)n >= a.lengths[b]) continue;          // keys that are not there
-        const f16* p = reinterpret_cast<const f16*>(a.t[which].p + h * a.t[which].s1 + n * a.t[which].s2 + b * a.t[which].s3);
-        for (int d = lane; d < a.width[which]; d += 64) most = fmaxf(most, fabsf((float)p[d]));
+        if (left <= 0 || (which == 0 && a.lengths && (int)n >= a.lengths[b])) continue;     // keys that are not there
+        float f[8];
+        unpack<f16>(load_chunk<f16>(a.t[which].p + h * a.t[which].s1 + n * a.t[which].s2 + b * a.t[which].s3 + chunk * 16, left), f);
+#pragma unroll
+        for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(f[e]));
     }
+    __shared__ float red[4];
     most = lane_max<64>(most);
-    if (lane == 0 && most > 0.f) atomicMax(a.most + which, __float_as_uint(most));
+    if (lane == 0) red[threadIdx.x / 64] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) a.most[2 + which * kMostBlocks + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+__global__ __launch_bounds__(128) void diff_most_of_all_kernel(float* most, int blocks) {
+    const int which = threadIdx.x / 64;
+    float m = 0.f;
+    for (int i = threadIdx.x % 64; i < blocks; i += 64) m = fmaxf(m, most[2 + which * kMostBlocks + i]);
+    m = lane_max<64>(m);
+    if (threadIdx.x % 64 == 0) most[which] = m;
 }
 
 // --------------------------------------------------------------------------------- host
@@ -509,7 +522,7 @@ BackPlan back_plan(const DiffShape& s, int size, bool causal) {
     };
     p.dots = take((size_t)s.B * s.H * 2 * s.M * sizeof(float));
     p.tiles_lam = take((size_t)((rows + 63) / 64) * p.q_splits * s.B * s.H * sizeof(double));   // of the smallest tiles
-    p.most = take(2 * sizeof(unsigned));
+    p.most = take((2 + 2 * kMostBlocks) * sizeof(float));
     const size_t q_part = p.q_splits > 1 ? (size_t)p.q_splits * pairs * rows * 2 * p.dp : 0;
     const size_t k_part = p.k_splits > 1 ? (size_t)p.k_splits * pairs * s.N * (2 * p.dp + p.vp) : 0;
     p.part = take(std::max(q_part, k_part) * sizeof(float));         // one after the other
@@ -601,7 +614,7 @@ STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tenso
         char* ws = static_cast<char*>(workspace);
         a.dots = reinterpret_cast<float*>(ws + p.dots);
         a.tiles_lam = reinterpret_cast<double*>(ws + p.tiles_lam);
-        unsigned* most = reinterpret_cast<unsigned*>(ws + p.most);
+        float* most = reinterpret_cast<float*>(ws + p.most);
         a.most = most;
         const hipStream_t st = as_stream(stream);
         const long long pairs = s.B * s.Hk;
@@ -618,14 +631,16 @@ STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tenso
                     m.rows[0] = s.B * s.N * s.Hk, m.rows[1] = s.B * s.M * s.H;
                     m.d1[0] = FastDiv((unsigned)s.Hk), m.d1[1] = FastDiv((unsigned)s.H);
                     m.d2[0] = FastDiv((unsigned)std::max(1LL, s.N)), m.d2[1] = FastDiv((unsigned)std::max(1LL, s.M));
-                    m.width[0] = m.width[1] = s.V;
+                    m.width = s.V;
+                    while (8 << m.log_lanes < s.V) m.log_lanes++;
                     m.lengths = lengths;
                     m.most = most;
                     STX_REQUIRE(m.rows[0] < (1LL << 32) && m.rows[1] < (1LL << 32), "%s: 2^32 rows or more", op);
-                    hipLaunchKernelGGL(diff_clear_kernel, dim3(1), dim3(2), 0, st, most);
-                    const long long blocks = std::max(1LL, std::min(2LL * kCus, (std::max(m.rows[0], m.rows[1]) + 15) / 16));
-                    hipLaunchKernelGGL(diff_most_kernel, dim3((unsigned)blocks, 2), dim3(256), 0, st, m);
+                    const int blocks = (int)std::max(1LL, std::min<long long>(kMostBlocks, (std::max(m.rows[0], m.rows[1]) << m.log_lanes) / 1024));
+                    hipLaunchKernelGGL(diff_most_kernel, dim3(blocks, 2), dim3(256), 0, st, m);
                     launch_check("diff_most_kernel");
+                    hipLaunchKernelGGL(diff_most_of_all_kernel, dim3(1), dim3(128), 0, st, most, blocks);
+                    launch_check("diff_most_of_all_kernel");
                 }
                 float* part = reinterpret_cast<float*>(ws + p.part);
                 if (s.M > 0) {
