@@ -888,7 +888,8 @@ STX_API size_t     stx_group_norm_cl_forward_workspace_size(const stx_tensor* a,
  *   dst = R(pos) (w * x / sqrt(mean(x^2) + eps)).
  * w_q and w_k: device float[dim], or with per_head != 0 float[heads][dim] and float[kv heads][dim]; either may be
  * NULL (1). pos, pos_stride and params as in stx_rope_scaled; so are strides, limits and the outputs that may be the
- * inputs. Mean squares are formed in double, the rest in float, rounded once. Rows of up to 1,024 elements; eps >= 0. */
+ * inputs. A row's mean square is added in double from sums of at most 16 squares in float (in double where they leave
+ * fp32's range); the rest is float, rounded once. Rows of up to 1,024 elements; eps >= 0. */
 STX_API stx_status stx_qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
                                     int64_t pos_stride, const stx_rope_params* params, const float* w_q,
                                     const float* w_k, int per_head, double eps, const stx_tensor* q_dst,
@@ -967,7 +968,8 @@ STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, 
  * sequence's length on), dlambda (device float[H]); any may be NULL. Scores are formed again; sums are float
  * (dlambda's over rows double), the maps' gradients rounded to the type for their products (16-bit types; fp16's scaled by
  * powers of two, so that they keep its range). dlambda comes from the maps themselves, not from the rounded second. The
- * same rules for masked keys, strides and workspace; dy is finite; outputs overlap nothing else. */
+ * same rules for masked keys, strides and workspace; dy and q are finite, also at queries that see no key; outputs overlap
+ * nothing else. */
 STX_API size_t     stx_diff_attention_back_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
                                                           stx_type type);
 STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tensor* q, const stx_tensor* k,

@@ -144,7 +144,10 @@ __device__ __forceinline__ float sum_over(float v, int lanes) {
     return v;
 }
 
-constexpr float kLog2e = 1.44269504088896340736f;
+// e^v, of a score less the row's largest: in that order, since the type's lowest values, which hide keys too, times log2 e are
+// infinite, and a row of them alone is a row of equal scores.
+__device__ __forceinline__ float natural_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896340736f); }
+constexpr float kLowest = -0x1.fffffep127f;
 
 // A row's maximum and sum of exponentials, of a wave's lanes already, over the block's waves: an exchange of both at
 // once, in one of two places by turns, so that one barrier a row is enough.
@@ -158,13 +161,12 @@ __device__ __forceinline__ void join_waves(float& m, float& s, float2 (&red)[2][
         for (int w = 1; w < WAVES; w++) top = fmaxf(top, red[turn][w].x);
         s = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) s += red[turn][w].y * __builtin_amdgcn_exp2f(red[turn][w].x - top);
+        for (int w = 0; w < WAVES; w++) s += red[turn][w].y * natural_exp(red[turn][w].x - top);
         m = top;
     }
 }
 
-// Scores in units of log2, so that the exponential is the hardware's 2^y. K vectors a lane, those of the next row
-// on their way while one is worked on; K 0: rows of any length, read twice.
+// K vectors a lane, those of the next row on their way while one is worked on; K 0: rows of any length, read twice.
 template <class T, int WAVES, int K>
 __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
     constexpr int V = kVec<T>;
@@ -177,9 +179,9 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
     __syncthreads();
     const int span = 2 * a.reach + 1;
     for (int e = threadIdx.x; e < span; e += kRelThreads)
-        near[e] = a.table[(long long)bucket_of(a, edges, e - a.reach) * a.heads + h] * kLog2e;
+        near[e] = a.table[(long long)bucket_of(a, edges, e - a.reach) * a.heads + h];
     __syncthreads();
-    const float left = near[0], right = near[span - 1], scale = a.scale * kLog2e;
+    const float left = near[0], right = near[span - 1], scale = a.scale;
     const int lanes = WAVES == 1 ? 1 << a.log_lanes : kRelThreads, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes;
     const int vectors = (a.n + V - 1) / V, rounds = kRelThreads / lanes;
 
@@ -235,13 +237,13 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
                     for (int e = 0; e < V; e++) m = fmaxf(m, z[k][e]);
                 }
                 m = max_over(m, min(lanes, 64));
-                m = m == -__builtin_inff() ? -0x1p126f : m;          // a row of nothing: zeros
+                m = m == -__builtin_inff() ? kLowest : m;            // a row of nothing: zeros
                 const float mine = m;
 #pragma unroll
                 for (int k = 0; k < K; k++) {
                     const int lo = Place<V>(lane + k * lanes, a.n, limit).lo;
 #pragma unroll
-                    for (int e = 0; e < V; e++) z[k][e] = __builtin_amdgcn_exp2f(z[k][e] - mine);
+                    for (int e = 0; e < V; e++) z[k][e] = natural_exp(z[k][e] - mine);
                     if (every(lo == 0)) {
 #pragma unroll
                         for (int e = 0; e < V; e++) s += z[k][e];
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
                 }
                 s = sum_over(s, min(lanes, 64));
                 join_waves<WAVES>(m, s, red, turn);
-                const float inv = s == 0.f ? 0.f : (WAVES > 1 ? __builtin_amdgcn_exp2f(mine - m) : 1.f) / s;
+                const float inv = s == 0.f ? 0.f : (WAVES > 1 ? natural_exp(mine - m) : 1.f) / s;
                 if (!valid) continue;
 #pragma unroll
                 for (int k = 0; k < K; k++) {
@@ -280,14 +282,14 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
 #pragma unroll
                     for (int e = 0; e < V; e++) top = fmaxf(top, z[e]);
                     const float base = top == -__builtin_inff() ? 0.f : top;
-                    s *= __builtin_amdgcn_exp2f(m - base);
+                    s *= natural_exp(m - base);
 #pragma unroll
-                    for (int e = 0; e < V; e++) s += __builtin_amdgcn_exp2f(z[e] - base);
+                    for (int e = 0; e < V; e++) s += natural_exp(z[e] - base);
                     m = top;
                 }
                 float top = max_over(m, min(lanes, 64));
-                top = top == -__builtin_inff() ? -0x1p126f : top;
-                s = sum_over(s * __builtin_amdgcn_exp2f(m - top), min(lanes, 64));
+                top = top == -__builtin_inff() ? kLowest : top;
+                s = sum_over(s * natural_exp(m - top), min(lanes, 64));
                 join_waves<WAVES>(top, s, red, turn);
                 const float inv = s == 0.f ? 0.f : 1.f / s;
                 for (int c = lane; c < vectors; c += lanes) {
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
                         scores(load_row<T>(x + c * V, a.n - c * V), c * V, at, z);
                         hide(limit - c * V, z);
 #pragma unroll
-                        for (int e = 0; e < V; e++) y.v[e] = from_f32<T>(__builtin_amdgcn_exp2f(z[e] - top) * inv);
+                        for (int e = 0; e < V; e++) y.v[e] = from_f32<T>(natural_exp(z[e] - top) * inv);
                     }
                     store_row<T>(out + c * V, y, a.n - c * V);
                 }

@@ -8,8 +8,8 @@ result's type relative to the value, plus half the smallest subnormal step of fp
           g = w dz, dx = r (g - xh mean(g xh)): each term's roundings, 8 u r (|w| D + |xh| mean(|w| D |xh|)).
           dw: sums of dz xh over n rows in float of at most n / 4 + 64 terms: each partial sum is at most S = sum |D xh|,
           a random walk of sqrt(n) roundings u S / ... bounded by (8 + 4 sqrt(n)) u S.
-  rel     an exponent in units of log2 has the roundings of scale log2e, of the fused product and bias, of the bias and of
-          the difference to the row's largest: 5 u (|scale x| + |bias|) of the natural one; at most 5 u Z relative to
+  rel     an exponent has the roundings of the fused product and bias, of the difference to the row's largest, which is
+          of twice their size, and of log2e and the product with it: 5 u (|scale x| + |bias|); at most 5 u Z relative to
           each exponential, Z the row's largest |scale x| + |bias|, as much of their sum, 2 u of the hardware's 2^y each,
           and of the sum a rounding for each of a lane's terms and 16 of the tree. Backward: products and sums are in
           double, so one rounding to float and one to the type; the table's sums one.
@@ -342,6 +342,31 @@ def test_rel_infinite_scores(device):
     assert torch.allclose(y[0, 0, 0, :5], torch.full((5,), 0.2, device=device)) and bool((y[0, 0, 0, 5:] == 0).all())
     assert bool((y[0, 0, 1] == 0).all()) and torch.allclose(y[0, 0, 2], torch.full((70,), 1 / 70, device=device))
     assert bool(y[0, 0, 3].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [3, 70, 700, 5000, 20000])
+def test_rel_lowest_values(device, dtype, N):
+    """Keys hidden by the type's lowest value, at scale 1, in rows of every width: none of the sum beside other
+    scores, an equal share each where a row has nothing else, and so beside -infinity; and biases of the lowest float.
+    Exponentials and their sums are exact here; 8 u are the quotient's."""
+    dt = TYPES[dtype]
+    low = torch.finfo(dt).min
+    x = torch.zeros((1, 1, 5, N), dtype=dt, device=device)
+    x[0, 0, 0, 2:] = low
+    x[0, 0, 1] = low
+    x[0, 0, 2] = -math.inf
+    x[0, 0, 2, N - 2:] = low
+    x[0, 0, 3, 1:] = torch.finfo(dt).max
+    x[0, 0, 4, 0] = low
+    y = stx.soft_max_rel(x, torch.zeros((32, 1), device=device), stx.rel_params(), 1.0)
+    wide = x[0, 0].to(F64)
+    want = torch.softmax(wide, -1)
+    close(y[0, 0], want, 8 * U * want, "y")
+    table = torch.full((32, 1), torch.finfo(torch.float32).min, device=device)
+    y = stx.soft_max_rel(torch.zeros_like(x), table, stx.rel_params(), 1.0)
+    want = torch.full_like(want, 1 / N)
+    close(y[0, 0], want, 8 * U * want, "y")
 
 
 def test_rel_strides_and_empty(device):
