@@ -19,6 +19,10 @@ namespace {
 // that rounding the result alone has (60 x 801 frames, lambda about 0.5: 2.5e-3 in bf16 where it is 1.65e-3), for the maps cancel and
 // their errors do not. The first map, which weighs more, is taken in two parts, 1.06 times; 204 -> 232 us.
 // fp16's P is scaled by 2^6 so that shares of 2^-20 keep all their bits.
+//
+// Those 60 x 801 frames of 4 heads of 64 and 128 take 215 to 230 us (551 TFLOP/s of the formula's products), 4 x 4 heads of 8,192 x 8,192
+// 960 us (860): exponentials (vector units 57 % busy) and products (matrix cores 42 %), which two waves a SIMD overlap in part.
+// One token of 8 sequences over caches of up to 16,384 (210 MB): 40 us, 5 TB/s, and 5 us to join the parts.
 template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 6.f : 0.f;
 

@@ -16,6 +16,11 @@ namespace {
 // dS and P are rounded to 16 bits for their products (16-bit data). fp16's range would cut them: P is
 // scaled by 2^8, and dP - D by a power of two of the row (first kernel) or the call (second) that keeps
 // 2^8 P (dP - D) max(1, |lambda|) below 2^15, from |dP - D| <= 2 V max|v| max|dy|.
+//
+// 16,384 x 16,384 causal, 8 heads to 2, bf16: 1,030 us (801 TFLOP/s of the first kernel's products; vector units 68 %, matrix cores 39 %
+// busy) and 1,725 us (637 TFLOP/s; 42 and 28 %): a wave of 16 keys reads the rows' q and dy from LDS both ways, 32 KB for 32
+// matrix instructions, twice what the 32 rows of a wave of the first need; 32 keys do not fit the registers of two waves a
+// SIMD, and one wave a SIMD was no faster. 1,344 x 2,688, 4 heads, fp32: 120 and 188 us, matrix cores 71 and 65 % busy.
 template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 8.f : 0.f;
 
