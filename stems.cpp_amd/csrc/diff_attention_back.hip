@@ -20,7 +20,7 @@ namespace {
 // 16,384 x 16,384 causal, 8 heads to 2, bf16: 1,030 us (801 TFLOP/s of the first kernel's products; vector units 68 %, matrix cores 39 %
 // busy) and 1,725 us (637 TFLOP/s; 42 and 28 %): a wave of 16 keys reads the rows' q and dy from LDS both ways, 32 KB for 32
 // matrix instructions, twice what the 32 rows of a wave of the first need; 32 keys do not fit the registers of two waves a
-// SIMD, and one wave a SIMD was no faster. 1,344 x 2,688, 4 heads, fp32: 120 and 188 us, matrix cores 71 and 65 % busy.
+// SIMD (v in LDS instead: 45 of them spilled, the call 3,670 us where it is 2,650), and one wave a SIMD was no faster. 1,344 x 2,688, 4 heads, fp32: 120 and 188 us, matrix cores 71 and 65 % busy.
 template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 8.f : 0.f;
 
@@ -233,9 +233,9 @@ struct RowStats {
     int limit[kRows];
 };
 
-template <class T, int DP, int VP, int NK, bool ALIGNED>
+template <class T, int DP, int VP, bool ALIGNED>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_dkv_kernel(DiffArgs a) {
-    constexpr int NT = 256, RG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, NV = VP / 16, KEYS = 64 * NK;
+    constexpr int NT = 256, RG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, NV = VP / 16, KEYS = 64;
     using QL = Loader<T, DP, kRows, 2, NT, ALIGNED>;
     using YL = Loader<T, VP, kRows, 1, NT, ALIGNED>;
     constexpr int STAGE = QL::BYTES + YL::BYTES;
@@ -304,16 +304,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
     };
     if (begin < end) fetch(head, i0, 0);
 
-    u32x4 kf[2][NK][GD], vf[NK][GV];
+    u32x4 kf[2][GD], vf[GV];
+    const int key = key0 + wave * 16 + s;
+    const bool there = key < mask.length;
 #pragma unroll
-    for (int n = 0; n < NK; n++) {
-        const int key = key0 + (wave * NK + n) * 16 + s;
-        const bool in = key < mask.length;
-#pragma unroll
-        for (int m = 0; m < 2; m++) load_fragments<T, DP>(kf[m][n], in ? a.k.p + (2LL * kvh + m) * a.k.s1 + key * a.k.s2 + b * a.k.s3 : nullptr, a.dim, lane);
-        load_fragments<T, VP>(vf[n], in ? a.v.p + (long long)kvh * a.v.s1 + key * a.v.s2 + b * a.v.s3 : nullptr, a.vdim, lane);
-    }
-    f32x4 dk[2][NK][ND] = {}, dv[NK][NV] = {};
+    for (int m = 0; m < 2; m++) load_fragments<T, DP>(kf[m], there ? a.k.p + (2LL * kvh + m) * a.k.s1 + key * a.k.s2 + b * a.k.s3 : nullptr, a.dim, lane);
+    load_fragments<T, VP>(vf, there ? a.v.p + (long long)kvh * a.v.s1 + key * a.v.s2 + b * a.v.s3 : nullptr, a.vdim, lane);
+    f32x4 dk[2][ND] = {}, dv[NV] = {};
     const float c = a.scale * kLog2e;
     int stage = 0;
     for (long long t = begin; t < end; t++) {
@@ -326,96 +323,77 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
         const RowStats& st = stats[stage];
 #pragma unroll 1
         for (int k0 = 0; k0 < kRows; k0 += RG) {
-            f32x4 z[2][NK][RG / 16], dp[NK][RG / 16];
+            f32x4 z[2][RG / 16], dp[RG / 16];
 #pragma unroll
             for (int t = 0; t < RG / 16; t++) {
-#pragma unroll
-                for (int n = 0; n < NK; n++) z[0][n][t] = z[1][n][t] = dp[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                z[0][t] = z[1][t] = dp[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int m = 0; m < 2; m++)
 #pragma unroll
                     for (int g = 0; g < GD; g++) {
                         const u32x4 qf = Tile<T, DP>::plain(qs + m * kRows * Tile<T, DP>::BYTES, k0 + t * 16, g, lane);
-#pragma unroll
-                        for (int n = 0; n < NK; n++) z[m][n][t] = mma(qf, kf[m][n][g], z[m][n][t], T{});
+                        z[m][t] = mma(qf, kf[m][g], z[m][t], T{});
                     }
 #pragma unroll
                 for (int g = 0; g < GV; g++) {
                     const u32x4 yf = Tile<T, VP>::plain(ys, k0 + t * 16, g, lane);
-#pragma unroll
-                    for (int n = 0; n < NK; n++) dp[n][t] = mma(yf, vf[n][g], dp[n][t], T{});
+                    dp[t] = mma(yf, vf[g], dp[t], T{});
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            u32x4 mix[NK], ds[2][NK];
-            f32x4 pm[NK][RG / 16];
+            f32x4 pm[RG / 16];
 #pragma unroll
             for (int t = 0; t < RG / 16; t++) {
                 const int at = k0 + t * 16 + lane / 16 * 4;
                 const f32x4 base1 = *reinterpret_cast<const f32x4*>(&st.base[0][at]), base2 = *reinterpret_cast<const f32x4*>(&st.base[1][at]);
                 const f32x4 dot1 = *reinterpret_cast<const f32x4*>(&st.dot[0][at]), dot2 = *reinterpret_cast<const f32x4*>(&st.dot[1][at]);
 #pragma unroll
-                for (int n = 0; n < NK; n++) {
-                    const int key = key0 + (wave * NK + n) * 16 + s;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float p1 = __builtin_amdgcn_exp2f(fmaf(z[0][n][t][e], c, -base1[e])), p2 = lam * __builtin_amdgcn_exp2f(fmaf(z[1][n][t][e], c, -base2[e]));
-                        if (!whole) {
-                            const bool in = key < st.limit[at + e];
-                            p1 = in ? p1 : 0.f;
-                            p2 = in ? p2 : 0.f;
-                        }
-                        pm[n][t][e] = p1 + p2;
-                        z[0][n][t][e] = p1 * fmaf(dp[n][t][e], unit, -dot1[e]);
-                        z[1][n][t][e] = p2 * fmaf(dp[n][t][e], unit, -dot2[e]);
+                for (int e = 0; e < 4; e++) {
+                    float p1 = __builtin_amdgcn_exp2f(fmaf(z[0][t][e], c, -base1[e])), p2 = lam * __builtin_amdgcn_exp2f(fmaf(z[1][t][e], c, -base2[e]));
+                    if (!whole) {
+                        const bool in = key < st.limit[at + e];
+                        p1 = in ? p1 : 0.f;
+                        p2 = in ? p2 : 0.f;
                     }
+                    pm[t][e] = p1 + p2;
+                    z[0][t][e] = p1 * fmaf(dp[t][e], unit, -dot1[e]);
+                    z[1][t][e] = p2 * fmaf(dp[t][e], unit, -dot2[e]);
                 }
             }
-#pragma unroll
-            for (int n = 0; n < NK; n++) {
-                mix[n] = chunk_of<T>(pm[n]);
-#pragma unroll
-                for (int m = 0; m < 2; m++) ds[m][n] = chunk_of<T>(z[m][n]);
-            }
+            const u32x4 mix = chunk_of<T>(pm), ds[2] = {chunk_of<T>(z[0]), chunk_of<T>(z[1])};
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const u32x4 yf = Tile<T, VP>::columns(ys, k0, i, lane);
-#pragma unroll
-                for (int n = 0; n < NK; n++) dv[n][i] = mma(yf, mix[n], dv[n][i], T{});
+                dv[i] = mma(yf, mix, dv[i], T{});
             }
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
                 for (int i = 0; i < ND; i++) {
                     const u32x4 qf = Tile<T, DP>::columns(qs + m * kRows * Tile<T, DP>::BYTES, k0, i, lane);
-#pragma unroll
-                    for (int n = 0; n < NK; n++) dk[m][n][i] = mma(qf, ds[m][n], dk[m][n][i], T{});
+                    dk[m][i] = mma(qf, ds[m], dk[m][i], T{});
                 }
         }
         stage ^= 1;
     }
     const float fk = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / unit, fv = __builtin_amdgcn_exp2f(-kShift<T>);
+    if (key >= a.keys) return;
+    float* to = a.part ? a.part + (((long long)part * (gridDim.x / a.tile_div.d) + per) * a.keys + key) * (2 * DP + VP) : nullptr;
 #pragma unroll
-    for (int n = 0; n < NK; n++) {
-        const int key = key0 + (wave * NK + n) * 16 + s;
-        if (key >= a.keys) continue;
-        float* to = a.part ? a.part + (((long long)part * (gridDim.x / a.tile_div.d) + per) * a.keys + key) * (2 * DP + VP) : nullptr;
+    for (int m = 0; m < 3; m++) {        // dk of both maps, dv
+        const Strided& d = m < 2 ? a.dk : a.dv;
+        char* out = const_cast<char*>(d.p) + (m < 2 ? 2LL * kvh + m : (long long)kvh) * d.s1 + key * d.s2 + b * d.s3;
+        const int width = m < 2 ? a.dim : a.vdim;
+        const float f = m < 2 ? fk : fv;
 #pragma unroll
-        for (int m = 0; m < 3; m++) {    // dk of both maps, dv
-            const Strided& d = m < 2 ? a.dk : a.dv;
-            char* out = const_cast<char*>(d.p) + (m < 2 ? 2LL * kvh + m : (long long)kvh) * d.s1 + key * d.s2 + b * d.s3;
-            const int width = m < 2 ? a.dim : a.vdim;
-            const float f = m < 2 ? fk : fv;
-#pragma unroll
-            for (int i = 0; i < (m < 2 ? ND : NV); i++) {
-                const int at = i * 16 + lane / 16 * 4;
-                const f32x4 v = (m < 2 ? dk[m < 2 ? m : 0][n][m < 2 ? i : 0] : dv[n][i]) * f;
-                if (to) {
-                    *reinterpret_cast<f32x4*>(to + m * DP + at) = v;
-                } else if (d.p) {
-                    const float o[4] = {v[0], v[1], v[2], v[3]};
-                    store4<T>(out + at * sizeof(T), width - at, o);
-                }
+        for (int i = 0; i < (m < 2 ? ND : NV); i++) {
+            const int at = i * 16 + lane / 16 * 4;
+            const f32x4 v = (m < 2 ? dk[m < 2 ? m : 0][m < 2 ? i : 0] : dv[i]) * f;
+            if (to) {
+                *reinterpret_cast<f32x4*>(to + m * DP + at) = v;
+            } else if (d.p) {
+                const float o[4] = {v[0], v[1], v[2], v[3]};
+                store4<T>(out + at * sizeof(T), width - at, o);
             }
         }
     }
@@ -502,7 +480,7 @@ __global__ __launch_bounds__(128) void diff_most_of_all_kernel(float* most, int 
 constexpr int kCus = 256;
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 struct BackPlan {
-    int nq, nk, dp, vp, q_splits, k_splits;
+    int nq, dp, vp, q_splits, k_splits;
     long long q_tiles, k_tiles;
     size_t dots, tiles_lam, most, part, total;
 };
@@ -512,9 +490,8 @@ BackPlan back_plan(const DiffShape& s, int size, bool causal) {
     const bool small = s.D <= 64 && s.V <= 128 && size == 2;
     with_dims(s.D, s.V, [&](auto d, auto v) { p.dp = d(), p.vp = v(); });
     p.nq = small && rows > 64 ? 2 : 1;
-    p.nk = 1;
     p.q_tiles = (rows + 64 * p.nq - 1) / (64 * p.nq);
-    p.k_tiles = (s.N + 64 * p.nk - 1) / (64 * p.nk);
+    p.k_tiles = (s.N + 63) / 64;
     // Parts of the keys or rows: as many as give two blocks a CU, or eight where causality makes tiles differ in length,
     // of 256 keys or rows at least.
     const long long want = (causal ? 8LL : 4LL) * kCus;
@@ -543,8 +520,8 @@ void launch_dq(const DiffArgs& a, const BackPlan& p, bool aligned, unsigned bloc
 }
 template <class T, int DP, int VP>
 void launch_dkv(const DiffArgs& a, bool aligned, unsigned blocks, hipStream_t stream) {
-    if (aligned) hipLaunchKernelGGL((diff_dkv_kernel<T, DP, VP, 1, true>), dim3(blocks), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((diff_dkv_kernel<T, DP, VP, 1, false>), dim3(blocks), dim3(256), 0, stream, a);
+    if (aligned) hipLaunchKernelGGL((diff_dkv_kernel<T, DP, VP, true>), dim3(blocks), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((diff_dkv_kernel<T, DP, VP, false>), dim3(blocks), dim3(256), 0, stream, a);
     launch_check("diff_dkv_kernel");
 }
 
