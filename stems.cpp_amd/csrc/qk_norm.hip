@@ -78,7 +78,9 @@ struct Spot {
     }
 };
 
-// Where the partners of unit `at` start; `at` itself where they are in the unit or there are none.
+// Where the partners of unit `at` start; `at` itself where they are in the unit or there are none. In mode 2 the units over a
+// half's end (`torn`) have theirs in two places; kernels without TORN are for calls that have none (with it, 60 x 801 tokens of
+// 16 rows of 64 elements in mode 0 took 101 us instead of 84, and their gradient 103 instead of 82).
 template <int V>
 __device__ __forceinline__ int partner(const QkArgs& a, int at) {
     const int half = a.at.n_dims / 2;
@@ -86,9 +88,19 @@ __device__ __forceinline__ int partner(const QkArgs& a, int at) {
     if (a.mode == 0) return V == 1 ? at ^ 1 : at;
     return at < half ? at + half : at - half;
 }
+template <int V, bool TORN>
+__device__ __forceinline__ bool torn(const QkArgs& a, int at) {
+    const int half = a.at.n_dims / 2;
+    return TORN && V > 1 && ((at < half && at + V > half) || (at < a.at.n_dims && at + V > a.at.n_dims));
+}
+// Element e's partner in mode 2, or -1.
+__device__ __forceinline__ int partner_of(const QkArgs& a, int e) {
+    const int half = a.at.n_dims / 2;
+    return e < half ? e + half : e < a.at.n_dims ? e - half : -1;
+}
 
 // The rotation of unit `at` with values f and partners p, in place.
-template <int V>
+template <int V, bool TORN>
 __device__ __forceinline__ void rotate(const QkArgs& a, int at, const float2* tab, float (&f)[V], const float (&p)[V]) {
     const int half = a.at.n_dims / 2;
     if (V > 1 && a.mode == 0) {
@@ -100,6 +112,14 @@ __device__ __forceinline__ void rotate(const QkArgs& a, int at, const float2* ta
             const float x0 = f[v], x1 = f[v + 1];
             f[v] = fmaf(x0, r.x, -(x1 * r.y));
             f[v + 1] = fmaf(x0, r.y, x1 * r.x);
+        }
+    } else if (torn<V, TORN>(a, at)) {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int e = at + v;
+            if (e >= a.at.n_dims) continue;
+            const float2 r = tab[e < half ? e : e - half];
+            f[v] = e < half ? fmaf(f[v], r.x, -(p[v] * r.y)) : fmaf(p[v], r.y, f[v] * r.x);
         }
     } else if (at < a.at.n_dims) {
         const bool first = a.mode == 0 ? at % 2 == 0 : at < half;
@@ -117,6 +137,25 @@ __device__ __forceinline__ void take(const T* p, float (&f)[V]) {
     const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(p);
 #pragma unroll
     for (int v = 0; v < V; v++) f[v] = to_f32(x.v[v]);
+}
+// The partners of unit `at` of the row at p; f stays as it is where there are none.
+template <class T, int V, bool TORN>
+__device__ __forceinline__ void take_partners(const QkArgs& a, const T* p, int at, float (&f)[V]) {
+    const int other = partner<V>(a, at);
+    if (other == at) return;
+    if (torn<V, TORN>(a, at)) {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int e = partner_of(a, at + v);
+            if (e >= 0) f[v] = to_f32(p[e]);
+        }
+    } else {
+        Pack<T, V> x;
+        if constexpr (TORN) __builtin_memcpy(&x, p + other, sizeof x);   // at any alignment
+        else x = *reinterpret_cast<const Pack<T, V>*>(p + other);
+#pragma unroll
+        for (int v = 0; v < V; v++) f[v] = to_f32(x.v[v]);
+    }
 }
 template <class T, int V>
 __device__ __forceinline__ void give(T* p, const float (&f)[V]) {
@@ -169,7 +208,7 @@ __device__ __forceinline__ bool outside(const QkArgs& a, float sum) {
 }
 
 // The weights of a lane's units and of their partners.
-template <int V, int K, bool PARTNERS>
+template <int V, int K, bool PARTNERS, bool TORN>
 struct Weights {
     float f[K][V], p[PARTNERS ? K : 1][V];
     __device__ __forceinline__ void load(const QkArgs& a, const float* w, int lane) {
@@ -177,12 +216,22 @@ struct Weights {
         for (int k = 0; k < K; k++) {
             const int u = lane + (k << a.log_lanes), at = min(u, a.units - 1) * V;
             weights<V>(w, at, f[k]);
-            if constexpr (PARTNERS) weights<V>(w, partner<V>(a, at), p[k]);
+            if constexpr (PARTNERS) {
+                if (torn<V, TORN>(a, at)) {
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        const int e = partner_of(a, at + v);
+                        p[k][v] = w && e >= 0 ? w[e] : 1.f;
+                    }
+                } else {
+                    weights<V>(w, partner<V>(a, at), p[k]);
+                }
+            }
         }
     }
 };
 
-template <class T, int V, int K>
+template <class T, int V, int K, bool TORN>
 __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
     extern __shared__ float2 cs[];       // [tile][n_dims / 2], then frequencies
     const int half = a.at.n_dims / 2;
@@ -196,7 +245,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
         Spot s(a, t0, tk0, min(group, total - 1) - tk0 * rows.d);
         Walk<const char> x(side.x, side.x1, side.x2, side.x3, s.h, s.i2, s.b, heads, tokens, rows.d, a.at.n.d);
         Walk<char> out(side.out, side.o1, side.o2, side.o3, s.h, s.i2, s.b, heads, tokens, rows.d, a.at.n.d);
-        Weights<V, K, true> w;
+        Weights<V, K, true, TORN> w;
         if (a.w_stride == 0) w.load(a, side.w, lane);
         for (unsigned row = group; row - group < total; row += groups, s.next(a, rows.d, heads, tokens, x, out)) {
             const bool valid = row < total;                          // every lane takes part in the sums
@@ -209,8 +258,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
                 for (int v = 0; v < V; v++) f[k][v] = p[k][v] = 0.f;
                 if (!valid || u >= a.units) continue;
                 take<T, V>(src + at, f[k]);
-                const int other = partner<V>(a, at);
-                if (other != at) take<T, V>(src + other, p[k]);
+                take_partners<T, V, TORN>(a, src, at, p[k]);
             }
             if (a.w_stride != 0) w.load(a, side.w ? side.w + (long long)s.h * a.w_stride : nullptr, lane);
 #pragma unroll
@@ -240,7 +288,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
                     f[k][v] = f[k][v] * rstd * w.f[k][v];
                     p[k][v] = p[k][v] * rstd * w.p[k][v];
                 }
-                rotate<V>(a, at, cs + s.tk * half, f[k], p[k]);
+                rotate<V, TORN>(a, at, cs + s.tk * half, f[k], p[k]);
                 give<T, V>(to + at, f[k]);
             }
         }
@@ -252,7 +300,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
 // Sums over the rows of dz x r are kept by the lanes that hold the elements, over the tokens of a block, of q and then of k:
 // where heads share weights, a group takes any row; where they do not (PER_HEAD), it keeps to a head, or takes its
 // heads one after another. Added up in LDS in order, and over the blocks by qk_fold_kernel.
-template <class T, int V, int K, bool PER_HEAD>
+template <class T, int V, int K, bool PER_HEAD, bool TORN>
 __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a) {
     extern __shared__ float2 cs[];       // [tile][n_dims / 2], frequencies, then sums [groups][units * V]
     const int half = a.at.n_dims / 2;
@@ -267,7 +315,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a)
         Walk<const char> x(side.x, side.x1, side.x2, side.x3, s.h, s.i2, s.b, heads, tokens, rows, a.at.n.d);
         Walk<const char> dy(side.dy, side.y1, side.y2, side.y3, s.h, s.i2, s.b, heads, tokens, rows, a.at.n.d);
         Walk<char> out(side.out, side.o1, side.o2, side.o3, s.h, s.i2, s.b, heads, tokens, rows, a.at.n.d);
-        Weights<V, K, false> w;
+        Weights<V, K, false, false> w;
         w.load(a, side.w ? side.w + (long long)s.h * a.w_stride : nullptr, lane);
         s.tk = tk0;
         for (unsigned round = 0; round < rounds; round++, s.next(a, rows, heads, tokens, x, dy, out)) {
@@ -282,13 +330,12 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a)
                 if (!valid || u >= a.units) continue;
                 take<T, V>(src + at, f[k]);
                 take<T, V>(dsrc + at, z[k]);
-                const int other = partner<V>(a, at);
-                if (other != at) take<T, V>(dsrc + other, p[k]);
+                take_partners<T, V, TORN>(a, dsrc, at, p[k]);
             }
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int u = lane + (k << a.log_lanes), at = u * V;
-                if (valid && u < a.units) rotate<V>(a, at, cs + s.tk * half, z[k], p[k]);
+                if (valid && u < a.units) rotate<V, TORN>(a, at, cs + s.tk * half, z[k], p[k]);
                 float xx[V], gx[V];
 #pragma unroll
                 for (int v = 0; v < V; v++) {
@@ -396,11 +443,12 @@ __global__ __launch_bounds__(1024) void qk_fold_kernel(const float* part, long l
 }
 
 // --------------------------------------------------------------------------------- host
-// The widest access (16, then 8 bytes, then an element) that every row's start, its length and, in mode 2, both halves allow.
-int width_of(std::initializer_list<const stx_tensor*> all, long long dim, const stx_rope_params* p, int size) {
+// The widest access (16, then 8 bytes, then an element) that every row's start and its length allow. (Where the halves of mode 2
+// had to allow it too, 15 x 775 tokens of 5 rows of 80 bf16 values, 38 of them rotated, took 129 us, now 38.)
+int width_of(std::initializer_list<const stx_tensor*> all, long long dim, int size) {
     for (int bytes : {16, 8}) {
         const int w = bytes / size;
-        bool ok = dim % w == 0 && (p->mode == 0 || p->n_dims / 2 % w == 0);
+        bool ok = dim % w == 0;
         for (const stx_tensor* t : all) ok = ok && rows_aligned(t, bytes);
         if (ok) return w;
     }
@@ -467,14 +515,20 @@ QkSide side(const stx_tensor* x, const stx_tensor* dy, const stx_tensor* out, co
     return s;
 }
 
-// Calls f(V, K) as constants: units of w elements, as many a lane as a row of them needs.
+// Calls f(V, K, TORN) as constants: units of w elements, as many a lane as a row of them needs, and whether halves end in them.
 template <class T, class F>
-void with_units(int w, int units, F&& f) {
+void with_units(int w, const QkArgs& a, F&& f) {
     constexpr int W = 16 / sizeof(T);
     auto lanes = [&](auto v) {
         constexpr int V = v();
-        if (units <= 64) f(v, std::integral_constant<int, 1>{});
-        else f(v, std::integral_constant<int, kQkDim / 64 / V>{});
+        auto torn = [&](auto t) {
+            if (a.units <= 64) f(v, std::integral_constant<int, 1>{}, t);
+            else f(v, std::integral_constant<int, kQkDim / 64 / V>{}, t);
+        };
+        if constexpr (V > 1) {
+            if (a.mode != 0 && a.at.n_dims / 2 % V != 0) return torn(std::true_type{});
+        }
+        torn(std::false_type{});
     };
     if (w == W) lanes(std::integral_constant<int, W>{});
     else if (w == W / 2) lanes(std::integral_constant<int, W / 2>{});
@@ -503,7 +557,7 @@ void qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const
         if (d) check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, weight_bytes(q, per_head)}, {"w_k", w_k, weight_bytes(k, per_head)}});
     if (s.empty()) return;
     STX_REQUIRE(pos != nullptr, "%s: pos is NULL", op);
-    const int w = width_of({q, k, q_dst, k_dst}, s.dim, p, size);
+    const int w = width_of({q, k, q_dst, k_dst}, s.dim, size);
     QkArgs a = args_of(q, s, at, p, pos, eps, per_head, w);
     a.q = side(q, nullptr, q_dst, w_q);
     if (k) a.k = side(k, nullptr, k_dst, w_k);
@@ -514,10 +568,10 @@ void qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const
     const size_t lds = sizeof(float2) * (tile + 1) * (a.at.n_dims / 2);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        with_units<T>(w, a.units, [&](auto v, auto n) {
+        with_units<T>(w, a, [&](auto v, auto n, auto torn) {
             launch_all((s.tokens + tile - 1) / tile, [&](dim3 grid, unsigned first) {
                 a.base = first;
-                hipLaunchKernelGGL((qk_norm_rope_kernel<T, v(), n()>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
+                hipLaunchKernelGGL((qk_norm_rope_kernel<T, v(), n(), torn()>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
                 launch_check("qk_norm_rope_kernel");
             });
         });
@@ -567,7 +621,7 @@ void qk_norm_rope_back(const stx_tensor* dyq, const stx_tensor* dyk, const stx_t
     long long blocks = 0;
     if (!s.empty()) {
         STX_REQUIRE(pos != nullptr, "%s: pos is NULL", op);
-        const int w = width_of({q, k, dyq, dyk, dq, dk}, s.dim, p, size);
+        const int w = width_of({q, k, dyq, dyk, dq, dk}, s.dim, size);
         QkArgs a = args_of(q, s, at, p, pos, eps, per_head, w);
         a.q = side(q, dyq, dq, w_q);
         if (k) a.k = side(k, dyk, dk, w_k);
@@ -577,11 +631,11 @@ void qk_norm_rope_back(const stx_tensor* dyq, const stx_tensor* dyk, const stx_t
         const size_t lds = sizeof(float2) * (tile + 1) * (p->n_dims / 2) + (sums ? sizeof(float) * (kQkThreads >> a.log_lanes) * a.units * w : 0);
         with_type(type, [&](auto t) {
             using T = decltype(t);
-            with_units<T>(w, a.units, [&](auto v, auto n) {
+            with_units<T>(w, a, [&](auto v, auto n, auto torn) {
                 launch_all(blocks, [&](dim3 grid, unsigned first) {
                     a.base = first;
-                    if (per_head) hipLaunchKernelGGL((qk_norm_rope_back_kernel<T, v(), n(), true>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
-                    else hipLaunchKernelGGL((qk_norm_rope_back_kernel<T, v(), n(), false>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
+                    if (per_head) hipLaunchKernelGGL((qk_norm_rope_back_kernel<T, v(), n(), true, torn()>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
+                    else hipLaunchKernelGGL((qk_norm_rope_back_kernel<T, v(), n(), false, torn()>), grid, dim3(kQkThreads), lds, as_stream(stream), a);
                     launch_check("qk_norm_rope_back_kernel");
                 });
             });

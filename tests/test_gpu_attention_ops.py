@@ -60,7 +60,12 @@ QK = [
     (3, 17, 4, 2, 64, 64, 0, {}, 5, "heads"),
     (2, 33, 4, 1, 128, 96, 2, YARN, 100000, "heads"),
     (2, 70, 32, 8, 128, 96, 2, YARN, 0, "heads"),               # more rows than groups of lanes
-    (2, 9, 3, 1, 80, 38, 2, dict(freq_scale=0.25), 1000, "shared"),   # 19 pairs: element by element
+    (2, 9, 3, 1, 80, 38, 2, dict(freq_scale=0.25), 1000, "shared"),   # 19 pairs: vectors over the halves' ends
+    (1, 9, 2, 1, 16, 2, 2, {}, 3, "heads"),                     # both ends in one vector
+    (2, 7, 2, 1, 8, 6, 2, {}, 3, "shared"),
+    (1, 9, 3, 1, 96, 46, 2, YARN, 1150, "heads"),
+    (1, 3, 1, 1, 600, 502, 2, YARN, 40, "shared"),
+    (1, 3, 2, 1, 1024, 1022, 2, {}, 40, "heads"),
     (2, 9, 3, 1, 80, 38, 0, dict(freq_scale=0.25), 1000, "none"),     # the last rotated pair inside a vector
     (2, 9, 3, 1, 80, 40, 2, {}, 3, "heads"),                    # halves of 20: vectors of 8 bytes
     (1, 700, 2, 2, 32, 30, 0, {}, 0, "shared"),
