@@ -14,7 +14,7 @@ namespace {
 // one product are, where they stand, the operand of the next, whose other operand is read transposed from the tile.
 //
 // dS and P are rounded to 16 bits for their products (16-bit data). fp16's range would cut them: P is
-// scaled by 2^8, and dP - D by a power of two of the row (first kernel) or the call (second) that keeps
+// scaled by 2^8 (the second kernel's by less where lambda is large), and dP - D by a power of two of the row (first kernel) or the call (second) that keeps
 // 2^8 P (dP - D) max(1, |lambda|) below 2^15, from |dP - D| <= 2 V max|v| max|dy|.
 //
 // 16,384 x 16,384 causal, 8 heads to 2, bf16: 1,030 us (801 TFLOP/s of the first kernel's products; vector units 68 %, matrix cores 39 %
@@ -259,11 +259,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
     ql.space(a.q.s2, a.q.s1);
     yl.space(a.dy.s2, 0);
     float held[5];                       // a row's stats on their way
-    float unit = 1.f;
+    float unit = 1.f, shift = kShift<T>;
     if constexpr (std::is_same_v<T, f16>) {
         float lam = 0.f;
         for (int g = 0; g < a.group; g++) lam = fmaxf(lam, fabsf(a.lam[kvh * a.group + g]));
-        unit = range_scale(a, a.most[1], lam);
+        // P1 - lambda P2 is dv's operand: from |lambda| 2^6 on both maps give way, so that 2^shift |lambda| stays below 2^14.
+        const float over = fminf(fmaxf(ceilf(__builtin_amdgcn_logf(lam)) - 6.f, 0.f), 100.f);
+        shift -= over;
+        unit = range_scale(a, a.most[1], lam) * __builtin_amdgcn_exp2f(over);
     }
     auto fetch = [&](int head, int i0, int stage) {
         const char* q = a.q.p + 2LL * head * a.q.s1 + i0 * a.q.s2 + b * a.q.s3;
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
             const long long at = ((long long)b * a.heads + head) * 2 * a.queries + i;
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                held[m] = fmaf(a.lse[at + m * a.queries], kLog2e, -kShift<T>);
+                held[m] = fmaf(a.lse[at + m * a.queries], kLog2e, -shift);
                 held[2 + m] = a.dots[at + m * a.queries] * unit;
             }
             held[4] = __int_as_float(i0 + tid < a.queries ? mask.limit(i) : 0);
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
         }
         stage ^= 1;
     }
-    const float fk = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / unit, fv = __builtin_amdgcn_exp2f(-kShift<T>);
+    const float fv = __builtin_amdgcn_exp2f(-shift), fk = a.scale * fv / unit;
     if (key >= a.keys) return;
     float* to = a.part ? a.part + (((long long)part * (gridDim.x / a.tile_div.d) + per) * a.keys + key) * (2 * DP + VP) : nullptr;
 #pragma unroll
