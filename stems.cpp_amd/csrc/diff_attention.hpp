@@ -25,7 +25,9 @@ struct DiffArgs {
     float* lse;                          // [sequence][head][map][query]
     float* dots;                         // backward: dy . o of each map, laid out as lse
     double* tiles_lam;                   // backward: a block's shares of lambda's gradient, [block][group]
-    const float* most;                   // fp16's backward: largest |v| and |dy| of the call
+    const float* most;                   // fp16's backward: largest |v| of a tile of keys, [sequence][key head][tile],
+    float* loud;                         // and largest |dy| max(1, |lambda|) of a wave's rows, [sequence][key head][loud_count]
+    int loud_rows, loud_count;
     float* part;                         // split keys (forward) or rows (keys' gradients)
     float* part_stat;
     const int *lengths, *starts;

@@ -14,20 +14,30 @@ namespace {
 // one product are, where they stand, the operand of the next, whose other operand is read transposed from the tile.
 //
 // dS and P are rounded to 16 bits for their products (16-bit data). fp16's range would cut them: P is
-// scaled by 2^8 (the second kernel's by less where lambda is large), and dP - D by a power of two of the row (first kernel) or the call (second) that keeps
-// 2^8 P (dP - D) max(1, |lambda|) below 2^15, from |dP - D| <= 2 V max|v| max|dy|.
+// scaled by 2^8 (the second kernel's by less where lambda is large), and dP - D by a power of two that keeps
+// 2^8 P (dP - D) max(1, |lambda|) below 2^15, from |dP - D| <= 2 V max|v| max|dy|. The maxima are those of what meets in a block,
+// so that what other sequences, key heads and hidden keys hold costs no bits: in the first kernel, a row's dy and
+// the values up to the last key that the block's rows see; in the second, the key head's values and the rows that see a key
+// of the block. (With the call's maxima a sequence of gradients 2^16 below another's kept 7 bits. A power for each key or
+// row, lowered as elements pass fp16's range, cost 13 % of the first kernel and 7 of the second.)
 //
 // 16,384 x 16,384 causal, 8 heads to 2, bf16: 1,030 us (801 TFLOP/s of the first kernel's products; vector units 68 %, matrix cores 39 %
 // busy) and 1,725 us (637 TFLOP/s; 42 and 28 %): a wave of 16 keys reads the rows' q and dy from LDS both ways, 32 KB for 32
 // matrix instructions, twice what the 32 rows of a wave of the first need; 32 keys do not fit the registers of two waves a
 // SIMD (v in LDS instead: 45 of them spilled, the call 3,670 us where it is 2,650), and one wave a SIMD was no faster. 1,344 x 2,688, 4 heads, fp32: 120 and 188 us, matrix cores 71 and 65 % busy.
+constexpr int kMostKeys = 64;            // keys of a block of the second kernel, and of a largest |v|
 template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 8.f : 0.f;
 
-__device__ __forceinline__ float range_scale(const DiffArgs& a, float dy, float lam) {
-    const float bound = 2.f * a.vdim * a.most[0] * dy * fmaxf(1.f, fabsf(lam));
-    if (!(bound > 0.f && bound < 0x1p120f)) return 1.f;
-    return __builtin_amdgcn_exp2f(fminf(fmaxf(7.f - ceilf(__builtin_amdgcn_logf(bound)), -100.f), 100.f));
+__device__ __forceinline__ float range_scale(const DiffArgs& a, float v, float dy, float shift) {
+    return __builtin_amdgcn_exp2f(fminf(fmaxf(15.f - shift - ceilf(__builtin_amdgcn_logf(2.f * a.vdim * v * dy)), -100.f), 100.f));
+}
+// The largest of values [from, to) at p, by `threads` threads of which this is `t`: this thread's share.
+__device__ __forceinline__ float largest(const float* p, int from, int to, int t, int threads) {
+    float most = 0.f;
+#pragma unroll 4
+    for (int i = from + t; i < to; i += threads) most = fmaxf(most, p[i]);
+    return most;
 }
 
 template <class T, int DP, int VP, int NQ, bool ALIGNED>
@@ -72,6 +82,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
     float base[2][NQ], dot[2][NQ], lam[NQ], unit[NQ];                 // lse in units of log2; D; of the row
     float share[NQ], rest[NQ];           // of lambda's gradient; what rounding left of it
     const float c = a.scale * kLog2e;
+    float values = 0.f, loud = 0.f;      // fp16: largest |v| of the keys that the block sees; largest |dy| max(1, |lambda|) of the wave's rows
+    if constexpr (std::is_same_v<T, f16>)
+        values = lane_max<64>(largest(a.most + (long long)per * ((a.keys + kMostKeys - 1) / kMostKeys), 0, (most + kMostKeys - 1) / kMostKeys, lane, 64));
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int r = r0 + (wave * NQ + n) * 16 + s;
@@ -108,9 +121,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
             if (lane < 16 && r < a.rows && part == 0) a.dots[at] = dot[m][n];
         }
         if constexpr (std::is_same_v<T, f16>) {
-            unit[n] = range_scale(a, most, lam[n]);
+            most *= fmaxf(1.f, fabsf(lam[n]));
+            unit[n] = range_scale(a, values, most, kShift<T>);
+            loud = fmaxf(loud, most);
             dot[0][n] *= unit[n], dot[1][n] *= unit[n];
         }
+    }
+    if constexpr (std::is_same_v<T, f16>) {
+        loud = lane_max<64>(loud);
+        if (lane == 0 && part == 0) a.loud[((long long)per * a.tiles + tile) * 4 + wave] = loud;
     }
     f32x4 acc[2][NQ][ND] = {};
     constexpr int KS = KG;
@@ -235,7 +254,7 @@ struct RowStats {
 
 template <class T, int DP, int VP, bool ALIGNED>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_dkv_kernel(DiffArgs a) {
-    constexpr int NT = 256, RG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, NV = VP / 16, KEYS = 64;
+    constexpr int NT = 256, RG = Tile<T, DP>::KEYS, GD = Tile<T, DP>::GROUPS, GV = Tile<T, VP>::GROUPS, ND = DP / 16, NV = VP / 16, KEYS = kMostKeys;
     using QL = Loader<T, DP, kRows, 2, NT, ALIGNED>;
     using YL = Loader<T, VP, kRows, 1, NT, ALIGNED>;
     constexpr int STAGE = QL::BYTES + YL::BYTES;
@@ -264,9 +283,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
         float lam = 0.f;
         for (int g = 0; g < a.group; g++) lam = fmaxf(lam, fabsf(a.lam[kvh * a.group + g]));
         // P1 - lambda P2 is dv's operand: from |lambda| 2^6 on both maps give way, so that 2^shift |lambda| stays below 2^14.
-        const float over = fminf(fmaxf(ceilf(__builtin_amdgcn_logf(lam)) - 6.f, 0.f), 100.f);
-        shift -= over;
-        unit = range_scale(a, a.most[1], lam) * __builtin_amdgcn_exp2f(over);
+        shift -= fminf(fmaxf(ceilf(__builtin_amdgcn_logf(lam)) - 6.f, 0.f), 100.f);
+        __shared__ float red[2][4];
+        const int waves = (a.rows + a.loud_rows - 1) / a.loud_rows;
+        const float v = lane_max<64>(largest(a.most + (long long)per * a.tiles, 0, a.tiles, tid, NT));
+        const float y = lane_max<64>(largest(a.loud + (long long)per * a.loud_count, (int)((long long)first * a.group / a.loud_rows), waves, tid, NT));
+        if (lane == 0) red[0][wave] = v, red[1][wave] = y;
+        __syncthreads();
+        unit = range_scale(a, fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])), fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])), shift);
     }
     auto fetch = [&](int head, int i0, int stage) {
         const char* q = a.q.p + 2LL * head * a.q.s1 + i0 * a.q.s2 + b * a.q.s3;
@@ -442,41 +466,26 @@ __global__ __launch_bounds__(256) void diff_lambda_kernel(const double* shares, 
     if (threadIdx.x == 0) dlam[blockIdx.x] = (float)-((red[0] + red[1]) + (red[2] + red[3]));
 }
 
-// fp16: the largest |v| and |dy| of the call, of each block and then of all (8,192 waves' atomics on two words took 196 us).
-constexpr int kMostBlocks = 1024;
-struct MostArgs {
-    Strided t[2];
-    long long rows[2];
-    FastDiv d1[2], d2[2];                // row -> (heads), (tokens)
-    int width, log_lanes;                // elements of a row, and lanes that hold 8 each of one
-    const int* lengths;
-    float* most;                         // [2], then [2][kMostBlocks]
-};
-__global__ __launch_bounds__(256) void diff_most_kernel(MostArgs a) {
-    const int which = blockIdx.y, lane = threadIdx.x % 64, chunk = lane & ((1 << a.log_lanes) - 1), left = a.width - chunk * 8;
+// fp16: the largest |v| of each kMostKeys keys of a (sequence, key head), a block each; keys past the length are not there.
+__global__ __launch_bounds__(256) void diff_most_kernel(DiffArgs a, int tiles, float* mosts) {
+    const unsigned per = blockIdx.x / tiles;
+    const int key0 = (int)(blockIdx.x - per * tiles) * kMostKeys, b = (int)a.kv_div.div(per), kvh = (int)(per - b * a.kv_div.d);
+    const Mask mask(a, b);
+    const int chunks = (a.vdim + 7) / 8, rows = min(kMostKeys, mask.length - key0);
     float most = 0.f;
-    const long long step = (long long)gridDim.x * (256 >> a.log_lanes);
 #pragma unroll 4
-    for (long long r = blockIdx.x * (256LL >> a.log_lanes) + (threadIdx.x >> a.log_lanes); r < a.rows[which]; r += step) {
-        const unsigned i = a.d1[which].div((unsigned)r), h = (unsigned)r - i * a.d1[which].d, b = a.d2[which].div(i), n = i - b * a.d2[which].d;
-        if (left <= 0 || (which == 0 && a.lengths && (int)n >= a.lengths[b])) continue;     // keys that are not there
+    for (int e = threadIdx.x; e < rows * chunks; e += 256) {
+        const int r = e / chunks, c = e - r * chunks;
         float f[8];
-        unpack<f16>(load_chunk<f16>(a.t[which].p + h * a.t[which].s1 + n * a.t[which].s2 + b * a.t[which].s3 + chunk * 16, left), f);
+        unpack<f16>(load_chunk<f16>(a.v.p + (long long)kvh * a.v.s1 + (key0 + r) * a.v.s2 + b * a.v.s3 + c * 16, a.vdim - c * 8), f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(f[e]));
+        for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(f[i]));
     }
     __shared__ float red[4];
     most = lane_max<64>(most);
-    if (lane == 0) red[threadIdx.x / 64] = most;
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = most;
     __syncthreads();
-    if (threadIdx.x == 0) a.most[2 + which * kMostBlocks + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-__global__ __launch_bounds__(128) void diff_most_of_all_kernel(float* most, int blocks) {
-    const int which = threadIdx.x / 64;
-    float m = 0.f;
-    for (int i = threadIdx.x % 64; i < blocks; i += 64) m = fmaxf(m, most[2 + which * kMostBlocks + i]);
-    m = lane_max<64>(m);
-    if (threadIdx.x % 64 == 0) most[which] = m;
+    if (threadIdx.x == 0) mosts[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
 // --------------------------------------------------------------------------------- host
@@ -485,7 +494,7 @@ size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 struct BackPlan {
     int nq, dp, vp, q_splits, k_splits;
     long long q_tiles, k_tiles;
-    size_t dots, tiles_lam, most, part, total;
+    size_t dots, tiles_lam, most, loud, part, total;
 };
 BackPlan back_plan(const DiffShape& s, int size, bool causal) {
     BackPlan p{};
@@ -494,7 +503,7 @@ BackPlan back_plan(const DiffShape& s, int size, bool causal) {
     with_dims(s.D, s.V, [&](auto d, auto v) { p.dp = d(), p.vp = v(); });
     p.nq = small && rows > 64 ? 2 : 1;
     p.q_tiles = (rows + 64 * p.nq - 1) / (64 * p.nq);
-    p.k_tiles = (s.N + 63) / 64;
+    p.k_tiles = (s.N + kMostKeys - 1) / kMostKeys;
     // Parts of the keys or rows: as many as give two blocks a CU, or eight where causality makes tiles differ in length,
     // of 256 keys or rows at least.
     const long long want = (causal ? 8LL : 4LL) * kCus;
@@ -507,7 +516,8 @@ BackPlan back_plan(const DiffShape& s, int size, bool causal) {
     };
     p.dots = take((size_t)s.B * s.H * 2 * s.M * sizeof(float));
     p.tiles_lam = take((size_t)((rows + 63) / 64) * p.q_splits * s.B * s.H * sizeof(double));   // of the smallest tiles
-    p.most = take((2 + 2 * kMostBlocks) * sizeof(float));
+    p.most = take((size_t)p.k_tiles * pairs * sizeof(float));
+    p.loud = take((size_t)((rows + 63) / 64) * 4 * pairs * sizeof(float));                      // of the smallest tiles
     const size_t q_part = p.q_splits > 1 ? (size_t)p.q_splits * pairs * rows * 2 * p.dp : 0;
     const size_t k_part = p.k_splits > 1 ? (size_t)p.k_splits * pairs * s.N * (2 * p.dp + p.vp) : 0;
     p.part = take(std::max(q_part, k_part) * sizeof(float));         // one after the other
@@ -601,31 +611,22 @@ STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tenso
         a.tiles_lam = reinterpret_cast<double*>(ws + p.tiles_lam);
         float* most = reinterpret_cast<float*>(ws + p.most);
         a.most = most;
+        a.loud = reinterpret_cast<float*>(ws + p.loud);
         const hipStream_t st = as_stream(stream);
         const long long pairs = s.B * s.Hk;
         const bool keys_aligned = rows_in_chunks(k, size) && rows_in_chunks(v, size), rows_aligned = rows_in_chunks(q, size) && rows_in_chunks(dy, size);
         if (!keys_aligned && p.nq > 1) p.nq = 1, p.q_tiles = (a.rows + 63) / 64;
+        a.loud_rows = 16 * p.nq, a.loud_count = 4 * (int)p.q_tiles;
         STX_REQUIRE(p.q_tiles * p.q_splits * pairs < (1LL << 22) && p.k_tiles * p.k_splits * pairs < (1LL << 22), "%s: too many tiles", op);
         auto fold_blocks = [&](long long quads) { return dim3((unsigned)((quads + 255) / 256)); };   // split calls have few tiles
         with_type(type, [&](auto t) {
             using T = decltype(t);
             with_dims(s.D, s.V, [&](auto d, auto vd) {
                 if constexpr (std::is_same_v<T, f16>) {
-                    MostArgs m{};
-                    m.t[0] = a.v, m.t[1] = a.dy;
-                    m.rows[0] = s.B * s.N * s.Hk, m.rows[1] = s.B * s.M * s.H;
-                    m.d1[0] = FastDiv((unsigned)s.Hk), m.d1[1] = FastDiv((unsigned)s.H);
-                    m.d2[0] = FastDiv((unsigned)std::max(1LL, s.N)), m.d2[1] = FastDiv((unsigned)std::max(1LL, s.M));
-                    m.width = s.V;
-                    while (8 << m.log_lanes < s.V) m.log_lanes++;
-                    m.lengths = lengths;
-                    m.most = most;
-                    STX_REQUIRE(m.rows[0] < (1LL << 32) && m.rows[1] < (1LL << 32), "%s: 2^32 rows or more", op);
-                    const int blocks = (int)std::max(1LL, std::min<long long>(kMostBlocks, (std::max(m.rows[0], m.rows[1]) << m.log_lanes) / 1024));
-                    hipLaunchKernelGGL(diff_most_kernel, dim3(blocks, 2), dim3(256), 0, st, m);
-                    launch_check("diff_most_kernel");
-                    hipLaunchKernelGGL(diff_most_of_all_kernel, dim3(1), dim3(128), 0, st, most, blocks);
-                    launch_check("diff_most_of_all_kernel");
+                    if (s.N > 0) {
+                        hipLaunchKernelGGL(diff_most_kernel, dim3((unsigned)(p.k_tiles * pairs)), dim3(256), 0, st, a, (int)p.k_tiles, most);
+                        launch_check("diff_most_kernel");
+                    }
                 }
                 float* part = reinterpret_cast<float*>(ws + p.part);
                 if (s.M > 0) {

@@ -36,3 +36,68 @@ def test_diff_large_lambda(device, dtype, Hk, lams):
         close(g, w, bound + (held if name == "dv" else 0.0), "lambda " + name)
         if name != "dlam":
             norm_close(g, w, 2, "lambda " + name)
+
+
+def back_of(part, got, dy, q, k, v, lam, kept, mask, scale, what):
+    """dq, dk and dv against those of these operands alone; dk and dv of the keys `part`."""
+    want = diff_back_ref(dy, q, k, v, lam, *kept, mask, scale)
+    for g, (w, bound), name in zip(got, want, ("dq", "dk", "dv")):
+        w, bound = (t[:, part] if name != "dq" else t for t in (w, bound))
+        close(g, w, bound, f"{what} {name}")
+        norm_close(g, w, 2, f"{what} {name}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lowered", ["dy", "v"])
+def test_diff_back_of_a_quiet_sequence(device, dtype, lowered):
+    """A sequence whose dy, or v, is 2^16 or 2^13 times smaller than another's of the batch has the accuracy that it has alone."""
+    B, M, N, H, Hk, D, V = 2, 200, 200, 2, 1, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    dy = randn(device, (B, M, H, V), 7, 1.0)
+    if lowered == "dy":
+        dy[0] *= 2.0 ** 10
+        dy[1] *= 2.0 ** -6
+    else:
+        v[0] *= 2.0 ** 9
+        v[1] *= 2.0 ** -4
+    dy = dy.to(q.dtype)
+    kept = stx.diff_attention(q, k, v, lam, keep=True)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept)
+    mask = torch.ones(1, M, N, dtype=torch.bool, device=device)
+    back_of(slice(None), [t[1:] for t in got[:3]], dy[1:], q[1:], k[1:], v[1:], lam, [t[1:] for t in kept], mask, D ** -0.5, "quiet")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_diff_back_of_a_quiet_key_head(device, dtype):
+    """A key head whose values are 2^13 times smaller than its neighbour's."""
+    B, M, N, H, Hk, D, V = 1, 200, 200, 4, 2, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    v[:, :, 0] *= 2.0 ** 9
+    v[:, :, 1] *= 2.0 ** -4
+    dy = randn(device, (B, M, H, V), 7, dtype=q.dtype)
+    kept = stx.diff_attention(q, k, v, lam, keep=True)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept)
+    mask = torch.ones(B, M, N, dtype=torch.bool, device=device)
+    of = lambda t, heads: t[:, :, heads:]  # noqa: E731
+    back_of(slice(None), [of(got[0], 4), of(got[1], 2), of(got[2], 1)], of(dy, 2), of(q, 4), of(k, 2), of(v, 1), lam[2:],
+            [of(kept[0], 2), of(kept[1], 2), kept[2][:, 2:]], mask, D ** -0.5, "head")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,quiet", [(200, 90), (700, 290)])
+def test_diff_back_of_quiet_last_rows(device, dtype, M, quiet):
+    """The last queries of a causal sequence have gradients 2^16 times smaller than the others: the blocks of 64 keys that only
+    they see, and their own dq, keep the accuracy that those rows alone give."""
+    B, H, Hk, D, V = 1, 2, 1, 64, 128
+    first = M - quiet
+    keys = (first + 16 + 63) // 64 * 64
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, M, H, Hk, D, V, True, None))
+    dy = randn(device, (B, M, H, V), 7, 2.0 ** 10)
+    dy[:, first:] *= 2.0 ** -16
+    dy = dy.to(q.dtype)
+    kept = stx.diff_attention(q, k, v, lam, causal=True, keep=True)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept, causal=True)
+    mask, _ = seen_ref(B, M, M, None, None, True, device)
+    of = lambda t: t[:, first:]  # noqa: E731
+    back_of(slice(keys, None), [of(got[0]), got[1][:, keys:], got[2][:, keys:]], of(dy), of(q), k, v, lam, [of(kept[0]), of(kept[1]), kept[2][..., first:]],
+            mask[:, first:], D ** -0.5, "rows")
