@@ -889,14 +889,16 @@ STX_API size_t     stx_group_norm_cl_forward_workspace_size(const stx_tensor* a,
  * w_q and w_k: device float[dim], or with per_head != 0 float[heads][dim] and float[kv heads][dim]; either may be
  * NULL (1). pos, pos_stride and params as in stx_rope_scaled; so are strides, limits and the outputs that may be the
  * inputs. A row's mean square is added in double from sums of at most 16 squares in float (in double where they leave
- * fp32's range); the rest is float, rounded once. Rows of up to 1,024 elements; eps >= 0. */
+ * fp32's range); the rest is float, rounded once. A row whose sqrt(mean(x^2) + eps) is below 2^-128, so that its
+ * reciprocal is no float, gives infinities. Rows of up to 1,024 elements; eps >= 0. */
 STX_API stx_status stx_qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
                                     int64_t pos_stride, const stx_rope_params* params, const float* w_q,
                                     const float* w_k, int per_head, double eps, const stx_tensor* q_dst,
                                     const stx_tensor* k_dst, stx_stream stream);
 /* Its gradients, from dq_out and dk_out (of q_dst and k_dst) and the forward call's inputs: dq and dk (of q and k;
  * each may be the gradient that it comes from, or its q or k), dw_q and dw_k (of the weights, in their layout, summed
- * over tokens and batch and, where heads share them, over heads). Any may be NULL. workspace: device, 256-byte
+ * over tokens and batch and, where heads share them, over heads). Any may be NULL. The rotated gradient times w is float; the
+ * rest holds for x of any size. workspace: device, 256-byte
  * aligned, no initialisation; calls that share one must not overlap. None is needed without dw_q and dw_k. */
 STX_API size_t     stx_qk_norm_rope_back_workspace_size(const stx_tensor* q, const stx_tensor* k, stx_type type,
                                                         int n_dims, int per_head);

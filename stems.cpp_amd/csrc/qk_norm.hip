@@ -9,14 +9,14 @@ namespace {
 
 // A row x of one head (of q or k) gives y = R(pos) (w x r), r = 1 / sqrt(mean(x^2) + eps), R the rotation
 // of rope.hip. Its gradient: dz = R^T dy, dw = sum over the rows of dz x r, and with g = w dz
-//   dx = r (g - x r^2 mean(g x)).
+//   dx = r (g - x r mean(g x r)).
 // Both read and write every element once (the gradient reads x again instead of r), so HBM bounds them.
 // A row is held by `lanes` lanes of a wave, V elements a unit and K units a lane, all of them loaded
 // before the first is stored: outputs may be inputs. A lane whose pair partner lies in another unit
 // (mode 2, or units of one element) loads it too, from the same lines: units stay dense for any
 // n_dims, where units of a pair of halves would leave 6 of 16 lanes idle at 128 elements, 96 rotated.
-// A lane's squares and products g x are added in float, by halves (three roundings at V 8), the lanes' in double; a wave that
-// meets a row whose squares leave fp32 forms them again in double, so data of any size keeps its norm. (In
+// A lane's squares and products g x r (of g's size for any x) are added in float, by halves (three roundings at V 8), the lanes' in double; a wave that
+// meets a row whose squares leave fp32 forms them again in double, so data of any size keeps its norm; so are products past 10^30. (In
 // double throughout, with a double division and root, these took more time than the memory's: the gradient of 2 x
 // 16,384 tokens of 40 rows of 128 bf16 values 297 us.)
 // 60 x 801 tokens of 16 rows of 64 fp32 values, slices of a projection (394 MB): 79 us, 5.0 TB/s, the rate of a large copy;
@@ -300,8 +300,13 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkArgs a) {
 // Sums over the rows of dz x r are kept by the lanes that hold the elements, over the tokens of a block, of q and then of k:
 // where heads share weights, a group takes any row; where they do not (PER_HEAD), it keeps to a head, or takes its
 // heads one after another. Added up in LDS in order, and over the blocks by qk_fold_kernel.
+// Waves a SIMD that a row of eight elements a lane is held to (98 registers instead of 96 in fp16 leave four: 104 us
+// instead of 80 for 60 x 801 tokens of 16 rows of 64).
+template <int V, int K, bool PER_HEAD, bool TORN>
+constexpr int kBackWaves = V * K > 8 ? 1 : V < 8 || TORN ? 4 : PER_HEAD ? 5 : 6;
+
 template <class T, int V, int K, bool PER_HEAD, bool TORN>
-__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a) {
+__global__ __launch_bounds__(kQkThreads, (kBackWaves<V, K, PER_HEAD, TORN>)) void qk_norm_rope_back_kernel(QkArgs a) {
     extern __shared__ float2 cs[];       // [tile][n_dims / 2], frequencies, then sums [groups][units * V]
     const int half = a.at.n_dims / 2;
     const unsigned block = a.base + blockIdx.x, t0 = block * a.tile, nt = min(a.tile, a.tokens - t0);
@@ -336,29 +341,42 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a)
             for (int k = 0; k < K; k++) {
                 const int u = lane + (k << a.log_lanes), at = u * V;
                 if (valid && u < a.units) rotate<V, TORN>(a, at, cs + s.tk * half, z[k], p[k]);
-                float xx[V], gx[V];
+                float xx[V];
 #pragma unroll
                 for (int v = 0; v < V; v++) {
                     xx[v] = f[k][v] * f[k][v];
                     p[k][v] = w.f[k][v] * z[k][v];
-                    gx[v] = p[k][v] * f[k][v];
                 }
                 squares += by_halves<V>(xx);
-                products += by_halves<V>(gx);
             }
-            double sxx = squares, sgx = products;
+            double sum = squares;
             if (outside(a, squares)) {
-                sxx = sgx = 0.0;
+                sum = 0.0;
 #pragma unroll
                 for (int k = 0; k < K; k++)
 #pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        sxx = fma((double)f[k][v], (double)f[k][v], sxx);
-                        sgx = fma((double)p[k][v], (double)f[k][v], sgx);
-                    }
+                    for (int v = 0; v < V; v++) sum = fma((double)f[k][v], (double)f[k][v], sum);
             }
-            const float rstd = inverse_root(fma(lane_sum_dyn(sxx, lanes), a.per_dim, a.eps));
-            const float mean = (float)(lane_sum_dyn(sgx, lanes) * a.per_dim * (double)rstd);
+            const float rstd = inverse_root(fma(lane_sum_dyn(sum, lanes), a.per_dim, a.eps));
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                float gx[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    f[k][v] *= rstd;
+                    gx[v] = p[k][v] * f[k][v];
+                }
+                products += by_halves<V>(gx);
+            }
+            sum = products;
+            if (__builtin_amdgcn_ballot_w64(!(fabsf(products) < 1e30f))) {
+                sum = 0.0;
+#pragma unroll
+                for (int k = 0; k < K; k++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) sum = fma((double)p[k][v], (double)f[k][v], sum);
+            }
+            const float mean = (float)(lane_sum_dyn(sum, lanes) * a.per_dim);
             if (!valid) continue;
             T* to = reinterpret_cast<T*>(out.p);
 #pragma unroll
@@ -367,9 +385,8 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_back_kernel(QkArgs a)
                 if (u >= a.units) continue;
 #pragma unroll
                 for (int v = 0; v < V; v++) {
-                    const float xh = f[k][v] * rstd;
-                    acc[k][v] = fmaf(z[k][v], xh, acc[k][v]);
-                    f[k][v] = rstd * fmaf(-xh, mean, p[k][v]);
+                    acc[k][v] = fmaf(z[k][v], f[k][v], acc[k][v]);
+                    f[k][v] = rstd * fmaf(-f[k][v], mean, p[k][v]);
                 }
                 if (side.out) give<T, V>(to + at, f[k]);
             }

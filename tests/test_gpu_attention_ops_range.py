@@ -1,12 +1,12 @@
-"""The attention operators (diff_attention*.hip) at values far from 1. Bounds are those of test_gpu_attention_ops.py, with what
-each test adds to them."""
+"""The attention operators (qk_norm.hip, diff_attention*.hip) at values far from 1. Bounds are those of test_gpu_attention_ops.py,
+with what each test adds to them."""
 import math
 
 import pytest
 
 import stx
-from test_gpu_attention_ops import check_diff, diff_back_ref, diff_inputs, seen_ref
-from test_gpu_layer_ops import F64, TYPES, close, norm_close, randn
+from test_gpu_attention_ops import check_diff, diff_back_ref, diff_inputs, qk_back_ref, seen_ref
+from test_gpu_layer_ops import F64, TYPES, U, close, norm_close, randn
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -101,3 +101,19 @@ def test_diff_back_of_quiet_last_rows(device, dtype, M, quiet):
     of = lambda t: t[:, first:]  # noqa: E731
     back_of(slice(keys, None), [of(got[0]), got[1][:, keys:], got[2][:, keys:]], of(dy), of(q), k, v, lam, [of(kept[0]), of(kept[1]), kept[2][..., first:]],
             mask[:, first:], D ** -0.5, "rows")
+
+
+# ------------------------------------------------------------------------- norms and rotation
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 1024, 33])
+@pytest.mark.parametrize("x_size,dy_size,eps", [(1e14, 1e25, 1e-6), (1e16, 1e30, 0.0), (1e-10, 1e-30, 0.0), (1e-18, 1e-25, 0.0), (1e25, 1e12, 0.0),
+                                                (1e-25, 1e-8, 0.0)])
+def test_qk_back_products_that_leave_fp32(device, dtype, D, x_size, dy_size, eps):
+    """Rows whose products w dy x are not floats, or below their normal range, while the squares and the gradient are."""
+    B, N, H = 2, 9, 3
+    x, dy = randn(device, (B, N, H, D), 1, x_size, dtype=TYPES[dtype]), randn(device, (B, N, H, D), 2, dy_size, dtype=TYPES[dtype])
+    w, pos = randn(device, (D,), 3, 0.3, 1.0), torch.arange(3, 3 + N, device=device, dtype=torch.int32)
+    dx, dw, _, _ = stx.qk_norm_rope_back(dy, x, pos, stx.rope_params(32), w, eps=eps)
+    want, bound, dww, dwm = qk_back_ref(dy, x, w, pos, eps, 32, 0)
+    close(dx, want, bound, "dx")
+    close(dw, dww.sum((0, 1, 2)), (8 + 4 * math.sqrt(B * N * H)) * U * dwm.sum((0, 1, 2)), "dw")
