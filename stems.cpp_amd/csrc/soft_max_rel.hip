@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
             const int r = min(r0 + group, it.rows - 1);
             const bool valid = r0 + group < it.rows;
             const long long at = it.at(r);
-            const int limit = it.limit(a, r);
+            const int limit = K > 0 || valid ? it.limit(a, r) : 0;       // K 0 in place: a row is its lanes' alone
             T* out = reinterpret_cast<T*>(os + r * a.o1);
             float m = -__builtin_inff(), s = 0.f;
             turn ^= 1;
@@ -295,6 +295,7 @@ __global__ __launch_bounds__(kRelThreads) void soft_max_rel_kernel(RelArgs a) {
                 s = sum_over(s * natural_exp(m - top), min(lanes, 64));
                 join_waves<WAVES>(top, s, red, turn);
                 const float inv = s == 0.f ? 0.f : 1.f / s;
+                if (!valid) continue;
                 for (int c = lane; c < vectors; c += lanes) {
                     Pack<T, V> y{};
                     if (c * V < limit) {

@@ -1,5 +1,5 @@
-"""The attention operators (qk_norm.hip, diff_attention*.hip) at values far from 1. Bounds are those of test_gpu_attention_ops.py,
-with what each test adds to them."""
+"""The attention operators (qk_norm.hip, soft_max_rel.hip, diff_attention*.hip) at values far from 1, and in place in short rows.
+Bounds are those of test_gpu_attention_ops.py, with what each test adds to them."""
 import math
 
 import pytest
@@ -117,3 +117,18 @@ def test_qk_back_products_that_leave_fp32(device, dtype, D, x_size, dy_size, eps
     want, bound, dww, dwm = qk_back_ref(dy, x, w, pos, eps, 32, 0)
     close(dx, want, bound, "dx")
     close(dw, dww.sum((0, 1, 2)), (8 + 4 * math.sqrt(B * N * H)) * U * dwm.sum((0, 1, 2)), "dw")
+
+
+# ------------------------------------------------------------------ softmax with a position bias
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 2, 3, 5, 7])
+@pytest.mark.parametrize("M", [5, 61, 300])
+def test_rel_short_rows_in_place(device, dtype, N, M):
+    """Rows shorter than a vector, a lane each: in place the bits of a call into other memory."""
+    B, H, dt = 40, 8, TYPES[dtype]
+    x, table, p = randn(device, (B, H, M, N), 1, 4.0, dtype=dt), randn(device, (32, H), 2), stx.rel_params()
+    want = stx.soft_max_rel(x, table, p)
+    for _ in range(3):
+        y = x.clone()
+        stx.soft_max_rel(y, table, p, out=y)
+        assert torch.equal(y, want)
