@@ -1,12 +1,12 @@
-"""The attention operators (qk_norm.hip, soft_max_rel.hip, diff_attention*.hip) at values far from 1, and in place in short rows.
-Bounds are those of test_gpu_attention_ops.py, with what each test adds to them."""
+"""The attention operators (qk_norm.hip, soft_max_rel.hip, diff_attention*.hip) at values far from 1, in place in short rows, and with
+some of their outputs alone. Bounds are those of test_gpu_attention_ops.py, with what each test adds to them."""
 import math
 
 import pytest
 
 import stx
 from test_gpu_attention_ops import check_diff, diff_back_ref, diff_inputs, qk_back_ref, seen_ref
-from test_gpu_layer_ops import F64, TYPES, U, close, norm_close, randn
+from test_gpu_layer_ops import F64, TYPES, U, close, half_step, norm_close, randn
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -101,6 +101,119 @@ def test_diff_back_of_quiet_last_rows(device, dtype, M, quiet):
     of = lambda t: t[:, first:]  # noqa: E731
     back_of(slice(keys, None), [of(got[0]), got[1][:, keys:], got[2][:, keys:]], of(dy), of(q), k, v, lam, [of(kept[0]), of(kept[1]), kept[2][..., first:]],
             mask[:, first:], D ** -0.5, "rows")
+
+
+@pytest.mark.parametrize("dtype,size", [("f32", 1e-25), ("f32", 1e-6), ("bf16", 1e-25), ("bf16", 1e-6), ("bf16", 1e20), ("f16", 1e-3), ("f16", 3e3)])
+def test_diff_back_sizes(device, dtype, size):
+    """Gradients of these sizes as they are, a third of the rows a hundredth of the others. Where fp16's results are subnormal
+    they are off by 2^-25 at most, a root mean square of 2^-25 / sqrt(3)."""
+    B, M, N, H, Hk, D, V = 1, 80, 150, 2, 1, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    dy = randn(device, (B, M, H, V), 7, size)
+    dy[:, ::3] *= 1e-2
+    dy, mask = dy.to(q.dtype), torch.ones(B, M, N, dtype=torch.bool, device=device)
+    kept = stx.diff_attention(q, k, v, lam, keep=True)
+    got = stx.diff_attention_back(dy, q, k, v, lam, *kept)
+    want = diff_back_ref(dy, q, k, v, lam, *kept, mask, D ** -0.5)
+    for g, (w, bound), name in zip(got, want, ("dq", "dk", "dv", "dlam")):
+        close(g, w, bound, "size " + name)
+        if name != "dlam" and dtype != "f32":
+            low = 2.0 ** -25 * math.sqrt(w.numel() / 3) * 1.2 if dtype == "f16" else 0.0
+            assert float((g.to(F64) - w).norm()) <= half_step(g.dtype) * math.sqrt(2 / 3) * 1.2 * float(w.norm()) + low, name
+
+
+def tensor(t):
+    """The C ABI's description of a tensor (batch, tokens, heads, elements), or NULL."""
+    import ctypes
+    if t is None:
+        return None
+    d = stx.Tensor()
+    d.data = t.data_ptr()
+    for i in range(4):
+        d.ne[i], d.nb[i] = t.shape[3 - i], t.stride(3 - i) * t.element_size()
+    return ctypes.byref(d)
+
+
+def pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+TYPE = {torch.float32: stx.TYPE_F32, torch.float16: stx.TYPE_F16, torch.bfloat16: stx.TYPE_BF16}
+
+
+def ask_alone(outputs, want, call, groups):
+    """call(outputs, those not asked for None) for each group alone: the bits of the full call, the rest untouched."""
+    for group in groups:
+        for i, t in enumerate(outputs):
+            t.fill_(7.0)
+        call([t if i in group else None for i, t in enumerate(outputs)])
+        for i, t in enumerate(outputs):
+            assert torch.equal(t, want[i]) if i in group else bool((t == 7.0).all()), (group, i)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 90, 700, 4, 2), (1, 700, 90, 2, 1), (40, 130, 150, 4, 4)], ids=["split keys", "split rows", "whole"])
+def test_diff_back_outputs_alone(device, dtype, shape):
+    B, M, N, H, Hk = shape
+    D, V, dt = 64, 128, TYPES[dtype]
+    q, k, v, lam, _, _ = diff_inputs(device, dt, (*shape, D, V, True, None))
+    dy = randn(device, (B, M, H, V), 7, dtype=dt)
+    kept = stx.diff_attention(q, k, v, lam, causal=True, keep=True)
+    want = stx.diff_attention_back(dy, q, k, v, lam, *kept, causal=True)
+    L, t = stx.lib(), TYPE[dt]
+    a = [tensor(x) for x in (dy, q, k, v)]
+    ws = torch.empty(L.stx_diff_attention_back_workspace_size(*a[1:], t), dtype=torch.uint8, device=device)
+    s = torch.cuda.current_stream().cuda_stream
+
+    def call(o):
+        stx.check(L.stx_diff_attention_back(*a, t, lam.data_ptr(), D ** -0.5, 1, None, None, tensor(kept[0]), tensor(kept[1]), kept[2].data_ptr(),
+                                            tensor(o[0]), tensor(o[1]), tensor(o[2]), pointer(o[3]), ws.data_ptr(), ws.numel(), s))
+
+    ask_alone([torch.empty_like(x) for x in want], want, call, ({0}, {1, 2}, {3}, {0, 3}, {1, 2, 3}, {0, 1, 2}, set()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("per_head", [False, True])
+def test_qk_back_outputs_alone(device, dtype, per_head):
+    import ctypes
+    B, N, H, Hk, D, dt = 2, 300, 4, 2, 64, TYPES[dtype]
+    q, k = randn(device, (B, N, H, D), 1, dtype=dt), randn(device, (B, N, Hk, D), 2, dtype=dt)
+    dyq, dyk = randn(device, q.shape, 3, dtype=dt), randn(device, k.shape, 4, dtype=dt)
+    wq, wk = (randn(device, (n, D) if per_head else (D,), 5 + n, 0.3, 1.0) for n in (H, Hk))
+    pos, p = torch.arange(N, device=device, dtype=torch.int32), stx.rope_params(D)
+    full = stx.qk_norm_rope_back(dyq, q, pos, p, wq, dyk, k, wk)
+    want = [full[i] for i in (0, 2, 1, 3)]                        # dq, dk, dw_q, dw_k
+    L, t = stx.lib(), TYPE[dt]
+    a = [tensor(x) for x in (dyq, dyk, q, k)]
+    ws = torch.empty(L.stx_qk_norm_rope_back_workspace_size(a[2], a[3], t, D, per_head), dtype=torch.uint8, device=device)
+    s = torch.cuda.current_stream().cuda_stream
+
+    def call(o):
+        sums = o[2] is not None or o[3] is not None
+        stx.check(L.stx_qk_norm_rope_back(*a, t, pos.data_ptr(), 0, ctypes.byref(p), wq.data_ptr(), wk.data_ptr(), per_head, 1e-6, tensor(o[0]), tensor(o[1]),
+                                          pointer(o[2]), pointer(o[3]), ws.data_ptr() if sums else None, ws.numel() if sums else 0, s))
+
+    ask_alone([torch.empty_like(x) for x in want], want, call, ({0}, {1}, {2}, {3}, {0, 1}, {2, 3}, {0, 3}, set()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [5, 150, 2500])
+def test_rel_back_outputs_alone(device, dtype, N):
+    import ctypes
+    B, H, M, dt = 3, 2, 70, TYPES[dtype]
+    p = stx.rel_params(16, 40)
+    y = stx.soft_max_rel(randn(device, (B, H, M, N), 1, dtype=dt), randn(device, (16, H), 2), p)
+    dy = randn(device, y.shape, 3, dtype=dt)
+    want = stx.soft_max_rel_back(dy, y, p, 0.5)
+    L, t = stx.lib(), TYPE[dt]
+    ws = torch.empty(L.stx_soft_max_rel_back_workspace_size(tensor(y), t, 16), dtype=torch.uint8, device=device)
+    s = torch.cuda.current_stream().cuda_stream
+
+    def call(o):
+        stx.check(L.stx_soft_max_rel_back(tensor(dy), tensor(y), t, ctypes.byref(p), 0.5, None, None, tensor(o[0]), pointer(o[1]),
+                                          pointer(ws) if o[1] is not None else None, ws.numel() if o[1] is not None else 0, s))
+
+    ask_alone([torch.empty_like(x) for x in want], want, call, ({0}, {1}, set()))
 
 
 # ------------------------------------------------------------------------- norms and rotation
