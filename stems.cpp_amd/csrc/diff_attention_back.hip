@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
         const RowAt row(a, kvh, min(r, a.rows - 1));
         limit[n] = mask.limit(row.query);
         lam[n] = a.lam[row.head];
-        unit[n] = 1.f, share[n] = rest[n] = 0.f;
+        share[n] = rest[n] = 0.f;
 #pragma unroll
         for (int m = 0; m < 2; m++) load_fragments<T, DP>(qf[m][n], row.at(a.q, b, 2, m), a.dim, lane);
         load_fragments<T, VP>(yf[n], row.at(a.dy, b, 1, 0), a.vdim, lane);
@@ -120,11 +120,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
             base[m][n] = fmaf(a.lse[at], kLog2e, -kShift<T>);
             if (lane < 16 && r < a.rows && part == 0) a.dots[at] = dot[m][n];
         }
+        unit[n] = 1.f;
         if constexpr (std::is_same_v<T, f16>) {
             most *= fmaxf(1.f, fabsf(lam[n]));
             unit[n] = range_scale(a, values, most, kShift<T>);
             loud = fmaxf(loud, most);
             dot[0][n] *= unit[n], dot[1][n] *= unit[n];
+        }
+        // The 16-bit products round low by a hundredth of an ulp in the mean, which dlambda's sum over rows and keys keeps: every
+        // other query has -dy and so -dP, and a negative unit.
+        if (sizeof(T) == 2 && (row.query + b) % 2) {
+            unit[n] = -unit[n];
+#pragma unroll
+            for (int g = 0; g < GV; g++) yf[n][g] ^= 0x80008000u;
         }
     }
     if constexpr (std::is_same_v<T, f16>) {
@@ -210,7 +218,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int at = (wave * NQ + n) * 16 + s;
-        const float sum = column_sum(share[n]);
+        const float sum = column_sum(share[n]) * copysignf(1.f, unit[n]);
         if (lane < 16) shares[at] = r0 + at < a.rows ? sum * __builtin_amdgcn_exp2f(-kShift<T>) : 0.f;
     }
     __syncthreads();
@@ -225,7 +233,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
         const int r = r0 + (wave * NQ + n) * 16 + s;
         if (r >= a.rows) continue;
         const RowAt row(a, kvh, r);
-        const float f = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / unit[n];
+        const float f = a.scale * __builtin_amdgcn_exp2f(-kShift<T>) / fabsf(unit[n]);
         float* to = a.part ? a.part + (((long long)part * (gridDim.x / a.tile_div.d) + per) * a.rows + r) * (2 * DP) : nullptr;
 #pragma unroll
         for (int m = 0; m < 2; m++) {

@@ -5,7 +5,7 @@ import math
 import pytest
 
 import stx
-from test_gpu_attention_ops import check_diff, diff_back_ref, diff_inputs, qk_back_ref, seen_ref
+from test_gpu_attention_ops import check_diff, diff_back_ref, diff_inputs, diff_maps, qk_back_ref, seen_ref
 from test_gpu_layer_ops import F64, TYPES, U, close, half_step, norm_close, randn
 
 pytestmark = pytest.mark.gpu
@@ -101,6 +101,25 @@ def test_diff_back_of_quiet_last_rows(device, dtype, M, quiet):
     of = lambda t: t[:, first:]  # noqa: E731
     back_of(slice(keys, None), [of(got[0]), got[1][:, keys:], got[2][:, keys:]], of(dy), of(q), k, v, lam, [of(kept[0]), of(kept[1]), kept[2][..., first:]],
             mask[:, first:], D ** -0.5, "rows")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(24, 801, 801, 4, 4), (4096, 1, 70, 4, 1), (24, 400, 300, 4, 1)], ids=lambda s: "-".join(map(str, s)))
+def test_diff_lambda_gradient_is_odd(device, dtype, shape):
+    """-dy gives -dlambda. Its share of a row is a mean of dP by the second map, of products each rounded by less than an ulp of dP;
+    over the rows of a head such roundings are a walk, 2 sqrt(rows) u of the mean share, unless they all go one way, as the matrix
+    instructions' do. 4 u |dlambda| are the results'."""
+    B, M, N, H, Hk = shape
+    D, V = 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (*shape, D, V, False, None))
+    dy = randn(device, (B, M, H, V), 7, dtype=q.dtype)
+    kept = stx.diff_attention(q, k, v, lam, keep=True)
+    one, other = (stx.diff_attention_back(y, q, k, v, lam, *kept)[3].to(F64) for y in (dy, -dy))
+    few = slice(0, max(1, 500 // M))
+    p, _, _, _, _, v64 = diff_maps(q[few], k[few], v[few], torch.ones(q[few].shape[0], M, N, dtype=torch.bool, device=device), D ** -0.5)
+    dp = torch.matmul(dy[few].to(F64).transpose(1, 2).contiguous(), v64.transpose(2, 3).contiguous())
+    share = (p[1] * dp.abs()).sum(-1).mean((0, 2))
+    assert bool(((one + other).abs() <= 2 * math.sqrt(B * M) * U * share + 4 * U * one.abs()).all()), (one + other).tolist()
 
 
 @pytest.mark.parametrize("dtype,size", [("f32", 1e-25), ("f32", 1e-6), ("bf16", 1e-25), ("bf16", 1e-6), ("bf16", 1e20), ("f16", 1e-3), ("f16", 3e3)])
