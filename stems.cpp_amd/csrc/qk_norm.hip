@@ -552,6 +552,12 @@ void with_units(int w, const QkArgs& a, F&& f) {
     else lanes(std::integral_constant<int, 1>{});
 }
 
+// Positions and factors of a call, as memory that its outputs leave alone.
+size_t pos_bytes(const stx_tensor* q, int64_t pos_stride) {
+    return q->ne[2] > 0 && q->ne[3] > 0 ? ((size_t)(q->ne[3] - 1) * pos_stride + q->ne[2]) * sizeof(int32_t) : 0;
+}
+size_t factor_bytes(const stx_rope_params* p) { return p->n_dims / 2 * sizeof(float); }
+
 void check_eps(double eps, const char* op) { STX_REQUIRE(eps >= 0.0 && std::isfinite(eps), "%s: eps must be finite and not negative", op); }
 
 size_t weight_bytes(const stx_tensor* t, int per_head) { return t ? (size_t)t->ne[0] * (per_head ? t->ne[1] : 1) * sizeof(float) : 0; }
@@ -571,7 +577,9 @@ void qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const
     const RopeAngles at = rope_angles(p, s.dim, pos_stride, 1.f, op);
     check_eps(eps, op);
     for (const stx_tensor* d : {q_dst, k_dst})
-        if (d) check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, weight_bytes(q, per_head)}, {"w_k", w_k, weight_bytes(k, per_head)}});
+        if (d)
+            check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, weight_bytes(q, per_head)}, {"w_k", w_k, weight_bytes(k, per_head)},
+                                                       {"pos", pos, pos_bytes(q, pos_stride)}, {"freq_factors", p->freq_factors, factor_bytes(p)}});
     if (s.empty()) return;
     STX_REQUIRE(pos != nullptr, "%s: pos is NULL", op);
     const int w = width_of({q, k, q_dst, k_dst}, s.dim, size);
@@ -630,9 +638,11 @@ void qk_norm_rope_back(const stx_tensor* dyq, const stx_tensor* dyk, const stx_t
     const size_t need = sums && !s.empty() ? back_part(s, tile, per_head) : 0, wq = weight_bytes(q, per_head), wk = weight_bytes(k, per_head);
     check_workspace(ws, ws_bytes, need, op);
     check_apart(op, {{"dw_q", dw_q, wq}, {"dw_k", dw_k, wk}, {"the workspace", need ? ws : nullptr, need}},
-                {{"q", q, size}, {"k", k, size}, {"dq_out", dyq, size}, {"dk_out", dyk, size}, {"dq", dq, size}, {"dk", dk, size}, {"w_q", w_q, wq}, {"w_k", w_k, wk}});
+                {{"q", q, size}, {"k", k, size}, {"dq_out", dyq, size}, {"dk_out", dyk, size}, {"dq", dq, size}, {"dk", dk, size}, {"w_q", w_q, wq}, {"w_k", w_k, wk},
+                 {"pos", pos, pos_bytes(q, pos_stride)}, {"freq_factors", p->freq_factors, factor_bytes(p)}});
     for (const stx_tensor* d : {dq, dk})
-        if (d) check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, wq}, {"w_k", w_k, wk}});
+        if (d)
+            check_apart(op, {{"an output", d, size}}, {{"w_q", w_q, wq}, {"w_k", w_k, wk}, {"pos", pos, pos_bytes(q, pos_stride)}, {"freq_factors", p->freq_factors, factor_bytes(p)}});
     if (!dq && !dk && !sums) return;
     float* part = sums ? static_cast<float*>(ws) : nullptr;
     long long blocks = 0;
