@@ -951,8 +951,8 @@ STX_API stx_status stx_soft_max_rel_back(const stx_tensor* dy, const stx_tensor*
  * q [D, 2 H, queries, batch], k [D, 2 kv heads, keys, batch], v [V, kv heads, keys, batch], dst [V, H, queries, batch]; kv
  * heads divide H, D is at most 128 and V at most 256. lambda: device float[H]. lengths: device int32[batch], keys of each
  * sequence, taken as 0 .. keys (NULL: all); causal: query i of sequence b sees keys up to starts[b] + i (starts: device
- * int32[batch], NULL: 0). A query that sees no key gets zeros. Keys from a sequence's length on are not looked at,
- * whatever they hold; k and v before it are finite, also where causality hides them. For the gradients, second (as dst, the second map's output, before
+ * int32[batch], NULL: 0). A query that sees no key gets zeros, whatever it holds. Keys that no query sees, those from a
+ * sequence's length on among them, are not looked at; those that some see are finite. For the gradients, second (as dst, the second map's output, before
  * lambda) and lse (device float [batch][H][2][queries], each map's ln sum exp of the scaled scores, -infinity for a query without
  * keys) receive what stx_diff_attention_back takes; NULL otherwise. Scores, sums and products are float, the maps
  * rounded to the type for their product with v (16-bit types). Rows are contiguous, other strides any; 16-byte aligned rows of k and v are
@@ -970,8 +970,7 @@ STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, 
  * sequence's length on), dlambda (device float[H]); any may be NULL. Scores are formed again; sums are float
  * (dlambda's over rows double), the maps' gradients rounded to the type for their products (16-bit types; fp16's scaled by
  * powers of two, so that they keep its range). dlambda comes from the maps themselves, not from the rounded second. The
- * same rules for masked keys, strides and workspace; dy and q are finite, also at queries that see no key; outputs overlap
- * nothing else. */
+ * same rules for masked keys and queries (dy as q), strides and workspace; outputs overlap nothing else. */
 STX_API size_t     stx_diff_attention_back_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
                                                           stx_type type);
 STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tensor* q, const stx_tensor* k,

@@ -42,12 +42,13 @@ struct DiffArgs {
 
 // A sequence's masks.
 struct Mask {
-    int length;
+    int length;                          // keys that a query sees are below it
     long long start;
     bool causal;
     __device__ __forceinline__ Mask(const DiffArgs& a, int b) : causal(a.causal) {
         length = a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
         start = a.starts ? a.starts[b] : 0;
+        if (causal) length = (int)min((long long)length, max(0LL, start + a.queries));
     }
     __device__ __forceinline__ int limit(int query) const { return causal ? (int)min((long long)length, max(0LL, query + start + 1)) : length; }
 };

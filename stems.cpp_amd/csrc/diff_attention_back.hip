@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void diff_d
         share[n] = rest[n] = 0.f;
 #pragma unroll
         for (int m = 0; m < 2; m++) load_fragments<T, DP>(qf[m][n], row.at(a.q, b, 2, m), a.dim, lane);
-        load_fragments<T, VP>(yf[n], row.at(a.dy, b, 1, 0), a.vdim, lane);
+        load_fragments<T, VP>(yf[n], limit[n] > 0 ? row.at(a.dy, b, 1, 0) : nullptr, a.vdim, lane);   // a row without keys holds anything
         const char *out = row.at(a.out, b, 1, 0), *second = row.at(a.second, b, 1, 0);
         float d1 = 0.f, d2 = 0.f, most = 0.f;
 #pragma unroll

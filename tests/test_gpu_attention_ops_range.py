@@ -38,6 +38,27 @@ def test_diff_large_lambda(device, dtype, Hk, lams):
             norm_close(g, w, 2, "lambda " + name)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+@pytest.mark.parametrize("shape", [(3, 1, 300, 8, 2, 64, 128), (3, 70, 300, 4, 2, 64, 128), (3, 6, 90, 2, 1, 128, 256), (3, 140, 200, 2, 1, 33, 47)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_diff_what_causality_hides(device, dtype, what, shape):
+    """Keys behind a sequence's last query (a cache that is not filled yet, without lengths) and queries that see no key hold anything."""
+    B, M, N, H, Hk, D, V = shape
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (*shape, False, None))
+    dy = randn(device, (B, M, H, V), 7, dtype=q.dtype)
+    starts = torch.tensor([N // 3, 0, -(M // 2) - 1], device=device, dtype=torch.int32)
+    results = []
+    for fill in (0.0, what):
+        for b, at in enumerate(starts.tolist()):
+            k[b, max(0, at + M):] = v[b, max(0, at + M):] = fill
+            q[b, :max(0, -at)] = dy[b, :max(0, -at)] = fill
+        kept = stx.diff_attention(q, k, v, lam, causal=True, starts=starts, keep=True)
+        results.append([*kept, *stx.diff_attention_back(dy, q, k, v, lam, *kept, causal=True, starts=starts)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert bool((results[1][3][2, :M // 2 + 1] == 0).all())
+
+
 def back_of(part, got, dy, q, k, v, lam, kept, mask, scale, what):
     """dq, dk and dv against those of these operands alone; dk and dv of the keys `part`."""
     want = diff_back_ref(dy, q, k, v, lam, *kept, mask, scale)
