@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "rope_angles.hpp"
+#include "typed.hpp"
 
 namespace stx {
 namespace {

@@ -152,6 +152,30 @@ inline void check_apart(const char* op, std::initializer_list<Operand> written, 
     }
 }
 
+// Whether every row of a tensor (NULL: of none) starts at a multiple of `bytes`.
+inline bool rows_aligned(const stx_tensor* t, int bytes) {
+    if (!t) return true;
+    bool ok = reinterpret_cast<uintptr_t>(t->data) % bytes == 0;
+    for (int i = 1; i < 4; i++) ok = ok && (t->ne[i] <= 1 || t->nb[i] % bytes == 0);
+    return ok;
+}
+
+// Checks of an output of src's shape that may be src, by the strides of both.
+inline void check_row_output(const stx_tensor* src, const stx_tensor* dst, int size, const char* what) {
+    check_typed(src, size, what);
+    check_typed(dst, size, what);
+    check_same_shape(src, dst, what);
+    bool same = src->data == dst->data;
+    for (int i = 1; i < 4; i++) {
+        STX_REQUIRE(dst->ne[i] <= 1 || dst->nb[i] > 0, "%s: output stride nb[%d] is 0", what, i);
+        same = same && (dst->ne[i] <= 1 || dst->nb[i] == src->nb[i]);
+    }
+    STX_REQUIRE(nelem(view(dst)) == 0 || nested(dst, size), "%s: rows of the output overlap", what);
+    // In place with other strides, or in part over the input, rows would be read after they were written.
+    STX_REQUIRE(same || src->data != dst->data || nelem(view(src)) == 0, "%s: in place with other strides", what);
+    STX_REQUIRE(same || shared(src, dst, size) != Shared::yes, "%s: the output overlaps the input in part", what);
+}
+
 inline void check_workspace(const void* ws, size_t have, size_t need, const char* what) {
     if (need == 0) return;
     STX_REQUIRE(ws != nullptr && have >= need, "%s: workspace of %zu bytes needed, %zu given", what, need, ws ? have : (size_t)0);
