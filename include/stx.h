@@ -896,10 +896,10 @@ STX_API stx_status stx_qk_norm_rope(const stx_tensor* q, const stx_tensor* k, st
                                     const float* w_k, int per_head, double eps, const stx_tensor* q_dst,
                                     const stx_tensor* k_dst, stx_stream stream);
 /* Its gradients, from dq_out and dk_out (of q_dst and k_dst) and the forward call's inputs: dq and dk (of q and k;
- * each may be the gradient that it comes from, or its q or k), dw_q and dw_k (of the weights, in their layout, summed
- * over tokens and batch and, where heads share them, over heads). Any may be NULL. The rotated gradient times w is float; the
- * rest holds for x of any size. workspace: device, 256-byte
- * aligned, no initialisation; calls that share one must not overlap. None is needed without dw_q and dw_k. */
+ * each may be the gradient that it comes from, or its q or k), dw_q and dw_k (of the weights, in their layout,
+ * summed over tokens and batch and, where heads share them, over heads). Any may be NULL. The rotated gradient times
+ * w is float; the rest holds for x of any size. workspace: device, 256-byte aligned, no initialisation; calls that
+ * share one must not overlap. None is needed without dw_q and dw_k. */
 STX_API size_t     stx_qk_norm_rope_back_workspace_size(const stx_tensor* q, const stx_tensor* k, stx_type type,
                                                         int n_dims, int per_head);
 STX_API stx_status stx_qk_norm_rope_back(const stx_tensor* dq_out, const stx_tensor* dk_out, const stx_tensor* q,
@@ -924,14 +924,14 @@ typedef struct {
     int32_t  causal;               /* a query sees no key after its own position */
 } stx_rel_params;
 
-/* stx_soft_max_ext with a learned position bias and masks, which that op refuses, over scores x [keys, queries, heads,
- * batch] of any of the types:
+/* stx_soft_max_ext with a learned position bias and masks, which that op refuses, over scores x [keys, queries,
+ * heads, batch] of any of the types:
  *   dst = softmax over the keys of scale * x + table[bucket(key - (query + start))][head].
- * table: device float [n_buckets][heads] (ggml [heads, n_buckets]). lengths: device int32[batch], keys of each sequence,
- * taken as 0 .. keys (NULL: all); starts: device int32[batch], the position of its first query (NULL: 0). Masked scores
- * are not read into the result whatever they hold, NaN among it, and get zeros; a row that sees no key, or only scores of
- * -infinity, is zeros. Sums are float. Rows are contiguous; any other strides. dst may be x, and overlaps nothing else. Fewer than 2^30 keys and
- * queries, at most 65,535 heads and 2^24 - 1 sequences. */
+ * table: device float [n_buckets][heads] (ggml [heads, n_buckets]). lengths: device int32[batch], keys of each
+ * sequence, taken as 0 .. keys (NULL: all); starts: device int32[batch], the position of its first query (NULL: 0).
+ * Masked scores are not read into the result whatever they hold, NaN among it, and get zeros; a row that sees no
+ * key, or only scores of -infinity, is zeros. Sums are float. Rows are contiguous; any other strides. dst may be x,
+ * and overlaps nothing else. Fewer than 2^30 keys and queries, at most 65,535 heads and 2^24 - 1 sequences. */
 STX_API stx_status stx_soft_max_rel(const stx_tensor* x, stx_type type, const float* table,
                                     const stx_rel_params* params, float scale, const int32_t* lengths,
                                     const int32_t* starts, const stx_tensor* dst, stx_stream stream);
@@ -948,29 +948,36 @@ STX_API stx_status stx_soft_max_rel_back(const stx_tensor* dy, const stx_tensor*
 /* Differential attention (Ye et al., "Differential Transformer", 2024): the difference of two softmax maps over the
  * same values, so that what both attend to cancels. For head h of H, over the keys that a query sees,
  *   dst_h = softmax(scale * q_2h k_2g^T) v_g - lambda_h * softmax(scale * q_2h+1 k_2g+1^T) v_g,  g = h / (H / kv heads).
- * q [D, 2 H, queries, batch], k [D, 2 kv heads, keys, batch], v [V, kv heads, keys, batch], dst [V, H, queries, batch]; kv
- * heads divide H, D is at most 128 and V at most 256. lambda: device float[H]. lengths: device int32[batch], keys of each
- * sequence, taken as 0 .. keys (NULL: all); causal: query i of sequence b sees keys up to starts[b] + i (starts: device
- * int32[batch], NULL: 0). A query that sees no key gets zeros, whatever it holds. Keys that no query sees, those from a
- * sequence's length on among them, are not looked at; those that some see are finite. For the gradients, second (as dst, the second map's output, before
- * lambda) and lse (device float [batch][H][2][queries], each map's ln sum exp of the scaled scores, -infinity for a query without
- * keys) receive what stx_diff_attention_back takes; NULL otherwise. Scores, sums and products are float, the maps
- * rounded to the type for their product with v (16-bit types). Rows are contiguous, other strides any; 16-byte aligned rows of k and v are
- * faster. Outputs overlap nothing else and their strides nest. workspace: device, 256-byte aligned, no initialisation (0
- * bytes where the call does not split the keys); calls that share one must not overlap. scale > 0. Fewer than 2^28 queries and keys, 2^30 queries to a key head, 2^16 heads,
- * 2^20 sequences, and 2^22 tiles: sequences * kv heads * ceil(queries * heads / kv heads / 64). */
+ * q [D, 2 H, queries, batch], k [D, 2 kv heads, keys, batch], v [V, kv heads, keys, batch], dst [V, H, queries,
+ * batch]; kv heads divide H, D is at most 128 and V at most 256. lambda: device float[H]. lengths: device
+ * int32[batch], keys of each sequence, taken as 0 .. keys (NULL: all); causal: query i of sequence b sees keys up to
+ * starts[b] + i (starts: device int32[batch], NULL: 0). A query that sees no key gets zeros, whatever it holds. Keys
+ * that no query sees, those from a sequence's length on among them, are not looked at; those that some see are
+ * finite, and scaled scores below 2^26 in size.
+ * For the gradients, second (as dst, the second map's output, before lambda) and lse (device float
+ * [batch][H][2][queries], each map's ln sum exp of the scaled scores, -infinity for a query without keys) receive
+ * what stx_diff_attention_back takes; NULL otherwise. Scores, sums and products are float, the maps rounded to the
+ * type for their product with v (16-bit types; the first in two parts). Rows are contiguous, other strides any;
+ * 16-byte aligned rows of k and v are faster. Outputs overlap nothing else and their strides nest. workspace:
+ * device, 256-byte aligned, no initialisation (0 bytes where the call does not split the keys); calls that share one
+ * must not overlap. scale > 0. Fewer than 2^28 queries and keys, 2^30 queries to a key head, 2^16 heads, 2^20
+ * sequences, and 2^22 tiles: sequences * kv heads * ceil(queries * heads / kv heads / 64). */
 STX_API size_t     stx_diff_attention_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
                                                      stx_type type);
 STX_API stx_status stx_diff_attention(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v, stx_type type,
                                       const float* lambda, float scale, int causal, const int32_t* lengths,
                                       const int32_t* starts, const stx_tensor* dst, const stx_tensor* second, float* lse,
                                       void* workspace, size_t workspace_bytes, stx_stream stream);
-/* Its gradients, from dy (of dst), the forward call's inputs and masks and what it kept: out (its dst), second and lse. dq
- * (of q), dk and dv (of k and v, together or neither; summed over the heads that share a key head; zeros for keys from a
- * sequence's length on), dlambda (device float[H]); any may be NULL. Scores are formed again; sums are float
- * (dlambda's over rows double), the maps' gradients rounded to the type for their products (16-bit types; fp16's scaled by
- * powers of two, so that they keep its range). dlambda comes from the maps themselves, not from the rounded second. The
- * same rules for masked keys and queries (dy as q), strides and workspace; outputs overlap nothing else. */
+/* Its gradients, from dy (of dst), the forward call's inputs and masks and what it kept: out (its dst), second and
+ * lse. dq (of q), dk and dv (of k and v, together or neither; summed over the heads that share a key head; zeros for
+ * keys that no query sees), dlambda (device float[H]); any may be NULL. Scores are formed again; sums are float
+ * (dlambda's over rows double). In 16-bit types the maps and their gradients are rounded to the type for their
+ * products, fp16's after a scaling by powers of two from the largest |v|, |dy| and |lambda| that meet in a block of
+ * rows and keys, so that what other sequences and key heads hold costs no bits. dlambda comes from the maps
+ * themselves, not from the rounded second. lse is float, so the maps are off by |lse| 2^-24 of themselves; the first
+ * map's row dots are dy (out + lambda second), so that its dq and dk carry |lambda| times the rounding of out where
+ * |lambda| is far above 1. The same rules for masked keys and queries (dy as q), strides and workspace; outputs
+ * overlap nothing else. */
 STX_API size_t     stx_diff_attention_back_workspace_size(const stx_tensor* q, const stx_tensor* k, const stx_tensor* v,
                                                           stx_type type);
 STX_API stx_status stx_diff_attention_back(const stx_tensor* dy, const stx_tensor* q, const stx_tensor* k,

@@ -143,6 +143,23 @@ def test_diff_lambda_gradient_is_odd(device, dtype, shape):
     assert bool(((one + other).abs() <= 2 * math.sqrt(B * M) * U * share + 4 * U * one.abs()).all()), (one + other).tolist()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 40, 150])
+def test_diff_large_scores(device, dtype, M):
+    """Scaled scores of up to 2^26, of which fp32 keeps so few digits that a row is nearly one key's: the maps stay maps (outputs
+    within sqrt(2) times the largest value) and lse follows the largest score."""
+    B, N, H, Hk, D, V = 1, 300, 2, 1, 64, 128
+    q, k, v, lam, _, _ = diff_inputs(device, TYPES[dtype], (B, M, N, H, Hk, D, V, False, None))
+    q, k = q * 2.0 ** 10, k * 2.0 ** 10
+    mask = torch.ones(B, M, N, dtype=torch.bool, device=device)
+    scale = 2.0 ** 25.9 / float(diff_maps(q, k, v, mask, 1.0)[2].max())
+    out, second, lse = stx.diff_attention(q, k, v, lam, scale=scale, keep=True)
+    top = float(v.to(F64).abs().max()) * math.sqrt(2)
+    assert float(second.to(F64).abs().max()) <= top and float(out.to(F64).abs().max()) <= top * (1 + float(lam.abs().max()))
+    _, want, size, _, _, _ = diff_maps(q, k, v, mask, scale)
+    assert bool(((lse.to(F64) - want).abs() <= ((D + 8) * U * size.squeeze(-1).permute(1, 2, 0, 3) + 4 * U * want.abs())).all())
+
+
 @pytest.mark.parametrize("dtype,size", [("f32", 1e-25), ("f32", 1e-6), ("bf16", 1e-25), ("bf16", 1e-6), ("bf16", 1e20), ("f16", 1e-3), ("f16", 3e3)])
 def test_diff_back_sizes(device, dtype, size):
     """Gradients of these sizes as they are, a third of the rows a hundredth of the others. Where fp16's results are subnormal
