@@ -21,7 +21,8 @@ namespace {
 // fp16's P is scaled by 2^6 so that shares of 2^-20 keep all their bits.
 //
 // Those 60 x 801 frames of 4 heads of 64 and 128 take 215 to 230 us (551 TFLOP/s of the formula's products), 4 x 4 heads of 8,192 x 8,192
-// 960 us (860): exponentials (vector units 57 % busy) and products (matrix cores 42 %), which two waves a SIMD overlap in part.
+// 960 us (860): exponentials (vector units 56 % busy) and products (matrix cores 42 %), which two waves a SIMD overlap in part. Of 801 rows the
+// last tile of 128 has 33, so two of its waves work for nothing, and 1,680 blocks are 3.3 rounds of the 512 that fit.
 // One token of 8 sequences over caches of up to 16,384 (210 MB): 40 us, 5 TB/s, and 5 us to join the parts.
 template <class T>
 constexpr float kShift = std::is_same_v<T, f16> ? 6.f : 0.f;

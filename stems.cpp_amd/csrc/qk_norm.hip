@@ -15,13 +15,13 @@ namespace {
 // before the first is stored: outputs may be inputs. A lane whose pair partner lies in another unit
 // (mode 2, or units of one element) loads it too, from the same lines: units stay dense for any
 // n_dims, where units of a pair of halves would leave 6 of 16 lanes idle at 128 elements, 96 rotated.
-// A lane's squares and products g x r (of g's size for any x) are added in float, by halves (three roundings at V 8), the lanes' in double; a wave that
-// meets a row whose squares leave fp32 forms them again in double, so data of any size keeps its norm; so are products past 10^30. (In
-// double throughout, with a double division and root, these took more time than the memory's: the gradient of 2 x
-// 16,384 tokens of 40 rows of 128 bf16 values 297 us.)
+// A lane's squares and products g x r (of g's size for any x) are added in float, by halves (three roundings at V 8), the lanes' in
+// double; a wave that meets a row whose squares leave fp32, or products past 10^30, forms them again in double, so data of any
+// size keeps its norm. (In double throughout, with a double division and root, these took more time than the memory's: the
+// gradient of 2 x 16,384 tokens of 40 rows of 128 bf16 values 297 us.)
 // 60 x 801 tokens of 16 rows of 64 fp32 values, slices of a projection (394 MB): 79 us, 5.0 TB/s, the rate of a large copy;
-// its bf16 gradient with weights of each head (295 MB) 79 us, 3.7 TB/s, vector units 86 % busy (short rows pay the sums across
-// lanes and the root as long ones do); that of 2 x 16,384 tokens above (1.0 GB) 211 us, 4.8 TB/s. One token of 16 rows: 5.0 us.
+// its bf16 gradient with weights of each head (295 MB) 80 us, 3.7 TB/s, vector units 84 % busy (short rows pay the sums across
+// lanes and the root as long ones do); that of 2 x 16,384 tokens above (1.0 GB) 212 us, 4.8 TB/s. One token of 16 rows: 5.0 us.
 struct QkSide {
     const char *x, *dy;
     char* out;

@@ -17,7 +17,7 @@ namespace {
 // than 2^14 16-bit or 2^13 32-bit scores are read twice), vectors of 16 bytes at any alignment. The bias
 // costs no bytes: buckets change only where |j - at| is below the last edge `reach`, so a block keeps the head's
 // biases by distance in LDS, and vectors beyond take a constant.
-// HBM bounds both, vector units 70 to 76 % busy beside it: 8 x 1,344 x 1,344 fp32 scores (116 MB) 26 us, 4.5 TB/s; gradients
+// HBM bounds both, vector units 68 to 78 % busy beside it: 8 x 1,344 x 1,344 fp32 scores (116 MB) 26 us, 4.5 TB/s; gradients
 // of 8 x 8,192 x 8,192 bf16 scores (3.2 GB) 718 us, 4.5 TB/s, and of 12 x 8 x 801 x 801 fp32 scores of ragged lengths 161 us,
 // 3.9 TB/s (rows at no alignment). 8 clips of one query: 5.2 us.
 constexpr int kRelThreads = 256;
