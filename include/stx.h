@@ -890,7 +890,7 @@ STX_API size_t     stx_group_norm_cl_forward_workspace_size(const stx_tensor* a,
  * NULL (1). pos, pos_stride and params as in stx_rope_scaled; so are strides, limits and the outputs that may be the
  * inputs. A row's mean square is added in double from sums of at most 16 squares in float (in double where they leave
  * fp32's range); the rest is float, rounded once. A row whose sqrt(mean(x^2) + eps) is below 2^-128, so that its
- * reciprocal is no float, gives infinities. Rows of up to 1,024 elements; eps >= 0. */
+ * reciprocal is no float, gives infinities or NaN. Rows of up to 1,024 elements; eps >= 0. */
 STX_API stx_status stx_qk_norm_rope(const stx_tensor* q, const stx_tensor* k, stx_type type, const int32_t* pos,
                                     int64_t pos_stride, const stx_rope_params* params, const float* w_q,
                                     const float* w_k, int per_head, double eps, const stx_tensor* q_dst,
@@ -930,8 +930,9 @@ typedef struct {
  * table: device float [n_buckets][heads] (ggml [heads, n_buckets]). lengths: device int32[batch], keys of each
  * sequence, taken as 0 .. keys (NULL: all); starts: device int32[batch], the position of its first query (NULL: 0).
  * Masked scores are not read into the result whatever they hold, NaN among it, and get zeros; a row that sees no
- * key, or only scores of -infinity, is zeros. Sums are float. Rows are contiguous; any other strides. dst may be x,
- * and overlaps nothing else. Fewer than 2^30 keys and queries, at most 65,535 heads and 2^24 - 1 sequences. */
+ * key, or only scores of -infinity, is zeros. Scaled scores and sums are float (scale * x past its range is
+ * infinite). Rows are contiguous; any other strides. dst may be x, and overlaps nothing else. Fewer than 2^30 keys
+ * and queries, at most 65,535 heads and 2^24 - 1 sequences. */
 STX_API stx_status stx_soft_max_rel(const stx_tensor* x, stx_type type, const float* table,
                                     const stx_rel_params* params, float scale, const int32_t* lengths,
                                     const int32_t* starts, const stx_tensor* dst, stx_stream stream);
